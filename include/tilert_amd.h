@@ -47,6 +47,10 @@
  *                                the format tl_indexer_fp8_scores_paged reads)
  *   tl_flash_sparse_mla    flash_sparse_mla_op            .../ops/flash_sparse_mla.py:18-93
  *                          (golden FlashSparseMLACombine.golden_forward :152-196)
+ *   tl_mla_cache_write     rmsnorm_kv_op, the key half of qkv_rope_op  .../ops/rmsnorm_kv.py:20-43, qkv_rope.py:42-50
+ *   tl_mla_cache_read      the cache's bf16 form (MlaNsaProfile.convert)  pd_vllm/profiles/mla_nsa.py:150-185
+ *   tl_flash_paged_mla     the dense form of flash_sparse_mla_op over those pages
+ *   tl_add_rmsnorm_quant   rmsnorm_quant_op behind a residual sum  tilert/models/common.py:92-133
  *   tl_topk_rows           topk_accurate_op               .../ops/topk.py:62-109
  *   tl_indexer_fp8_topk    sparse_index_topk_dsv32_op (fp8 cache)  .../ops/sparse_index.py:72-128
  *   tl_indexer_bf16_scores sparse_index_op (bf16, the reference's own)  .../ops/sparse_index.py:11-69
@@ -420,6 +424,65 @@ int tl_flash_sparse_mla(const void* q_nope_bf16, const void* q_pe_bf16, const vo
                         int64_t seqlen, int64_t heads, int64_t topk, int64_t kv_rows,
                         float softmax_scale, void* out_bf16, float* out_acc, float* lse,
                         float* lse_acc, void* stream);
+
+/* RMSNorm of a residual sum with activation quantisation (RMSNorm.forward with a residual,
+ * tilert/models/common.py:92-133, then act_quant): for x, residual bf16 [rows, dim] and gamma
+ * fp32 [dim], h = x + residual in fp32, sum_bf16 = bf16(h), n = gamma * h * 1/sqrt(mean(h^2) +
+ * eps), y_bf16 = bf16(n), and per 1x128 group y_scale = the act_quant scale of max |n|
+ * (scale_mode as tl_act_quant), y_fp8 = e4m3fn(clamp(n / y_scale)): norm and codes come from
+ * unrounded values, where tl_rmsnorm_quant's codes are those of its bf16 output.  sum_bf16 may
+ * be x or residual itself; no other output may overlap an input.  Either y_bf16 or
+ * (y_fp8, y_scale) may be null.  dim % 128 == 0, dim <= 16384; pointers 16-byte aligned. */
+int tl_add_rmsnorm_quant(const void* x_bf16, const void* residual_bf16, const float* gamma, float eps,
+                         int64_t rows, int64_t dim, void* sum_bf16, void* y_bf16, void* y_fp8,
+                         float* y_scale, int scale_mode, void* stream);
+
+/* ---- The paged latent cache.  kv_pages u8 [n_pages, 41216], 16-byte aligned: page p holds 64
+ * keys as 64 x 512 e4m3fn codes, 64 fp32 scales, 64 x 64 bf16 rope parts; a key's latent is
+ * code * scale.  A batch of n_seqs sequences over it (int32, on the device): sequence b owns
+ * the call's tokens cu_seqlens[b] .. cu_seqlens[b+1]-1 (cu_seqlens [n_seqs + 1], ascending from
+ * 0), its cache holds seq_lens[b] keys with them, and its key at position p is row p % 64 of
+ * page block_table[b, p / 64] (block_table [n_seqs, max_pages]): token t stands at position
+ * seq_lens[b] - (cu_seqlens[b+1] - cu_seqlens[b]) + t - cu_seqlens[b].  n_tokens is the number
+ * of rows of the call's tensors: rows from cu_seqlens[n_seqs] on are left as they are.  No
+ * metadata makes a kernel leave the pages: a position below 0 or past the table, and a page id
+ * outside [0, n_pages), name no key. */
+
+/* The new tokens' keys: kv bf16 [n_tokens, 512], n = RMSNorm(kv) * gamma in fp32 (gamma fp32
+ * [512]; null: n = kv), scale = the act_quant scale of the key's max |n| (scale_mode as
+ * tl_act_quant; NaN for a key with a NaN or an infinity, whose codes are finite all the same),
+ * code = e4m3fn(clamp(n / scale)); pe bf16 [n_tokens, 64] turned by freqs fp32 [n_tokens, 64]
+ * ((cos, sin) interleaved; null: not turned), dims (2i, 2i + 1) paired (interleaved = 1) or (i,
+ * i + 32) (0), as bf16.  Replaces rmsnorm_kv_op and the key half of qkv_rope_op
+ * (ops/rmsnorm_kv.py:20-43, ops/qkv_rope.py:42-50).  kv and gamma 16-byte aligned. */
+int tl_mla_cache_write(const void* kv_bf16, const void* pe_bf16, void* kv_pages, int64_t n_pages,
+                       const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
+                       const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, const float* gamma,
+                       const float* freqs, float eps, int interleaved, int scale_mode, void* stream);
+
+/* Keys in flat bf16 form: row t of kv bf16 [n_tokens, 512] = bf16(code * scale) and of pe bf16
+ * [n_tokens, 64] from the key of token t; rows with no key are left as they are.  The caches
+ * tl_flash_sparse_mla reads (MlaNsaProfile.convert, pd_vllm/profiles/mla_nsa.py:150-185).  kv
+ * and pe 16-byte aligned. */
+int tl_mla_cache_read(const void* kv_pages, int64_t n_pages, const int32_t* block_table, int64_t max_pages,
+                      const int32_t* cu_seqlens, const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens,
+                      void* kv_bf16, void* pe_bf16, void* stream);
+
+/* Causal MLA attention of the batch's tokens: q_nope bf16 [n_tokens, heads, 512], q_pe bf16
+ * [n_tokens, heads, 64]; token t at position p sees the keys 0 .. p of its sequence:
+ *   s[j] = (q_nope . latent[j] + q_pe . rope[j]) * softmax_scale,  out = softmax(s) . latent
+ * out bf16 [n_tokens, heads, 512], lse fp32 [n_tokens, heads] (nullable) = ln sum e^s; 0 and
+ * -inf where no key is seen.  fp32 scores, statistics and sums; probabilities times key
+ * scales are rounded to bf16.  1 <= heads <= 128, n_tokens * heads < 2^31; q and out 16-byte
+ * aligned.  workspace: tl_flash_paged_mla_workspace_bytes bytes (0: none), 16-byte aligned, its
+ * contents of no account before or after; calls that overlap in time need one each.  The
+ * dense form of flash_sparse_mla_op (ops/flash_sparse_mla.py:18-93). */
+size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads);
+int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const void* kv_pages, int64_t n_pages,
+                       const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
+                       const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t heads,
+                       float softmax_scale, void* out_bf16, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* Exact per-row top-k.  logits fp32 [rows, ld]; row i considers columns
  * [0, valid_base + 1 + i) (clamped to [0, ld]) -- topk_accurate's convention with

@@ -60,6 +60,16 @@ def _require_cuda(name: str, *ts: torch.Tensor | None) -> None:
             raise ValueError(f"{name}: tensors on different devices ({ts[0].device} vs {t.device})")
 
 
+def _call(t: torch.Tensor, name: str, *args) -> None:
+    """``_lib.call`` with t's GPU as the current one: a launch goes to the current device."""
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args)
+
+
 def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt: str | None = None
               ) -> tuple[torch.Tensor, torch.Tensor]:
     """Quantise ``x`` (bf16, [..., K]) per 1x128 group to e4m3fn with fp32 scales.
