@@ -260,20 +260,21 @@ typedef __attribute__((address_space(3))) uint8_t* lds_u8_ptr;
 // are invisible to it, and the kernel's own s_waitcnt (and s_barrier, where waves share a
 // stage) order them.  m0 is saved into a scratch SGPR and restored inside the statement: it is a
 // reserved register that the compiler may keep live, so the assembly leaves it as it found it.
+// The s_nop is the wait state that the copy needs between the write of m0 and its use.
 // NT: a non-temporal copy, for weights that are streamed once.
 template <bool NT = false>
 __device__ inline void dma_lds16(const void* src, uint32_t lds) {
   uint32_t saved;
   if constexpr (NT)
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off nt\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt\n\ts_mov_b32 m0, %0"
                  : "=&s"(saved) : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
   else
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(saved) : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
 }
 __device__ inline void dma_lds4(const void* src, uint32_t lds) {
   uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(saved) : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
 }
 
