@@ -2,7 +2,20 @@
 // position p, and head h, over the keys j <= p:
 //   s[j] = (q_nope[t,h] . latent[j] + q_pe[t,h] . rope[j]) * softmax_scale
 //   out[t,h] = sum_j softmax(s)[j] latent[j],  lse[t,h] = ln sum_j e^s[j]      (0 and -inf where no key is seen)
+//
+// A sequence's rows (token, head), token-major, are cut into tiles of BM; a workgroup takes a tile through the
+// sequence's pages, 64 keys a step.  The latents go into both products as the codes they are stored as, on the fp8
+// MFMA; the other operand is split into two e4m3 numbers, x = hi + lo / 32:
+//   q / sigma (sigma: a power of two that brings the row's largest magnitude into [128, 256)): exact for
+//     values down to 2^-15 of the row's largest, below that within 2^-23 of it;
+//   p * scale_j * kP / s_ref (kept <= 256): 8 to 9 significant bits, as bf16, down to 2^-21 of the largest.
+// Two fp8 products take the time of one in bf16, and no code is converted: with codes turned into bf16 the
+// conversions alone (64 a page and wave for each product and 32 rows) would take as long as the products.
+// Scores are U = scale_j * (codes . q / sigma) + (q_pe / sigma) . rope (bf16 MFMA), the exponent U * (sigma *
+// softmax_scale * log2 e) - m; all statistics and sums are fp32.
 #include <math.h>
+
+#include <type_traits>
 
 #include "paged.h"
 #include "../../include/tilert_amd.h"
@@ -11,64 +24,702 @@ namespace tl {
 
 typedef uint32_t u32x4p __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2p __attribute__((ext_vector_type(2)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
 
-// One wave a row (token, head): 8 latent dims and one rope dim a lane, key after key, with the running
-// maximum and sum.
-__global__ __launch_bounds__(256) void paged_mla_rows_kernel(const uint16_t* __restrict__ q_nope, const uint16_t* __restrict__ q_pe,
-                                                             const uint8_t* __restrict__ pages, PagedBatch p, int heads,
-                                                             float scale, uint16_t* __restrict__ out, float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = static_cast<int>(r / heads);
-  if (t >= p.n_tokens) return;
-  const int b = find_seq(p.cu, p.n_seqs, t);
-  if (b < 0 || b >= p.n_seqs) return;
-  const int64_t first = p.cu[b], end = p.cu[b + 1];
-  if (t < first || t >= end) return;
-  const int64_t seen = min(p.lens[b] - end + t + 1, static_cast<int64_t>(p.max_pages) * kKvPageKeys);
-  float q[8], o[8], qp = bf16_to_f32(q_pe[r * kKvRope + lane]);
-  const u32x4p raw = reinterpret_cast<const u32x4p*>(q_nope + r * kKvLatent)[lane];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    q[i] = __uint_as_float(i & 1 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
-    o[i] = 0.f;
+constexpr int kPagedWgs = 256;      // workgroups of a split launch: one per CU
+constexpr int kPagedMaxTiles = 1024;  // tiles (and sequences) that a split launch plans in LDS
+constexpr int kPagedMinPages = 1;     // pages a workgroup takes at least
+constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
+constexpr int kSlots = 3;
+constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
+constexpr float kP = 32.0f;          // p * scale / s_ref is held at kP at most when m and s_ref were last set,
+constexpr float kPMost = 256.0f;     // and at kPMost until they are set again
+constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
+
+// NW waves: wave w scores the keys 16 (w % 4) .. +15 of a page for the row group w / 4 (RT tiles of 16 rows) and
+// multiplies P with the latent dims 512 / NW * w .. for all rows.
+template <int NW, int RT>
+struct PagedCfg {
+  static constexpr int kThreads = NW * 64;
+  static constexpr int BM = 16 * RT * (NW / 4);
+  static constexpr int RT2 = (BM + 31) / 32;     // 32-row tiles of the second product
+  static constexpr int PR = RT2 * 32;            // rows of P in LDS
+  static constexpr int DT = 16 / NW;             // 32-dim tiles a wave
+  static constexpr int kDma = 40 / NW;           // 1 KB pieces of a page a wave
+  static constexpr int SCALE_OFF = kSlots * kSlotBytes;
+  static constexpr int P_OFF = SCALE_OFF + kSlots * kKvPageKeys * 4;
+  static constexpr int P_BYTES = PR * kPStride;  // one of hi, lo of one buffer
+  static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;   // [4][BM] f32
+  static constexpr int ALPHA_OFF = STAT_OFF + 4 * BM * 4;  // [PR] f32
+  static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;      // [PR] f32
+  static constexpr int FLAG_OFF = ROWL_OFF + PR * 4;       // [4] i32
+  static constexpr int SCAN_OFF = FLAG_OFF + 16;           // [NW] i32
+  static constexpr int SEQ_OFF = SCAN_OFF + NW * 4;        // [kPagedMaxTiles] i32: tiles up to sequence b and with it
+  static constexpr int TILE_OFF = SEQ_OFF + kPagedMaxTiles * 4;  // [kPagedMaxTiles] i32: pages up to tile t and with it
+  static constexpr int BYTES = TILE_OFF + kPagedMaxTiles * 4;
+  static constexpr size_t kPartFloats = static_cast<size_t>(PR) * kKvLatent;
+};
+
+// What a split launch leaves for the combine kernel, in the workspace: for every workgroup the tile that it
+// continues, if it is the second on it; two slots of partial sums a workgroup (0: of the tile that it continues, 1: of
+// the tile that another one goes on with).
+struct SplitTile {
+  int64_t row0;
+  int rows, parts;
+};
+
+struct PagedArgs {
+  const uint16_t* q_nope;
+  const uint16_t* q_pe;
+  const uint8_t* pages;
+  PagedBatch p;
+  int heads;
+  float scale;  // softmax_scale * log2 e
+  uint16_t* out;
+  float* lse;
+  SplitTile* split;  // [kPagedWgs]; null: one workgroup a tile
+  float2* part_ml;   // [2 kPagedWgs][PR]
+  float* part_o;     // [2 kPagedWgs][kPartFloats]
+  int tile_cap;      // tiles that the launch makes room for
+};
+
+// A sequence's row tiles and what they see, from untrusted metadata.
+struct SeqRows {
+  int first, n_tok;   // tokens
+  int64_t base;       // position of the first
+  __device__ inline SeqRows(const PagedBatch& p, int b) {
+    const int c0 = p.cu[b], c1 = p.cu[b + 1];
+    first = min(max(c0, 0), p.n_tokens);
+    const int end = min(max(c1, first), p.n_tokens);
+    n_tok = end - first;
+    base = static_cast<int64_t>(p.lens[b]) - c1 + first;
   }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < seen; ++j) {
-    const int pg = p.table[static_cast<int64_t>(b) * p.max_pages + (j >> 6)];
-    if (pg < 0 || pg >= p.n_pages) continue;
-    const int row = static_cast<int>(j & 63);
-    const uint8_t* page = pages + static_cast<int64_t>(pg) * kKvPageBytes;
-    const uint2 code = reinterpret_cast<const uint2*>(page + row * kKvLatent)[lane];
-    const float ks = *reinterpret_cast<const float*>(page + kKvScaleAt + row * 4);
-    float k[8];
-    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(code.x, false), c = __builtin_amdgcn_cvt_pk_f32_fp8(code.x, true);
-    const v2f d = __builtin_amdgcn_cvt_pk_f32_fp8(code.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8(code.y, true);
-    k[0] = a.x; k[1] = a.y; k[2] = c.x; k[3] = c.y; k[4] = d.x; k[5] = d.y; k[6] = e.x; k[7] = e.y;
-    float dot = qp * bf16_to_f32(reinterpret_cast<const uint16_t*>(page + kKvRopeAt)[row * kKvRope + lane]);
+  __device__ inline int tiles(int heads, int bm) const { return (n_tok * heads + bm - 1) / bm; }
+  // keys that the row'th row of the sequence sees
+  __device__ inline int seen(const PagedBatch& p, int row, int heads) const {
+    const int64_t n = base + row / heads + 1, most = min(static_cast<int64_t>(p.max_pages) * kKvPageKeys, static_cast<int64_t>(0x7fffffc0));
+    return static_cast<int>(n < 0 ? 0 : (n > most ? most : n));
+  }
+  __device__ inline int pages(const PagedBatch& p, int tile, int heads, int bm) const {
+    return (seen(p, min(n_tok * heads, (tile + 1) * bm) - 1, heads) + kKvPageKeys - 1) / kKvPageKeys;
+  }
+};
+
+// Inclusive sum over the workgroup's threads, and the total of all; `part` holds one int a wave.
+template <int NW>
+__device__ inline int block_scan(int v, int* part, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      k[i] *= ks;
-      dot = __builtin_fmaf(q[i], k[i], dot);
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int x = part[w];
+    before += w < wave ? x : 0;
+    total += x;
+  }
+  __syncthreads();
+  return v + before;
+}
+
+// The first index of an ascending array that is > x.
+__device__ inline int upper(const int* a, int n, int x) {
+  int lo = 0;
+  while (n > 0) {
+    const int h = n >> 1;
+    if (a[lo + h] <= x) { lo += h + 1; n -= h + 1; }
+    else n = h;
+  }
+  return lo;
+}
+
+__device__ inline v4f mfma16_fp8(const v8i& a, const v8i& b, v4f c, int scale_b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, kScaleOne, 0, scale_b);
+}
+__device__ inline v16f mfma32_fp8(const v8i& a, const v8i& b, v16f c, int scale_b) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, kScaleOne, 0, scale_b);
+}
+__device__ inline v8i two_v4i(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Four values (finite, <= 256 in magnitude, or NaN) as hi + lo / 32, four codes each.
+__device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
+  const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 32.0f, (x[1] - a[1]) * 32.0f, 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 32.0f, (x[3] - b[1]) * 32.0f, lo, true);
+}
+
+template <int NW, int RT>
+__global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedArgs A) {
+  using C = PagedCfg<NW, RT>;
+  constexpr int BM = C::BM, RT2 = C::RT2, DT = C::DT;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kq = wave & 3, rh = wave >> 2;  // key quarter, row group
+  const int n16 = lane & 15, g = lane >> 4;
+  const int n32 = lane & 31, half = lane >> 5;
+  const PagedBatch& p = A.p;
+  int* seq_end = reinterpret_cast<int*>(smem + C::SEQ_OFF);
+  int* unit_end = reinterpret_cast<int*>(smem + C::TILE_OFF);
+  int* scan = reinterpret_cast<int*>(smem + C::SCAN_OFF);
+  float* stat = reinterpret_cast<float*>(smem + C::STAT_OFF);
+  float* alpha_l = reinterpret_cast<float*>(smem + C::ALPHA_OFF);
+  float* rowl = reinterpret_cast<float*>(smem + C::ROWL_OFF);
+  int* flag = reinterpret_cast<int*>(smem + C::FLAG_OFF);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8_ptr)smem));
+  const int w = blockIdx.x;
+
+  // ---- the work of this workgroup
+  int n_tiles = 0, u = 0, u_end = 1, quota = 1, tile = 0, seq = 0, seq_tile0 = 0;
+  if (A.split) {
+    // units are pages of tiles (a tile that sees nothing counts one); every workgroup takes `quota` of them in a row
+    for (int b0 = 0; b0 < p.n_seqs; b0 += C::kThreads) {
+      const int b = b0 + tid;
+      int total;
+      const int t = block_scan<NW>(b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), A.tile_cap) : 0, scan, total);
+      if (b < p.n_seqs) seq_end[b] = min(n_tiles + t, A.tile_cap);
+      n_tiles = min(n_tiles + total, A.tile_cap);
     }
-    const float s = wave_sum_f32(dot) * scale;
-    const float mn = fmaxf(m, s), keep = m == -INFINITY ? 0.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(s - mn);
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + w * k[i];
-    m = mn;
+    __syncthreads();
+    const int per = (n_tiles + C::kThreads - 1) / C::kThreads, t0 = tid * per, t1 = min(t0 + per, n_tiles);
+    int sum = 0;
+    if (t0 < t1) {
+      int b = upper(seq_end, p.n_seqs, t0);
+      SeqRows s(p, b);
+      for (int t = t0; t < t1; ++t) {
+        while (t >= seq_end[b]) s = SeqRows(p, ++b);
+        sum += max(1, s.pages(p, t - (b ? seq_end[b - 1] : 0), A.heads, BM));
+        unit_end[t] = sum;
+      }
+    }
+    int units;
+    const int before = block_scan<NW>(sum, scan, units) - sum;
+    for (int t = t0; t < t1; ++t) unit_end[t] += before;
+    __syncthreads();
+    quota = max(kPagedMinPages, (units + kPagedWgs - 1) / kPagedWgs);
+    u = min(w * quota, units);
+    u_end = min(u + quota, units);
+    tile = upper(unit_end, n_tiles, u);
+    if (tid == 0) {
+      SplitTile info{0, 0, 0};
+      if (u < u_end) {
+        const int first = tile ? unit_end[tile - 1] : 0;
+        if (first < u && first >= u - quota) {  // the second workgroup on its first tile
+          const int b = upper(seq_end, p.n_seqs, tile);
+          const SeqRows s(p, b);
+          const int j = tile - (b ? seq_end[b - 1] : 0);
+          info.row0 = static_cast<int64_t>(s.first) * A.heads + static_cast<int64_t>(j) * BM;
+          info.rows = min(BM, s.n_tok * A.heads - j * BM);
+          info.parts = (unit_end[tile] - 1) / quota - first / quota + 1;
+        }
+      }
+      A.split[w] = info;
+    }
+  } else {
+    // one workgroup a tile: its sequence, from the tile counts in order
+    tile = w;
+    seq = -1;
+    for (int b0 = 0; b0 < p.n_seqs; b0 += C::kThreads) {
+      const int b = b0 + tid;
+      int total;
+      const int mine = b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), static_cast<int>(gridDim.x)) : 0;
+      const int t = n_tiles + block_scan<NW>(mine, scan, total);
+      if (w >= t - mine && w < t) { scan[0] = b; scan[1] = t - mine; }
+      __syncthreads();
+      if (w < n_tiles + total) { seq = scan[0]; seq_tile0 = scan[1]; break; }
+      n_tiles += total;
+      __syncthreads();
+    }
+    if (seq < 0) return;
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  u32x4p w;
+
+  while (u < u_end) {
+    // ---- the tile: rows row0 .. row0 + rows - 1 of the call's (token, head) rows, pages pg0 .. pg0 + n - 1
+    int tile_u0 = 0, tile_u1 = 1;
+    if (A.split) {
+      seq = upper(seq_end, p.n_seqs, tile);
+      seq_tile0 = seq ? seq_end[seq - 1] : 0;
+      tile_u0 = tile ? unit_end[tile - 1] : 0;
+      tile_u1 = unit_end[tile];
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    const SeqRows s(p, seq);
+    const int j = tile - seq_tile0;
+    const int in_seq = j * BM;
+    const int64_t row0 = static_cast<int64_t>(s.first) * A.heads + in_seq;
+    const int rows = min(BM, s.n_tok * A.heads - in_seq);
+    const int n_pages = s.pages(p, j, A.heads, BM);
+    const int seen_all = s.seen(p, in_seq, A.heads);  // every row sees these
+    const int pg0 = __builtin_amdgcn_readfirstlane(u - tile_u0);
+    const int n = __builtin_amdgcn_readfirstlane(min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0));
+    const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
+
+    // page k of the tile into its slot: 1 KB pieces, 32 of codes and 8 of rope parts; the 16-byte chunk c of a row
+    // goes to c ^ (row & 7), so that the rows' chunks that a read takes together are in different banks
+    auto fetch = [&](int k) {
+      int id = table[k];
+      if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.n_pages)) id = 0;  // its keys are masked
+      const uint8_t* page = A.pages + static_cast<int64_t>(id) * kKvPageBytes;
+      const uint32_t slot = lds0 + (k % kSlots) * kSlotBytes;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = bf16x2_bits(v2f{o[2 * i] * inv, o[2 * i + 1] * inv});
-  reinterpret_cast<u32x4p*>(out + r * kKvLatent)[lane] = w;
-  if (lse && lane == 0) lse[r] = l == 0.f ? -INFINITY : m + logf(l);
+      for (int i = 0; i < C::kDma; ++i) {
+        const int blk = wave * C::kDma + i;
+        if (blk < 32) {
+          const int row = 2 * blk + (lane >> 5);
+          dma_lds16(page + row * kKvLatent + ((lane & 31) ^ (row & 7)) * 16, slot + blk * 1024);
+        } else {
+          dma_lds16(page + kKvRopeAt + (blk - 32) * 1024 + (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16, slot + blk * 1024);
+        }
+      }
+      dma_lds4(page + kKvScaleAt + lane * 4, lds0 + C::SCALE_OFF + (k % kSlots) * kKvPageKeys * 4);
+    };
+    __syncthreads();  // the slots, P and the statistics are free again
+    if (tid < 4) flag[tid] = 0;
+    if (n > 0) fetch(0);
+    if (n > 1) fetch(1);
+
+    // ---- the rows' queries as hi + lo / 32, and what each row sees
+    v8i qhi[RT][4], qlo[RT][4];
+    v8bf qr[RT][2];
+    float f[RT], m[RT], l[RT], psum[RT];
+    int seen[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = (rh * RT + rt) * 16 + n16;
+      const bool live = r < rows;
+      const int64_t row = row0 + (live ? r : 0);
+      const u32x4p* qn = reinterpret_cast<const u32x4p*>(A.q_nope + row * kKvLatent);
+      const u32x4p* qp = reinterpret_cast<const u32x4p*>(A.q_pe + row * kKvRope);
+      u32x4p raw[4][4], rawr[2];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) raw[ks][c] = qn[ks * 16 + g * 4 + c];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) rawr[ks] = qp[ks * 4 + g];
+      uint32_t most = 0;  // the largest magnitude's bits (bf16, upper half)
+      auto look = [&](uint32_t x) { most = max(most, max(x & 0x7fff0000u, (x << 16) & 0x7fff0000u)); };
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) look(raw[ks][c][i]);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) look(rawr[ks][i]);
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+      const bool bad = most >= 0x7f800000u;  // a NaN or an infinity: every output of the row is NaN
+      int e = static_cast<int>(most >> 23) - 127 - 7;  // sigma = 2^e
+      e = bad || !live ? 0 : max(e, -120);
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      f[rt] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale;
+      const bool zero = bad || !live;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t x0 = zero ? 0u : raw[ks][c >> 1][(c & 1) * 2], x1 = zero ? 0u : raw[ks][c >> 1][(c & 1) * 2 + 1];
+          const float v[4] = {__uint_as_float(x0 << 16) * inv, __uint_as_float(x0 & 0xffff0000u) * inv,
+                              __uint_as_float(x1 << 16) * inv, __uint_as_float(x1 & 0xffff0000u) * inv};
+          int hi, lo;
+          split4(v, hi, lo);
+          qhi[rt][ks][c] = hi;
+          qlo[rt][ks][c] = lo;
+        }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4p x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t y = zero ? 0u : rawr[ks][i];
+          x[i] = bf16x2_bits(v2f{__uint_as_float(y << 16) * inv, __uint_as_float(y & 0xffff0000u) * inv});
+        }
+        qr[rt][ks] = __builtin_bit_cast(v8bf, x);
+      }
+      seen[rt] = live ? s.seen(p, in_seq + r, A.heads) : 0;
+      m[rt] = -INFINITY;
+      l[rt] = bad && live && seen[rt] > 0 ? __builtin_nanf("") : 0.f;
+      psum[rt] = 0.f;
+      __builtin_amdgcn_sched_barrier(0);  // one tile's loads at a time: the codes are what has to stay in registers
+    }
+    v16f o[RT2][DT];
+#pragma unroll
+    for (int a = 0; a < RT2; ++a)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[a][d][i] = 0.f;
+    float s_ref = 0.f, kf = 0.f;
+    v4f U[RT];
+
+    // U of page k (in its slot); MASK: some row does not see all of it
+    auto scores = [&](int k, auto mask) {
+      constexpr bool MASK = decltype(mask)::value;
+      const int slot = k % kSlots;
+      const uint8_t* codes = smem + slot * kSlotBytes;
+      const int key = kq * 16 + n16;
+      v4f R[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) { U[rt] = v4f{0.f, 0.f, 0.f, 0.f}; R[rt] = v4f{0.f, 0.f, 0.f, 0.f}; }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const v8bf a = *reinterpret_cast<const v8bf*>(codes + kKvPageKeys * kKvLatent + key * 128 + ((ks * 4 + g) ^ (key & 7)) * 16);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) R[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qr[rt][ks], R[rt], 0, 0, 0);
+      }
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const int c = ks * 8 + g * 2;
+        const v4i a0 = *reinterpret_cast<const v4i*>(codes + key * kKvLatent + (c ^ (key & 7)) * 16);
+        const v4i a1 = *reinterpret_cast<const v4i*>(codes + key * kKvLatent + ((c + 1) ^ (key & 7)) * 16);
+        const v8i a = two_v4i(a0, a1);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) U[rt] = mfma16_fp8(a, qhi[rt][ks], U[rt], kScaleOne);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) U[rt] = mfma16_fp8(a, qlo[rt][ks], U[rt], kScaleLo);
+      }
+      v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + kq * 16 + 4 * g) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sk[i] = __builtin_fabsf(sk[i]) < INFINITY ? sk[i] : __builtin_nanf("");  // not -inf, a masked score
+      const int at = (pg0 + k) * kKvPageKeys + kq * 16 + 4 * g;
+      const bool there = !MASK || static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = __builtin_fmaf(U[rt][i], sk[i], R[rt][i]);
+          U[rt][i] = !MASK || (there && at + i < seen[rt]) ? x : -INFINITY;
+        }
+    };
+
+    // P of page k from U, m and s_ref: codes to buffer k % 2, psum; whether all were <= kPMost
+    auto weights = [&](int k) {
+      const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + ((k % kSlots) * kKvPageKeys + kq * 16 + 4 * g) * 4) * kf;
+      uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES;
+      float pmax = 0.f;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float mu = m[rt] == -INFINITY ? 0.f : m[rt];
+        float x[4], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool none = U[rt][i] == -INFINITY;  // a masked key's scale may be anything
+          const float e = none ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(U[rt][i], f[rt], -mu));
+          sum += e;
+          x[i] = none ? 0.f : e * sk[i];
+          pmax = fmaxf(pmax, __builtin_fabsf(x[i]));
+        }
+        psum[rt] = sum;
+        int hi, lo;
+        split4(x, hi, lo);
+        const int at = ((rh * RT + rt) * 16 + n16) * kPStride + kq * 16 + 4 * g;
+        *reinterpret_cast<int*>(P + at) = hi;
+        *reinterpret_cast<int*>(P + C::P_BYTES + at) = lo;
+      }
+      return !__any(pmax > kPMost);
+    };
+
+    // New m and s_ref from page k's scores, O and l brought to them, P again.  Every wave comes here, or none.
+    auto settle = [&](int k) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float x = fmaxf(fmaxf(U[rt][0], U[rt][1]), fmaxf(U[rt][2], U[rt][3]));
+        x = fmaxf(x, __shfl_xor(x, 16));
+        x = fmaxf(x, __shfl_xor(x, 32));
+        if (g == 0) stat[kq * BM + (rh * RT + rt) * 16 + n16] = x;
+      }
+      // the largest finite scale of the page's keys that some row sees
+      const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + (k % kSlots) * kKvPageKeys * 4)[lane]);
+      const bool use = (pg0 + k) * kKvPageKeys + lane < s.seen(p, in_seq + rows - 1, A.heads) && sk < INFINITY &&
+                       static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
+      const float most = fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f);
+      const float ratio = s_ref > 0.f ? s_ref / fmaxf(s_ref, most) : 0.f;
+      s_ref = fmaxf(s_ref, most);
+      kf = kP / s_ref;
+      __syncthreads();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = (rh * RT + rt) * 16 + n16;
+        const float x = fmaxf(fmaxf(stat[r], stat[BM + r]), fmaxf(stat[2 * BM + r], stat[3 * BM + r]));
+        const float mn = fmaxf(m[rt], x == -INFINITY ? -INFINITY : x * f[rt]);
+        const float a = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+        l[rt] *= m[rt] == -INFINITY ? 1.0f : a;  // (0, or a bad row's NaN, before the first key)
+        m[rt] = mn;
+        if (kq == 0 && g == 0) alpha_l[r] = a * ratio;
+      }
+      weights(k);
+      __syncthreads();
+#pragma unroll
+      for (int a = 0; a < RT2; ++a) {
+        const float x = alpha_l[min(a * 32 + n32, BM - 1)];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[a][d][i] *= x;
+      }
+    };
+
+    // a page's codes before a masked step: a NaN code would reach rows that do not see its key through 0 * NaN, so it
+    // becomes 0 and the key's scale NaN
+    auto clean = [&](int k) {
+      uint8_t* codes = smem + (k % kSlots) * kSlotBytes;
+      for (int i = tid; i < kKvPageKeys * kKvLatent / 16; i += C::kThreads) {
+        v4i x = reinterpret_cast<v4i*>(codes)[i];
+        bool found = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t y = static_cast<uint32_t>(x[c]) & 0x7f7f7f7fu;
+          // bytes equal to 0x7f: adding 1 to a 7-bit value carries into bit 7 only from 0x7f
+          const uint32_t nan = ((y + 0x01010101u) & 0x80808080u) >> 7;
+          found = found || nan;
+          x[c] &= ~static_cast<int>(nan * 0xffu);
+        }
+        if (found) {
+          reinterpret_cast<v4i*>(codes)[i] = x;
+          reinterpret_cast<float*>(smem + C::SCALE_OFF)[(k % kSlots) * kKvPageKeys + i / (kKvLatent / 16)] = __builtin_nanf("");
+        }
+      }
+      __syncthreads();
+    };
+
+    // O^T += latent^T P^T of page k: rows of A are dims, of B the tile's rows, 64 keys in one MFMA.  The operand lane
+    // (dim n32, half) needs 32 keys of its dim, a column of the key-major codes: ds_read_b64_tr_b8 gives lane i of a
+    // 16-lane group byte i % 8 of the 8 bytes at lane 2 j + i / 8's address as its byte j, so lane i addresses key
+    // 32 half + 8 r + i / 2, half i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
+    auto product = [&](int k) {
+      const uint8_t* codes = smem + (k % kSlots) * kSlotBytes + (32 * half + (n16 >> 1)) * kKvLatent + (lane & 1) * 8;
+      const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + n32 * kPStride + half * 32;
+      v8i ph[RT2], pl[RT2];
+#pragma unroll
+      for (int a = 0; a < RT2; ++a) {
+        const v4i* hi = reinterpret_cast<const v4i*>(P + a * 32 * kPStride);
+        const v4i* lo = reinterpret_cast<const v4i*>(P + a * 32 * kPStride + C::P_BYTES);
+        ph[a] = two_v4i(hi[0], hi[1]);
+        pl[a] = two_v4i(lo[0], lo[1]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int chunk = (wave * DT + d) * 2 + (g & 1);
+        const uint8_t* src = codes + (chunk ^ (n16 >> 1)) * 16;
+        v8i v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + r * 8 * kKvLatent));
+          v[2 * r] = x[0];
+          v[2 * r + 1] = x[1];
+        }
+#pragma unroll
+        for (int a = 0; a < RT2; ++a) {
+          o[a][d] = mfma32_fp8(v, ph[a], o[a][d], kScaleOne);
+          o[a][d] = mfma32_fp8(v, pl[a], o[a][d], kScaleLo);
+        }
+      }
+    };
+
+    // O stays in accumulation registers from step to step: left to itself the compiler holds it in
+    // vector registers between the products and moves all of it to and fro
+    auto pin_o = [&] {
+#pragma unroll
+      for (int a = 0; a < RT2; ++a)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) asm volatile("" : "+a"(o[a][d]));
+    };
+
+    // ---- the pages.  Step k: the scores of page k + 1, the product of page k, the weights of page k + 1; one
+    // barrier a step, before which the fetch of page k + 2 has arrived
+    auto begin = [&](int k) {  // page k's scores
+      if ((pg0 + k + 1) * kKvPageKeys > seen_all || static_cast<uint32_t>(table[k]) >= static_cast<uint32_t>(p.n_pages)) {
+        clean(k);
+        scores(k, std::true_type{});
+      } else {
+        scores(k, std::false_type{});
+      }
+    };
+    auto arrive = [&] {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+    };
+    if (n > 0) {
+      arrive();
+      begin(0);
+      settle(0);
+      for (int k = 0; k < n; ++k) {
+        // here: P of page k is whole, page k + 1 is in its slot
+        pin_o();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) l[rt] += psum[rt];
+        if (k + 2 < n) fetch(k + 2);
+        if (tid == 0) flag[(k + 2) & 3] = 0;
+        if (k + 1 < n) begin(k + 1);
+        product(k);
+        pin_o();
+        if (k + 1 < n) {
+          if (!weights(k + 1) && lane == 0) flag[(k + 1) & 3] = 1;
+          arrive();
+          if (flag[(k + 1) & 3]) settle(k + 1);
+        }
+      }
+    }
+
+    // ---- the tile's sums: l over the lanes and waves of a row, then the rows' results or partial sums
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float x = l[rt] + __shfl_xor(l[rt], 16);
+      x += __shfl_xor(x, 32);
+      const int r = (rh * RT + rt) * 16 + n16;
+      if (g == 0) {
+        stat[kq * BM + r] = x;
+        if (kq == 0) alpha_l[r] = m[rt];
+      }
+    }
+    __syncthreads();
+    if (tid < BM) rowl[tid] = (stat[tid] + stat[BM + tid]) + (stat[2 * BM + tid] + stat[3 * BM + tid]);
+    __syncthreads();
+    const bool whole = !A.split || (u == tile_u0 && u_end >= tile_u1);
+    if (whole) {
+      if (A.lse && tid < rows) A.lse[row0 + tid] = rowl[tid] == 0.f ? -INFINITY : (alpha_l[tid] + log2f(rowl[tid])) * 0.6931471805599453f;
+#pragma unroll
+      for (int a = 0; a < RT2; ++a) {
+        const int r = a * 32 + n32;
+        if (r < rows) {
+          const float L = rowl[r], x = L == 0.f ? 0.f : s_ref / (kP * L);
+          uint16_t* dst = A.out + (row0 + r) * kKvLatent + wave * DT * 32 + 4 * half;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<u32x2p*>(dst + d * 32 + 8 * i) = u32x2p{bf16x2_bits(v2f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x}),
+                                                                       bf16x2_bits(v2f{o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x})};
+        }
+      }
+    } else {
+      const int slot = 2 * w + (u == tile_u0 ? 1 : 0);
+      if (tid < rows) A.part_ml[static_cast<int64_t>(slot) * C::PR + tid] = float2{alpha_l[tid], rowl[tid]};
+      const float x = s_ref / kP;
+      v4f* dst = reinterpret_cast<v4f*>(A.part_o + static_cast<int64_t>(slot) * C::kPartFloats);
+#pragma unroll
+      for (int a = 0; a < RT2; ++a)
+        if (a * 32 + n32 < rows) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              dst[((a * 16 + wave * DT + d) * 4 + i) * 64 + lane] =
+                  v4f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x, o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x};
+        }
+    }
+    if (!A.split) return;
+    u = min(tile_u1, u_end);
+    ++tile;
+  }
+}
+
+// The split tiles' partial sums joined.  An item is 32 rows x 4 dims of a tile: lane n32 a row, the eight half-waves the
+// parts in turn, joined in LDS in a fixed order.
+template <int PR>
+__global__ __launch_bounds__(256) void paged_mla_combine_kernel(const SplitTile* __restrict__ split, const float2* __restrict__ part_ml,
+                                                                const float* __restrict__ part_o, uint16_t* __restrict__ out,
+                                                                float* __restrict__ lse) {
+  __shared__ int list[kPagedWgs], count[4];
+  __shared__ float top[8][32], sums[8][32];
+  __shared__ v4f acc[8][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  static_assert(kPagedWgs == 256, "one thread a workgroup of the split launch");
+  const uint64_t mine = __ballot(split[tid].parts > 1);
+  if (lane == 0) count[wave] = __popcll(mine);
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { before += i < wave ? count[i] : 0; total += count[i]; }
+  if (mine >> lane & 1) list[before + __popcll(mine & ((1ull << lane) - 1))] = tid;
+  __syncthreads();
+  constexpr int kItems = PR / 32 * 128;  // of a tile
+  const int n32 = tid & 31, part0 = tid >> 5;
+  for (int item = blockIdx.x; item < total * kItems; item += gridDim.x) {
+    const int w = list[item / kItems], a = item % kItems / 128, d4 = item % 128;
+    const SplitTile t = split[w];
+    const int r = a * 32 + n32;
+    const bool live = r < t.rows;
+    // part i: workgroup w - 1's slot 1, then the slots 0 of w, w + 1, ...
+    float mx = -INFINITY;
+    if (live)
+      for (int i = part0; i < t.parts; i += 8)
+        mx = fmaxf(mx, part_ml[static_cast<int64_t>(i ? 2 * (w + i - 1) : 2 * w - 1) * PR + r].x);
+    top[part0][n32] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, top[i][n32]);
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    if (live)
+      for (int i = part0; i < t.parts; i += 8) {
+        const int64_t slot = i ? 2 * (w + i - 1) : 2 * w - 1;
+        const float2 ml = part_ml[slot * PR + r];
+        const float x = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+        l += ml.x == -INFINITY ? ml.y : ml.y * x;  // (0, or a bad row's NaN)
+        // dims 4 d4 .. +3: 32-dim tile d4 / 8, group (d4 % 8) / 2 of 8 dims, half d4 % 2
+        o += reinterpret_cast<const v4f*>(part_o + slot * (static_cast<int64_t>(PR) * kKvLatent))[((a * 16 + d4 / 8) * 4 + (d4 % 8) / 2) * 64 + (d4 & 1) * 32 + n32] * x;
+      }
+    sums[part0][n32] = l;
+    acc[part0][n32] = o;
+    __syncthreads();
+    if (part0 == 0 && live) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) { l += sums[i][n32]; o += acc[i][n32]; }
+      const float x = l == 0.f ? 0.f : 1.0f / l;
+      const int64_t row = t.row0 + r;
+      *reinterpret_cast<u32x2p*>(out + row * kKvLatent + 4 * d4) = u32x2p{bf16x2_bits(v2f{o[0] * x, o[1] * x}), bf16x2_bits(v2f{o[2] * x, o[3] * x})};
+      if (lse && d4 == 0) lse[row] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
+    }
+    __syncthreads();
+  }
+}
+
+// The launch: rows a tile, whether tiles are split, and the workspace.
+struct PagedPlan {
+  int bm, pr;
+  int64_t tiles;  // at most
+  bool split;
+  size_t ml_at, o_at, bytes;
+};
+inline PagedPlan paged_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
+  PagedPlan d{};
+  const int64_t rows = n_tokens * heads, each = cdiv(rows, n_seqs);
+  d.bm = each <= 16 ? 16 : 32;
+  d.pr = d.bm < 32 ? 32 : d.bm;
+  d.tiles = rows / d.bm + (n_seqs < n_tokens ? n_seqs : n_tokens);
+  d.split = d.tiles <= kPagedMaxTiles && n_seqs <= kPagedMaxTiles;
+  if (d.split) {
+    d.ml_at = kPagedWgs * sizeof(SplitTile);
+    d.o_at = d.ml_at + static_cast<size_t>(2 * kPagedWgs) * d.pr * sizeof(float2);
+    d.bytes = d.o_at + static_cast<size_t>(2 * kPagedWgs) * d.pr * kKvLatent * sizeof(float);
+  }
+  return d;
 }
 
 }  // namespace tl
 
 using namespace tl;
+
+extern "C" size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
+  if (n_seqs < 1 || n_tokens < 1 || heads < 1 || heads > 128 || n_seqs > (1ll << 20) || n_tokens * heads >= (1ll << 27)) return 0;
+  return paged_plan(n_seqs, n_tokens, heads).bytes;
+}
 
 extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const void* kv_pages, int64_t n_pages,
                                   const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
@@ -78,19 +729,42 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
   if (int rc = check_batch("flash_paged_mla", kv_pages, n_pages, block_table, max_pages, cu_seqlens, seq_lens, n_seqs, n_tokens)) return rc;
   if (heads < 1 || heads > 128) { set_error("flash_paged_mla: heads=%lld must be in [1, 128]", (long long)heads); return kErrUnsupported; }
   if (n_seqs == 0 || n_tokens == 0) return kOk;
-  if (n_tokens * heads >= (1ll << 31)) { set_error("flash_paged_mla: %lld tokens x %lld heads: too many rows", (long long)n_tokens, (long long)heads); return kErrUnsupported; }
+  if (n_tokens * heads >= (1ll << 27) || n_seqs > (1ll << 20) || max_pages > (1ll << 20)) {
+    set_error("flash_paged_mla: %lld tokens x %lld heads, %lld sequences, %lld pages a sequence: at most 2^27 rows, 2^20 "
+              "sequences and 2^20 pages", (long long)n_tokens, (long long)heads, (long long)n_seqs, (long long)max_pages);
+    return kErrUnsupported;
+  }
+  if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) { set_error("flash_paged_mla: softmax_scale must be positive and finite"); return kErrArg; }
   if (!q_nope_bf16 || !q_pe_bf16 || !out_bf16) { set_error("flash_paged_mla: null pointer"); return kErrArg; }
-  if ((reinterpret_cast<uintptr_t>(q_nope_bf16) | reinterpret_cast<uintptr_t>(q_pe_bf16) | reinterpret_cast<uintptr_t>(out_bf16)) & 15) {
-    set_error("flash_paged_mla: q and out must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(q_nope_bf16) | reinterpret_cast<uintptr_t>(q_pe_bf16) | reinterpret_cast<uintptr_t>(out_bf16) |
+       reinterpret_cast<uintptr_t>(workspace)) & 15) {
+    set_error("flash_paged_mla: q, out and workspace must be 16-byte aligned");
     return kErrArg;
   }
-  const PagedBatch p{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens};
-  hipLaunchKernelGGL(paged_mla_rows_kernel, dim3(cdiv(n_tokens * heads, 4)), dim3(256), 0, (hipStream_t)stream,
-                     (const uint16_t*)q_nope_bf16, (const uint16_t*)q_pe_bf16, (const uint8_t*)kv_pages, p, (int)heads,
-                     softmax_scale, (uint16_t*)out_bf16, lse);
-  return check_launch("flash_paged_mla");
-}
+  const PagedPlan d = paged_plan(n_seqs, n_tokens, heads);
+  if (d.bytes && (!workspace || workspace_bytes < d.bytes)) {
+    set_error("flash_paged_mla: needs a workspace of %zu bytes (got %zu)", d.bytes, workspace_bytes);
+    return kErrArg;
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const PagedArgs args{(const uint16_t*)q_nope_bf16, (const uint16_t*)q_pe_bf16, (const uint8_t*)kv_pages,
+                       PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
+                       (int)heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
+                       d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
+                       reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0)};
+  const hipStream_t st = (hipStream_t)stream;
+  auto launch = [&](auto nw, auto rt) -> int {
+    using C = PagedCfg<decltype(nw)::value, decltype(rt)::value>;
+    const auto kern = paged_mla_kernel<decltype(nw)::value, decltype(rt)::value>;
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), C::BYTES, "flash_paged_mla")) return rc;
+    hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(d.tiles)), dim3(C::kThreads), C::BYTES, st, args);
+    if (int rc = check_launch("flash_paged_mla")) return rc;
+    if (!d.split) return kOk;
+    hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(512), dim3(256), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
+    return check_launch("flash_paged_mla");
+  };
+  using std::integral_constant;
+  if (d.bm == 16) return launch(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  return launch(integral_constant<int, 4>{}, integral_constant<int, 2>{});
 
-extern "C" size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
-  return 0;
 }
