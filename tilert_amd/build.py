@@ -34,9 +34,11 @@ FLAGS = [
 
 
 # Per-source extra flags.  indexer: MFMA results in VGPRs (its epilogue reads every result
-# with VALU ops; in AGPRs each element would first need a v_accvgpr_read).
+# with VALU ops; in AGPRs each element would first need a v_accvgpr_read).  paged_mla: the same;
+# and with two waves a SIMD the registers are not halved into VGPRs and AGPRs.
 EXTRA = {
     "indexer": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_mla": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -39,27 +39,29 @@ constexpr float kP = 32.0f;          // p * scale / s_ref is held at kP at most 
 constexpr float kPMost = 256.0f;     // and at kPMost until they are set again
 constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
 
-// NW waves: wave w scores the keys 16 (w % 4) .. +15 of a page for the row group w / 4 (RT tiles of 16 rows) and
+// NW waves in RG groups of 16 rows: wave w scores the rows of group w / KG against the 16 KT keys w % KG of a page, and
 // multiplies P with the latent dims 512 / NW * w .. for all rows.
-template <int NW, int RT>
+template <int NW, int RG>
 struct PagedCfg {
   static constexpr int kThreads = NW * 64;
-  static constexpr int BM = 16 * RT * (NW / 4);
+  static constexpr int BM = 16 * RG;
+  static constexpr int KG = NW / RG, KT = 4 / KG;
   static constexpr int RT2 = (BM + 31) / 32;     // 32-row tiles of the second product
   static constexpr int PR = RT2 * 32;            // rows of P in LDS
   static constexpr int DT = 16 / NW;             // 32-dim tiles a wave
-  static constexpr int kDma = 40 / NW;           // 1 KB pieces of a page a wave
   static constexpr int SCALE_OFF = kSlots * kSlotBytes;
   static constexpr int P_OFF = SCALE_OFF + kSlots * kKvPageKeys * 4;
   static constexpr int P_BYTES = PR * kPStride;  // one of hi, lo of one buffer
-  static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;   // [4][BM] f32
-  static constexpr int ALPHA_OFF = STAT_OFF + 4 * BM * 4;  // [PR] f32
+  static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;   // [KG][BM] f32
+  static constexpr int ALPHA_OFF = STAT_OFF + KG * BM * 4;  // [PR] f32
   static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;      // [PR] f32
   static constexpr int FLAG_OFF = ROWL_OFF + PR * 4;       // [4] i32
   static constexpr int SCAN_OFF = FLAG_OFF + 16;           // [NW] i32
   static constexpr int SEQ_OFF = SCAN_OFF + NW * 4;        // [kPagedMaxTiles] i32: tiles up to sequence b and with it
   static constexpr int TILE_OFF = SEQ_OFF + kPagedMaxTiles * 4;  // [kPagedMaxTiles] i32: pages up to tile t and with it
-  static constexpr int BYTES = TILE_OFF + kPagedMaxTiles * 4;
+  static constexpr bool kRopeLds = BM >= 64;      // the queries' rope parts in LDS, where registers are short
+  static constexpr int ROPE_OFF = TILE_OFF + kPagedMaxTiles * 4;  // [BM][64] bf16, chunks placed as a page's
+  static constexpr int BYTES = ROPE_OFF + (kRopeLds ? BM * kKvRope * 2 : 0);
   static constexpr size_t kPartFloats = static_cast<size_t>(PR) * kKvLatent;
 };
 
@@ -150,6 +152,36 @@ __device__ inline v16f mfma32_fp8(const v8i& a, const v8i& b, v16f c, int scale_
 }
 __device__ inline v8i two_v4i(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+// N copies of 1 KB to LDS at `lds` and behind, from base + off[i] + 1024 i: lane l's 16 bytes go to its place in
+// piece i.  The offset field moves both addresses, so m0 is written once; the copy of the base gives m0 its wait
+// state, and the copies a base that no vector instruction has just written.
+template <int N>
+__device__ inline void dma_pieces(const uint8_t* base, const uint32_t (&off)[N], uint32_t lds) {
+  static_assert(N == 1 || N == 2 || N == 4, "");
+  uint32_t saved;
+  uint64_t from;
+  if constexpr (N == 4)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
+        "global_load_lds_dwordx4 %5, %1 offset:1024\n\tglobal_load_lds_dwordx4 %6, %1 offset:2048\n\t"
+        "global_load_lds_dwordx4 %7, %1 offset:3072\n\ts_mov_b32 m0, %0"
+        : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
+        "global_load_lds_dwordx4 %5, %1 offset:1024\n\ts_mov_b32 m0, %0"
+        : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]) : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]) : "memory");
+}
+__device__ inline void dma_words(const uint8_t* base, uint32_t off, uint32_t lds) {  // 4 bytes a lane
+  uint32_t saved;
+  uint64_t from;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dword %4, %1\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off) : "memory");
+}
+
 // Four values (finite, <= 256 in magnitude, or NaN) as hi + lo / 32, four codes each.
 __device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
@@ -159,16 +191,30 @@ __device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
   lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 32.0f, (x[3] - b[1]) * 32.0f, lo, true);
 }
 
-template <int NW, int RT>
+template <int NW, int RG>
 __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedArgs A) {
-  using C = PagedCfg<NW, RT>;
-  constexpr int BM = C::BM, RT2 = C::RT2, DT = C::DT;
+  using C = PagedCfg<NW, RG>;
+  constexpr int BM = C::BM, KG = C::KG, KT = C::KT, RT2 = C::RT2, DT = C::DT;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kq = wave & 3, rh = wave >> 2;  // key quarter, row group
+  const int kg = wave % KG, rg = wave / KG;  // key group, row group
   const int n16 = lane & 15, g = lane >> 4;
   const int n32 = lane & 31, half = lane >> 5;
+  // lane parts of the addresses: a 16-byte chunk c of a page's row is kept at c ^ (row & 7), so that the rows' chunks
+  // that a read takes together are in different banks; c's bits above the third are whole steps of 128 bytes
+  const uint32_t fetch_code = half * 512 + (n32 ^ half) * 16;  // rows 2 i, 2 i + 1 (i % 4 = 0; ^ 32 (i % 4) for others)
+  const uint32_t fetch_rope = (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
+  const int my_key = kg * KT * 16 + n16;  // and 16, 32, .. behind it
+  const int at_code = my_key * kKvLatent + ((2 * g) ^ (my_key & 7)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31)
+  const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (my_key & 7)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
+  const int at_value = (32 * half + (n16 >> 1)) * kKvLatent + (wave * DT >> 2) * 128 + (lane & 1) * 8 +
+                       (((wave * DT * 2 & 7) + (g & 1)) ^ (n16 >> 1)) * 16;  // 32-dim tile d: ^ 32 d
+  const int at_p = n32 * kPStride + half * 32;
+  const int my_row = rg * 16 + n16;
+  const int my_quad = kg * KT * 16 + 4 * g;  // the keys of this lane's scores: my_quad .. +3, and 16, 32, .. behind them
+  const int put_rope = my_row * 128 + (g ^ (my_row & 7)) * 16;
+  const int put_p = my_row * kPStride + my_quad;
   const PagedBatch& p = A.p;
   int* seq_end = reinterpret_cast<int*>(smem + C::SEQ_OFF);
   int* unit_end = reinterpret_cast<int*>(smem + C::TILE_OFF);
@@ -207,10 +253,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
     const int before = block_scan<NW>(sum, scan, units) - sum;
     for (int t = t0; t < t1; ++t) unit_end[t] += before;
     __syncthreads();
+    units = __builtin_amdgcn_readfirstlane(units);
     quota = max(kPagedMinPages, (units + kPagedWgs - 1) / kPagedWgs);
     u = min(w * quota, units);
     u_end = min(u + quota, units);
-    tile = upper(unit_end, n_tiles, u);
+    tile = __builtin_amdgcn_readfirstlane(upper(unit_end, n_tiles, u));
     if (tid == 0) {
       SplitTile info{0, 0, 0};
       if (u < u_end) {
@@ -250,10 +297,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
     if (A.split) {
       seq = upper(seq_end, p.n_seqs, tile);
       seq_tile0 = seq ? seq_end[seq - 1] : 0;
-      tile_u0 = tile ? unit_end[tile - 1] : 0;
-      tile_u1 = unit_end[tile];
+      tile_u0 = __builtin_amdgcn_readfirstlane(tile ? unit_end[tile - 1] : 0);
+      tile_u1 = __builtin_amdgcn_readfirstlane(unit_end[tile]);
     }
     seq = __builtin_amdgcn_readfirstlane(seq);
+    seq_tile0 = __builtin_amdgcn_readfirstlane(seq_tile0);
     const SeqRows s(p, seq);
     const int j = tile - seq_tile0;
     const int in_seq = j * BM;
@@ -261,44 +309,44 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
     const int rows = min(BM, s.n_tok * A.heads - in_seq);
     const int n_pages = s.pages(p, j, A.heads, BM);
     const int seen_all = s.seen(p, in_seq, A.heads);  // every row sees these
-    const int pg0 = __builtin_amdgcn_readfirstlane(u - tile_u0);
-    const int n = __builtin_amdgcn_readfirstlane(min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0));
+    const int pg0 = u - tile_u0;
+    const int n = min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0);
     const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
 
-    // page k of the tile into its slot: 1 KB pieces, 32 of codes and 8 of rope parts; the 16-byte chunk c of a row
-    // goes to c ^ (row & 7), so that the rows' chunks that a read takes together are in different banks
-    auto fetch = [&](int k) {
+    // page k of the tile into its slot, in 1 KB pieces: 32 of codes, four at a time, and 8 of rope parts; every wave
+    // also fetches the scales, all of them the same
+    auto fetch = [&](int k, int slot) {
       int id = table[k];
       if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.n_pages)) id = 0;  // its keys are masked
       const uint8_t* page = A.pages + static_cast<int64_t>(id) * kKvPageBytes;
-      const uint32_t slot = lds0 + (k % kSlots) * kSlotBytes;
+      const uint32_t to = lds0 + slot * kSlotBytes;
+      const uint32_t off[4] = {fetch_code, fetch_code ^ 32, fetch_code ^ 64, fetch_code ^ 96};
 #pragma unroll
-      for (int i = 0; i < C::kDma; ++i) {
-        const int blk = wave * C::kDma + i;
-        if (blk < 32) {
-          const int row = 2 * blk + (lane >> 5);
-          dma_lds16(page + row * kKvLatent + ((lane & 31) ^ (row & 7)) * 16, slot + blk * 1024);
-        } else {
-          dma_lds16(page + kKvRopeAt + (blk - 32) * 1024 + (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16, slot + blk * 1024);
-        }
+      for (int i = 0; i < 8 / NW; ++i) {
+        const int at = (wave * (8 / NW) + i) * 4096;
+        dma_pieces<4>(page + at, off, to + at);
       }
-      dma_lds4(page + kKvScaleAt + lane * 4, lds0 + C::SCALE_OFF + (k % kSlots) * kKvPageKeys * 4);
+      constexpr int kRope = 8 / NW;
+      uint32_t rope[kRope];
+#pragma unroll
+      for (int i = 0; i < kRope; ++i) rope[i] = fetch_rope;
+      const int at = wave * kRope * 1024;
+      dma_pieces<kRope>(page + kKvRopeAt + at, rope, to + kKvPageKeys * kKvLatent + at);
+      dma_words(page + kKvScaleAt, lane * 4, lds0 + C::SCALE_OFF + slot * kKvPageKeys * 4);
     };
     __syncthreads();  // the slots, P and the statistics are free again
     if (tid < 4) flag[tid] = 0;
-    if (n > 0) fetch(0);
-    if (n > 1) fetch(1);
+    if (n > 0) fetch(0, 0);
+    if (n > 1) fetch(1, 1);
 
     // ---- the rows' queries as hi + lo / 32, and what each row sees
-    v8i qhi[RT][4], qlo[RT][4];
-    v8bf qr[RT][2];
-    float f[RT], m[RT], l[RT], psum[RT];
-    int seen[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = (rh * RT + rt) * 16 + n16;
-      const bool live = r < rows;
-      const int64_t row = row0 + (live ? r : 0);
+    v8i qhi[4], qlo[4];
+    v8bf qr[2];
+    float f, m = -INFINITY, l, psum = 0.f;
+    int seen;
+    {
+      const bool live = my_row < rows;
+      const int64_t row = row0 + (live ? my_row : 0);
       const u32x4p* qn = reinterpret_cast<const u32x4p*>(A.q_nope + row * kKvLatent);
       const u32x4p* qp = reinterpret_cast<const u32x4p*>(A.q_pe + row * kKvRope);
       u32x4p raw[4][4], rawr[2];
@@ -322,12 +370,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
         for (int i = 0; i < 4; ++i) look(rawr[ks][i]);
       most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
       most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
-      const bool bad = most >= 0x7f800000u;  // a NaN or an infinity: every output of the row is NaN
-      int e = static_cast<int>(most >> 23) - 127 - 7;  // sigma = 2^e
-      e = bad || !live ? 0 : max(e, -120);
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      f[rt] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale;
+      const bool bad = live && most >= 0x7f800000u;  // a NaN or an infinity: every output of the row is NaN
       const bool zero = bad || !live;
+      const int e = zero ? 0 : max(static_cast<int>(most >> 23) - 127 - 7, -120);  // sigma = 2^e
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -337,8 +384,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
                               __uint_as_float(x1 << 16) * inv, __uint_as_float(x1 & 0xffff0000u) * inv};
           int hi, lo;
           split4(v, hi, lo);
-          qhi[rt][ks][c] = hi;
-          qlo[rt][ks][c] = lo;
+          qhi[ks][c] = hi;
+          qlo[ks][c] = lo;
         }
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -348,13 +395,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
           const uint32_t y = zero ? 0u : rawr[ks][i];
           x[i] = bf16x2_bits(v2f{__uint_as_float(y << 16) * inv, __uint_as_float(y & 0xffff0000u) * inv});
         }
-        qr[rt][ks] = __builtin_bit_cast(v8bf, x);
+        if constexpr (!C::kRopeLds) qr[ks] = __builtin_bit_cast(v8bf, x);
+        else if (kg == 0) *reinterpret_cast<u32x4p*>(smem + C::ROPE_OFF + (put_rope ^ (ks * 64))) = x;
       }
-      seen[rt] = live ? s.seen(p, in_seq + r, A.heads) : 0;
-      m[rt] = -INFINITY;
-      l[rt] = bad && live && seen[rt] > 0 ? __builtin_nanf("") : 0.f;
-      psum[rt] = 0.f;
-      __builtin_amdgcn_sched_barrier(0);  // one tile's loads at a time: the codes are what has to stay in registers
+      seen = live ? s.seen(p, in_seq + my_row, A.heads) : 0;
+      l = bad && seen > 0 ? __builtin_nanf("") : 0.f;
     }
     v16f o[RT2][DT];
 #pragma unroll
@@ -364,86 +409,97 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[a][d][i] = 0.f;
     float s_ref = 0.f, kf = 0.f;
-    v4f U[RT];
+    v4f U[KT];
 
-    // U of page k (in its slot); MASK: some row does not see all of it
-    auto scores = [&](int k, auto mask) {
-      constexpr bool MASK = decltype(mask)::value;
-      const int slot = k % kSlots;
-      const uint8_t* codes = smem + slot * kSlotBytes;
-      const int key = kq * 16 + n16;
-      v4f R[RT];
+    // the keys' operands of page k, and the products with the queries: U (codes) and R (rope parts)
+    // U of a page: 4 KT items of 128 dims, each item's operand read kAhead items before its
+    // two products.  The order is held by barriers: with all reads first the registers do not suffice, and a spilled
+    // register's reload waits for the page that is being fetched.
+    auto load_key = [&](int slot, int i) {
+      const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i % 4) * 128;
+      return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
+    };
+    auto score_products = [&](int slot) {
+      constexpr int kItems = 4 * KT, kAhead = KT > 1 ? 2 : 3;
+      v8i a[kItems];
+      v8bf r[KT][2];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) { U[rt] = v4f{0.f, 0.f, 0.f, 0.f}; R[rt] = v4f{0.f, 0.f, 0.f, 0.f}; }
+      for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const v8bf a = *reinterpret_cast<const v8bf*>(codes + kKvPageKeys * kKvLatent + key * 128 + ((ks * 4 + g) ^ (key & 7)) * 16);
+      for (int kt = 0; kt < KT; ++kt) U[kt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) R[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qr[rt][ks], R[rt], 0, 0, 0);
-      }
+      for (int i = 0; i < kItems; ++i) {
+        if (i + kAhead < kItems) a[i + kAhead] = load_key(slot, i + kAhead);
+        if (i + kAhead == kItems) {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const int c = ks * 8 + g * 2;
-        const v4i a0 = *reinterpret_cast<const v4i*>(codes + key * kKvLatent + (c ^ (key & 7)) * 16);
-        const v4i a1 = *reinterpret_cast<const v4i*>(codes + key * kKvLatent + ((c + 1) ^ (key & 7)) * 16);
-        const v8i a = two_v4i(a0, a1);
+          for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) U[rt] = mfma16_fp8(a, qhi[rt][ks], U[rt], kScaleOne);
+            for (int ks = 0; ks < 2; ++ks)
+              r[kt][ks] = *reinterpret_cast<const v8bf*>(smem + slot * kSlotBytes + (at_rope ^ (ks * 64)) + kt * 16 * 128);
+          if constexpr (C::kRopeLds)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) U[rt] = mfma16_fp8(a, qlo[rt][ks], U[rt], kScaleLo);
-      }
-      v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + kq * 16 + 4 * g) * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sk[i] = __builtin_fabsf(sk[i]) < INFINITY ? sk[i] : __builtin_nanf("");  // not -inf, a masked score
-      const int at = (pg0 + k) * kKvPageKeys + kq * 16 + 4 * g;
-      const bool there = !MASK || static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = __builtin_fmaf(U[rt][i], sk[i], R[rt][i]);
-          U[rt][i] = !MASK || (there && at + i < seen[rt]) ? x : -INFINITY;
+            for (int ks = 0; ks < 2; ++ks) qr[ks] = *reinterpret_cast<const v8bf*>(smem + C::ROPE_OFF + (put_rope ^ (ks * 64)));
         }
+        U[i / 4] = mfma16_fp8(a[i], qhi[i % 4], U[i / 4], kScaleOne);
+        U[i / 4] = mfma16_fp8(a[i], qlo[i % 4], U[i / 4], kScaleLo);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) U[kt][i] *= __builtin_fabsf(sk[i]) < INFINITY ? sk[i] : __builtin_nanf("");  // not -inf, a masked score
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) U[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(r[kt][ks], qr[ks], U[kt], 0, 0, 0);
+      }
+    };
+    // the scores of page k, in `slot`, that a row does not see
+    auto mask_scores = [&](int k) {
+      const bool there = static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
+      const int at = (pg0 + k) * kKvPageKeys + my_quad;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) U[kt][i] = there && at + kt * 16 + i < seen ? U[kt][i] : -INFINITY;
     };
 
     // P of page k from U, m and s_ref: codes to buffer k % 2, psum; whether all were <= kPMost
-    auto weights = [&](int k) {
-      const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + ((k % kSlots) * kKvPageKeys + kq * 16 + 4 * g) * 4) * kf;
-      uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES;
-      float pmax = 0.f;
+    auto weights = [&](int k, int slot) {
+      uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p;
+      const float mu = m == -INFINITY ? 0.f : m;
+      float pmax = 0.f, sum = 0.f;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float mu = m[rt] == -INFINITY ? 0.f : m[rt];
-        float x[4], sum = 0.f;
+      for (int kt = 0; kt < KT; ++kt) {
+        const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4) * kf;
+        float x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool none = U[rt][i] == -INFINITY;  // a masked key's scale may be anything
-          const float e = none ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(U[rt][i], f[rt], -mu));
+          const bool none = U[kt][i] == -INFINITY;  // a masked key's scale may be anything
+          const float e = none ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mu));
           sum += e;
           x[i] = none ? 0.f : e * sk[i];
           pmax = fmaxf(pmax, __builtin_fabsf(x[i]));
         }
-        psum[rt] = sum;
         int hi, lo;
         split4(x, hi, lo);
-        const int at = ((rh * RT + rt) * 16 + n16) * kPStride + kq * 16 + 4 * g;
-        *reinterpret_cast<int*>(P + at) = hi;
-        *reinterpret_cast<int*>(P + C::P_BYTES + at) = lo;
+        *reinterpret_cast<int*>(P + kt * 16) = hi;
+        *reinterpret_cast<int*>(P + kt * 16 + C::P_BYTES) = lo;
       }
+      psum = sum;
       return !__any(pmax > kPMost);
     };
 
     // New m and s_ref from page k's scores, O and l brought to them, P again.  Every wave comes here, or none.
-    auto settle = [&](int k) {
+    auto settle = [&](int k, int slot) {
+      float x = -INFINITY;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float x = fmaxf(fmaxf(U[rt][0], U[rt][1]), fmaxf(U[rt][2], U[rt][3]));
-        x = fmaxf(x, __shfl_xor(x, 16));
-        x = fmaxf(x, __shfl_xor(x, 32));
-        if (g == 0) stat[kq * BM + (rh * RT + rt) * 16 + n16] = x;
-      }
+      for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(fmaxf(U[kt][0], U[kt][1]), fmaxf(U[kt][2], U[kt][3])));
+      x = fmaxf(x, __shfl_xor(x, 16));
+      x = fmaxf(x, __shfl_xor(x, 32));
+      if (g == 0) stat[kg * BM + my_row] = x;
       // the largest finite scale of the page's keys that some row sees
-      const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + (k % kSlots) * kKvPageKeys * 4)[lane]);
+      const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + slot * kKvPageKeys * 4)[lane]);
       const bool use = (pg0 + k) * kKvPageKeys + lane < s.seen(p, in_seq + rows - 1, A.heads) && sk < INFINITY &&
                        static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
       const float most = fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f);
@@ -452,16 +508,13 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
       kf = kP / s_ref;
       __syncthreads();
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int r = (rh * RT + rt) * 16 + n16;
-        const float x = fmaxf(fmaxf(stat[r], stat[BM + r]), fmaxf(stat[2 * BM + r], stat[3 * BM + r]));
-        const float mn = fmaxf(m[rt], x == -INFINITY ? -INFINITY : x * f[rt]);
-        const float a = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
-        l[rt] *= m[rt] == -INFINITY ? 1.0f : a;  // (0, or a bad row's NaN, before the first key)
-        m[rt] = mn;
-        if (kq == 0 && g == 0) alpha_l[r] = a * ratio;
-      }
-      weights(k);
+      for (int i = 0; i < KG; ++i) x = fmaxf(x, stat[i * BM + my_row]);
+      const float mn = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
+      const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= m == -INFINITY ? 1.0f : a;  // (0, or a bad row's NaN, before the first key)
+      m = mn;
+      if (kg == 0 && g == 0) alpha_l[my_row] = a * ratio;
+      weights(k, slot);
       __syncthreads();
 #pragma unroll
       for (int a = 0; a < RT2; ++a) {
@@ -475,8 +528,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
 
     // a page's codes before a masked step: a NaN code would reach rows that do not see its key through 0 * NaN, so it
     // becomes 0 and the key's scale NaN
-    auto clean = [&](int k) {
-      uint8_t* codes = smem + (k % kSlots) * kSlotBytes;
+    auto clean = [&](int slot) {
+      uint8_t* codes = smem + slot * kSlotBytes;
       for (int i = tid; i < kKvPageKeys * kKvLatent / 16; i += C::kThreads) {
         v4i x = reinterpret_cast<v4i*>(codes)[i];
         bool found = false;
@@ -490,7 +543,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
         }
         if (found) {
           reinterpret_cast<v4i*>(codes)[i] = x;
-          reinterpret_cast<float*>(smem + C::SCALE_OFF)[(k % kSlots) * kKvPageKeys + i / (kKvLatent / 16)] = __builtin_nanf("");
+          reinterpret_cast<float*>(smem + C::SCALE_OFF)[slot * kKvPageKeys + i / (kKvLatent / 16)] = __builtin_nanf("");
         }
       }
       __syncthreads();
@@ -500,95 +553,105 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
     // (dim n32, half) needs 32 keys of its dim, a column of the key-major codes: ds_read_b64_tr_b8 gives lane i of a
     // 16-lane group byte i % 8 of the 8 bytes at lane 2 j + i / 8's address as its byte j, so lane i addresses key
     // 32 half + 8 r + i / 2, half i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
-    auto product = [&](int k) {
-      const uint8_t* codes = smem + (k % kSlots) * kSlotBytes + (32 * half + (n16 >> 1)) * kKvLatent + (lane & 1) * 8;
-      const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + n32 * kPStride + half * 32;
-      v8i ph[RT2], pl[RT2];
+    auto product = [&](int k, int slot) {
+      const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + at_p;
+      v8i v[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const uint8_t* src = smem + slot * kSlotBytes + (at_value ^ (32 * d));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + r * 8 * kKvLatent));
+          v[d][2 * r] = x[0];
+          v[d][2 * r + 1] = x[1];
+        }
+      }
 #pragma unroll
       for (int a = 0; a < RT2; ++a) {
         const v4i* hi = reinterpret_cast<const v4i*>(P + a * 32 * kPStride);
         const v4i* lo = reinterpret_cast<const v4i*>(P + a * 32 * kPStride + C::P_BYTES);
-        ph[a] = two_v4i(hi[0], hi[1]);
-        pl[a] = two_v4i(lo[0], lo[1]);
-      }
+        const v8i ph = two_v4i(hi[0], hi[1]), pl = two_v4i(lo[0], lo[1]);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int chunk = (wave * DT + d) * 2 + (g & 1);
-        const uint8_t* src = codes + (chunk ^ (n16 >> 1)) * 16;
-        v8i v;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + r * 8 * kKvLatent));
-          v[2 * r] = x[0];
-          v[2 * r + 1] = x[1];
+        for (int d = 0; d < DT; ++d) {
+          o[a][d] = mfma32_fp8(v[d], ph, o[a][d], kScaleOne);
+          o[a][d] = mfma32_fp8(v[d], pl, o[a][d], kScaleLo);
         }
-#pragma unroll
-        for (int a = 0; a < RT2; ++a) {
-          o[a][d] = mfma32_fp8(v, ph[a], o[a][d], kScaleOne);
-          o[a][d] = mfma32_fp8(v, pl[a], o[a][d], kScaleLo);
-        }
+        if (a + 1 < RT2) __builtin_amdgcn_sched_barrier(0);  // the next rows' P not before: registers
       }
-    };
-
-    // O stays in accumulation registers from step to step: left to itself the compiler holds it in
-    // vector registers between the products and moves all of it to and fro
-    auto pin_o = [&] {
-#pragma unroll
-      for (int a = 0; a < RT2; ++a)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) asm volatile("" : "+a"(o[a][d]));
     };
 
     // ---- the pages.  Step k: the scores of page k + 1, the product of page k, the weights of page k + 1; one
     // barrier a step, before which the fetch of page k + 2 has arrived
-    auto begin = [&](int k) {  // page k's scores
-      if ((pg0 + k + 1) * kKvPageKeys > seen_all || static_cast<uint32_t>(table[k]) >= static_cast<uint32_t>(p.n_pages)) {
-        clean(k);
-        scores(k, std::true_type{});
-      } else {
-        scores(k, std::false_type{});
-      }
+    auto masked = [&](int k) {
+      return (pg0 + k + 1) * kKvPageKeys > seen_all || static_cast<uint32_t>(table[k]) >= static_cast<uint32_t>(p.n_pages);
     };
     auto arrive = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
     };
+    // With KT > 1 a spilled operand is reloaded among the scores, and its wait would be for the fetch too: the fetch
+    // follows them (2048 tokens over 16384 keys 1458 us with it first, 1286 so; KT = 1 spills nothing, and
+    // 60 sequences take 128 us with it first, 139 so).
+    constexpr bool kLate = KT > 1;
+    // P of page k is whole, page k + 1 in its slot: the scores of k + 1, the product of k, and between the product's
+    // MFMAs the weights of k + 1
+    auto step = [&](int k, int slot, int next, int free, auto mask) {
+      score_products(next);
+      if (kLate && k + 2 < n) fetch(k + 2, free);
+      if constexpr (decltype(mask)::value) mask_scores(k + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      product(k, slot);
+      const bool fits = weights(k + 1, next);
+      if (!fits && lane == 0) flag[(k + 1) & 3] = 1;
+    };
     if (n > 0) {
       arrive();
-      begin(0);
-      settle(0);
+      {
+        const bool cut = masked(0);
+        if (cut) clean(0);
+        score_products(0);
+        if (cut) mask_scores(0);
+      }
+      settle(0, 0);
+      int slot = 0, next = 1, free = 2;  // of pages k, k + 1, k + 2
       for (int k = 0; k < n; ++k) {
-        // here: P of page k is whole, page k + 1 is in its slot
-        pin_o();
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) l[rt] += psum[rt];
-        if (k + 2 < n) fetch(k + 2);
-        if (tid == 0) flag[(k + 2) & 3] = 0;
-        if (k + 1 < n) begin(k + 1);
-        product(k);
-        pin_o();
+          l += psum;
+        if (!kLate && k + 2 < n) fetch(k + 2, free);
         if (k + 1 < n) {
-          if (!weights(k + 1) && lane == 0) flag[(k + 1) & 3] = 1;
+          if (tid == 0) flag[(k + 2) & 3] = tid;  // (0, without a register that holds it)
+          if (masked(k + 1)) {
+            clean(next);
+            step(k, slot, next, free, std::true_type{});
+          } else {
+            step(k, slot, next, free, std::false_type{});
+          }
           arrive();
-          if (flag[(k + 1) & 3]) settle(k + 1);
+          if (flag[(k + 1) & 3]) settle(k + 1, next);
+        } else {
+          product(k, slot);
         }
+        const int was = slot;
+        slot = next;
+        next = free;
+        free = was;
       }
     }
 
     // ---- the tile's sums: l over the lanes and waves of a row, then the rows' results or partial sums
     __syncthreads();
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float x = l[rt] + __shfl_xor(l[rt], 16);
-      x += __shfl_xor(x, 32);
-      const int r = (rh * RT + rt) * 16 + n16;
-      if (g == 0) {
-        stat[kq * BM + r] = x;
-        if (kq == 0) alpha_l[r] = m[rt];
-      }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+      stat[kg * BM + my_row] = l;
+      if (kg == 0) alpha_l[my_row] = m;
     }
     __syncthreads();
-    if (tid < BM) rowl[tid] = (stat[tid] + stat[BM + tid]) + (stat[2 * BM + tid] + stat[3 * BM + tid]);
+    if (tid < BM) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < KG; ++i) x += stat[i * BM + tid];
+      rowl[tid] = x;
+    }
     __syncthreads();
     const bool whole = !A.split || (u == tile_u0 && u_end >= tile_u1);
     if (whole) {
@@ -700,7 +763,7 @@ struct PagedPlan {
 inline PagedPlan paged_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
   PagedPlan d{};
   const int64_t rows = n_tokens * heads, each = cdiv(rows, n_seqs);
-  d.bm = each <= 16 ? 16 : 32;
+  d.bm = each <= 16 ? 16 : (each <= 32 ? 32 : 64);
   d.pr = d.bm < 32 ? 32 : d.bm;
   d.tiles = rows / d.bm + (n_seqs < n_tokens ? n_seqs : n_tokens);
   d.split = d.tiles <= kPagedMaxTiles && n_seqs <= kPagedMaxTiles;
@@ -753,9 +816,9 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
                        d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
                        reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0)};
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto nw, auto rt) -> int {
-    using C = PagedCfg<decltype(nw)::value, decltype(rt)::value>;
-    const auto kern = paged_mla_kernel<decltype(nw)::value, decltype(rt)::value>;
+  auto launch = [&](auto nw, auto rg) -> int {
+    using C = PagedCfg<decltype(nw)::value, decltype(rg)::value>;
+    const auto kern = paged_mla_kernel<decltype(nw)::value, decltype(rg)::value>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), C::BYTES, "flash_paged_mla")) return rc;
     hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(d.tiles)), dim3(C::kThreads), C::BYTES, st, args);
     if (int rc = check_launch("flash_paged_mla")) return rc;
@@ -765,6 +828,6 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
   };
   using std::integral_constant;
   if (d.bm == 16) return launch(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  return launch(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-
+  if (d.bm == 32) return launch(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  return launch(integral_constant<int, 8>{}, integral_constant<int, 4>{});
 }
