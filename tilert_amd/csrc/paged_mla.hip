@@ -39,31 +39,35 @@ constexpr float kP = 32.0f;          // p * scale / s_ref is held at kP at most 
 constexpr float kPMost = 256.0f;     // and at kPMost until they are set again
 constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
 
-// NW waves in RG groups of 16 rows: wave w scores the rows of group w / KG against the 16 KT keys w % KG of a page, and
-// multiplies P with the latent dims 512 / NW * w .. for all rows.
-template <int NW, int RG>
+// Eight waves, two on a SIMD: 0 .. 3 score, 4 .. 7 multiply.  Scoring wave w takes the 16 rows of group w / KG against the
+// 16 KT keys w % KG of a page and writes P; multiplying wave w takes P of all rows with 128 of the latent's dims.
+// A SIMD's MFMA pipe always has the other wave's products while one wave turns scores into weights or waits for LDS, and
+// either wave's registers (queries 72, or sums up to 128) fit without the other's.  With every wave doing both, the two
+// waves of a SIMD stood at the same place of the step most of the time.
+template <int BM_>
 struct PagedCfg {
-  static constexpr int kThreads = NW * 64;
-  static constexpr int BM = 16 * RG;
-  static constexpr int KG = NW / RG, KT = 4 / KG;
+  static constexpr int BM = BM_;
+  static constexpr int RG = BM / 16, KG = 4 / RG, KT = 4 / KG;
   static constexpr int RT2 = (BM + 31) / 32;     // 32-row tiles of the second product
   static constexpr int PR = RT2 * 32;            // rows of P in LDS
-  static constexpr int DT = 16 / NW;             // 32-dim tiles a wave
   static constexpr int SCALE_OFF = kSlots * kSlotBytes;
   static constexpr int P_OFF = SCALE_OFF + kSlots * kKvPageKeys * 4;
   static constexpr int P_BYTES = PR * kPStride;  // one of hi, lo of one buffer
-  static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;   // [KG][BM] f32
+  static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;      // [KG][BM] f32
   static constexpr int ALPHA_OFF = STAT_OFF + KG * BM * 4;  // [PR] f32
-  static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;      // [PR] f32
-  static constexpr int FLAG_OFF = ROWL_OFF + PR * 4;       // [4] i32
-  static constexpr int SCAN_OFF = FLAG_OFF + 16;           // [NW] i32
-  static constexpr int SEQ_OFF = SCAN_OFF + NW * 4;        // [kPagedMaxTiles] i32: tiles up to sequence b and with it
+  static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;       // [PR] f32
+  static constexpr int SREF_OFF = ROWL_OFF + PR * 4;        // f32 (and padding)
+  static constexpr int FLAG_OFF = SREF_OFF + 16;            // [4] i32
+  static constexpr int SCAN_OFF = FLAG_OFF + 16;            // [8] i32
+  static constexpr int SEQ_OFF = SCAN_OFF + 32;             // [kPagedMaxTiles] i32: tiles up to sequence b and with it
   static constexpr int TILE_OFF = SEQ_OFF + kPagedMaxTiles * 4;  // [kPagedMaxTiles] i32: pages up to tile t and with it
-  static constexpr bool kRopeLds = BM >= 64;      // the queries' rope parts in LDS, where registers are short
-  static constexpr int ROPE_OFF = TILE_OFF + kPagedMaxTiles * 4;  // [BM][64] bf16, chunks placed as a page's
-  static constexpr int BYTES = ROPE_OFF + (kRopeLds ? BM * kKvRope * 2 : 0);
+  static constexpr int BYTES = TILE_OFF + kPagedMaxTiles * 4;
   static constexpr size_t kPartFloats = static_cast<size_t>(PR) * kKvLatent;
 };
+constexpr int kPagedThreads = 512;
+// 32 rows' queries on their way into registers, in slot 2: hi codes [32][512], lo codes, rope parts bf16 [32][64]
+constexpr int kQueryLo = 32 * kKvLatent, kQueryRope = 2 * kQueryLo;
+static_assert(kQueryRope + 32 * kKvRope * 2 <= kSlotBytes, "");
 
 // What a split launch leaves for the combine kernel, in the workspace: for every workgroup the tile that it
 // continues, if it is the second on it; two slots of partial sums a workgroup (0: of the tile that it continues, 1: of
@@ -110,27 +114,39 @@ struct SeqRows {
   }
 };
 
+// Inclusive sum over the wave (row shifts, then the broadcasts of lanes 15 and 31).
+__device__ inline int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
 // Inclusive sum over the workgroup's threads, and the total of all; `part` holds one int a wave.
-template <int NW>
 __device__ inline int block_scan(int v, int* part, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v = wave_scan(v);
   if (lane == 63) part[wave] = v;
   __syncthreads();
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
+  for (int w = 0; w < kPagedThreads / 64; ++w) {
     const int x = part[w];
     before += w < wave ? x : 0;
     total += x;
   }
   __syncthreads();
   return v + before;
+}
+
+// Max over each 16-lane row, in every lane of it.
+__device__ inline uint32_t row16_max_u32(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xf, 0xf, false)));
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xf, 0xf, false)));
 }
 
 // The first index of an ascending array that is > x.
@@ -191,30 +207,15 @@ __device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
   lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 32.0f, (x[3] - b[1]) * 32.0f, lo, true);
 }
 
-template <int NW, int RG>
-__global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedArgs A) {
-  using C = PagedCfg<NW, RG>;
-  constexpr int BM = C::BM, KG = C::KG, KT = C::KT, RT2 = C::RT2, DT = C::DT;
+template <int BM>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const PagedArgs A) {
+  using C = PagedCfg<BM>;
+  constexpr int KG = C::KG, KT = C::KT, RT2 = C::RT2, DT = 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kg = wave % KG, rg = wave / KG;  // key group, row group
   const int n16 = lane & 15, g = lane >> 4;
   const int n32 = lane & 31, half = lane >> 5;
-  // lane parts of the addresses: a 16-byte chunk c of a page's row is kept at c ^ (row & 7), so that the rows' chunks
-  // that a read takes together are in different banks; c's bits above the third are whole steps of 128 bytes
-  const uint32_t fetch_code = half * 512 + (n32 ^ half) * 16;  // rows 2 i, 2 i + 1 (i % 4 = 0; ^ 32 (i % 4) for others)
-  const uint32_t fetch_rope = (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
-  const int my_key = kg * KT * 16 + n16;  // and 16, 32, .. behind it
-  const int at_code = my_key * kKvLatent + ((2 * g) ^ (my_key & 7)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31)
-  const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (my_key & 7)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
-  const int at_value = (32 * half + (n16 >> 1)) * kKvLatent + (wave * DT >> 2) * 128 + (lane & 1) * 8 +
-                       (((wave * DT * 2 & 7) + (g & 1)) ^ (n16 >> 1)) * 16;  // 32-dim tile d: ^ 32 d
-  const int at_p = n32 * kPStride + half * 32;
-  const int my_row = rg * 16 + n16;
-  const int my_quad = kg * KT * 16 + 4 * g;  // the keys of this lane's scores: my_quad .. +3, and 16, 32, .. behind them
-  const int put_rope = my_row * 128 + (g ^ (my_row & 7)) * 16;
-  const int put_p = my_row * kPStride + my_quad;
   const PagedBatch& p = A.p;
   int* seq_end = reinterpret_cast<int*>(smem + C::SEQ_OFF);
   int* unit_end = reinterpret_cast<int*>(smem + C::TILE_OFF);
@@ -222,6 +223,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
   float* stat = reinterpret_cast<float*>(smem + C::STAT_OFF);
   float* alpha_l = reinterpret_cast<float*>(smem + C::ALPHA_OFF);
   float* rowl = reinterpret_cast<float*>(smem + C::ROWL_OFF);
+  float* sref_l = reinterpret_cast<float*>(smem + C::SREF_OFF);
   int* flag = reinterpret_cast<int*>(smem + C::FLAG_OFF);
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8_ptr)smem));
   const int w = blockIdx.x;
@@ -230,15 +232,15 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
   int n_tiles = 0, u = 0, u_end = 1, quota = 1, tile = 0, seq = 0, seq_tile0 = 0;
   if (A.split) {
     // units are pages of tiles (a tile that sees nothing counts one); every workgroup takes `quota` of them in a row
-    for (int b0 = 0; b0 < p.n_seqs; b0 += C::kThreads) {
+    for (int b0 = 0; b0 < p.n_seqs; b0 += kPagedThreads) {
       const int b = b0 + tid;
       int total;
-      const int t = block_scan<NW>(b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), A.tile_cap) : 0, scan, total);
+      const int t = block_scan(b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), A.tile_cap) : 0, scan, total);
       if (b < p.n_seqs) seq_end[b] = min(n_tiles + t, A.tile_cap);
       n_tiles = min(n_tiles + total, A.tile_cap);
     }
     __syncthreads();
-    const int per = (n_tiles + C::kThreads - 1) / C::kThreads, t0 = tid * per, t1 = min(t0 + per, n_tiles);
+    const int per = (n_tiles + kPagedThreads - 1) / kPagedThreads, t0 = tid * per, t1 = min(t0 + per, n_tiles);
     int sum = 0;
     if (t0 < t1) {
       int b = upper(seq_end, p.n_seqs, t0);
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
       }
     }
     int units;
-    const int before = block_scan<NW>(sum, scan, units) - sum;
+    const int before = block_scan(sum, scan, units) - sum;
     for (int t = t0; t < t1; ++t) unit_end[t] += before;
     __syncthreads();
     units = __builtin_amdgcn_readfirstlane(units);
@@ -277,11 +279,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
     // one workgroup a tile: its sequence, from the tile counts in order
     tile = w;
     seq = -1;
-    for (int b0 = 0; b0 < p.n_seqs; b0 += C::kThreads) {
+    for (int b0 = 0; b0 < p.n_seqs; b0 += kPagedThreads) {
       const int b = b0 + tid;
       int total;
       const int mine = b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), static_cast<int>(gridDim.x)) : 0;
-      const int t = n_tiles + block_scan<NW>(mine, scan, total);
+      const int t = n_tiles + block_scan(mine, scan, total);
       if (w >= t - mine && w < t) { scan[0] = b; scan[1] = t - mine; }
       __syncthreads();
       if (w < n_tiles + total) { seq = scan[0]; seq_tile0 = scan[1]; break; }
@@ -308,237 +310,48 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
     const int64_t row0 = static_cast<int64_t>(s.first) * A.heads + in_seq;
     const int rows = min(BM, s.n_tok * A.heads - in_seq);
     const int n_pages = s.pages(p, j, A.heads, BM);
-    const int seen_all = s.seen(p, in_seq, A.heads);  // every row sees these
+    const int seen_first = s.seen(p, in_seq, A.heads);             // every row sees these
+    const int seen_last = s.seen(p, in_seq + rows - 1, A.heads);   // some row sees these
     const int pg0 = u - tile_u0;
     const int n = min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0);
     const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
 
     // page k of the tile into its slot, in 1 KB pieces: 32 of codes, four at a time, and 8 of rope parts; every wave
-    // also fetches the scales, all of them the same
+    // also fetches the scales, all of them the same.  A 16-byte chunk c of a row is kept at c ^ (row & 7), so
+    // that the rows' chunks that a read takes together are in different banks
     auto fetch = [&](int k, int slot) {
       int id = table[k];
       if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.n_pages)) id = 0;  // its keys are masked
       const uint8_t* page = A.pages + static_cast<int64_t>(id) * kKvPageBytes;
       const uint32_t to = lds0 + slot * kSlotBytes;
-      const uint32_t off[4] = {fetch_code, fetch_code ^ 32, fetch_code ^ 64, fetch_code ^ 96};
-#pragma unroll
-      for (int i = 0; i < 8 / NW; ++i) {
-        const int at = (wave * (8 / NW) + i) * 4096;
-        dma_pieces<4>(page + at, off, to + at);
-      }
-      constexpr int kRope = 8 / NW;
-      uint32_t rope[kRope];
-#pragma unroll
-      for (int i = 0; i < kRope; ++i) rope[i] = fetch_rope;
-      const int at = wave * kRope * 1024;
-      dma_pieces<kRope>(page + kKvRopeAt + at, rope, to + kKvPageKeys * kKvLatent + at);
+      const uint32_t code = half * 512 + (n32 ^ half) * 16;  // rows 2 i, 2 i + 1 of piece i
+      const uint32_t off[4] = {code, code ^ 32, code ^ 64, code ^ 96};
+      dma_pieces<4>(page + wave * 4096, off, to + wave * 4096);
+      const uint32_t rope[1] = {static_cast<uint32_t>((lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16)};
+      dma_pieces<1>(page + kKvRopeAt + wave * 1024, rope, to + kKvPageKeys * kKvLatent + wave * 1024);
       dma_words(page + kKvScaleAt, lane * 4, lds0 + C::SCALE_OFF + slot * kKvPageKeys * 4);
     };
-    __syncthreads();  // the slots, P and the statistics are free again
-    if (tid < 4) flag[tid] = 0;
-    if (n > 0) fetch(0, 0);
-    if (n > 1) fetch(1, 1);
-
-    // ---- the rows' queries as hi + lo / 32, and what each row sees
-    v8i qhi[4], qlo[4];
-    v8bf qr[2];
-    float f, m = -INFINITY, l, psum = 0.f;
-    int seen;
-    {
-      const bool live = my_row < rows;
-      const int64_t row = row0 + (live ? my_row : 0);
-      const u32x4p* qn = reinterpret_cast<const u32x4p*>(A.q_nope + row * kKvLatent);
-      const u32x4p* qp = reinterpret_cast<const u32x4p*>(A.q_pe + row * kKvRope);
-      u32x4p raw[4][4], rawr[2];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) raw[ks][c] = qn[ks * 16 + g * 4 + c];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) rawr[ks] = qp[ks * 4 + g];
-      uint32_t most = 0;  // the largest magnitude's bits (bf16, upper half)
-      auto look = [&](uint32_t x) { most = max(most, max(x & 0x7fff0000u, (x << 16) & 0x7fff0000u)); };
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) look(raw[ks][c][i]);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) look(rawr[ks][i]);
-      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
-      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
-      const bool bad = live && most >= 0x7f800000u;  // a NaN or an infinity: every output of the row is NaN
-      const bool zero = bad || !live;
-      const int e = zero ? 0 : max(static_cast<int>(most >> 23) - 127 - 7, -120);  // sigma = 2^e
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t x0 = zero ? 0u : raw[ks][c >> 1][(c & 1) * 2], x1 = zero ? 0u : raw[ks][c >> 1][(c & 1) * 2 + 1];
-          const float v[4] = {__uint_as_float(x0 << 16) * inv, __uint_as_float(x0 & 0xffff0000u) * inv,
-                              __uint_as_float(x1 << 16) * inv, __uint_as_float(x1 & 0xffff0000u) * inv};
-          int hi, lo;
-          split4(v, hi, lo);
-          qhi[ks][c] = hi;
-          qlo[ks][c] = lo;
-        }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        u32x4p x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t y = zero ? 0u : rawr[ks][i];
-          x[i] = bf16x2_bits(v2f{__uint_as_float(y << 16) * inv, __uint_as_float(y & 0xffff0000u) * inv});
-        }
-        if constexpr (!C::kRopeLds) qr[ks] = __builtin_bit_cast(v8bf, x);
-        else if (kg == 0) *reinterpret_cast<u32x4p*>(smem + C::ROPE_OFF + (put_rope ^ (ks * 64))) = x;
-      }
-      seen = live ? s.seen(p, in_seq + my_row, A.heads) : 0;
-      l = bad && seen > 0 ? __builtin_nanf("") : 0.f;
-    }
-    v16f o[RT2][DT];
-#pragma unroll
-    for (int a = 0; a < RT2; ++a)
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[a][d][i] = 0.f;
-    float s_ref = 0.f, kf = 0.f;
-    v4f U[KT];
-
-    // the keys' operands of page k, and the products with the queries: U (codes) and R (rope parts)
-    // U of a page: 4 KT items of 128 dims, each item's operand read kAhead items before its
-    // two products.  The order is held by barriers: with all reads first the registers do not suffice, and a spilled
-    // register's reload waits for the page that is being fetched.
-    auto load_key = [&](int slot, int i) {
-      const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i % 4) * 128;
-      return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
+    auto masked = [&](int k) {
+      return (pg0 + k + 1) * kKvPageKeys > seen_first || static_cast<uint32_t>(table[k]) >= static_cast<uint32_t>(p.n_pages);
     };
-    auto score_products = [&](int slot) {
-      constexpr int kItems = 4 * KT, kAhead = KT > 1 ? 2 : 3;
-      v8i a[kItems];
-      v8bf r[KT][2];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) U[kt] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        if (i + kAhead < kItems) a[i + kAhead] = load_key(slot, i + kAhead);
-        if (i + kAhead == kItems) {
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-              r[kt][ks] = *reinterpret_cast<const v8bf*>(smem + slot * kSlotBytes + (at_rope ^ (ks * 64)) + kt * 16 * 128);
-          if constexpr (C::kRopeLds)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) qr[ks] = *reinterpret_cast<const v8bf*>(smem + C::ROPE_OFF + (put_rope ^ (ks * 64)));
-        }
-        U[i / 4] = mfma16_fp8(a[i], qhi[i % 4], U[i / 4], kScaleOne);
-        U[i / 4] = mfma16_fp8(a[i], qlo[i % 4], U[i / 4], kScaleLo);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) U[kt][i] *= __builtin_fabsf(sk[i]) < INFINITY ? sk[i] : __builtin_nanf("");  // not -inf, a masked score
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) U[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(r[kt][ks], qr[ks], U[kt], 0, 0, 0);
-      }
-    };
-    // the scores of page k, in `slot`, that a row does not see
-    auto mask_scores = [&](int k) {
-      const bool there = static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
-      const int at = (pg0 + k) * kKvPageKeys + my_quad;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) U[kt][i] = there && at + kt * 16 + i < seen ? U[kt][i] : -INFINITY;
-    };
-
-    // P of page k from U, m and s_ref: codes to buffer k % 2, psum; whether all were <= kPMost
-    auto weights = [&](int k, int slot) {
-      uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p;
-      const float mu = m == -INFINITY ? 0.f : m;
-      float pmax = 0.f, sum = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4) * kf;
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool none = U[kt][i] == -INFINITY;  // a masked key's scale may be anything
-          const float e = none ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mu));
-          sum += e;
-          x[i] = none ? 0.f : e * sk[i];
-          pmax = fmaxf(pmax, __builtin_fabsf(x[i]));
-        }
-        int hi, lo;
-        split4(x, hi, lo);
-        *reinterpret_cast<int*>(P + kt * 16) = hi;
-        *reinterpret_cast<int*>(P + kt * 16 + C::P_BYTES) = lo;
-      }
-      psum = sum;
-      return !__any(pmax > kPMost);
-    };
-
-    // New m and s_ref from page k's scores, O and l brought to them, P again.  Every wave comes here, or none.
-    auto settle = [&](int k, int slot) {
-      float x = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(fmaxf(U[kt][0], U[kt][1]), fmaxf(U[kt][2], U[kt][3])));
-      x = fmaxf(x, __shfl_xor(x, 16));
-      x = fmaxf(x, __shfl_xor(x, 32));
-      if (g == 0) stat[kg * BM + my_row] = x;
-      // the largest finite scale of the page's keys that some row sees
-      const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + slot * kKvPageKeys * 4)[lane]);
-      const bool use = (pg0 + k) * kKvPageKeys + lane < s.seen(p, in_seq + rows - 1, A.heads) && sk < INFINITY &&
-                       static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
-      const float most = fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f);
-      const float ratio = s_ref > 0.f ? s_ref / fmaxf(s_ref, most) : 0.f;
-      s_ref = fmaxf(s_ref, most);
-      kf = kP / s_ref;
+    // every wave's part of a fetch has arrived, and what it wrote to LDS is there
+    auto arrive = [&] {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < KG; ++i) x = fmaxf(x, stat[i * BM + my_row]);
-      const float mn = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
-      const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= m == -INFINITY ? 1.0f : a;  // (0, or a bad row's NaN, before the first key)
-      m = mn;
-      if (kg == 0 && g == 0) alpha_l[my_row] = a * ratio;
-      weights(k, slot);
-      __syncthreads();
-#pragma unroll
-      for (int a = 0; a < RT2; ++a) {
-        const float x = alpha_l[min(a * 32 + n32, BM - 1)];
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[a][d][i] *= x;
-      }
     };
-
     // a page's codes before a masked step: a NaN code would reach rows that do not see its key through 0 * NaN, so it
     // becomes 0 and the key's scale NaN
     auto clean = [&](int slot) {
       uint8_t* codes = smem + slot * kSlotBytes;
-      for (int i = tid; i < kKvPageKeys * kKvLatent / 16; i += C::kThreads) {
+#pragma unroll 1
+      for (int i = tid; i < kKvPageKeys * kKvLatent / 16; i += kPagedThreads) {
         v4i x = reinterpret_cast<v4i*>(codes)[i];
-        bool found = false;
+        uint32_t found = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t y = static_cast<uint32_t>(x[c]) & 0x7f7f7f7fu;
           // bytes equal to 0x7f: adding 1 to a 7-bit value carries into bit 7 only from 0x7f
-          const uint32_t nan = ((y + 0x01010101u) & 0x80808080u) >> 7;
-          found = found || nan;
+          const uint32_t nan = (((static_cast<uint32_t>(x[c]) & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+          found |= nan;
           x[c] &= ~static_cast<int>(nan * 0xffu);
         }
         if (found) {
@@ -549,142 +362,356 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_mla_kernel(const PagedA
       __syncthreads();
     };
 
-    // O^T += latent^T P^T of page k: rows of A are dims, of B the tile's rows, 64 keys in one MFMA.  The operand lane
-    // (dim n32, half) needs 32 keys of its dim, a column of the key-major codes: ds_read_b64_tr_b8 gives lane i of a
-    // 16-lane group byte i % 8 of the 8 bytes at lane 2 j + i / 8's address as its byte j, so lane i addresses key
-    // 32 half + 8 r + i / 2, half i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
-    auto product = [&](int k, int slot) {
-      const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + at_p;
-      v8i v[DT];
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const uint8_t* src = smem + slot * kSlotBytes + (at_value ^ (32 * d));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + r * 8 * kKvLatent));
-          v[d][2 * r] = x[0];
-          v[d][2 * r + 1] = x[1];
-        }
-      }
-#pragma unroll
-      for (int a = 0; a < RT2; ++a) {
-        const v4i* hi = reinterpret_cast<const v4i*>(P + a * 32 * kPStride);
-        const v4i* lo = reinterpret_cast<const v4i*>(P + a * 32 * kPStride + C::P_BYTES);
-        const v8i ph = two_v4i(hi[0], hi[1]), pl = two_v4i(lo[0], lo[1]);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          o[a][d] = mfma32_fp8(v[d], ph, o[a][d], kScaleOne);
-          o[a][d] = mfma32_fp8(v[d], pl, o[a][d], kScaleLo);
-        }
-        if (a + 1 < RT2) __builtin_amdgcn_sched_barrier(0);  // the next rows' P not before: registers
-      }
-    };
+    __syncthreads();  // the slots, P and the statistics are free again
+    if (tid < 4) flag[tid] = 0;
 
-    // ---- the pages.  Step k: the scores of page k + 1, the product of page k, the weights of page k + 1; one
-    // barrier a step, before which the fetch of page k + 2 has arrived
-    auto masked = [&](int k) {
-      return (pg0 + k + 1) * kKvPageKeys > seen_all || static_cast<uint32_t>(table[k]) >= static_cast<uint32_t>(p.n_pages);
-    };
-    auto arrive = [&] {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __syncthreads();
-    };
-    // With KT > 1 a spilled operand is reloaded among the scores, and its wait would be for the fetch too: the fetch
-    // follows them (2048 tokens over 16384 keys 1458 us with it first, 1286 so; KT = 1 spills nothing, and
-    // 60 sequences take 128 us with it first, 139 so).
-    constexpr bool kLate = KT > 1;
-    // P of page k is whole, page k + 1 in its slot: the scores of k + 1, the product of k, and between the product's
-    // MFMAs the weights of k + 1
-    auto step = [&](int k, int slot, int next, int free, auto mask) {
-      score_products(next);
-      if (kLate && k + 2 < n) fetch(k + 2, free);
-      if constexpr (decltype(mask)::value) mask_scores(k + 1);
+    // ---- the rows' queries as hi + lo / 32, through slot 2: 16 lanes a row, 32 rows a round.  Their loads are first, as
+    // their wait would be for the pages too
+    v8i qhi[4], qlo[4];
+    v8bf qr[2];
+    float f = 0.f;
+    const int kg = wave % KG, rg = wave / KG;  // a scoring wave's keys and rows
+    const int my_row = rg * 16 + n16;
+#pragma unroll
+    for (int round = 0; round < RT2; ++round) {
+      const int r = round * 32 + wave * 4 + g, place = wave * 4 + g;
+      const bool live = r < rows;
+      const int64_t row = row0 + (live ? r : 0);
+      u32x4p raw[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = reinterpret_cast<const u32x4p*>(A.q_nope + row * kKvLatent)[n16 + 16 * i];
+      raw[4] = reinterpret_cast<const u32x4p*>(A.q_pe + row * kKvRope)[n16 & 7];
+      uint32_t most = 0;  // the largest magnitude's bits (bf16, upper half)
+#pragma unroll
+      for (int i = 0; i < 5; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) most = max(most, max(raw[i][c] & 0x7fff0000u, (raw[i][c] << 16) & 0x7fff0000u));
+      most = row16_max_u32(most);
       __builtin_amdgcn_sched_barrier(0);
-      product(k, slot);
-      const bool fits = weights(k + 1, next);
-      if (!fits && lane == 0) flag[(k + 1) & 3] = 1;
-    };
-    if (n > 0) {
-      arrive();
-      {
-        const bool cut = masked(0);
-        if (cut) clean(0);
-        score_products(0);
-        if (cut) mask_scores(0);
+      if (round == 0) {
+        if (n > 0) fetch(0, 0);
+        if (n > 1) fetch(1, 1);
       }
-      settle(0, 0);
-      int slot = 0, next = 1, free = 2;  // of pages k, k + 1, k + 2
-      for (int k = 0; k < n; ++k) {
-          l += psum;
-        if (!kLate && k + 2 < n) fetch(k + 2, free);
-        if (k + 1 < n) {
-          if (tid == 0) flag[(k + 2) & 3] = tid;  // (0, without a register that holds it)
-          if (masked(k + 1)) {
-            clean(next);
-            step(k, slot, next, free, std::true_type{});
-          } else {
-            step(k, slot, next, free, std::false_type{});
-          }
-          arrive();
-          if (flag[(k + 1) & 3]) settle(k + 1, next);
-        } else {
-          product(k, slot);
+      const bool bad = most >= 0x7f800000u;  // a NaN or an infinity: every output of the row is NaN
+      const bool zero = bad || !live;
+      const int e = zero ? 0 : max(static_cast<int>(most >> 23) - 127 - 7, -120);  // sigma = 2^e
+      const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      uint8_t* to = smem + 2 * kSlotBytes;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v2i hi, lo;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t x0 = zero ? 0u : raw[i][2 * c], x1 = zero ? 0u : raw[i][2 * c + 1];
+          const float v[4] = {__uint_as_float(x0 << 16) * inv, __uint_as_float(x0 & 0xffff0000u) * inv,
+                              __uint_as_float(x1 << 16) * inv, __uint_as_float(x1 & 0xffff0000u) * inv};
+          int a, b;
+          split4(v, a, b);
+          hi[c] = a;
+          lo[c] = b;
         }
-        const int was = slot;
-        slot = next;
-        next = free;
-        free = was;
+        const int at = place * kKvLatent + (((n16 >> 1) ^ (place & 7)) + 8 * i) * 16 + (n16 & 1) * 8;
+        *reinterpret_cast<v2i*>(to + at) = hi;
+        *reinterpret_cast<v2i*>(to + kQueryLo + at) = lo;
       }
+      if (n16 < 8) {
+        u32x4p x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t y = zero ? 0u : raw[4][c];
+          x[c] = bf16x2_bits(v2f{__uint_as_float(y << 16) * inv, __uint_as_float(y & 0xffff0000u) * inv});
+        }
+        *reinterpret_cast<u32x4p*>(to + kQueryRope + place * 128 + (n16 ^ (place & 7)) * 16) = x;
+      }
+      // (a bad row's factor is NaN, which makes its sum NaN)
+      if (n16 == 0 && r < BM) rowl[r] = bad && live ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale;
+      __syncthreads();
+      if (wave < 4 && my_row / 32 == round) {
+        const int q = my_row & 31;
+        const uint8_t* from = smem + 2 * kSlotBytes + q * kKvLatent;
+        const int c0 = ((2 * g) ^ (q & 7)) * 16;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          qhi[ks] = two_v4i(*reinterpret_cast<const v4i*>(from + c0 + ks * 128), *reinterpret_cast<const v4i*>(from + (c0 ^ 16) + ks * 128));
+          qlo[ks] = two_v4i(*reinterpret_cast<const v4i*>(from + kQueryLo + c0 + ks * 128), *reinterpret_cast<const v4i*>(from + kQueryLo + (c0 ^ 16) + ks * 128));
+        }
+        const int r0 = kQueryRope + q * 128 + (g ^ (q & 7)) * 16;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) qr[ks] = *reinterpret_cast<const v8bf*>(smem + 2 * kSlotBytes + (r0 ^ (ks * 64)));
+        f = rowl[my_row];
+      }
+      if (round + 1 < RT2) __syncthreads();
     }
 
-    // ---- the tile's sums: l over the lanes and waves of a row, then the rows' results or partial sums
-    __syncthreads();
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (g == 0) {
-      stat[kg * BM + my_row] = l;
-      if (kg == 0) alpha_l[my_row] = m;
-    }
-    __syncthreads();
-    if (tid < BM) {
-      float x = 0.f;
+    // ---- the pages.  Step k: the scoring waves make P of page k + 1, the others multiply that of page k; one barrier a
+    // step, before which page k + 2 has arrived.  P is made with the maxima and s_ref that were set last; where a
+    // weight would not fit (flag), every wave goes through settle() before it is used.
+    if (wave < 4) {
+      const int my_key = kg * KT * 16 + n16;       // and 16, 32, .. behind it
+      const int my_quad = kg * KT * 16 + 4 * g;    // the keys of this lane's scores: my_quad .. +3, and 16, 32, ..
+      const int at_code = my_key * kKvLatent + ((2 * g) ^ (my_key & 7)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31)
+      const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (my_key & 7)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
+      const int put_p = my_row * kPStride + my_quad;
+      const int seen = my_row < rows ? s.seen(p, in_seq + my_row, A.heads) : 0;
+      float m = -INFINITY, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f, kf = 0.f;
+      if (f != f) f = 0.f;
+      v4f U[KT];
+
+      // U of a page: scale * (codes . q) + rope . q, 4 KT items of 128 dims, each item's operand read ahead of its products
+      auto load_key = [&](int slot, int i) {
+        const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i % 4) * 128;
+        return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
+      };
+      auto scores = [&](int k, int slot) {
+        constexpr int kItems = 4 * KT, kAhead = 4;
+        v8i a[kItems];
 #pragma unroll
-      for (int i = 0; i < KG; ++i) x += stat[i * BM + tid];
-      rowl[tid] = x;
-    }
-    __syncthreads();
-    const bool whole = !A.split || (u == tile_u0 && u_end >= tile_u1);
-    if (whole) {
-      if (A.lse && tid < rows) A.lse[row0 + tid] = rowl[tid] == 0.f ? -INFINITY : (alpha_l[tid] + log2f(rowl[tid])) * 0.6931471805599453f;
+        for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int a = 0; a < RT2; ++a) {
-        const int r = a * 32 + n32;
-        if (r < rows) {
-          const float L = rowl[r], x = L == 0.f ? 0.f : s_ref / (kP * L);
-          uint16_t* dst = A.out + (row0 + r) * kKvLatent + wave * DT * 32 + 4 * half;
+        for (int kt = 0; kt < KT; ++kt) {
+          v4f x = {0.f, 0.f, 0.f, 0.f};
+          const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
+          v8bf r[2];
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+          for (int ks = 0; ks < 2; ++ks) r[ks] = *reinterpret_cast<const v8bf*>(smem + slot * kSlotBytes + (at_rope ^ (ks * 64)) + kt * 16 * 128);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<u32x2p*>(dst + d * 32 + 8 * i) = u32x2p{bf16x2_bits(v2f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x}),
-                                                                       bf16x2_bits(v2f{o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x})};
+          for (int ks = 0; ks < 4; ++ks) {
+            const int i = kt * 4 + ks;
+            if (i + kAhead < kItems) a[i + kAhead] = load_key(slot, i + kAhead);
+            x = mfma16_fp8(a[i], qhi[ks], x, kScaleOne);
+            x = mfma16_fp8(a[i], qlo[ks], x, kScaleLo);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] *= __builtin_fabsf(sk[i]) < INFINITY ? sk[i] : __builtin_nanf("");  // not -inf, a masked score
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(r[ks], qr[ks], x, 0, 0, 0);
+          U[kt] = x;
+        }
+        if (masked(k)) {
+          const bool there = static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
+          const int at = (pg0 + k) * kKvPageKeys + my_quad;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) U[kt][i] = there && at + kt * 16 + i < seen ? U[kt][i] : -INFINITY;
+        }
+      };
+
+      // P of page k from U, m and s_ref: codes to buffer k % 2, psum; whether all were <= kPMost
+      auto weights = [&](int k, int slot) {
+        uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p;
+        const float mu = m == -INFINITY ? 0.f : m;
+        float pmax = 0.f, sum = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4) * kf;
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool none = U[kt][i] == -INFINITY;  // a masked key's scale may be anything
+            const float e = none ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mu));
+            sum += e;
+            x[i] = none ? 0.f : e * sk[i];
+            pmax = fmaxf(pmax, __builtin_fabsf(x[i]));
+          }
+          int hi, lo;
+          split4(x, hi, lo);
+          *reinterpret_cast<int*>(P + kt * 16) = hi;
+          *reinterpret_cast<int*>(P + kt * 16 + C::P_BYTES) = lo;
+        }
+        psum = sum;
+        return !__any(pmax > kPMost);
+      };
+
+      // New m and s_ref from page k's scores, O and l brought to them, P again.  Every wave comes here, or none.
+      auto settle = [&](int k, int slot) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(fmaxf(U[kt][0], U[kt][1]), fmaxf(U[kt][2], U[kt][3])));
+        x = fmaxf(x, __shfl_xor(x, 16));
+        x = fmaxf(x, __shfl_xor(x, 32));
+        if (KG > 1 && g == 0) stat[kg * BM + my_row] = x;
+        // the largest finite scale of the page's keys that some row sees
+        const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + slot * kKvPageKeys * 4)[lane]);
+        const bool use = (pg0 + k) * kKvPageKeys + lane < seen_last && sk < INFINITY &&
+                         static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
+        const float most = fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f);
+        const float ratio = s_ref > 0.f ? s_ref / fmaxf(s_ref, most) : 0.f;
+        s_ref = fmaxf(s_ref, most);
+        kf = kP / s_ref;
+        if (tid == 0) *sref_l = s_ref;
+        __syncthreads();
+        if constexpr (KG > 1)
+#pragma unroll
+          for (int i = 0; i < KG; ++i) x = fmaxf(x, stat[i * BM + my_row]);
+        const float mn = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
+        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= m == -INFINITY ? 1.0f : a;  // (0, or a bad row's NaN, before the first key)
+        m = mn;
+        if (kg == 0 && g == 0) alpha_l[my_row] = a * ratio;
+        weights(k, slot);
+        __syncthreads();
+      };
+
+      if (n > 0) {
+        arrive();
+        if (masked(0)) clean(0);
+        scores(0, 0);
+        settle(0, 0);
+        int next = 1, free = 2, slot = 0;
+#pragma unroll 1
+        for (int k = 0; k < n; ++k) {
+          l += psum;
+          if (k + 2 < n) fetch(k + 2, free);
+          if (k + 1 < n) {
+            if (tid == 0) flag[(k + 2) & 3] = tid;  // (0, without a register that holds it)
+            if (masked(k + 1)) clean(next);
+            scores(k + 1, next);
+            if (!weights(k + 1, next) && lane == 0) flag[(k + 1) & 3] = 1;
+            arrive();
+            if (flag[(k + 1) & 3]) settle(k + 1, next);
+          }
+          const int was = slot;
+          slot = next;
+          next = free;
+          free = was;
         }
       }
+      // l over the lanes and waves of a row
+      __syncthreads();
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      if (g == 0) {
+        stat[kg * BM + my_row] = l;
+        if (kg == 0) alpha_l[my_row] = m;
+      }
+      __syncthreads();
+      if (tid < BM) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < KG; ++i) x += stat[i * BM + tid];
+        rowl[tid] = x;
+      }
+      __syncthreads();
     } else {
-      const int slot = 2 * w + (u == tile_u0 ? 1 : 0);
-      if (tid < rows) A.part_ml[static_cast<int64_t>(slot) * C::PR + tid] = float2{alpha_l[tid], rowl[tid]};
-      const float x = s_ref / kP;
-      v4f* dst = reinterpret_cast<v4f*>(A.part_o + static_cast<int64_t>(slot) * C::kPartFloats);
+      const int dw = wave - 4;  // dims 128 dw ..
+      const int at_value = (32 * half + (n16 >> 1)) * kKvLatent + dw * 128 + (lane & 1) * 8 + ((g & 1) ^ (n16 >> 1)) * 16;  // 32-dim tile d: ^ 32 d
+      const int at_p = n32 * kPStride + half * 32;
+      v16f o[RT2][DT];
 #pragma unroll
       for (int a = 0; a < RT2; ++a)
-        if (a * 32 + n32 < rows) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[a][d][i] = 0.f;
+
+      // O^T += latent^T P^T of page k: rows of A are dims, of B the tile's rows, 64 keys in one MFMA.  The operand lane
+      // (dim n32, half) needs 32 keys of its dim, a column of the key-major codes: ds_read_b64_tr_b8 gives lane i of a
+      // 16-lane group byte i % 8 of the 8 bytes at lane 2 j + i / 8's address as its byte j, so lane i addresses key
+      // 32 half + 8 r + i / 2, half i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
+      auto product = [&](int k, int slot) {
+        const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + at_p;
+        v8i v[DT], ph[RT2], pl[RT2];
+#pragma unroll
+        for (int a = 0; a < RT2; ++a) {
+          const v4i* hi = reinterpret_cast<const v4i*>(P + a * 32 * kPStride);
+          const v4i* lo = reinterpret_cast<const v4i*>(P + a * 32 * kPStride + C::P_BYTES);
+          ph[a] = two_v4i(hi[0], hi[1]);
+          pl[a] = two_v4i(lo[0], lo[1]);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const uint8_t* src = smem + slot * kSlotBytes + (at_value ^ (32 * d));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + r * 8 * kKvLatent));
+            v[d][2 * r] = x[0];
+            v[d][2 * r + 1] = x[1];
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int a = 0; a < RT2; ++a) {
+            o[a][d] = mfma32_fp8(v[d], ph[a], o[a][d], kScaleOne);
+            o[a][d] = mfma32_fp8(v[d], pl[a], o[a][d], kScaleLo);
+          }
+      };
+      auto settle = [&](bool first) {
+        __syncthreads();
+        __syncthreads();
+        if (first) return;  // (nothing to bring along)
+#pragma unroll
+        for (int a = 0; a < RT2; ++a) {
+          const float x = alpha_l[min(a * 32 + n32, BM - 1)];
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              dst[((a * 16 + wave * DT + d) * 4 + i) * 64 + lane] =
-                  v4f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x, o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x};
+            for (int i = 0; i < 16; ++i) o[a][d][i] *= x;
         }
+      };
+
+      if (n > 0) {
+        arrive();
+        if (masked(0)) clean(0);
+        settle(true);
+        int next = 1, free = 2, slot = 0;
+#pragma unroll 1
+        for (int k = 0; k < n; ++k) {
+          if (k + 2 < n) fetch(k + 2, free);
+          if (k + 1 < n && masked(k + 1)) clean(next);
+          product(k, slot);
+          if (k + 1 < n) {
+            arrive();
+            if (flag[(k + 1) & 3]) settle(false);
+          }
+          const int was = slot;
+          slot = next;
+          next = free;
+          free = was;
+        }
+      }
+      __syncthreads();
+      __syncthreads();
+      __syncthreads();
+
+      // ---- the rows' results, or the tile's partial sums
+      const float s_ref = n > 0 ? *sref_l : 0.f;
+      if (!A.split || (u == tile_u0 && u_end >= tile_u1)) {
+        const int t = tid - 256;
+        if (A.lse && t < rows) A.lse[row0 + t] = rowl[t] == 0.f ? -INFINITY : (alpha_l[t] + log2f(rowl[t])) * 0.6931471805599453f;
+#pragma unroll
+        for (int a = 0; a < RT2; ++a) {
+          const int r = a * 32 + n32;
+          if (r < rows) {
+            const float L = rowl[r], x = L == 0.f ? 0.f : s_ref / (kP * L);
+            uint16_t* dst = A.out + (row0 + r) * kKvLatent + dw * 128 + 4 * half;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<u32x2p*>(dst + d * 32 + 8 * i) = u32x2p{bf16x2_bits(v2f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x}),
+                                                                         bf16x2_bits(v2f{o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x})};
+          }
+        }
+      } else {
+        const int slot = 2 * w + (u == tile_u0 ? 1 : 0), t = tid - 256;
+        if (t < rows) A.part_ml[static_cast<int64_t>(slot) * C::PR + t] = float2{alpha_l[t], rowl[t]};
+        const float x = s_ref / kP;
+        v4f* dst = reinterpret_cast<v4f*>(A.part_o + static_cast<int64_t>(slot) * C::kPartFloats);
+#pragma unroll
+        for (int a = 0; a < RT2; ++a)
+          if (a * 32 + n32 < rows) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                dst[((a * 16 + dw * DT + d) * 4 + i) * 64 + lane] =
+                    v4f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x, o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x};
+          }
+      }
     }
     if (!A.split) return;
     u = min(tile_u1, u_end);
@@ -816,18 +843,18 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
                        d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
                        reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0)};
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto nw, auto rg) -> int {
-    using C = PagedCfg<decltype(nw)::value, decltype(rg)::value>;
-    const auto kern = paged_mla_kernel<decltype(nw)::value, decltype(rg)::value>;
+  auto launch = [&](auto bm) -> int {
+    using C = PagedCfg<decltype(bm)::value>;
+    const auto kern = paged_mla_kernel<decltype(bm)::value>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), C::BYTES, "flash_paged_mla")) return rc;
-    hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(d.tiles)), dim3(C::kThreads), C::BYTES, st, args);
+    hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(d.tiles)), dim3(kPagedThreads), C::BYTES, st, args);
     if (int rc = check_launch("flash_paged_mla")) return rc;
     if (!d.split) return kOk;
     hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(512), dim3(256), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
     return check_launch("flash_paged_mla");
   };
   using std::integral_constant;
-  if (d.bm == 16) return launch(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  if (d.bm == 32) return launch(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-  return launch(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  if (d.bm == 16) return launch(integral_constant<int, 16>{});
+  if (d.bm == 32) return launch(integral_constant<int, 32>{});
+  return launch(integral_constant<int, 64>{});
 }
