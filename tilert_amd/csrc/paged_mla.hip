@@ -58,8 +58,8 @@ struct PagedCfg {
   static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;       // [PR] f32
   static constexpr int SREF_OFF = ROWL_OFF + PR * 4;        // f32 (and padding)
   static constexpr int FLAG_OFF = SREF_OFF + 16;            // [4] i32
-  static constexpr int SCAN_OFF = FLAG_OFF + 16;            // [8] i32
-  static constexpr int SEQ_OFF = SCAN_OFF + 32;             // [kPagedMaxTiles] i32: tiles up to sequence b and with it
+  static constexpr int SCAN_OFF = FLAG_OFF + 16;            // [24] i32
+  static constexpr int SEQ_OFF = SCAN_OFF + 96;             // [kPagedMaxTiles] i32: tiles up to sequence b and with it
   static constexpr int TILE_OFF = SEQ_OFF + kPagedMaxTiles * 4;  // [kPagedMaxTiles] i32: pages up to tile t and with it
   static constexpr int BYTES = TILE_OFF + kPagedMaxTiles * 4;
   static constexpr size_t kPartFloats = static_cast<size_t>(PR) * kKvLatent;
@@ -83,6 +83,7 @@ struct PagedArgs {
   const uint8_t* pages;
   PagedBatch p;
   int heads;
+  uint64_t per_head;  // ceil(2^40 / heads): x / heads = x * per_head >> 40 for x < 2^33
   float scale;  // softmax_scale * log2 e
   uint16_t* out;
   float* lse;
@@ -94,23 +95,22 @@ struct PagedArgs {
 
 // A sequence's row tiles and what they see, from untrusted metadata.
 struct SeqRows {
-  int first, n_tok;   // tokens
-  int64_t base;       // position of the first
-  __device__ inline SeqRows(const PagedBatch& p, int b) {
-    const int c0 = p.cu[b], c1 = p.cu[b + 1];
-    first = min(max(c0, 0), p.n_tokens);
-    const int end = min(max(c1, first), p.n_tokens);
-    n_tok = end - first;
-    base = static_cast<int64_t>(p.lens[b]) - c1 + first;
+  int first, n_rows;  // token, (token, head) rows
+  int64_t base;       // position of the first token
+  __device__ inline SeqRows(const PagedArgs& A, int b) {
+    const int c0 = A.p.cu[b], c1 = A.p.cu[b + 1];
+    first = min(max(c0, 0), A.p.n_tokens);
+    n_rows = (min(max(c1, first), A.p.n_tokens) - first) * A.heads;
+    base = static_cast<int64_t>(A.p.lens[b]) - c1 + first;
   }
-  __device__ inline int tiles(int heads, int bm) const { return (n_tok * heads + bm - 1) / bm; }
+  __device__ inline int tiles(int bm) const { return (n_rows + bm - 1) / bm; }
   // keys that the row'th row of the sequence sees
-  __device__ inline int seen(const PagedBatch& p, int row, int heads) const {
-    const int64_t n = base + row / heads + 1, most = min(static_cast<int64_t>(p.max_pages) * kKvPageKeys, static_cast<int64_t>(0x7fffffc0));
+  __device__ inline int seen(const PagedArgs& A, int row) const {
+    const int64_t n = base + static_cast<int>(row * A.per_head >> 40) + 1, most = static_cast<int64_t>(A.p.max_pages) * kKvPageKeys;  // <= 2^26
     return static_cast<int>(n < 0 ? 0 : (n > most ? most : n));
   }
-  __device__ inline int pages(const PagedBatch& p, int tile, int heads, int bm) const {
-    return (seen(p, min(n_tok * heads, (tile + 1) * bm) - 1, heads) + kKvPageKeys - 1) / kKvPageKeys;
+  __device__ inline int pages(const PagedArgs& A, int tile, int bm) const {
+    return (seen(A, min(n_rows, (tile + 1) * bm) - 1) + kKvPageKeys - 1) / kKvPageKeys;
   }
 };
 
@@ -139,6 +139,34 @@ __device__ inline int block_scan(int v, int* part, int& total) {
   }
   __syncthreads();
   return v + before;
+}
+
+// Inclusive sums of two values at once and their totals; whether `no` is false everywhere.
+__device__ inline bool block_scan2(int& a, int& b, bool no, int* part, int& total_a, int& total_b) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  a = wave_scan(a);
+  b = wave_scan(b);
+  const bool any = __any(no);
+  if (lane == 63) {
+    part[wave] = a;
+    part[8 + wave] = b;
+    part[16 + wave] = any;
+  }
+  __syncthreads();
+  int before_a = 0, before_b = 0, bad = 0;
+  total_a = total_b = 0;
+#pragma unroll
+  for (int w = 0; w < kPagedThreads / 64; ++w) {
+    const int x = part[w], y = part[8 + w];
+    before_a += w < wave ? x : 0;
+    before_b += w < wave ? y : 0;
+    total_a += x;
+    total_b += y;
+    bad |= part[16 + w];
+  }
+  a += before_a;
+  b += before_b;
+  return !bad;
 }
 
 // Max over each 16-lane row, in every lane of it.
@@ -202,9 +230,9 @@ __device__ inline void dma_words(const uint8_t* base, uint32_t off, uint32_t lds
 __device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
-  const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 32.0f, (x[1] - a[1]) * 32.0f, 0, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 32.0f, (x[3] - b[1]) * 32.0f, lo, true);
+  const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 32.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 32.0f, true);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_fmaf(x[0], 32.0f, -a[0]), __builtin_fmaf(x[1], 32.0f, -a[1]), 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_fmaf(x[2], 32.0f, -b[0]), __builtin_fmaf(x[3], 32.0f, -b[1]), lo, true);
 }
 
 template <int BM>
@@ -212,10 +240,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   using C = PagedCfg<BM>;
   constexpr int KG = C::KG, KT = C::KT, RT2 = C::RT2, DT = 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 63;
+  int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n16 = lane & 15, g = lane >> 4;
-  const int n32 = lane & 31, half = lane >> 5;
   const PagedBatch& p = A.p;
   int* seq_end = reinterpret_cast<int*>(smem + C::SEQ_OFF);
   int* unit_end = reinterpret_cast<int*>(smem + C::TILE_OFF);
@@ -232,29 +258,49 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   int n_tiles = 0, u = 0, u_end = 1, quota = 1, tile = 0, seq = 0, seq_tile0 = 0;
   if (A.split) {
     // units are pages of tiles (a tile that sees nothing counts one); every workgroup takes `quota` of them in a row
-    for (int b0 = 0; b0 < p.n_seqs; b0 += kPagedThreads) {
-      const int b = b0 + tid;
-      int total;
-      const int t = block_scan(b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), A.tile_cap) : 0, scan, total);
-      if (b < p.n_seqs) seq_end[b] = min(n_tiles + t, A.tile_cap);
-      n_tiles = min(n_tiles + total, A.tile_cap);
-    }
-    __syncthreads();
-    const int per = (n_tiles + kPagedThreads - 1) / kPagedThreads, t0 = tid * per, t1 = min(t0 + per, n_tiles);
-    int sum = 0;
-    if (t0 < t1) {
-      int b = upper(seq_end, p.n_seqs, t0);
-      SeqRows s(p, b);
-      for (int t = t0; t < t1; ++t) {
-        while (t >= seq_end[b]) s = SeqRows(p, ++b);
-        sum += max(1, s.pages(p, t - (b ? seq_end[b - 1] : 0), A.heads, BM));
-        unit_end[t] = sum;
+    int units;
+    bool done = false;
+    if (p.n_seqs <= kPagedThreads) {  // a decode step: where no sequence has two tiles, one pass does
+      int tiles = 0, pages = 0;
+      if (tid < p.n_seqs) {
+        const SeqRows s(A, tid);
+        tiles = min(s.tiles(BM), A.tile_cap);
+        pages = tiles ? max(1, s.pages(A, 0, BM)) : 0;
+      }
+      int t = tiles, q = pages;
+      done = block_scan2(t, q, tiles > 1, scan, n_tiles, units);
+      n_tiles = min(n_tiles, A.tile_cap);
+      if (tid < p.n_seqs) {
+        seq_end[tid] = min(t, A.tile_cap);
+        if (done && tiles && t <= A.tile_cap) unit_end[t - 1] = q;
+      }
+    } else {
+      for (int b0 = 0; b0 < p.n_seqs; b0 += kPagedThreads) {
+        const int b = b0 + tid;
+        int total;
+        const int t = block_scan(b < p.n_seqs ? min(SeqRows(A, b).tiles(BM), A.tile_cap) : 0, scan, total);
+        if (b < p.n_seqs) seq_end[b] = min(n_tiles + t, A.tile_cap);
+        n_tiles = min(n_tiles + total, A.tile_cap);
       }
     }
-    int units;
-    const int before = block_scan(sum, scan, units) - sum;
-    for (int t = t0; t < t1; ++t) unit_end[t] += before;
     __syncthreads();
+    if (!done) {
+      const int per = (n_tiles + kPagedThreads - 1) / kPagedThreads, t0 = tid * per, t1 = min(t0 + per, n_tiles);
+      int sum = 0;
+      if (t0 < t1) {
+        int b = upper(seq_end, p.n_seqs, t0);
+        SeqRows s(A, b);
+        for (int t = t0; t < t1; ++t) {
+          while (t >= seq_end[b]) s = SeqRows(A, ++b);
+          sum += max(1, s.pages(A, t - (b ? seq_end[b - 1] : 0), BM));
+          unit_end[t] = sum;
+        }
+      }
+      const int before = block_scan(sum, scan, units) - sum;
+      for (int t = t0; t < t1; ++t) unit_end[t] += before;
+      __syncthreads();
+    }
+    if (done) units = n_tiles ? unit_end[n_tiles - 1] : 0;  // (as many tiles as there is room for)
     units = __builtin_amdgcn_readfirstlane(units);
     quota = max(kPagedMinPages, (units + kPagedWgs - 1) / kPagedWgs);
     u = min(w * quota, units);
@@ -266,10 +312,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         const int first = tile ? unit_end[tile - 1] : 0;
         if (first < u && first >= u - quota) {  // the second workgroup on its first tile
           const int b = upper(seq_end, p.n_seqs, tile);
-          const SeqRows s(p, b);
+          const SeqRows s(A, b);
           const int j = tile - (b ? seq_end[b - 1] : 0);
           info.row0 = static_cast<int64_t>(s.first) * A.heads + static_cast<int64_t>(j) * BM;
-          info.rows = min(BM, s.n_tok * A.heads - j * BM);
+          info.rows = min(BM, s.n_rows - j * BM);
           info.parts = (unit_end[tile] - 1) / quota - first / quota + 1;
         }
       }
@@ -282,7 +328,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     for (int b0 = 0; b0 < p.n_seqs; b0 += kPagedThreads) {
       const int b = b0 + tid;
       int total;
-      const int mine = b < p.n_seqs ? min(SeqRows(p, b).tiles(A.heads, BM), static_cast<int>(gridDim.x)) : 0;
+      const int mine = b < p.n_seqs ? min(SeqRows(A, b).tiles(BM), static_cast<int>(gridDim.x)) : 0;
       const int t = n_tiles + block_scan(mine, scan, total);
       if (w >= t - mine && w < t) { scan[0] = b; scan[1] = t - mine; }
       __syncthreads();
@@ -294,6 +340,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   }
 
   while (u < u_end) {
+    // what follows from the lane is computed anew for each tile: taken out of this loop, it would fill the registers that
+    // the products need
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63;
+    const int n16 = lane & 15, g = lane >> 4;
+    const int n32 = lane & 31, half = lane >> 5;
     // ---- the tile: rows row0 .. row0 + rows - 1 of the call's (token, head) rows, pages pg0 .. pg0 + n - 1
     int tile_u0 = 0, tile_u1 = 1;
     if (A.split) {
@@ -304,14 +356,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     }
     seq = __builtin_amdgcn_readfirstlane(seq);
     seq_tile0 = __builtin_amdgcn_readfirstlane(seq_tile0);
-    const SeqRows s(p, seq);
+    const SeqRows s(A, seq);
     const int j = tile - seq_tile0;
     const int in_seq = j * BM;
     const int64_t row0 = static_cast<int64_t>(s.first) * A.heads + in_seq;
-    const int rows = min(BM, s.n_tok * A.heads - in_seq);
-    const int n_pages = s.pages(p, j, A.heads, BM);
-    const int seen_first = s.seen(p, in_seq, A.heads);             // every row sees these
-    const int seen_last = s.seen(p, in_seq + rows - 1, A.heads);   // some row sees these
+    const int rows = min(BM, s.n_rows - in_seq);
+    const int n_pages = s.pages(A, j, BM);
+    const int seen_first = s.seen(A, in_seq);             // every row sees these
+    const int seen_last = s.seen(A, in_seq + rows - 1);   // some row sees these
     const int pg0 = u - tile_u0;
     const int n = min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0);
     const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
@@ -372,26 +424,35 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     float f = 0.f;
     const int kg = wave % KG, rg = wave / KG;  // a scoring wave's keys and rows
     const int my_row = rg * 16 + n16;
+    u32x4p raws[RT2][5];
+    uint32_t largest[RT2];  // a row's largest magnitude's bits (bf16, upper half)
+    const int place = wave * 4 + g;
 #pragma unroll
     for (int round = 0; round < RT2; ++round) {
-      const int r = round * 32 + wave * 4 + g, place = wave * 4 + g;
-      const bool live = r < rows;
-      const int64_t row = row0 + (live ? r : 0);
-      u32x4p raw[5];
+      const int r = round * 32 + place;
+      const int64_t row = row0 + (r < rows ? r : 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = reinterpret_cast<const u32x4p*>(A.q_nope + row * kKvLatent)[n16 + 16 * i];
-      raw[4] = reinterpret_cast<const u32x4p*>(A.q_pe + row * kKvRope)[n16 & 7];
-      uint32_t most = 0;  // the largest magnitude's bits (bf16, upper half)
+      for (int i = 0; i < 4; ++i) raws[round][i] = reinterpret_cast<const u32x4p*>(A.q_nope + row * kKvLatent)[n16 + 16 * i];
+      raws[round][4] = reinterpret_cast<const u32x4p*>(A.q_pe + row * kKvRope)[n16 & 7];
+    }
+#pragma unroll
+    for (int round = 0; round < RT2; ++round) {
+      uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < 5; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) most = max(most, max(raw[i][c] & 0x7fff0000u, (raw[i][c] << 16) & 0x7fff0000u));
-      most = row16_max_u32(most);
-      __builtin_amdgcn_sched_barrier(0);
-      if (round == 0) {
-        if (n > 0) fetch(0, 0);
-        if (n > 1) fetch(1, 1);
-      }
+        for (int c = 0; c < 4; ++c) most = max(most, max(raws[round][i][c] & 0x7fff0000u, (raws[round][i][c] << 16) & 0x7fff0000u));
+      largest[round] = row16_max_u32(most);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (n > 0) fetch(0, 0);
+    if (n > 1) fetch(1, 1);
+#pragma unroll
+    for (int round = 0; round < RT2; ++round) {
+      const int r = round * 32 + place;
+      const bool live = r < rows;
+      const u32x4p (&raw)[5] = raws[round];
+      const uint32_t most = largest[round];
       const bool bad = most >= 0x7f800000u;  // a NaN or an infinity: every output of the row is NaN
       const bool zero = bad || !live;
       const int e = zero ? 0 : max(static_cast<int>(most >> 23) - 127 - 7, -120);  // sigma = 2^e
@@ -452,7 +513,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       const int at_code = my_key * kKvLatent + ((2 * g) ^ (my_key & 7)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31)
       const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (my_key & 7)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
       const int put_p = my_row * kPStride + my_quad;
-      const int seen = my_row < rows ? s.seen(p, in_seq + my_row, A.heads) : 0;
+      const int seen = my_row < rows ? s.seen(A, in_seq + my_row) : 0;
       float m = -INFINITY, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f, kf = 0.f;
       if (f != f) f = 0.f;
       v4f U[KT];
@@ -719,64 +780,102 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   }
 }
 
-// The split tiles' partial sums joined.  An item is 32 rows x 4 dims of a tile: lane n32 a row, the eight half-waves the
-// parts in turn, joined in LDS in a fixed order.
+// The split tiles' partial sums joined, in a fixed order.  An item is 32 rows x 64 / G dims of a tile: a thread takes one
+// row, 4 dims and every G'th part, so that it has few parts (up to eight, all their loads in flight together; a
+// context split over all workgroups: sixteen), and the G half-waves of the same dims are joined in LDS.
+constexpr int kCombineThreads = 512, kHalfWaves = kCombineThreads / 32;
+__device__ inline int part_groups(int parts) { return parts <= 8 ? 1 : (parts <= 16 ? 2 : (parts <= 32 ? 4 : (parts <= 64 ? 8 : 16))); }
 template <int PR>
-__global__ __launch_bounds__(256) void paged_mla_combine_kernel(const SplitTile* __restrict__ split, const float2* __restrict__ part_ml,
-                                                                const float* __restrict__ part_o, uint16_t* __restrict__ out,
-                                                                float* __restrict__ lse) {
-  __shared__ int list[kPagedWgs], count[4];
-  __shared__ float top[8][32], sums[8][32];
-  __shared__ v4f acc[8][32];
+__global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(const SplitTile* __restrict__ split,
+                                                                            const float2* __restrict__ part_ml,
+                                                                            const float* __restrict__ part_o,
+                                                                            uint16_t* __restrict__ out, float* __restrict__ lse) {
+  __shared__ int item_end[kPagedWgs], count[4];
+  __shared__ float top[kHalfWaves][32], sums[kHalfWaves][32];
+  __shared__ v4f acc[kHalfWaves][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  static_assert(kPagedWgs == 256, "one thread a workgroup of the split launch");
-  const uint64_t mine = __ballot(split[tid].parts > 1);
-  if (lane == 0) count[wave] = __popcll(mine);
+  static_assert(kPagedWgs == 256, "four waves' scan");
+  const int parts = tid < kPagedWgs ? split[tid].parts : 0;
+  const int mine = wave_scan(parts < 2 ? 0 : (PR / 32) * 8 * part_groups(parts));
+  if (lane == 63 && wave < 4) count[wave] = mine;
   __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { before += i < wave ? count[i] : 0; total += count[i]; }
-  if (mine >> lane & 1) list[before + __popcll(mine & ((1ull << lane) - 1))] = tid;
+  const int e0 = count[0], e1 = e0 + count[1], e2 = e1 + count[2], total = e2 + count[3];
+  if (static_cast<int>(blockIdx.x) >= total) return;
+  if (wave < 4) item_end[tid] = mine + (wave == 0 ? 0 : (wave == 1 ? e0 : (wave == 2 ? e1 : e2)));
   __syncthreads();
-  constexpr int kItems = PR / 32 * 128;  // of a tile
-  const int n32 = tid & 31, part0 = tid >> 5;
-  for (int item = blockIdx.x; item < total * kItems; item += gridDim.x) {
-    const int w = list[item / kItems], a = item % kItems / 128, d4 = item % 128;
-    const SplitTile t = split[w];
-    const int r = a * 32 + n32;
-    const bool live = r < t.rows;
-    // part i: workgroup w - 1's slot 1, then the slots 0 of w, w + 1, ...
-    float mx = -INFINITY;
-    if (live)
-      for (int i = part0; i < t.parts; i += 8)
-        mx = fmaxf(mx, part_ml[static_cast<int64_t>(i ? 2 * (w + i - 1) : 2 * w - 1) * PR + r].x);
-    top[part0][n32] = mx;
-    __syncthreads();
+  const int n32 = tid & 31, hw = tid >> 5;
+  // part i of the tile that workgroup w continues: workgroup w - 1's slot 1, then the slots 0 of w, w + 1, ...
+  auto slot_of = [](int w, int i) -> int64_t { return i ? 2 * (w + i - 1) : 2 * w - 1; };
+  auto sums_at = [&](int64_t slot, int a, int d4) {  // dims 4 d4 .. +3: 32-dim tile d4 / 8, group (d4 % 8) / 2 of 8 dims, half d4 % 2
+    return reinterpret_cast<const v4f*>(part_o + slot * (static_cast<int64_t>(PR) * kKvLatent))[((a * 16 + d4 / 8) * 4 + (d4 % 8) / 2) * 64 + (d4 & 1) * 32 + n32];
+  };
+  auto store = [&](int64_t row, int d4, const v4f& o, float l, float mx) {
+    const float x = l == 0.f ? 0.f : 1.0f / l;
+    *reinterpret_cast<u32x2p*>(out + row * kKvLatent + 4 * d4) = u32x2p{bf16x2_bits(v2f{o[0] * x, o[1] * x}), bf16x2_bits(v2f{o[2] * x, o[3] * x})};
+    if (lse && d4 == 0) lse[row] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
+  };
+  // N parts i0, i0 + step, .. below `end`, added to (mx, l, o); their loads are all in flight together
+  auto add = [&](auto count_tag, int w, int a, int d4, int r, int i0, int step, int end, float& mx, float& l, v4f& o) {
+    constexpr int N = decltype(count_tag)::value;
+    float2 ml[N];
+    v4f x[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, top[i][n32]);
-    v4f o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (live)
-      for (int i = part0; i < t.parts; i += 8) {
-        const int64_t slot = i ? 2 * (w + i - 1) : 2 * w - 1;
-        const float2 ml = part_ml[slot * PR + r];
-        const float x = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-        l += ml.x == -INFINITY ? ml.y : ml.y * x;  // (0, or a bad row's NaN)
-        // dims 4 d4 .. +3: 32-dim tile d4 / 8, group (d4 % 8) / 2 of 8 dims, half d4 % 2
-        o += reinterpret_cast<const v4f*>(part_o + slot * (static_cast<int64_t>(PR) * kKvLatent))[((a * 16 + d4 / 8) * 4 + (d4 % 8) / 2) * 64 + (d4 & 1) * 32 + n32] * x;
-      }
-    sums[part0][n32] = l;
-    acc[part0][n32] = o;
-    __syncthreads();
-    if (part0 == 0 && live) {
-#pragma unroll
-      for (int i = 1; i < 8; ++i) { l += sums[i][n32]; o += acc[i][n32]; }
-      const float x = l == 0.f ? 0.f : 1.0f / l;
-      const int64_t row = t.row0 + r;
-      *reinterpret_cast<u32x2p*>(out + row * kKvLatent + 4 * d4) = u32x2p{bf16x2_bits(v2f{o[0] * x, o[1] * x}), bf16x2_bits(v2f{o[2] * x, o[3] * x})};
-      if (lse && d4 == 0) lse[row] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
+    for (int i = 0; i < N; ++i) {
+      const int64_t slot = slot_of(w, min(i0 + i * step, end - 1));
+      ml[i] = part_ml[slot * PR + r];
+      x[i] = sums_at(slot, a, d4);
     }
-    __syncthreads();
+    float top = mx;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, i0 + i * step < end ? ml[i].x : -INFINITY);
+    const float keep = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mx - top);  // (0, or a bad row's NaN, before the first)
+    l *= keep;
+    o *= keep;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i0 + i * step >= end) continue;
+      const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - top);
+      l += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * f;
+      o += x[i] * f;
+    }
+    mx = top;
+  };
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    const int w = upper(item_end, kPagedWgs, item);
+    const SplitTile t = split[w];
+    const int groups = part_groups(t.parts), dims = kHalfWaves / groups;  // float4s of dims an item
+    const int at = item - (w ? item_end[w - 1] : 0), items = 8 * groups;    // items of 32 rows
+    const int a = at / items, d4 = at % items * dims + hw % dims, part0 = hw / dims, r = a * 32 + n32;
+    const bool live = r < t.rows;
+    float mx = -INFINITY, l = 0.f;
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      const int each = (t.parts + groups - 1) / groups;
+      if (each <= 2) add(std::integral_constant<int, 2>{}, w, a, d4, r, part0, groups, t.parts, mx, l, o);
+      else if (each <= 4) add(std::integral_constant<int, 4>{}, w, a, d4, r, part0, groups, t.parts, mx, l, o);
+      else
+#pragma unroll 1
+        for (int i = part0; i < t.parts; i += 8 * groups)
+          add(std::integral_constant<int, 8>{}, w, a, d4, r, i, groups, t.parts, mx, l, o);
+    }
+    if (groups > 1) {
+      top[hw][n32] = mx;
+      sums[hw][n32] = l;
+      acc[hw][n32] = o;
+      __syncthreads();
+      if (part0 == 0 && live) {
+        for (int i = hw + dims; i < kHalfWaves; i += dims) mx = fmaxf(mx, top[i][n32]);
+        l = 0.f;
+        o = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int i = hw; i < kHalfWaves; i += dims) {
+          const float f = top[i][n32] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[i][n32] - mx);
+          l += top[i][n32] == -INFINITY ? sums[i][n32] : sums[i][n32] * f;
+          o += acc[i][n32] * f;
+        }
+      }
+      __syncthreads();
+    }
+    if (part0 == 0 && live) store(t.row0 + r, d4, o, l, mx);
   }
 }
 
@@ -839,7 +938,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const PagedArgs args{(const uint16_t*)q_nope_bf16, (const uint16_t*)q_pe_bf16, (const uint8_t*)kv_pages,
                        PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
-                       (int)heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
+                       (int)heads, ((1ull << 40) + heads - 1) / heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
                        d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
                        reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0)};
   const hipStream_t st = (hipStream_t)stream;
@@ -850,7 +949,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
     hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(d.tiles)), dim3(kPagedThreads), C::BYTES, st, args);
     if (int rc = check_launch("flash_paged_mla")) return rc;
     if (!d.split) return kOk;
-    hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(512), dim3(256), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
+    hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(512), dim3(kCombineThreads), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
     return check_launch("flash_paged_mla");
   };
   using std::integral_constant;
