@@ -35,8 +35,8 @@ constexpr int kPagedMinPages = 1;     // pages a workgroup takes at least
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
 constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
-constexpr float kP = 32.0f;          // p * scale / s_ref is held at kP at most when m and s_ref were last set,
-constexpr float kPMost = 256.0f;     // and at kPMost until they are set again
+constexpr float kP = 32.0f;          // a weight times key scale is kP at most when m and s_ref are set,
+constexpr float kPMost = 256.0f;     // and kPMost until they are set again
 constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
 
 // Eight waves, two on a SIMD: 0 .. 3 score, 4 .. 7 multiply.  Scoring wave w takes the 16 rows of group w / KG against the
@@ -56,8 +56,7 @@ struct PagedCfg {
   static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;      // [KG][BM] f32
   static constexpr int ALPHA_OFF = STAT_OFF + KG * BM * 4;  // [PR] f32
   static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;       // [PR] f32
-  static constexpr int SREF_OFF = ROWL_OFF + PR * 4;        // f32 (and padding)
-  static constexpr int FLAG_OFF = SREF_OFF + 16;            // [4] i32
+  static constexpr int FLAG_OFF = ROWL_OFF + PR * 4;        // [4] i32
   static constexpr int SCAN_OFF = FLAG_OFF + 16;            // [24] i32
   static constexpr int SEQ_OFF = SCAN_OFF + 96;             // [kPagedMaxTiles] i32: tiles up to sequence b and with it
   static constexpr int TILE_OFF = SEQ_OFF + kPagedMaxTiles * 4;  // [kPagedMaxTiles] i32: pages up to tile t and with it
@@ -249,7 +248,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   float* stat = reinterpret_cast<float*>(smem + C::STAT_OFF);
   float* alpha_l = reinterpret_cast<float*>(smem + C::ALPHA_OFF);
   float* rowl = reinterpret_cast<float*>(smem + C::ROWL_OFF);
-  float* sref_l = reinterpret_cast<float*>(smem + C::SREF_OFF);
   int* flag = reinterpret_cast<int*>(smem + C::FLAG_OFF);
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8_ptr)smem));
   const int w = blockIdx.x;
@@ -368,24 +366,27 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     const int n = min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0);
     const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
 
-    // page k of the tile into its slot, in 1 KB pieces: 32 of codes, four at a time, and 8 of rope parts; every wave
-    // also fetches the scales, all of them the same.  A 16-byte chunk c of a row is kept at c ^ (row & 7), so
+    // the page `id` into a slot, by the multiplying waves, in 1 KB pieces: 32 of codes, four at a time, and 8 of rope
+    // parts; each also fetches the scales, all of them the same.  A 16-byte chunk c of a row is kept at c ^ (row & 7), so
     // that the rows' chunks that a read takes together are in different banks
-    auto fetch = [&](int k, int slot) {
-      int id = table[k];
-      if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.n_pages)) id = 0;  // its keys are masked
+    auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.n_pages); };
+    auto fetch = [&](int id, int slot) {
+      if (!valid(id)) id = 0;  // its keys are masked
       const uint8_t* page = A.pages + static_cast<int64_t>(id) * kKvPageBytes;
       const uint32_t to = lds0 + slot * kSlotBytes;
+      const int piece = (wave - 4) * 8;
       const uint32_t code = half * 512 + (n32 ^ half) * 16;  // rows 2 i, 2 i + 1 of piece i
       const uint32_t off[4] = {code, code ^ 32, code ^ 64, code ^ 96};
-      dma_pieces<4>(page + wave * 4096, off, to + wave * 4096);
-      const uint32_t rope[1] = {static_cast<uint32_t>((lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16)};
-      dma_pieces<1>(page + kKvRopeAt + wave * 1024, rope, to + kKvPageKeys * kKvLatent + wave * 1024);
+      dma_pieces<4>(page + piece * 1024, off, to + piece * 1024);
+      dma_pieces<4>(page + piece * 1024 + 4096, off, to + piece * 1024 + 4096);
+      const uint32_t part = (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
+      const uint32_t rope[2] = {part, part};
+      dma_pieces<2>(page + kKvRopeAt + piece * 256, rope, to + kKvPageKeys * kKvLatent + piece * 256);
       dma_words(page + kKvScaleAt, lane * 4, lds0 + C::SCALE_OFF + slot * kKvPageKeys * 4);
     };
-    auto masked = [&](int k) {
-      return (pg0 + k + 1) * kKvPageKeys > seen_first || static_cast<uint32_t>(table[k]) >= static_cast<uint32_t>(p.n_pages);
-    };
+    // whether some row does not see all of page k; an id that is not valid is one whose keys nobody sees
+    auto masked = [&](int k, int id) { return (pg0 + k + 1) * kKvPageKeys > seen_first || !valid(id); };
+    auto id_of = [&](int k) { return table[min(k, n - 1)]; };
     // every wave's part of a fetch has arrived, and what it wrote to LDS is there
     auto arrive = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -445,8 +446,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       largest[round] = row16_max_u32(most);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (n > 0) fetch(0, 0);
-    if (n > 1) fetch(1, 1);
+    const int id0 = n > 0 ? id_of(0) : 0, id1 = n > 0 ? id_of(1) : 0;
+    if (wave >= 4) {
+      if (n > 0) fetch(id0, 0);
+      if (n > 1) fetch(id1, 1);
+    }
 #pragma unroll
     for (int round = 0; round < RT2; ++round) {
       const int r = round * 32 + place;
@@ -514,7 +518,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (my_key & 7)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
       const int put_p = my_row * kPStride + my_quad;
       const int seen = my_row < rows ? s.seen(A, in_seq + my_row) : 0;
-      float m = -INFINITY, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f, kf = 0.f;
+      // weights are e = exp2(U * f - mk), mk = m - log2(kP / s_ref): m the row's largest U * f and s_ref the largest
+      // key scale when they were last set, so that e * scale <= kP then.  l and O are sums of such e and need no
+      // s_ref in the end.
+      float m = -INFINITY, mk = 0.f, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f;
       if (f != f) f = 0.f;
       v4f U[KT];
 
@@ -523,8 +530,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i % 4) * 128;
         return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
       };
-      auto scores = [&](int k, int slot) {
-        constexpr int kItems = 4 * KT, kAhead = 4;
+      auto scores = [&](int slot) {
+        constexpr int kItems = 4 * KT, kAhead = kItems < 6 ? kItems : 6;
         v8i a[kItems];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
@@ -550,29 +557,29 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           for (int ks = 0; ks < 2; ++ks) x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(r[ks], qr[ks], x, 0, 0, 0);
           U[kt] = x;
         }
-        if (masked(k)) {
-          const bool there = static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
-          const int at = (pg0 + k) * kKvPageKeys + my_quad;
+      };
+      // the scores of page k that the row does not see
+      auto mask_scores = [&](int k, int id) {
+        const int at = (pg0 + k) * kKvPageKeys + my_quad, end = valid(id) ? seen : 0;
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) U[kt][i] = there && at + kt * 16 + i < seen ? U[kt][i] : -INFINITY;
-        }
+          for (int i = 0; i < 4; ++i) U[kt][i] = at + kt * 16 + i < end ? U[kt][i] : -INFINITY;
       };
 
-      // P of page k from U, m and s_ref: codes to buffer k % 2, psum; whether all were <= kPMost
-      auto weights = [&](int k, int slot) {
+      // P of page k from U, mk: codes to buffer k % 2, psum; whether all were <= kPMost
+      auto weights = [&](int k, int slot, auto mask) {
+        constexpr bool MASK = decltype(mask)::value;
         uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p;
-        const float mu = m == -INFINITY ? 0.f : m;
         float pmax = 0.f, sum = 0.f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-          const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4) * kf;
+          const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
           float x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool none = U[kt][i] == -INFINITY;  // a masked key's scale may be anything
-            const float e = none ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mu));
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mk));
+            const bool none = MASK && U[kt][i] == -INFINITY;  // a masked key's scale may be anything
             sum += e;
             x[i] = none ? 0.f : e * sk[i];
             pmax = fmaxf(pmax, __builtin_fabsf(x[i]));
@@ -587,7 +594,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       };
 
       // New m and s_ref from page k's scores, O and l brought to them, P again.  Every wave comes here, or none.
-      auto settle = [&](int k, int slot) {
+      auto settle = [&](int k, int slot, int id) {
         float x = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(fmaxf(U[kt][0], U[kt][1]), fmaxf(U[kt][2], U[kt][3])));
@@ -596,49 +603,55 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         if (KG > 1 && g == 0) stat[kg * BM + my_row] = x;
         // the largest finite scale of the page's keys that some row sees
         const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + slot * kKvPageKeys * 4)[lane]);
-        const bool use = (pg0 + k) * kKvPageKeys + lane < seen_last && sk < INFINITY &&
-                         static_cast<uint32_t>(table[k]) < static_cast<uint32_t>(p.n_pages);
-        const float most = fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f);
-        const float ratio = s_ref > 0.f ? s_ref / fmaxf(s_ref, most) : 0.f;
-        s_ref = fmaxf(s_ref, most);
-        kf = kP / s_ref;
-        if (tid == 0) *sref_l = s_ref;
+        const bool use = (pg0 + k) * kKvPageKeys + lane < seen_last && sk < INFINITY && valid(id);
+        s_ref = fmaxf(s_ref, fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f));
         __syncthreads();
         if constexpr (KG > 1)
 #pragma unroll
           for (int i = 0; i < KG; ++i) x = fmaxf(x, stat[i * BM + my_row]);
-        const float mn = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
-        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= m == -INFINITY ? 1.0f : a;  // (0, or a bad row's NaN, before the first key)
-        m = mn;
-        if (kg == 0 && g == 0) alpha_l[my_row] = a * ratio;
-        weights(k, slot);
+        const float was = mk;
+        const bool none = m == -INFINITY;
+        m = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
+        mk = m == -INFINITY ? 0.f : m - __builtin_amdgcn_logf(kP / s_ref);  // (base 2)
+        const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(was - mk);
+        l *= alpha;
+        if (kg == 0 && g == 0) alpha_l[my_row] = alpha;
+        weights(k, slot, std::true_type{});
         __syncthreads();
       };
 
       if (n > 0) {
         arrive();
-        if (masked(0)) clean(0);
-        scores(0, 0);
-        settle(0, 0);
-        int next = 1, free = 2, slot = 0;
+        if (masked(0, id0)) clean(0);
+        scores(0);
+        if (masked(0, id0)) mask_scores(0, id0);
+        settle(0, 0, id0);
+        int next = 1, free = 2, slot = 0, id = id1, id_after = id_of(2);
 #pragma unroll 1
-        for (int k = 0; k < n; ++k) {
+        for (int k = 0; k + 1 < n; ++k) {  // id: page k + 1's
           l += psum;
-          if (k + 2 < n) fetch(k + 2, free);
-          if (k + 1 < n) {
-            if (tid == 0) flag[(k + 2) & 3] = tid;  // (0, without a register that holds it)
-            if (masked(k + 1)) clean(next);
-            scores(k + 1, next);
-            if (!weights(k + 1, next) && lane == 0) flag[(k + 1) & 3] = 1;
-            arrive();
-            if (flag[(k + 1) & 3]) settle(k + 1, next);
+          if (tid == 0) flag[(k + 2) & 3] = tid;  // (0, without a register that holds it)
+          bool fits;
+          if (masked(k + 1, id)) {
+            clean(next);
+            scores(next);
+            mask_scores(k + 1, id);
+            fits = weights(k + 1, next, std::true_type{});
+          } else {
+            scores(next);
+            fits = weights(k + 1, next, std::false_type{});
           }
+          if (!fits && lane == 0) flag[(k + 1) & 3] = 1;
+          arrive();
+          if (flag[(k + 1) & 3]) settle(k + 1, next, id);
+          id = id_after;
+          id_after = id_of(k + 3);
           const int was = slot;
           slot = next;
           next = free;
           free = was;
         }
+        l += psum;
       }
       // l over the lanes and waves of a row
       __syncthreads();
@@ -646,7 +659,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       l += __shfl_xor(l, 32);
       if (g == 0) {
         stat[kg * BM + my_row] = l;
-        if (kg == 0) alpha_l[my_row] = m;
+        if (kg == 0) alpha_l[my_row] = m == -INFINITY ? -INFINITY : mk;
       }
       __syncthreads();
       if (tid < BM) {
@@ -716,30 +729,30 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 
       if (n > 0) {
         arrive();
-        if (masked(0)) clean(0);
+        if (masked(0, id0)) clean(0);
         settle(true);
-        int next = 1, free = 2, slot = 0;
+        int next = 1, free = 2, slot = 0, id = id1, id_after = id_of(2);
 #pragma unroll 1
-        for (int k = 0; k < n; ++k) {
-          if (k + 2 < n) fetch(k + 2, free);
-          if (k + 1 < n && masked(k + 1)) clean(next);
+        for (int k = 0; k + 1 < n; ++k) {  // id: page k + 1's
+          if (k + 2 < n) fetch(id_after, free);
+          if (masked(k + 1, id)) clean(next);
+          id = id_after;
+          id_after = id_of(k + 3);
           product(k, slot);
-          if (k + 1 < n) {
-            arrive();
-            if (flag[(k + 1) & 3]) settle(false);
-          }
+          arrive();
+          if (flag[(k + 1) & 3]) settle(false);
           const int was = slot;
           slot = next;
           next = free;
           free = was;
         }
+        product(n - 1, slot);
       }
       __syncthreads();
       __syncthreads();
       __syncthreads();
 
       // ---- the rows' results, or the tile's partial sums
-      const float s_ref = n > 0 ? *sref_l : 0.f;
       if (!A.split || (u == tile_u0 && u_end >= tile_u1)) {
         const int t = tid - 256;
         if (A.lse && t < rows) A.lse[row0 + t] = rowl[t] == 0.f ? -INFINITY : (alpha_l[t] + log2f(rowl[t])) * 0.6931471805599453f;
@@ -747,7 +760,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         for (int a = 0; a < RT2; ++a) {
           const int r = a * 32 + n32;
           if (r < rows) {
-            const float L = rowl[r], x = L == 0.f ? 0.f : s_ref / (kP * L);
+            const float L = rowl[r], x = L == 0.f ? 0.f : 1.0f / L;
             uint16_t* dst = A.out + (row0 + r) * kKvLatent + dw * 128 + 4 * half;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -760,7 +773,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       } else {
         const int slot = 2 * w + (u == tile_u0 ? 1 : 0), t = tid - 256;
         if (t < rows) A.part_ml[static_cast<int64_t>(slot) * C::PR + t] = float2{alpha_l[t], rowl[t]};
-        const float x = s_ref / kP;
         v4f* dst = reinterpret_cast<v4f*>(A.part_o + static_cast<int64_t>(slot) * C::kPartFloats);
 #pragma unroll
         for (int a = 0; a < RT2; ++a)
@@ -770,7 +782,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 dst[((a * 16 + dw * DT + d) * 4 + i) * 64 + lane] =
-                    v4f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x, o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x};
+                    v4f{o[a][d][4 * i], o[a][d][4 * i + 1], o[a][d][4 * i + 2], o[a][d][4 * i + 3]};
           }
       }
     }
