@@ -53,7 +53,8 @@ CASES = [  # new tokens, cache lengths, heads, padding
     ([7], [70], 3, 0), ([33], [40], 16, 0), ([1], [4000], 16, 0), ([2], [5000], 128, 0), ([257], [700], 16, 5),
     ([64], [64], 20, 0), ([1, 1, 1], [10, 200, 64], 16, 0), ([1, 5, 0, 40, 1], [90, 5, 33, 400, 1], 16, 3),
     ([0, 0, 3], [0, 9, 64], 8, 1), ([1] * 70, list(range(1, 211, 3)), 16, 4), ([100, 1, 1], [130, 3000, 1], 20, 0),
-    ([1] * 5, [64 * i for i in range(1, 6)], 128, 0), ([500], [1500], 8, 0),
+    ([1] * 5, [64 * i for i in range(1, 6)], 128, 0), ([500], [1500], 8, 0), ([1], [40000], 16, 0), ([3], [30000], 8, 0),
+    ([4], [30000], 16, 0), ([700, 300], [2000, 2500], 16, 0), ([1] * 40, [100 * i + 1 for i in range(40)], 16, 0),
 ]
 
 
@@ -113,6 +114,25 @@ def test_pages_outside_the_pool_are_not_seen(cuda, new):
     out, lse = run(cuda, q, qp, pages, table, cu, lens)
     check(cuda, q, qp, pages, table, cu, lens, out, lse)
     assert torch.isneginf(lse[2 * new:]).all()
+
+
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_bad_pages_among_many(cuda, new):
+    """Enough pages that a workgroup takes several, bad ones first, last and between them, also the first pages of a cache."""
+    total = [4000, 5000, 3500] if new > 4 else [12000, 9000, 15000]
+    pages, table, cu, lens, rows = _paged.batch([new] * 3, total, seed=59)
+    _paged.fill(pages, table, total)
+    g = torch.Generator().manual_seed(61)
+    for b, n in enumerate(total):
+        need = -(-n // 64)
+        bad = torch.randperm(need, generator=g)[:need // 3]
+        table[b, bad] = torch.where(bad % 2 == 0, -1, pages.shape[0]).to(torch.int32)
+        table[b, :4] = -1
+    table[2, :-(-total[2] // 64) - 1] = -3  # one page is left, the last
+    q, qp = queries(rows, 16, 63)
+    out, lse = run(cuda, q, qp, pages, table, cu, lens)
+    check(cuda, q, qp, pages, table, cu, lens, out, lse)
+    assert torch.isfinite(out).all()
 
 
 @pytest.mark.parametrize("new", [1, 40])

@@ -612,7 +612,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         const float was = mk;
         const bool none = m == -INFINITY;
         m = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
-        mk = m == -INFINITY ? 0.f : m - __builtin_amdgcn_logf(kP / s_ref);  // (base 2)
+        mk = m == -INFINITY ? -300.f : m - __builtin_amdgcn_logf(kP / s_ref);  // (base 2; with no score yet, any one is flagged)
         const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(was - mk);
         l *= alpha;
         if (kg == 0 && g == 0) alpha_l[my_row] = alpha;
@@ -627,6 +627,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         if (masked(0, id0)) mask_scores(0, id0);
         settle(0, 0, id0);
         int next = 1, free = 2, slot = 0, id = id1, id_after = id_of(2);
+        bool fresh = !valid(id0);  // no page so far had keys: nothing is set yet
 #pragma unroll 1
         for (int k = 0; k + 1 < n; ++k) {  // id: page k + 1's
           l += psum;
@@ -641,7 +642,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
             scores(next);
             fits = weights(k + 1, next, std::false_type{});
           }
-          if (!fits && lane == 0) flag[(k + 1) & 3] = 1;
+          if ((!fits || fresh) && lane == 0) flag[(k + 1) & 3] = 1;
+          fresh = fresh && !valid(id);
           arrive();
           if (flag[(k + 1) & 3]) settle(k + 1, next, id);
           id = id_after;
