@@ -473,11 +473,13 @@ int tl_mla_cache_read(const void* kv_pages, int64_t n_pages, const int32_t* bloc
  *   s[j] = (q_nope . latent[j] + q_pe . rope[j]) * softmax_scale,  out = softmax(s) . latent
  * out bf16 [n_tokens, heads, 512], lse fp32 [n_tokens, heads] (nullable) = ln sum e^s; 0 and
  * -inf where no key is seen.  fp32 scores, statistics and sums; probabilities times key
- * scales are rounded to bf16.  1 <= heads <= 128, n_tokens * heads < 2^31; q and out 16-byte
- * aligned.  workspace: tl_flash_paged_mla_workspace_bytes bytes (0: none), 16-byte aligned, its
+ * scales are rounded as to bf16.  1 <= heads <= 128, n_tokens * heads < 2^26, n_seqs and
+ * max_pages <= 2^20; q and out 16-byte aligned.  workspace: the bytes that
+ * tl_flash_paged_mla_workspace_bytes names for these sizes (0: none), 16-byte aligned, its
  * contents of no account before or after; calls that overlap in time need one each.  The
  * dense form of flash_sparse_mla_op (ops/flash_sparse_mla.py:18-93). */
-size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads);
+size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads,
+                                          int64_t max_pages);
 int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const void* kv_pages, int64_t n_pages,
                        const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
                        const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t heads,

@@ -88,7 +88,7 @@ SIGNATURES: dict[str, tuple] = {
                                   _i64, _c_void_p, _c_void_p, ctypes.c_float, _int, _int, _c_void_p]),
     "tl_mla_cache_read": (_int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p,
                                  _c_void_p, _c_void_p]),
-    "tl_flash_paged_mla_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "tl_flash_paged_mla_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
     "tl_flash_paged_mla": (_int, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _i64,
                                   _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
     "tl_rmsnorm_projq_wqb": (_int, [_c_void_p, _c_void_p, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p,

@@ -29,9 +29,13 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
 
-constexpr int kPagedWgs = 256;      // workgroups of a split launch: one per CU
+constexpr int kPagedWgs = 256;        // workgroups of a split launch: one per CU
 constexpr int kPagedMaxTiles = 1024;  // tiles (and sequences) that a split launch plans in LDS
-constexpr int kPagedMinPages = 1;     // pages a workgroup takes at least
+constexpr int64_t kPagedMaxRows = 1 << 26;  // (token, head) rows: sums of 512 sequences' tiles, of 32 rows then, stay below 2^31
+// Pages that a sequence can have (a table's width), up to which no tile is split: one token, 16 heads, 512 keys take
+// 14.2 us in one workgroup and 8.5 + 4.6 us over eight and with the join, and the second launch costs the caller 4 us
+// (10.1 against 14.5 us a call); from there on the page loop, 1.0 us a page, decides.
+constexpr int kPagedFew = 8;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
 constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
@@ -82,7 +86,7 @@ struct PagedArgs {
   const uint8_t* pages;
   PagedBatch p;
   int heads;
-  uint64_t per_head;  // ceil(2^40 / heads): x / heads = x * per_head >> 40 for x < 2^33
+  uint64_t per_head;  // ceil(2^34 / heads): x / heads = x * per_head >> 34 for x < 2^34 / heads, so for every row
   float scale;  // softmax_scale * log2 e
   uint16_t* out;
   float* lse;
@@ -105,7 +109,7 @@ struct SeqRows {
   __device__ inline int tiles(int bm) const { return (n_rows + bm - 1) / bm; }
   // keys that the row'th row of the sequence sees
   __device__ inline int seen(const PagedArgs& A, int row) const {
-    const int64_t n = base + static_cast<int>(row * A.per_head >> 40) + 1, most = static_cast<int64_t>(A.p.max_pages) * kKvPageKeys;  // <= 2^26
+    const int64_t n = base + static_cast<int>(row * A.per_head >> 34) + 1, most = static_cast<int64_t>(A.p.max_pages) * kKvPageKeys;  // <= 2^26
     return static_cast<int>(n < 0 ? 0 : (n > most ? most : n));
   }
   __device__ inline int pages(const PagedArgs& A, int tile, int bm) const {
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     }
     if (done) units = n_tiles ? unit_end[n_tiles - 1] : 0;  // (as many tiles as there is room for)
     units = __builtin_amdgcn_readfirstlane(units);
-    quota = max(kPagedMinPages, (units + kPagedWgs - 1) / kPagedWgs);
+    quota = max(1, (units + kPagedWgs - 1) / kPagedWgs);
     u = min(w * quota, units);
     u_end = min(u + quota, units);
     tile = __builtin_amdgcn_readfirstlane(upper(unit_end, n_tiles, u));
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
       };
       auto scores = [&](int slot) {
-        constexpr int kItems = 4 * KT, kAhead = kItems < 6 ? kItems : 6;
+        constexpr int kItems = 4 * KT, kAhead = kItems < 4 ? kItems : 4;  // (8: 962 -> 979 us at 2048 tokens, 16 heads, 16384 keys; 6: 970)
         v8i a[kItems];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
@@ -893,20 +897,27 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
   }
 }
 
-// The launch: rows a tile, whether tiles are split, and the workspace.
+// The launch: rows a tile, whether tiles are split, and the workspace.  More rows a tile read a page for more rows at
+// once, and for 64 rows both 32-row products of a multiplying wave share its read of the page; fewer rows have their
+// queries split and their sums written in less time and waste less where a sequence's rows end.  Measured, for the rows
+// that a sequence has on average, in us with 16 / 32 / 64 rows a tile:
+//   16 rows (60 sequences, up to 32768 keys)          101 / 102 / 121;   (1 sequence, 500 keys)  13.8 / 14.5 / 22.5
+//   64 rows (4 tokens, 16 heads, 131072 keys)         48.4 / 40.3 / 41.9
+//   128 rows (1 token, 128 heads, 40000 keys)         47.0 / 37.5 / 44.4
+//   700 rows (7 sequences of 1 to 2048 tokens)        284 / 278 / 242
 struct PagedPlan {
   int bm, pr;
   int64_t tiles;  // at most
   bool split;
   size_t ml_at, o_at, bytes;
 };
-inline PagedPlan paged_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
+inline PagedPlan paged_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t max_pages) {
   PagedPlan d{};
   const int64_t rows = n_tokens * heads, each = cdiv(rows, n_seqs);
-  d.bm = each <= 16 ? 16 : (each <= 32 ? 32 : 64);
+  d.bm = each <= 16 ? 16 : (each <= 128 ? 32 : 64);
   d.pr = d.bm < 32 ? 32 : d.bm;
   d.tiles = rows / d.bm + (n_seqs < n_tokens ? n_seqs : n_tokens);
-  d.split = d.tiles <= kPagedMaxTiles && n_seqs <= kPagedMaxTiles;
+  d.split = d.tiles <= kPagedMaxTiles && n_seqs <= kPagedMaxTiles && max_pages > kPagedFew;
   if (d.split) {
     d.ml_at = kPagedWgs * sizeof(SplitTile);
     d.o_at = d.ml_at + static_cast<size_t>(2 * kPagedWgs) * d.pr * sizeof(float2);
@@ -919,9 +930,9 @@ inline PagedPlan paged_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
 
 using namespace tl;
 
-extern "C" size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads) {
-  if (n_seqs < 1 || n_tokens < 1 || heads < 1 || heads > 128 || n_seqs > (1ll << 20) || n_tokens * heads >= (1ll << 27)) return 0;
-  return paged_plan(n_seqs, n_tokens, heads).bytes;
+extern "C" size_t tl_flash_paged_mla_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t max_pages) {
+  if (n_seqs < 1 || n_tokens < 1 || heads < 1 || heads > 128 || n_seqs > (1ll << 20) || n_tokens * heads >= kPagedMaxRows) return 0;
+  return paged_plan(n_seqs, n_tokens, heads, max_pages).bytes;
 }
 
 extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const void* kv_pages, int64_t n_pages,
@@ -932,8 +943,8 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
   if (int rc = check_batch("flash_paged_mla", kv_pages, n_pages, block_table, max_pages, cu_seqlens, seq_lens, n_seqs, n_tokens)) return rc;
   if (heads < 1 || heads > 128) { set_error("flash_paged_mla: heads=%lld must be in [1, 128]", (long long)heads); return kErrUnsupported; }
   if (n_seqs == 0 || n_tokens == 0) return kOk;
-  if (n_tokens * heads >= (1ll << 27) || n_seqs > (1ll << 20) || max_pages > (1ll << 20)) {
-    set_error("flash_paged_mla: %lld tokens x %lld heads, %lld sequences, %lld pages a sequence: at most 2^27 rows, 2^20 "
+  if (n_tokens * heads >= kPagedMaxRows || n_seqs > (1ll << 20) || max_pages > (1ll << 20)) {
+    set_error("flash_paged_mla: %lld tokens x %lld heads, %lld sequences, %lld pages a sequence: fewer than 2^26 rows, up to 2^20 "
               "sequences and 2^20 pages", (long long)n_tokens, (long long)heads, (long long)n_seqs, (long long)max_pages);
     return kErrUnsupported;
   }
@@ -944,7 +955,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
     set_error("flash_paged_mla: q, out and workspace must be 16-byte aligned");
     return kErrArg;
   }
-  const PagedPlan d = paged_plan(n_seqs, n_tokens, heads);
+  const PagedPlan d = paged_plan(n_seqs, n_tokens, heads, max_pages);
   if (d.bytes && (!workspace || workspace_bytes < d.bytes)) {
     set_error("flash_paged_mla: needs a workspace of %zu bytes (got %zu)", d.bytes, workspace_bytes);
     return kErrArg;
@@ -952,7 +963,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const PagedArgs args{(const uint16_t*)q_nope_bf16, (const uint16_t*)q_pe_bf16, (const uint8_t*)kv_pages,
                        PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
-                       (int)heads, ((1ull << 40) + heads - 1) / heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
+                       (int)heads, ((1ull << 34) + heads - 1) / heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
                        d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
                        reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0)};
   const hipStream_t st = (hipStream_t)stream;

@@ -48,7 +48,7 @@ def flash_paged_mla(query: torch.Tensor, query_pe: torch.Tensor, kv_pages: torch
             scale = _SCALES[model_arch] = softmax_scale(model_arch)
     st = _stream(query)
     tokens = rows // heads
-    nbytes = _lib.query("tl_flash_paged_mla_workspace_bytes", n, tokens, heads)
+    nbytes = _lib.query("tl_flash_paged_mla_workspace_bytes", n, tokens, heads, block_table.shape[1])
     # taken from the allocator call by call: its memory is ordered on the stream, and a captured graph's is its own
     ws = query.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(query, "tl_flash_paged_mla", query.data_ptr(), query_pe.data_ptr(), kv_pages.data_ptr(), kv_pages.shape[0],
