@@ -27,21 +27,26 @@ struct PagedBatch {
   int n_seqs, max_pages, n_pages, n_tokens;
 };
 
-// The index of the last entry of cu[0 .. n_seqs] that is <= t, for a wave-uniform t: the token's sequence (-1 or
-// n_seqs: none; empty sequences are passed over).  64 entries a round, so one round up to 63 sequences, two up
-// to 4095.  Whatever cu holds, the result is in [-1, n_seqs].
-__device__ inline int find_seq(const int32_t* __restrict__ cu, int n_seqs, int t) {
+// The last index i of 0 .. n_seqs for which upto(i) holds, a wave-uniform predicate that holds up to some index (-1: for
+// none).  64 indices a round, so one round up to 63 sequences, two up to 4095.  Whatever upto says, it is asked about
+// 0 .. n_seqs only and the result is in [-1, n_seqs].
+template <class F>
+__device__ inline int last_seq(int n_seqs, F upto) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = n_seqs + 1;  // the first entry > t is in [lo, lo + n]
+  int lo = 0, n = n_seqs + 1;  // the first index for which it does not hold is in [lo, lo + n]
   while (n > 64) {
     const int step = (n + 63) >> 6, i = lane * step;
-    const int c = __popcll(__ballot(i < n && cu[lo + min(i, n - 1)] <= t));
+    const int c = __popcll(__ballot(i < n && upto(lo + i)));
     if (c == 0) return lo - 1;
     const int from = (c - 1) * step + 1;
     n = min(n, c * step) - from;
     lo += from;
   }
-  return lo + __popcll(__ballot(lane < n && cu[lo + min(lane, max(n - 1, 0))] <= t)) - 1;
+  return lo + __popcll(__ballot(lane < n && upto(lo + lane))) - 1;
+}
+// The sequence of token t (wave-uniform; -1 or n_seqs: none; empty sequences are passed over).
+__device__ inline int find_seq(const int32_t* __restrict__ cu, int n_seqs, int t) {
+  return last_seq(n_seqs, [&](int b) { return cu[b] <= t; });
 }
 
 // The place of token t of sequence b (any lane, any value): its page and row in the pool; page < 0: there is none.

@@ -31,7 +31,7 @@ typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar l
 
 constexpr int kPagedWgs = 256;        // workgroups of a split launch: one per CU
 constexpr int kPagedMaxTiles = 1024;  // tiles (and sequences) that a split launch plans in LDS
-constexpr int64_t kPagedMaxRows = 1 << 26;  // (token, head) rows: sums of 512 sequences' tiles, of 32 rows then, stay below 2^31
+constexpr int64_t kPagedMaxRows = 1 << 27;  // (token, head) rows, fewer than this (PagedArgs::per_head)
 // Pages that a sequence can have (a table's width), up to which no tile is split: one token, 16 heads, 512 keys take
 // 14.2 us in one workgroup and 8.5 + 4.6 us over eight and with the join, and the second launch costs the caller 4 us
 // (10.1 against 14.5 us a call); from there on the page loop, 1.0 us a page, decides.
@@ -86,7 +86,7 @@ struct PagedArgs {
   const uint8_t* pages;
   PagedBatch p;
   int heads;
-  uint64_t per_head;  // ceil(2^34 / heads): x / heads = x * per_head >> 34 for x < 2^34 / heads, so for every row
+  uint64_t per_head;  // ceil(2^34 / heads): x / heads = x * per_head >> 34 for x < 2^34 / heads
   float scale;  // softmax_scale * log2 e
   uint16_t* out;
   float* lse;
@@ -324,21 +324,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       A.split[w] = info;
     }
   } else {
-    // one workgroup a tile: its sequence, from the tile counts in order
+    // one workgroup a tile: sequence b's are the workgroups from `before(b)` on, which leaves it as many as it has tiles
+    auto before = [&](int b) { return min(max(p.cu[b], 0), p.n_tokens) * A.heads / BM + b; };
     tile = w;
-    seq = -1;
-    for (int b0 = 0; b0 < p.n_seqs; b0 += kPagedThreads) {
-      const int b = b0 + tid;
-      int total;
-      const int mine = b < p.n_seqs ? min(SeqRows(A, b).tiles(BM), static_cast<int>(gridDim.x)) : 0;
-      const int t = n_tiles + block_scan(mine, scan, total);
-      if (w >= t - mine && w < t) { scan[0] = b; scan[1] = t - mine; }
-      __syncthreads();
-      if (w < n_tiles + total) { seq = scan[0]; seq_tile0 = scan[1]; break; }
-      n_tiles += total;
-      __syncthreads();
-    }
-    if (seq < 0) return;
+    seq = last_seq(p.n_seqs, [&](int b) { return before(b) <= w; });
+    if (seq < 0 || seq >= p.n_seqs) return;
+    seq_tile0 = before(seq);
+    if (tile - seq_tile0 >= SeqRows(A, seq).tiles(BM)) return;
   }
 
   while (u < u_end) {
@@ -907,7 +899,7 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
 //   700 rows (7 sequences of 1 to 2048 tokens)        284 / 278 / 242
 struct PagedPlan {
   int bm, pr;
-  int64_t tiles;  // at most
+  int64_t tiles;  // of a split launch, at most
   bool split;
   size_t ml_at, o_at, bytes;
 };
@@ -944,7 +936,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
   if (heads < 1 || heads > 128) { set_error("flash_paged_mla: heads=%lld must be in [1, 128]", (long long)heads); return kErrUnsupported; }
   if (n_seqs == 0 || n_tokens == 0) return kOk;
   if (n_tokens * heads >= kPagedMaxRows || n_seqs > (1ll << 20) || max_pages > (1ll << 20)) {
-    set_error("flash_paged_mla: %lld tokens x %lld heads, %lld sequences, %lld pages a sequence: fewer than 2^26 rows, up to 2^20 "
+    set_error("flash_paged_mla: %lld tokens x %lld heads, %lld sequences, %lld pages a sequence: fewer than 2^27 rows, up to 2^20 "
               "sequences and 2^20 pages", (long long)n_tokens, (long long)heads, (long long)n_seqs, (long long)max_pages);
     return kErrUnsupported;
   }
@@ -971,7 +963,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
     using C = PagedCfg<decltype(bm)::value>;
     const auto kern = paged_mla_kernel<decltype(bm)::value>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), C::BYTES, "flash_paged_mla")) return rc;
-    hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(d.tiles)), dim3(kPagedThreads), C::BYTES, st, args);
+    hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(n_tokens * heads / d.bm + n_seqs)), dim3(kPagedThreads), C::BYTES, st, args);
     if (int rc = check_launch("flash_paged_mla")) return rc;
     if (!d.split) return kOk;
     hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(512), dim3(kCombineThreads), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
