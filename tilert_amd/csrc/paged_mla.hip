@@ -521,38 +521,70 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       if (f != f) f = 0.f;
       v4f U[KT];
 
-      // U of a page: scale * (codes . q) + rope . q, 4 KT items of 128 dims, each item's operand read ahead of its products
+      // A weight from its score; the largest and the sum so far.
+      auto weigh = [&](float score, float scale, float& sum, float& pmax) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score, f, -mk));
+        sum += e;
+        const float x = e * scale;
+        pmax = fmaxf(pmax, __builtin_fabsf(x));
+        return x;
+      };
+      auto put = [&](uint8_t* P, int kt, const float (&x)[4]) {
+        int hi, lo;
+        split4(x, hi, lo);
+        *reinterpret_cast<int*>(P + kt * 16) = hi;
+        *reinterpret_cast<int*>(P + kt * 16 + C::P_BYTES) = lo;
+      };
+      auto weights_at = [&](int k) { return smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p; };
+      // U of page k, and with WEIGH its weights, whose tile of 16 keys is one behind that of the products: the wave issues
+      // the vector instructions of the one while the matrix pipe works on the other.  Whether all weights were <= kPMost.
+      // 4 KT items of 128 dims, each item's operand read ahead of its products.
       auto load_key = [&](int slot, int i) {
         const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i % 4) * 128;
         return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
       };
-      auto scores = [&](int slot) {
+      auto scores = [&](int k, int slot, auto weigh_tag) {
+        constexpr bool WEIGH = decltype(weigh_tag)::value;
         constexpr int kItems = 4 * KT, kAhead = kItems < 4 ? kItems : 4;  // (8: 962 -> 979 us at 2048 tokens, 16 heads, 16384 keys; 6: 970)
+        uint8_t* P = weights_at(k);
+        float pmax = 0.f, sum = 0.f;
         v8i a[kItems];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
         __builtin_amdgcn_sched_barrier(0);
+        v4f x[KT], part[KT], sk[KT];  // of a tile: codes . q, rope . q, scales
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          v4f x = {0.f, 0.f, 0.f, 0.f};
-          const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
-          v8bf r[2];
+        for (int kt = 0; kt <= KT; ++kt) {
+          if (kt < KT) {
+            sk[kt] = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
+            x[kt] = part[kt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) r[ks] = *reinterpret_cast<const v8bf*>(smem + slot * kSlotBytes + (at_rope ^ (ks * 64)) + kt * 16 * 128);
+            for (int ks = 0; ks < 2; ++ks)
+              part[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  *reinterpret_cast<const v8bf*>(smem + slot * kSlotBytes + (at_rope ^ (ks * 64)) + kt * 16 * 128), qr[ks], part[kt], 0, 0, 0);
+          }
+          float w[4];
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            const int i = kt * 4 + ks;
-            if (i + kAhead < kItems) a[i + kAhead] = load_key(slot, i + kAhead);
-            x = mfma16_fp8(a[i], qhi[ks], x, kScaleOne);
-            x = mfma16_fp8(a[i], qlo[ks], x, kScaleLo);
+            if (kt < KT) {
+              const int i = kt * 4 + ks;
+              if (i + kAhead < kItems) a[i + kAhead] = load_key(slot, i + kAhead);
+              x[kt] = mfma16_fp8(a[i], qhi[ks], x[kt], kScaleOne);
+              x[kt] = mfma16_fp8(a[i], qlo[ks], x[kt], kScaleLo);
+            }
+            if (kt > 0) {
+              // (an infinite scale as NaN: a score of -inf is a masked one)
+              const float scale = __builtin_fmaf(sk[kt - 1][ks], 0.f, sk[kt - 1][ks]);
+              U[kt - 1][ks] = __builtin_fmaf(x[kt - 1][ks], scale, part[kt - 1][ks]);
+              if constexpr (WEIGH) w[ks] = weigh(U[kt - 1][ks], scale, sum, pmax);
+            }
             __builtin_amdgcn_sched_barrier(0);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] *= __builtin_fabsf(sk[i]) < INFINITY ? sk[i] : __builtin_nanf("");  // not -inf, a masked score
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(r[ks], qr[ks], x, 0, 0, 0);
-          U[kt] = x;
+          if constexpr (WEIGH)
+            if (kt > 0) put(P, kt - 1, w);
         }
+        psum = sum;
+        return !__any(pmax > kPMost);
       };
       // the scores of page k that the row does not see
       auto mask_scores = [&](int k, int id) {
@@ -563,27 +595,17 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           for (int i = 0; i < 4; ++i) U[kt][i] = at + kt * 16 + i < end ? U[kt][i] : -INFINITY;
       };
 
-      // P of page k from U, mk: codes to buffer k % 2, psum; whether all were <= kPMost
-      auto weights = [&](int k, int slot, auto mask) {
-        constexpr bool MASK = decltype(mask)::value;
-        uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p;
+      // The weights of page k from U where some are masked (-inf), whatever those keys' scales are.
+      auto weights = [&](int k, int slot) {
+        uint8_t* P = weights_at(k);
         float pmax = 0.f, sum = 0.f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
           const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
-          float x[4];
+          float w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mk));
-            const bool none = MASK && U[kt][i] == -INFINITY;  // a masked key's scale may be anything
-            sum += e;
-            x[i] = none ? 0.f : e * sk[i];
-            pmax = fmaxf(pmax, __builtin_fabsf(x[i]));
-          }
-          int hi, lo;
-          split4(x, hi, lo);
-          *reinterpret_cast<int*>(P + kt * 16) = hi;
-          *reinterpret_cast<int*>(P + kt * 16 + C::P_BYTES) = lo;
+          for (int i = 0; i < 4; ++i) w[i] = weigh(U[kt][i], U[kt][i] == -INFINITY ? 0.f : sk[i], sum, pmax);
+          put(P, kt, w);
         }
         psum = sum;
         return !__any(pmax > kPMost);
@@ -612,14 +634,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(was - mk);
         l *= alpha;
         if (kg == 0 && g == 0) alpha_l[my_row] = alpha;
-        weights(k, slot, std::true_type{});
+        weights(k, slot);
         __syncthreads();
       };
 
       if (n > 0) {
         arrive();
         if (masked(0, id0)) clean(0);
-        scores(0);
+        scores(0, 0, std::false_type{});
         if (masked(0, id0)) mask_scores(0, id0);
         settle(0, 0, id0);
         int next = 1, free = 2, slot = 0, id = id1, id_after = id_of(2);
@@ -631,12 +653,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           bool fits;
           if (masked(k + 1, id)) {
             clean(next);
-            scores(next);
+            scores(k + 1, next, std::false_type{});
             mask_scores(k + 1, id);
-            fits = weights(k + 1, next, std::true_type{});
+            fits = weights(k + 1, next);
           } else {
-            scores(next);
-            fits = weights(k + 1, next, std::false_type{});
+            fits = scores(k + 1, next, std::true_type{});
           }
           if ((!fits || fresh) && lane == 0) flag[(k + 1) & 3] = 1;
           fresh = fresh && !valid(id);
