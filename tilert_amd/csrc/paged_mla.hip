@@ -363,20 +363,22 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
 
     // the page `id` into a slot, by the multiplying waves, in 1 KB pieces: 32 of codes, four at a time, and 8 of rope
-    // parts; each also fetches the scales, all of them the same.  A 16-byte chunk c of a row is kept at c ^ (row & 7), so
-    // that the rows' chunks that a read takes together are in different banks
+    // parts; each also fetches the scales, all of them the same.  LDS has 64 banks of 4 bytes, 16 chunks of 16 bytes.  A row's
+    // chunk c of codes is kept at c ^ turn(row), turn = (row & 7) << 1 | (row >> 3 & 1): 16 rows' chunk c is then in 16
+    // places (a read of the scores), and so are the chunks 2 c and 2 c + 1 of 8 rows (a read of the values).  A chunk of a
+    // rope part, two rows to the 64 banks, is kept at c ^ (row >> 1 & 7).
     auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.n_pages); };
     auto fetch = [&](int id, int slot) {
       if (!valid(id)) id = 0;  // its keys are masked
       const uint8_t* page = A.pages + static_cast<int64_t>(id) * kKvPageBytes;
       const uint32_t to = lds0 + slot * kSlotBytes;
       const int piece = (wave - 4) * 8;
-      const uint32_t code = half * 512 + (n32 ^ half) * 16;  // rows 2 i, 2 i + 1 of piece i
-      const uint32_t off[4] = {code, code ^ 32, code ^ 64, code ^ 96};
+      const uint32_t code = half * 512 + (n32 ^ (2 * half)) * 16;  // rows 2 i, 2 i + 1 of piece i
+      const uint32_t off[4] = {code, code ^ 64, code ^ 128, code ^ 192}, odd[4] = {code ^ 16, code ^ 80, code ^ 144, code ^ 208};
       dma_pieces<4>(page + piece * 1024, off, to + piece * 1024);
-      dma_pieces<4>(page + piece * 1024 + 4096, off, to + piece * 1024 + 4096);
-      const uint32_t part = (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
-      const uint32_t rope[2] = {part, part};
+      dma_pieces<4>(page + piece * 1024 + 4096, odd, to + piece * 1024 + 4096);
+      const uint32_t part = (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 4)) * 16;
+      const uint32_t rope[2] = {part, part ^ 64};
       dma_pieces<2>(page + kKvRopeAt + piece * 256, rope, to + kKvPageKeys * kKvLatent + piece * 256);
       dma_words(page + kKvScaleAt, lane * 4, lds0 + C::SCALE_OFF + slot * kKvPageKeys * 4);
     };
@@ -510,8 +512,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     if (wave < 4) {
       const int my_key = kg * KT * 16 + n16;       // and 16, 32, .. behind it
       const int my_quad = kg * KT * 16 + 4 * g;    // the keys of this lane's scores: my_quad .. +3, and 16, 32, ..
-      const int at_code = my_key * kKvLatent + ((2 * g) ^ (my_key & 7)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31)
-      const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (my_key & 7)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
+      const int at_code = my_key * kKvLatent + ((2 * g) ^ ((n16 & 7) << 1) ^ (n16 >> 3)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31, ^ 128: 128 + 32 g ..)
+      const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (n16 >> 1)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
       const int put_p = my_row * kPStride + my_quad;
       const int seen = my_row < rows ? s.seen(A, in_seq + my_row) : 0;
       // weights are e = exp2(U * f - mk), mk = m - log2(kP / s_ref): m the row's largest U * f and s_ref the largest
@@ -540,8 +542,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       // the vector instructions of the one while the matrix pipe works on the other.  Whether all weights were <= kPMost.
       // 4 KT items of 128 dims, each item's operand read ahead of its products.
       auto load_key = [&](int slot, int i) {
-        const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i % 4) * 128;
-        return two_v4i(*reinterpret_cast<const v4i*>(at + at_code), *reinterpret_cast<const v4i*>(at + (at_code ^ 16)));
+        const uint8_t* at = smem + slot * kSlotBytes + (i / 4) * 16 * kKvLatent + (i & 2) * 128;
+        const int x = at_code ^ ((i & 1) * 128);
+        return two_v4i(*reinterpret_cast<const v4i*>(at + x), *reinterpret_cast<const v4i*>(at + (x ^ 16)));
       };
       auto scores = [&](int k, int slot, auto weigh_tag) {
         constexpr bool WEIGH = decltype(weigh_tag)::value;
@@ -690,7 +693,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       __syncthreads();
     } else {
       const int dw = wave - 4;  // dims 128 dw ..
-      const int at_value = (32 * half + (n16 >> 1)) * kKvLatent + dw * 128 + (lane & 1) * 8 + ((g & 1) ^ (n16 >> 1)) * 16;  // 32-dim tile d: ^ 32 d
+      const int at_value = (32 * half + (n16 >> 1)) * kKvLatent + (dw & 2) * 128 + (lane & 1) * 8 +
+                           ((8 * (dw & 1) + (g & 1)) ^ (n16 & 14)) * 16;  // 32-dim tile d: ^ 32 d; keys 8 .. 15 and 24 .. 31: ^ 16
       const int at_p = n32 * kPStride + half * 32;
       v16f o[RT2][DT];
 #pragma unroll
@@ -716,10 +720,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const uint8_t* src = smem + slot * kSlotBytes + (at_value ^ (32 * d));
+          const uint8_t* src = smem + slot * kSlotBytes;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + r * 8 * kKvLatent));
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + (at_value ^ (32 * d + 16 * (r & 1))) + r * 8 * kKvLatent));
             v[d][2 * r] = x[0];
             v[d][2 * r + 1] = x[1];
           }
