@@ -8,7 +8,8 @@
 // MFMA; the other operand is split into two e4m3 numbers, x = hi + lo / 32:
 //   q / sigma (sigma: a power of two that brings the row's largest magnitude into [128, 256)): exact for
 //     values down to 2^-15 of the row's largest, below that within 2^-23 of it;
-//   p * scale_j * kP / s_ref (kept <= 256): 8 to 9 significant bits, as bf16, down to 2^-21 of the largest.
+//   p * scale_j * r (r: a power of two that brings the largest to kP at most; kept <= 256): 8 to 9 significant bits,
+//     as bf16, down to 2^-20 of the largest.
 // Two fp8 products take the time of one in bf16, and no code is converted: with codes turned into bf16 the
 // conversions alone (64 a page and wave for each product and 32 rows) would take as long as the products.
 // Scores are U = scale_j * (codes . q / sigma) + (q_pe / sigma) . rope (bf16 MFMA), the exponent U * (sigma *
@@ -39,8 +40,8 @@ constexpr int kPagedFew = 8;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
 constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
-constexpr float kP = 32.0f;          // a weight times key scale is kP at most when m and s_ref are set,
-constexpr float kPMost = 256.0f;     // and kPMost until they are set again
+constexpr int kPLog = 5;             // a weight times key scale is below kP = 2^kPLog when m and r are set,
+constexpr float kPMost = 256.0f;     // and kPMost at most until they are set again
 constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
 
 // Eight waves, two on a SIMD: 0 .. 3 score, 4 .. 7 multiply.  Scoring wave w takes the 16 rows of group w / KG against the
@@ -516,14 +517,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (n16 >> 1)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
       const int put_p = my_row * kPStride + my_quad;
       const int seen = my_row < rows ? s.seen(A, in_seq + my_row) : 0;
-      // weights are e = exp2(U * f - mk), mk = m - log2(kP / s_ref): m the row's largest U * f and s_ref the largest
-      // key scale when they were last set, so that e * scale <= kP then.  l and O are sums of such e and need no
-      // s_ref in the end.
-      float m = -INFINITY, mk = 0.f, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f;
+      // weights are e = exp2(U * f - mk), mk = m: the row's largest U * f when it was last set (-300 where it had none
+      // yet: any score is then flagged).  P is e * scale * r, r = 2^kPLog over s_ref, the largest key scale so far, rounded
+      // up to a power of two, so that P < kP where m is set.  l is the sum of such e, O of P times codes.
+      float m = -INFINITY, mk = 0.f, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f, r = 1.f;
       if (f != f) f = 0.f;
       v4f U[KT];
 
-      // A weight from its score; the largest and the sum so far.
+      // A weight, times its key's scale * r, from its score; the largest and the sum so far.
       auto weigh = [&](float score, float scale, float& sum, float& pmax) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score, f, -mk));
         sum += e;
@@ -579,7 +580,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
               // (an infinite scale as NaN: a score of -inf is a masked one)
               const float scale = __builtin_fmaf(sk[kt - 1][ks], 0.f, sk[kt - 1][ks]);
               U[kt - 1][ks] = __builtin_fmaf(x[kt - 1][ks], scale, part[kt - 1][ks]);
-              if constexpr (WEIGH) w[ks] = weigh(U[kt - 1][ks], scale, sum, pmax);
+              if constexpr (WEIGH) w[ks] = weigh(U[kt - 1][ks], scale * r, sum, pmax);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -607,14 +608,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
           float w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = weigh(U[kt][i], U[kt][i] == -INFINITY ? 0.f : sk[i], sum, pmax);
+          for (int i = 0; i < 4; ++i) w[i] = weigh(U[kt][i], U[kt][i] == -INFINITY ? 0.f : sk[i] * r, sum, pmax);
           put(P, kt, w);
         }
         psum = sum;
         return !__any(pmax > kPMost);
       };
 
-      // New m and s_ref from page k's scores, O and l brought to them, P again.  Every wave comes here, or none.
+      // New m and r from page k's scores and scales, O and l brought to them, P again.  Every wave comes here, or none.
       auto settle = [&](int k, int slot, int id) {
         float x = -INFINITY;
 #pragma unroll
@@ -630,13 +631,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         if constexpr (KG > 1)
 #pragma unroll
           for (int i = 0; i < KG; ++i) x = fmaxf(x, stat[i * BM + my_row]);
-        const float was = mk;
+        const float was = mk, was_r = r;
         const bool none = m == -INFINITY;
         m = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
-        mk = m == -INFINITY ? -300.f : m - __builtin_amdgcn_logf(kP / s_ref);  // (base 2; with no score yet, any one is flagged)
+        mk = m == -INFINITY ? -300.f : m;
+        // s_ref < 2^(e - 126), e its exponent's bits, 27 .. 254
+        const uint32_t e = __builtin_amdgcn_readfirstlane(__float_as_uint(s_ref) >> 23);
+        r = __uint_as_float((127 + kPLog + 126 - e) << 23);
         const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(was - mk);
         l *= alpha;
-        if (kg == 0 && g == 0) alpha_l[my_row] = alpha;
+        if (kg == 0 && g == 0) alpha_l[my_row] = alpha * (r / was_r);
         weights(k, slot);
         __syncthreads();
       };
@@ -677,6 +681,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       }
       // l over the lanes and waves of a row
       __syncthreads();
+      if (tid == 0) scan[0] = static_cast<int>(__float_as_uint(1.0f / r));
       l += __shfl_xor(l, 16);
       l += __shfl_xor(l, 32);
       if (g == 0) {
@@ -774,6 +779,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       __syncthreads();
       __syncthreads();
       __syncthreads();
+      const float unit = __uint_as_float(scan[0]);  // 1 / r, a power of two
 
       // ---- the rows' results, or the tile's partial sums
       if (!A.split || (u == tile_u0 && u_end >= tile_u1)) {
@@ -783,7 +789,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         for (int a = 0; a < RT2; ++a) {
           const int r = a * 32 + n32;
           if (r < rows) {
-            const float L = rowl[r], x = L == 0.f ? 0.f : 1.0f / L;
+            const float L = rowl[r], x = L == 0.f ? 0.f : 1.0f / L * unit;
             uint16_t* dst = A.out + (row0 + r) * kKvLatent + dw * 128 + 4 * half;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -805,7 +811,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 dst[((a * 16 + dw * DT + d) * 4 + i) * 64 + lane] =
-                    v4f{o[a][d][4 * i], o[a][d][4 * i + 1], o[a][d][4 * i + 2], o[a][d][4 * i + 3]};
+                    v4f{o[a][d][4 * i], o[a][d][4 * i + 1], o[a][d][4 * i + 2], o[a][d][4 * i + 3]} * unit;
           }
       }
     }
