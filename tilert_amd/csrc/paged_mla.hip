@@ -371,17 +371,19 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.n_pages); };
     auto fetch = [&](int id, int slot) {
       if (!valid(id)) id = 0;  // its keys are masked
+      int at = lane;  // what follows from it is computed anew for each page: the products need the registers
+      asm volatile("" : "+v"(at));
       const uint8_t* page = A.pages + static_cast<int64_t>(id) * kKvPageBytes;
       const uint32_t to = lds0 + slot * kSlotBytes;
       const int piece = (wave - 4) * 8;
-      const uint32_t code = half * 512 + (n32 ^ (2 * half)) * 16;  // rows 2 i, 2 i + 1 of piece i
+      const uint32_t code = (at >> 5) * 512 + ((at & 31) ^ (at >> 5) * 2) * 16;  // rows 2 i, 2 i + 1 of piece i
       const uint32_t off[4] = {code, code ^ 64, code ^ 128, code ^ 192}, odd[4] = {code ^ 16, code ^ 80, code ^ 144, code ^ 208};
       dma_pieces<4>(page + piece * 1024, off, to + piece * 1024);
       dma_pieces<4>(page + piece * 1024 + 4096, odd, to + piece * 1024 + 4096);
-      const uint32_t part = (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 4)) * 16;
+      const uint32_t part = (at >> 3) * 128 + ((at & 7) ^ (at >> 4)) * 16;
       const uint32_t rope[2] = {part, part ^ 64};
       dma_pieces<2>(page + kKvRopeAt + piece * 256, rope, to + kKvPageKeys * kKvLatent + piece * 256);
-      dma_words(page + kKvScaleAt, lane * 4, lds0 + C::SCALE_OFF + slot * kKvPageKeys * 4);
+      dma_words(page + kKvScaleAt, at * 4, lds0 + C::SCALE_OFF + slot * kKvPageKeys * 4);
     };
     // whether some row does not see all of page k; an id that is not valid is one whose keys nobody sees
     auto masked = [&](int k, int id) { return (pg0 + k + 1) * kKvPageKeys > seen_first || !valid(id); };
@@ -715,7 +717,19 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       // 32 half + 8 r + i / 2, half i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
       auto product = [&](int k, int slot) {
         const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + at_p;
-        v8i v[DT], ph[RT2], pl[RT2];
+        const int at = slot * kSlotBytes + at_value;  // (a slot's place leaves bits 4 .. 8 alone)
+        auto load_value = [&](int d) {
+          v8i v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(smem + (at ^ (32 * d + 16 * (r & 1))) + r * 8 * kKvLatent));
+            v[2 * r] = x[0];
+            v[2 * r + 1] = x[1];
+          }
+          return v;
+        };
+        v8i v[2], ph[RT2], pl[RT2];
+        v[0] = load_value(0);
 #pragma unroll
         for (int a = 0; a < RT2; ++a) {
           const v4i* hi = reinterpret_cast<const v4i*>(P + a * 32 * kPStride);
@@ -725,21 +739,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const uint8_t* src = smem + slot * kSlotBytes;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(src + (at_value ^ (32 * d + 16 * (r & 1))) + r * 8 * kKvLatent));
-            v[d][2 * r] = x[0];
-            v[d][2 * r + 1] = x[1];
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
+          if (d + 1 < DT) v[(d + 1) & 1] = load_value(d + 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int a = 0; a < RT2; ++a) {
-            o[a][d] = mfma32_fp8(v[d], ph[a], o[a][d], kScaleOne);
-            o[a][d] = mfma32_fp8(v[d], pl[a], o[a][d], kScaleLo);
+            o[a][d] = mfma32_fp8(v[d & 1], ph[a], o[a][d], kScaleOne);
+            o[a][d] = mfma32_fp8(v[d & 1], pl[a], o[a][d], kScaleLo);
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       };
       auto settle = [&](bool first) {
         __syncthreads();
