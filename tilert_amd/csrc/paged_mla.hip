@@ -37,6 +37,12 @@ constexpr int64_t kPagedMaxRows = 1 << 27;  // (token, head) rows, fewer than th
 // 14.2 us in one workgroup and 8.5 + 4.6 us over eight and with the join, and the second launch costs the caller 4 us
 // (10.1 against 14.5 us a call); from there on the page loop, 1.0 us a page, decides.
 constexpr int kPagedFew = 8;
+// Pages' time that a tile is counted for besides its pages, where a launch has many tiles: its queries' way into registers,
+// the first scores, its results (18 thousand cycles at 64 rows, a page 3.4 thousand), rounded up for the tile that is cut in
+// two.  Seven sequences of 2 to 700 new tokens, 273 tiles of 6 to 79 pages: 244 us without, 184 with 5, 173 with 9, 170
+// with 18; with half as many tiles as workgroups or fewer, each takes part of one or two, and it makes no difference
+// (60 sequences, 102 us).
+constexpr int kPagedStart = 10;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
 constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
@@ -95,6 +101,7 @@ struct PagedArgs {
   float2* part_ml;   // [2 kPagedWgs][PR]
   float* part_o;     // [2 kPagedWgs][kPartFloats]
   int tile_cap;      // tiles that the launch makes room for
+  int start;         // pages' time that a tile takes before its first
 };
 
 // A sequence's row tiles and what they see, from untrusted metadata.
@@ -260,7 +267,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   // ---- the work of this workgroup
   int n_tiles = 0, u = 0, u_end = 1, quota = 1, tile = 0, seq = 0, seq_tile0 = 0;
   if (A.split) {
-    // units are pages of tiles (a tile that sees nothing counts one); every workgroup takes `quota` of them in a row
+    // units are pages of tiles (a tile that sees nothing counts one) and A.start more a tile, in front of its pages; every
+    // workgroup takes `quota` of them in a row
     int units;
     bool done = false;
     if (p.n_seqs <= kPagedThreads) {  // a decode step: where no sequence has two tiles, one pass does
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       if (tid < p.n_seqs) {
         const SeqRows s(A, tid);
         tiles = min(s.tiles(BM), A.tile_cap);
-        pages = tiles ? max(1, s.pages(A, 0, BM)) : 0;
+        pages = tiles ? max(1, s.pages(A, 0, BM)) + A.start : 0;
       }
       int t = tiles, q = pages;
       done = block_scan2(t, q, tiles > 1, scan, n_tiles, units);
@@ -295,7 +303,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         SeqRows s(A, b);
         for (int t = t0; t < t1; ++t) {
           while (t >= seq_end[b]) s = SeqRows(A, ++b);
-          sum += max(1, s.pages(A, t - (b ? seq_end[b - 1] : 0), BM));
+          sum += max(1, s.pages(A, t - (b ? seq_end[b - 1] : 0), BM)) + A.start;
           unit_end[t] = sum;
         }
       }
@@ -306,20 +314,28 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     if (done) units = n_tiles ? unit_end[n_tiles - 1] : 0;  // (as many tiles as there is room for)
     units = __builtin_amdgcn_readfirstlane(units);
     quota = max(1, (units + kPagedWgs - 1) / kPagedWgs);
-    u = min(w * quota, units);
-    u_end = min(u + quota, units);
-    tile = __builtin_amdgcn_readfirstlane(upper(unit_end, n_tiles, u));
+    // the units at which the workgroup before, this one and the next begin: lanes 0, 1, 2
+    int at = min((w - 1 + min(tid & 63, 2)) * quota, units);
+    const int in = upper(unit_end, n_tiles, at);
+    if (in < n_tiles) {
+      const int first = in ? unit_end[in - 1] : 0;
+      if (at <= first + A.start) at = first;  // all its pages
+    }
+    const int u_before = __builtin_amdgcn_readlane(at, 0);
+    u = __builtin_amdgcn_readlane(at, 1);
+    u_end = __builtin_amdgcn_readlane(at, 2);
+    tile = __builtin_amdgcn_readlane(in, 1);
     if (tid == 0) {
       SplitTile info{0, 0, 0};
       if (u < u_end) {
-        const int first = tile ? unit_end[tile - 1] : 0;
-        if (first < u && first >= u - quota) {  // the second workgroup on its first tile
+        const int before = tile ? unit_end[tile - 1] : 0;
+        if (before < u && u_before <= before) {  // the second workgroup on its first tile
           const int b = upper(seq_end, p.n_seqs, tile);
           const SeqRows s(A, b);
           const int j = tile - (b ? seq_end[b - 1] : 0);
           info.row0 = static_cast<int64_t>(s.first) * A.heads + static_cast<int64_t>(j) * BM;
           info.rows = min(BM, s.n_rows - j * BM);
-          info.parts = (unit_end[tile] - 1) / quota - first / quota + 1;
+          info.parts = (unit_end[tile] - 1) / quota - w + 2;  // those that begin inside it, and one
         }
       }
       A.split[w] = info;
@@ -346,8 +362,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     if (A.split) {
       seq = upper(seq_end, p.n_seqs, tile);
       seq_tile0 = seq ? seq_end[seq - 1] : 0;
-      tile_u0 = __builtin_amdgcn_readfirstlane(tile ? unit_end[tile - 1] : 0);
+      tile_u0 = __builtin_amdgcn_readfirstlane(tile ? unit_end[tile - 1] : 0) + A.start;
       tile_u1 = __builtin_amdgcn_readfirstlane(unit_end[tile]);
+      u = max(u, tile_u0);
     }
     seq = __builtin_amdgcn_readfirstlane(seq);
     seq_tile0 = __builtin_amdgcn_readfirstlane(seq_tile0);
@@ -996,7 +1013,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
                        PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
                        (int)heads, ((1ull << 34) + heads - 1) / heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
                        d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
-                       reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0)};
+                       reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0), d.split && d.tiles > kPagedWgs / 2 ? kPagedStart : 0};
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto bm) -> int {
     using C = PagedCfg<decltype(bm)::value>;
