@@ -12,6 +12,10 @@ typedef uint32_t u32x4c __attribute__((ext_vector_type(4)));
 // and the rope part turned by its token's angles (lanes 0 .. 31, a pair each).  A key that holds a
 // NaN or an infinity gets the scale NaN: its codes are finite whatever it held, so only rows of an attention that see
 // the key are touched by it.
+// A wave needs no other's values: no LDS, no barrier, and the row's loads are all under way before the token's place
+// is known.  Bound by the round trips one behind another (cu_seqlens, lengths, table, store) in small calls and by
+// bytes (1408 read and 644 written a token) in large ones: one token 2.6 us, 4000 tokens of 5 sequences 5.7 us,
+// 1.5 TB/s, where a launch that does nothing takes 2.
 template <bool NORM>
 __global__ __launch_bounds__(256) void mla_cache_write_kernel(const uint16_t* __restrict__ kv, const uint16_t* __restrict__ pe,
                                                               uint8_t* __restrict__ pages, PagedBatch p,
@@ -70,7 +74,9 @@ __global__ __launch_bounds__(256) void mla_cache_write_kernel(const uint16_t* __
   }
 }
 
-// One wave a key: its latent as bf16(code * scale), its rope part as it is.
+// One wave a key: its latent as bf16(code * scale), its rope part as it is.  Bound by bytes, 644 read and 1152 written a
+// key: 143 thousand keys of 9 sequences, 257 MB, 40 us (6.4 TB/s) where the Infinity Cache holds part of them, 59 us a
+// call (4.4 TB/s; a large copy 4.7) over caches that it does not; 2100 keys 3.2 us.
 __global__ __launch_bounds__(256) void mla_cache_read_kernel(const uint8_t* __restrict__ pages, PagedBatch p,
                                                              uint16_t* __restrict__ kv, uint16_t* __restrict__ pe) {
   const int lane = threadIdx.x & 63;

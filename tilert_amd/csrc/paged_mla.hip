@@ -31,7 +31,10 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
 
 constexpr int kPagedWgs = 256;        // workgroups of a split launch: one per CU
-constexpr int kPagedMaxTiles = 1024;  // tiles (and sequences) that a split launch plans in LDS
+// Tiles (and sequences) that a split launch plans in LDS; with more, a workgroup takes one and the last round of them is
+// short against the others.  273 tiles, ragged: 177 us split, 237 not; 512 tiles of 225 to 256 pages, two for every
+// workgroup: 966 split, 918 not.
+constexpr int kPagedMaxTiles = 1024;
 constexpr int64_t kPagedMaxRows = 1 << 27;  // (token, head) rows, fewer than this (PagedArgs::per_head)
 // Pages that a sequence can have (a table's width), up to which no tile is split: one token, 16 heads, 512 keys take
 // 14.2 us in one workgroup and 8.5 + 4.6 us over eight and with the join, and the second launch costs the caller 4 us
@@ -40,8 +43,10 @@ constexpr int kPagedFew = 8;
 // Pages' time that a tile is counted for besides its pages, where a launch has many tiles: its queries' way into registers,
 // the first scores, its results (18 thousand cycles at 64 rows, a page 3.4 thousand), rounded up for the tile that is cut in
 // two.  Seven sequences of 2 to 700 new tokens, 273 tiles of 6 to 79 pages: 244 us without, 184 with 5, 173 with 9, 170
-// with 18; with half as many tiles as workgroups or fewer, each takes part of one or two, and it makes no difference
-// (60 sequences, 102 us).
+// with 18.  32 tiles of 25 to 256 pages (1 token, 128 heads, 8 sequences): 36.2 without, 32.0 with 10; 60 tiles: 102 both
+// ways.  A launch of at most kPagedWgs / 16 tiles has few workgroups with two of them, and does without: 2 tiles of one
+// sequence (4 tokens over 131072 keys) are 38.9 us, 42.9 with it, as the workgroups on the same pages of both are then
+// no longer a multiple of 8, an XCD's L2, apart.
 constexpr int kPagedStart = 10;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
@@ -75,6 +80,15 @@ struct PagedCfg {
   static constexpr size_t kPartFloats = static_cast<size_t>(PR) * kKvLatent;
 };
 constexpr int kPagedThreads = 512;
+
+// What bounds it.  Decode: bytes; 60 sequences, 60 to 32768 keys, 447 MB of pages and rows: 102 us a call, 4.4 TB/s (a large
+// copy 4.7), 95 + 8.6 us in the two kernels.  Chunks: 2048 tokens, 16 heads over 16384 keys, 1.10 PFLOP: 0.94 to 0.97 ms,
+// 1.13 to 1.17 PFLOP/s; a large bf16 product of the library reaches 1.39.  A step of 64 rows x 64 keys takes 3750 cycles, in
+// which a SIMD's matrix pipe works for 2176; without the scoring waves' reads of the codes it takes 2980, without the
+// second product 3160, without writing P 3300, without fetches 3680, but then at 2.19 GHz instead of 1.95: the
+// clock gives way to the power drawn.  (Scoring waves of 32 rows would halve the reads; their queries' 144 registers leave
+// too few: with reloads from scratch memory 1.8 ms.)  Small calls: the latency of plan, queries, pages and join, one
+// behind another; 1 token over 500 keys 13.7 us in one kernel, of which seven pages' steps are 7.5.
 // 32 rows' queries on their way into registers, in slot 2: hi codes [32][512], lo codes, rope parts bf16 [32][64]
 constexpr int kQueryLo = 32 * kKvLatent, kQueryRope = 2 * kQueryLo;
 static_assert(kQueryRope + 32 * kKvRope * 2 <= kSlotBytes, "");
@@ -1013,7 +1027,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
                        PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
                        (int)heads, ((1ull << 34) + heads - 1) / heads, softmax_scale * 1.4426950408889634f, (uint16_t*)out_bf16, lse,
                        d.split ? reinterpret_cast<SplitTile*>(ws) : nullptr, reinterpret_cast<float2*>(ws + d.ml_at),
-                       reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0), d.split && d.tiles > kPagedWgs / 2 ? kPagedStart : 0};
+                       reinterpret_cast<float*>(ws + d.o_at), (int)(d.split ? d.tiles : 0), d.split && d.tiles > kPagedWgs / 16 ? kPagedStart : 0};
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto bm) -> int {
     using C = PagedCfg<decltype(bm)::value>;
