@@ -963,10 +963,11 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
 // once, and for 64 rows both 32-row products of a multiplying wave share its read of the page; fewer rows have their
 // queries split and their sums written in less time and waste less where a sequence's rows end.  Measured, for the rows
 // that a sequence has on average, in us with 16 / 32 / 64 rows a tile:
-//   16 rows (60 sequences, up to 32768 keys)          101 / 102 / 121;   (1 sequence, 500 keys)  13.8 / 14.5 / 22.5
-//   64 rows (4 tokens, 16 heads, 131072 keys)         48.4 / 40.3 / 41.9
-//   128 rows (1 token, 128 heads, 40000 keys)         47.0 / 37.5 / 44.4
-//   700 rows (7 sequences of 1 to 2048 tokens)        284 / 278 / 242
+//   16 rows (1 sequence, 500 keys)                         13.8 / 14.7 / 22.6
+//   17 rows (60 sequences of 60 to 32768 keys, padded)     101.5 / 102.1 / 117.9
+//   64 rows (4 tokens, 16 heads, 131072 keys)              48.7 / 38.8 / 42.5
+//   128 rows (8 sequences of 1589 to 16384 keys)           42.2 / 32.2 / 38.4
+//   2471 rows (7 sequences of 2 to 700 new tokens)         305 / 181 / 171
 struct PagedPlan {
   int bm, pr;
   int64_t tiles;  // of a split launch, at most
