@@ -161,6 +161,7 @@ ENTRIES = [("tl_mla_cache_write", _write_c), ("tl_mla_cache_read", _read_c), ("t
     (dict(pages=P + 8), "16-byte aligned"), (dict(n_pages=0), "n_pages"), (dict(n_pages=1 << 31), "n_pages"), (dict(max_pages=0), "max_pages"),
     (dict(max_pages=1 << 25), "max_pages"), (dict(n_seqs=-1), "out of range"), (dict(n_tokens=-1), "out of range"),
     (dict(n_seqs=1 << 24), "out of range"), (dict(n_tokens=1 << 31), "out of range"),
+    (dict(n_tokens=1 << 26), "out of range"),
 ])
 def test_c_entries_refuse_a_batch(name, args, change, text):
     _refused(name, args(**change), 1, text)
@@ -199,6 +200,11 @@ def test_an_empty_batch_is_no_error(name, args, nothing):
 def test_c_norm_refuses(change, text):
     a = {**dict(x=P, r=P, g=P, rows=4, dim=256, s=P, y=P, y8=P, ys=P, mode=0), **change}
     _refused("tl_add_rmsnorm_quant", (a["x"], a["r"], a["g"], 1e-6, a["rows"], a["dim"], a["s"], a["y"], a["y8"], a["ys"], a["mode"], None), 1, text)
+
+
+@pytest.mark.parametrize("rows,dim", [(1 << 24, 2048), (1 << 22, 2176), (1 << 22, 16384), (1 << 40, 128)])
+def test_c_norm_refuses_more_rows_than_a_launch_has(rows, dim):
+    _refused("tl_add_rmsnorm_quant", (P, P, P, 1e-6, rows, dim, P, P, P, P, 0, None), 3, "rows")
 
 
 def test_the_workspace_follows_the_sizes():

@@ -97,13 +97,17 @@ using namespace tl;
 extern "C" int tl_add_rmsnorm_quant(const void* x_bf16, const void* residual_bf16, const float* gamma, float eps,
                                     int64_t rows, int64_t dim, void* sum_bf16, void* y_bf16, void* y_fp8, float* y_scale,
                                     int scale_mode, void* stream) {
-  if (rows < 0 || rows > 0x7fffffff || dim <= 0 || dim % kBlock || dim > kAddNormMaxDim) {
+  if (rows < 0 || dim <= 0 || dim % kBlock || dim > kAddNormMaxDim) {
     set_error("add_rmsnorm_quant: dim=%lld must be a positive multiple of 128, at most %d (rows=%lld)", (long long)dim,
               kAddNormMaxDim, (long long)rows);
     return kErrArg;
   }
   if (scale_mode < 0 || scale_mode > 2) { set_error("add_rmsnorm_quant: bad scale_mode %d", scale_mode); return kErrArg; }
   if (rows == 0) return kOk;
+  if (rows >= (dim <= 2048 ? 1ll << 24 : 1ll << 22)) {  // a launch has fewer than 2^32 threads
+    set_error("add_rmsnorm_quant: %lld rows: at most 2^24 - 1 up to 2048 columns, 2^22 - 1 behind", (long long)rows);
+    return kErrUnsupported;
+  }
   if (!x_bf16 || !residual_bf16 || !gamma || !sum_bf16 || (!y_fp8) != (!y_scale) || (!y_bf16 && !y_fp8)) {
     set_error("add_rmsnorm_quant: null pointer (y_fp8 and y_scale are given together; y_bf16 may be left out beside them)");
     return kErrArg;
