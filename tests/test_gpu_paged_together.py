@@ -229,7 +229,7 @@ def test_a_pool_past_32_bit_offsets(cuda, new, total):
     assert torch.equal(flat[0], flat[2]) and torch.equal(flat[1], flat[3]) and flat[0].any()
 
 
-@pytest.mark.parametrize("n", [64, 600, 1100, 5000])
+@pytest.mark.parametrize("n", [64, 600, 1100, 2100, 5000])
 def test_many_sequences(cuda, n):
     """More sequences than one round, one pass, a split launch's plan and two rounds of the search take; some are
     empty, some have no new token."""
@@ -254,10 +254,11 @@ def test_many_sequences(cuda, n):
     assert torch.equal(flat_pe[where[:, 0].to(cuda)].cpu(), pe[where[:, 0]]) and torch.all(flat[int(cu[-1]):] == 7.0)
 
 
-def test_more_row_tiles_than_a_split_launch_plans(cuda):
-    """One workgroup a tile over a long table."""
-    pages, table, cu, lens, rows = _paged.batch([640, 1], [700, 3], seed=61)
-    _paged.fill(pages, table, [700, 3])
+@pytest.mark.parametrize("new", [640, 1100])
+def test_more_row_tiles_than_a_split_launch_plans(cuda, new):
+    """Many tiles over a long table: planned, and one workgroup a tile."""
+    pages, table, cu, lens, rows = _paged.batch([new, 1], [new + 60, 3], seed=61)
+    _paged.fill(pages, table, [new + 60, 3])
     d = _paged.to(cuda, *queries(rows, 128, 67), pages, table, cu, lens)
     check(cuda, *d[:4], cu, lens, *_attend(d))
 
@@ -299,3 +300,35 @@ def test_queries_of_zero_and_of_far_sizes(cuda, factor):
     else:
         flash_paged_mla(q, qp, *case[2:], out, lse, model_arch=ARCH)
         check(cuda, q, qp, *(t.cpu() for t in case[2:]), out, lse)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_metadata_that_does_not_make_sense_stays_inside(cuda, seed):
+    """cu_seqlens that do not ascend, lengths and pages that are not there, in both forms of the launch: what lies around
+    the call's tensors and the pool is left as it was, and a call that makes sense is right afterwards."""
+    g = torch.Generator().manual_seed(100 + seed)
+    B, heads = 1 + seed, (16, 5, 40)[seed % 3]
+    new = [1 + int(x) for x in torch.randint(0, 5, (B,), generator=g)]
+    total = [n + int(x) for n, x in zip(new, torch.randint(0, 900 if seed % 2 else 200, (B,), generator=g))]
+    pages, table, cu, lens, rows = _paged.batch(new, total, pad=seed % 3, seed=seed)
+    _paged.fill(pages, table, total)
+    good = _paged.to(cuda, *queries(rows, heads, seed), pages, table, cu, lens)
+    for _ in range(5):
+        bad_cu = torch.where(torch.rand(B + 1, generator=g) < 0.5, torch.randint(-4, rows + 4, (B + 1,), generator=g).to(I32), cu)
+        bad_lens = torch.where(torch.rand(B, generator=g) < 0.3, torch.randint(-50, 64 * table.shape[1] + 50, (B,), generator=g).to(I32), lens)
+        bad_table = torch.where(torch.rand(table.shape, generator=g) < 0.2, torch.randint(-5, pages.shape[0] + 5, table.shape, generator=g).to(I32), table)
+        pool = torch.full((pages.shape[0] + 4, paged.PAGE_BYTES), 0x55, dtype=torch.uint8, device=cuda)
+        pool[2:-2] = good[2]
+        out = torch.full((rows + 8, heads, 512), 7.0, dtype=BF16, device=cuda)
+        lse = torch.full((rows + 8, heads), 7.0, device=cuda)
+        flat, flat_pe = torch.full((rows + 8, 512), 7.0, dtype=BF16, device=cuda), torch.full((rows + 8, 64), 7.0, dtype=BF16, device=cuda)
+        meta = _paged.to(cuda, bad_table, bad_cu, bad_lens)
+        flash_paged_mla(good[0], good[1], pool[2:-2], *meta, out[4:-4], lse[4:-4], model_arch=ARCH)
+        mla_cache_read(pool[2:-2], *meta, flat[4:-4], flat_pe[4:-4])
+        kv, pe, gamma, _ = _inputs(rows, seed)
+        mla_cache_write(*_paged.to(cuda, kv, pe), pool[2:-2], *meta, gamma.to(cuda))
+        torch.cuda.synchronize()
+        for t in (out, lse, flat, flat_pe):
+            assert torch.all(t[:4] == 7.0) and torch.all(t[-4:] == 7.0)
+        assert torch.all(pool[:2] == 0x55) and torch.all(pool[-2:] == 0x55)
+    check(cuda, *good[:4], cu, lens, *_attend(good))

@@ -213,7 +213,7 @@ def test_the_workspace_follows_the_sizes():
     assert f(1, 1, 16, 8) == 0 and f(1, 1, 16, 9) > 0
     assert f(1, 1, 16, 9) == f(60, 60, 16, 4096) == f(1, 1, 16, 1 << 20)
     assert f(1, 8, 16, 9) == f(1, 2, 16, 9) < f(1, 9, 16, 9)
-    assert f(1, 4094, 16, 512) > 0 and f(1, 5000, 16, 512) == 0 and f(1025, 1025, 16, 512) == 0
+    assert f(1, 8188, 16, 512) > 0 and f(1, 8200, 16, 512) == 0 and f(2049, 2049, 16, 512) == 0
     assert f(0, 1, 16, 9) == f(1, 0, 16, 9) == f(1, 1, 0, 9) == f(1, 1, 129, 9) == 0
 
 

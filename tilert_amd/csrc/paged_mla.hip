@@ -33,8 +33,8 @@ typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar l
 constexpr int kPagedWgs = 256;        // workgroups of a split launch: one per CU
 // Tiles (and sequences) that a split launch plans in LDS; with more, a workgroup takes one and the last round of them is
 // short against the others.  273 tiles, ragged: 177 us split, 237 not; 512 tiles of 225 to 256 pages, two for every
-// workgroup: 966 split, 918 not.
-constexpr int kPagedMaxTiles = 1024;
+// workgroup: 966 split, 918 not; 1040 tiles (4160 tokens over 32768 keys), a few more than four: 3.77 ms split, 4.33 not.
+constexpr int kPagedMaxTiles = 2048;
 constexpr int64_t kPagedMaxRows = 1 << 27;  // (token, head) rows, fewer than this (PagedArgs::per_head)
 // Pages that a sequence can have (a table's width), up to which no tile is split: one token, 16 heads, 512 keys take
 // 14.2 us in one workgroup and 8.5 + 4.6 us over eight and with the join, and the second launch costs the caller 4 us
@@ -357,11 +357,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   } else {
     // one workgroup a tile: sequence b's are the workgroups from `before(b)` on, which leaves it as many as it has tiles
     auto before = [&](int b) { return min(max(p.cu[b], 0), p.n_tokens) * A.heads / BM + b; };
-    tile = w;
     seq = last_seq(p.n_seqs, [&](int b) { return before(b) <= w; });
     if (seq < 0 || seq >= p.n_seqs) return;
     seq_tile0 = before(seq);
-    if (tile - seq_tile0 >= SeqRows(A, seq).tiles(BM)) return;
+    const int j = w - seq_tile0, last = SeqRows(A, seq).tiles(BM) - 1;
+    if (j < 0 || j > last) return;  // (below 0 where cu_seqlens does not ascend)
+    tile = seq_tile0 + last - j;  // the last tile, which sees the most, first
   }
 
   while (u < u_end) {
