@@ -82,8 +82,8 @@ struct PagedCfg {
 constexpr int kPagedThreads = 512;
 
 // What bounds it.  Decode: bytes; 60 sequences, 60 to 32768 keys, 447 MB of pages and rows: 102 us a call, 4.4 TB/s (a large
-// copy 4.7), 95 + 8.6 us in the two kernels.  Chunks: 2048 tokens, 16 heads over 16384 keys, 1.10 PFLOP: 0.94 to 0.97 ms,
-// 1.13 to 1.17 PFLOP/s; a large bf16 product of the library reaches 1.39.  A step of 64 rows x 64 keys takes 3750 cycles, in
+// copy 4.7), 95 + 8.6 us in the two kernels.  Chunks: 2048 tokens, 16 heads over 16384 keys, 1.10 TFLOP: 0.94 to 0.99 ms,
+// 1.10 to 1.17 PFLOP/s; a large bf16 product of the library reaches 1.39.  A step of 64 rows x 64 keys takes 3750 cycles, in
 // which a SIMD's matrix pipe works for 2176; without the scoring waves' reads of the codes it takes 2980, without the
 // second product 3160, without writing P 3300, without fetches 3680, but then at 2.19 GHz instead of 1.95: the
 // clock gives way to the power drawn.  (Scoring waves of 32 rows would halve the reads; their queries' 144 registers leave
@@ -232,13 +232,13 @@ __device__ inline void dma_pieces(const uint8_t* base, const uint32_t (&off)[N],
   if constexpr (N == 4)
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
-        "global_load_lds_dwordx4 %5, %1 offset:1024\n\tglobal_load_lds_dwordx4 %6, %1 offset:2048\n\t"
-        "global_load_lds_dwordx4 %7, %1 offset:3072\n\ts_mov_b32 m0, %0"
+        "global_load_lds_dwordx4 %5, %1 offset:0x400\n\tglobal_load_lds_dwordx4 %6, %1 offset:0x800\n\t"
+        "global_load_lds_dwordx4 %7, %1 offset:0xc00\n\ts_mov_b32 m0, %0"
         : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory");
   else if constexpr (N == 2)
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
-        "global_load_lds_dwordx4 %5, %1 offset:1024\n\ts_mov_b32 m0, %0"
+        "global_load_lds_dwordx4 %5, %1 offset:0x400\n\ts_mov_b32 m0, %0"
         : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]) : "memory");
   else
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\ts_mov_b32 m0, %0"
@@ -863,8 +863,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 
 // The split tiles' partial sums joined, in a fixed order.  An item is 32 rows x 64 / G dims of a tile: a thread takes one
 // row, 4 dims and every G'th part, so that it has few parts (up to eight, all their loads in flight together; a
-// context split over all workgroups: sixteen), and the G half-waves of the same dims are joined in LDS.
-constexpr int kCombineThreads = 512, kHalfWaves = kCombineThreads / 32;
+// context split over all workgroups: sixteen), and the G half-waves of the same dims are joined in LDS.  Bound by round
+// trips (the tiles, then the sums, which other XCDs wrote) where few tiles are split, and by the sums' bytes where many
+// are: 256 parts of 32 rows, 17 MB, 8 us; 495 of 64, 65 MB, 21 us.  Four workgroups a CU: 60 sequences 101.2 us a call, 102.6
+// with two; sixteen do no better.
+constexpr int kCombineWgs = 1024, kCombineThreads = 512, kHalfWaves = kCombineThreads / 32;
 __device__ inline int part_groups(int parts) { return parts <= 8 ? 1 : (parts <= 16 ? 2 : (parts <= 32 ? 4 : (parts <= 64 ? 8 : 16))); }
 template <int PR>
 __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(const SplitTile* __restrict__ split,
@@ -1038,7 +1041,7 @@ extern "C" int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16
     hipLaunchKernelGGL(kern, dim3(d.split ? kPagedWgs : static_cast<unsigned>(n_tokens * heads / d.bm + n_seqs)), dim3(kPagedThreads), C::BYTES, st, args);
     if (int rc = check_launch("flash_paged_mla")) return rc;
     if (!d.split) return kOk;
-    hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(512), dim3(kCombineThreads), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
+    hipLaunchKernelGGL((paged_mla_combine_kernel<C::PR>), dim3(kCombineWgs), dim3(kCombineThreads), 0, st, args.split, args.part_ml, args.part_o, args.out, lse);
     return check_launch("flash_paged_mla");
   };
   using std::integral_constant;
