@@ -332,3 +332,18 @@ def test_metadata_that_does_not_make_sense_stays_inside(cuda, seed):
             assert torch.all(t[:4] == 7.0) and torch.all(t[-4:] == 7.0)
         assert torch.all(pool[:2] == 0x55) and torch.all(pool[-2:] == 0x55)
     check(cuda, *good[:4], cu, lens, *_attend(good))
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_sequences_that_share_pages(cuda, new):
+    """A prefix in the same pages for three sequences, and a page that a sequence names twice."""
+    total = [700, 800, 700]
+    pages, table, cu, lens, rows = _paged.batch([new] * 3, total, seed=83)
+    _paged.fill(pages, table, total)
+    table[1, :9], table[2, :11] = table[0, :9], table[0, :11]
+    table[2, 3] = table[2, 2]
+    d = _paged.to(cuda, *queries(rows, HEADS, 89), pages, table, cu, lens)
+    check(cuda, *d[:4], cu, lens, *_attend(d))
+    flat, pe = torch.zeros(sum(total), 512, dtype=BF16, device=cuda), torch.zeros(sum(total), 64, dtype=BF16, device=cuda)
+    mla_cache_read(d[2], d[3], *_meta(cuda, total, total), flat, pe)
+    assert torch.equal(flat[:64 * 9], flat[700:700 + 64 * 9]) and torch.equal(flat[1500 + 128:1500 + 192], flat[1500 + 192:1500 + 256])

@@ -226,7 +226,7 @@ __device__ inline v8i two_v4i(v4i a, v4i b) { return __builtin_shufflevector(a, 
 // state, and the copies a base that no vector instruction has just written.
 template <int N>
 __device__ inline void dma_pieces(const uint8_t* base, const uint32_t (&off)[N], uint32_t lds) {
-  static_assert(N == 1 || N == 2 || N == 4, "");
+  static_assert(N == 2 || N == 4, "");
   uint32_t saved;
   uint64_t from;
   if constexpr (N == 4)
@@ -235,14 +235,11 @@ __device__ inline void dma_pieces(const uint8_t* base, const uint32_t (&off)[N],
         "global_load_lds_dwordx4 %5, %1 offset:0x400\n\tglobal_load_lds_dwordx4 %6, %1 offset:0x800\n\t"
         "global_load_lds_dwordx4 %7, %1 offset:0xc00\n\ts_mov_b32 m0, %0"
         : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory");
-  else if constexpr (N == 2)
+  else
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
         "global_load_lds_dwordx4 %5, %1 offset:0x400\n\ts_mov_b32 m0, %0"
         : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]) : "memory");
-  else
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 %1, %3\n\tglobal_load_lds_dwordx4 %4, %1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off[0]) : "memory");
 }
 __device__ inline void dma_words(const uint8_t* base, uint32_t off, uint32_t lds) {  // 4 bytes a lane
   uint32_t saved;
