@@ -8,8 +8,9 @@
 // MFMA; the other operand is split into two e4m3 numbers, x = hi + lo / 32:
 //   q / sigma (sigma: a power of two that brings the row's largest magnitude into [128, 256)): exact for
 //     values down to 2^-15 of the row's largest, below that within 2^-23 of it;
-//   p * scale_j * r (r: a power of two that brings the largest to kP at most; kept <= 256): 8 to 9 significant bits,
-//     as bf16, down to 2^-20 of the largest.
+//   p * scale_j over a power of two that brings the largest of the row's 32 keys (one half of a page) into [128, 256), the
+//     scale of that operand in the MFMA: within 2^-8 of the value, as bf16, down to 2^-15 of the largest, below that
+//     within 2^-22 of it.  Nothing else sets that power: not the row's other keys, and no other row.
 // Two fp8 products take the time of one in bf16, and no code is converted: with codes turned into bf16 the
 // conversions alone (64 a page and wave for each product and 32 rows) would take as long as the products.
 // Scores are U = scale_j * (codes . q / sigma) + (q_pe / sigma) . rope (bf16 MFMA), the exponent U * (sigma *
@@ -26,6 +27,7 @@ namespace tl {
 typedef uint32_t u32x4p __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2p __attribute__((ext_vector_type(2)));
 typedef int v2i __attribute__((ext_vector_type(2)));
+typedef short v2s __attribute__((ext_vector_type(2)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
@@ -51,8 +53,9 @@ constexpr int kPagedStart = 10;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
 constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
-constexpr int kPLog = 5;             // a weight times key scale is below kP = 2^kPLog when m and r are set,
-constexpr float kPMost = 256.0f;     // and kPMost at most until they are set again
+// A weight times key scale, in units of 1 / r (the row's largest when m and r were set, below 2 then), until they are set
+// again: sums of 2^26 such times a code are far inside fp32's range.
+constexpr float kPMost = 0x1p40f;
 constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
 
 // Eight waves, two on a SIMD: 0 .. 3 score, 4 .. 7 multiply.  Scoring wave w takes the 16 rows of group w / KG against the
@@ -66,13 +69,20 @@ struct PagedCfg {
   static constexpr int RG = BM / 16, KG = 4 / RG, KT = 4 / KG;
   static constexpr int RT2 = (BM + 31) / 32;     // 32-row tiles of the second product
   static constexpr int PR = RT2 * 32;            // rows of P in LDS
+  // Keys of a P row that share a power of two: 32, a block of the MFMA.  With 16-row tiles a scoring wave has 16 keys and
+  // would have to wait for another's, so its odd 16 keys take the P row 16 behind, which has no other use: each P row holds
+  // every other 16 keys, with zeros between, and the two rows' sums are added at the end.
+  static constexpr bool kTwoRows = BM == 16;
+  static constexpr int BT = KT < 2 ? KT : 2;     // 16-key tiles of a block in a scoring wave
   static constexpr int SCALE_OFF = kSlots * kSlotBytes;
   static constexpr int P_OFF = SCALE_OFF + kSlots * kKvPageKeys * 4;
   static constexpr int P_BYTES = PR * kPStride;  // one of hi, lo of one buffer
-  static constexpr int STAT_OFF = P_OFF + 4 * P_BYTES;      // [KG][BM] f32
-  static constexpr int ALPHA_OFF = STAT_OFF + KG * BM * 4;  // [PR] f32
-  static constexpr int ROWL_OFF = ALPHA_OFF + PR * 4;       // [PR] f32
-  static constexpr int FLAG_OFF = ROWL_OFF + PR * 4;        // [4] i32
+  static constexpr int POW_OFF = P_OFF + 4 * P_BYTES;       // [2][32][2] u32: E8M0 of hi, lo of P rows n, n + 32; block
+  static constexpr int STAT_OFF = POW_OFF + 2 * 32 * 2 * 4; // [3][KG][BM] f32
+  static constexpr int ALPHA_OFF = STAT_OFF + 3 * KG * BM * 4;  // [BM] f32
+  static constexpr int ROWL_OFF = ALPHA_OFF + BM * 4;       // [BM] f32
+  static constexpr int UNIT_OFF = ROWL_OFF + BM * 4;        // [BM] f32
+  static constexpr int FLAG_OFF = UNIT_OFF + BM * 4;        // [4] i32
   static constexpr int SCAN_OFF = FLAG_OFF + 16;            // [24] i32
   static constexpr int SEQ_OFF = SCAN_OFF + 96;             // [kPagedMaxTiles] i32: tiles up to sequence b and with it
   static constexpr int TILE_OFF = SEQ_OFF + kPagedMaxTiles * 4;  // [kPagedMaxTiles] i32: pages up to tile t and with it
@@ -213,11 +223,26 @@ __device__ inline int upper(const int* a, int n, int x) {
   return lo;
 }
 
+// Max over the lanes i, i ^ 16, i ^ 32, i ^ 48, in all of them; the sum with lane i ^ 16.
+__device__ inline float four_max(float v) {
+  const u32x2p a = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  const float x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u32x2p b = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float pair_sum(float v) {
+  const u32x2p a = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 __device__ inline v4f mfma16_fp8(const v8i& a, const v8i& b, v4f c, int scale_b) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, kScaleOne, 0, scale_b);
 }
+// scale_b: byte SEL of the scale of b's column n, for the first 16 bytes of lanes n and n + 32 in lane n, for the others in lane
+// n + 32.
+template <int SEL>
 __device__ inline v16f mfma32_fp8(const v8i& a, const v8i& b, v16f c, int scale_b) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, kScaleOne, 0, scale_b);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, kScaleOne, SEL, scale_b);
 }
 __device__ inline v8i two_v4i(v4i a, v4i b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
@@ -248,6 +273,18 @@ __device__ inline void dma_words(const uint8_t* base, uint32_t off, uint32_t lds
                : "=&s"(saved), "=&s"(from) : "s"(lds), "s"(base), "v"(off) : "memory");
 }
 
+// Four values over a power of two as hi + lo / 32, four codes each; to_lo = the power / 32.
+__device__ inline void split4(const float (&x)[4], float power, float to_lo, int& hi, int& lo) {
+  v2s h = {0, 0}, l = {0, 0};
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[0], x[1], power, false);
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[2], x[3], power, true);
+  hi = __builtin_bit_cast(int, h);
+  const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, power, true);
+  l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, x[0] - a[0], x[1] - a[1], to_lo, false);
+  l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, x[2] - b[0], x[3] - b[1], to_lo, true);
+  lo = __builtin_bit_cast(int, l);
+}
+
 // Four values (finite, <= 256 in magnitude, or NaN) as hi + lo / 32, four codes each.
 __device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
@@ -260,7 +297,7 @@ __device__ inline void split4(const float (&x)[4], int& hi, int& lo) {
 template <int BM>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const PagedArgs A) {
   using C = PagedCfg<BM>;
-  constexpr int KG = C::KG, KT = C::KT, RT2 = C::RT2, DT = 4;
+  constexpr int KG = C::KG, KT = C::KT, BT = C::BT, RT2 = C::RT2, DT = 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -271,9 +308,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   float* stat = reinterpret_cast<float*>(smem + C::STAT_OFF);
   float* alpha_l = reinterpret_cast<float*>(smem + C::ALPHA_OFF);
   float* rowl = reinterpret_cast<float*>(smem + C::ROWL_OFF);
+  float* unit_l = reinterpret_cast<float*>(smem + C::UNIT_OFF);
   int* flag = reinterpret_cast<int*>(smem + C::FLAG_OFF);
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8_ptr)smem));
   const int w = blockIdx.x;
+
+  if constexpr (C::kTwoRows)  // the keys between a P row's own
+    for (int i = tid; i < 4 * C::P_BYTES / 16; i += kPagedThreads) reinterpret_cast<v4i*>(smem + C::P_OFF)[i] = v4i{0, 0, 0, 0};
 
   // ---- the work of this workgroup
   int n_tiles = 0, u = 0, u_end = 1, quota = 1, tile = 0, seq = 0, seq_tile0 = 0;
@@ -387,7 +428,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
     const int rows = min(BM, s.n_rows - in_seq);
     const int n_pages = s.pages(A, j, BM);
     const int seen_first = s.seen(A, in_seq);             // every row sees these
-    const int seen_last = s.seen(A, in_seq + rows - 1);   // some row sees these
     const int pg0 = u - tile_u0;
     const int n = min(A.split ? min(tile_u1, u_end) - u : n_pages, n_pages - pg0);
     const const_i32 table = (const_i32)(p.table + static_cast<int64_t>(seq) * p.max_pages + pg0);
@@ -546,30 +586,45 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       const int my_quad = kg * KT * 16 + 4 * g;    // the keys of this lane's scores: my_quad .. +3, and 16, 32, ..
       const int at_code = my_key * kKvLatent + ((2 * g) ^ ((n16 & 7) << 1) ^ (n16 >> 3)) * 16;  // dims 32 g .. +15 (^ 16: +16 .. +31, ^ 128: 128 + 32 g ..)
       const int at_rope = kKvPageKeys * kKvLatent + my_key * 128 + (g ^ (n16 >> 1)) * 16;  // rope dims 8 g .. (^ 64: 32 + 8 g ..)
-      const int put_p = my_row * kPStride + my_quad;
+      const int p_row = C::kTwoRows ? my_row + 16 * (kg & 1) : my_row;
+      const int put_p = p_row * kPStride + my_quad;
+      const int put_pow = C::POW_OFF + ((p_row & 31) * 2 + kg * KT / 2) * 4 + (p_row >> 5) * 2;  // the wave's first block
       const int seen = my_row < rows ? s.seen(A, in_seq + my_row) : 0;
-      // weights are e = exp2(U * f - mk), mk = m: the row's largest U * f when it was last set (-300 where it had none
-      // yet: any score is then flagged).  P is e * scale * r, r = 2^kPLog over s_ref, the largest key scale so far, rounded
-      // up to a power of two, so that P < kP where m is set.  l is the sum of such e, O of P times codes.
-      float m = -INFINITY, mk = 0.f, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, s_ref = 0.f, r = 1.f;
+      // Weights are e = exp2(U * f - mk), mk = m: the row's largest U * f when it was last set (-300 where it has none).
+      // P is e * scale * r; r = 1 / unit, a power of two of the row's largest e * scale when it was set.  l is the sum of such
+      // e, O of P times codes.  m and r are set where the row's first keys are, and where a P would pass kPMost: both follow
+      // from the row's own keys alone, and where they stay another row's change leaves the row's results as they were.
+      float m = -INFINITY, mk = 0.f, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, pmost = 0.f, r = 1.f;
       if (f != f) f = 0.f;
       v4f U[KT];
 
-      // A weight, times its key's scale * r, from its score; the largest and the sum so far.
-      auto weigh = [&](float score, float scale, float& sum, float& pmax) {
+      auto weights_at = [&](int k) { return smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p; };
+      // A weight, times its key's scale and r, from its score; the largest and the sum so far.  (scale * r may pass fp32's
+      // range where e is 0.)
+      auto weigh = [&](float score, float scale, float& sum, float& most) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(score, f, -mk));
         sum += e;
-        const float x = e * scale;
-        pmax = fmaxf(pmax, __builtin_fabsf(x));
+        const float x = e * scale * r;
+        most = fmaxf(most, __builtin_fabsf(x));
         return x;
       };
-      auto put = [&](uint8_t* P, int kt, const float (&x)[4]) {
-        int hi, lo;
-        split4(x, hi, lo);
-        *reinterpret_cast<int*>(P + kt * 16) = hi;
-        *reinterpret_cast<int*>(P + kt * 16 + C::P_BYTES) = lo;
+      // The P of block `b`'s weights, whose largest in this lane is `most`: over the power of two that brings the block's
+      // largest into [128, 256) (2^-114 at least, far below what is left in a sum).
+      auto put_block = [&](int k, int b, const float (&x)[BT][4], float most) {
+        most = four_max(most);
+        pmost = fmaxf(pmost, most);
+        const uint32_t top = max(__float_as_uint(most) & 0x7f800000u, 20u << 23);
+        uint8_t* P = weights_at(k);
+#pragma unroll
+        for (int i = 0; i < BT; ++i) {
+          int hi, lo;
+          split4(x[i], __uint_as_float(top - (7u << 23)), __uint_as_float(top - (12u << 23)), hi, lo);
+          *reinterpret_cast<int*>(P + (b * BT + i) * 16) = hi;
+          *reinterpret_cast<int*>(P + (b * BT + i) * 16 + C::P_BYTES) = lo;
+        }
+        const uint32_t e = top >> 23;
+        if (g == 0) *reinterpret_cast<uint16_t*>(smem + put_pow + b * 4 + (k & 1) * 256) = static_cast<uint16_t>(e - 7 | (e - 12) << 8);
       };
-      auto weights_at = [&](int k) { return smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + put_p; };
       // U of page k, and with WEIGH its weights, whose tile of 16 keys is one behind that of the products: the wave issues
       // the vector instructions of the one while the matrix pipe works on the other.  Whether all weights were <= kPMost.
       // 4 KT items of 128 dims, each item's operand read ahead of its products.
@@ -581,8 +636,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       auto scores = [&](int k, int slot, auto weigh_tag) {
         constexpr bool WEIGH = decltype(weigh_tag)::value;
         constexpr int kItems = 4 * KT, kAhead = kItems < 4 ? kItems : 4;  // (8: 962 -> 979 us at 2048 tokens, 16 heads, 16384 keys; 6: 970)
-        uint8_t* P = weights_at(k);
-        float pmax = 0.f, sum = 0.f;
+        float most = 0.f, sum = 0.f;
+        pmost = 0.f;
+        float w[BT][4];
         v8i a[kItems];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) a[i] = load_key(slot, i);
@@ -598,7 +654,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
               part[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                   *reinterpret_cast<const v8bf*>(smem + slot * kSlotBytes + (at_rope ^ (ks * 64)) + kt * 16 * 128), qr[ks], part[kt], 0, 0, 0);
           }
-          float w[4];
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             if (kt < KT) {
@@ -611,15 +666,18 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
               // (an infinite scale as NaN: a score of -inf is a masked one)
               const float scale = __builtin_fmaf(sk[kt - 1][ks], 0.f, sk[kt - 1][ks]);
               U[kt - 1][ks] = __builtin_fmaf(x[kt - 1][ks], scale, part[kt - 1][ks]);
-              if constexpr (WEIGH) w[ks] = weigh(U[kt - 1][ks], scale * r, sum, pmax);
+              if constexpr (WEIGH) w[(kt - 1) % BT][ks] = weigh(U[kt - 1][ks], scale, sum, most);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
           if constexpr (WEIGH)
-            if (kt > 0) put(P, kt - 1, w);
+            if (kt > 0 && kt % BT == 0) {
+              put_block(k, kt / BT - 1, w, most);
+              most = 0.f;
+            }
         }
         psum = sum;
-        return !__any(pmax > kPMost);
+        return !__any(pmost > kPMost);
       };
       // the scores of page k that the row does not see
       auto mask_scores = [&](int k, int id) {
@@ -630,48 +688,78 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           for (int i = 0; i < 4; ++i) U[kt][i] = at + kt * 16 + i < end ? U[kt][i] : -INFINITY;
       };
 
-      // The weights of page k from U where some are masked (-inf), whatever those keys' scales are.
+      // A key's scale, 0 where the row does not see it, whatever it holds.
+      auto scale_seen = [&](int kt, int slot) {
+        v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sk[i] = U[kt][i] == -INFINITY ? 0.f : sk[i];
+        return sk;
+      };
+      // The weights of page k from U where some are masked (-inf).
       auto weights = [&](int k, int slot) {
-        uint8_t* P = weights_at(k);
-        float pmax = 0.f, sum = 0.f;
+        float sum = 0.f;
+        pmost = 0.f;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const v4f sk = *reinterpret_cast<const v4f*>(smem + C::SCALE_OFF + (slot * kKvPageKeys + my_quad + kt * 16) * 4);
-          float w[4];
+        for (int b = 0; b < KT / BT; ++b) {
+          float w[BT][4], most = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = weigh(U[kt][i], U[kt][i] == -INFINITY ? 0.f : sk[i] * r, sum, pmax);
-          put(P, kt, w);
+          for (int i = 0; i < BT; ++i) {
+            const v4f sk = scale_seen(b * BT + i, slot);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[i][c] = weigh(U[b * BT + i][c], sk[c], sum, most);
+          }
+          put_block(k, b, w, most);
         }
         psum = sum;
-        return !__any(pmax > kPMost);
+        return !__any(pmost > kPMost);
       };
 
-      // New m and r from page k's scores and scales, O and l brought to them, P again.  Every wave comes here, or none.
-      auto settle = [&](int k, int slot, int id) {
-        float x = -INFINITY;
+      auto one_over = [](float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); };
+      // New m and r from page k's scores and scales for the rows that need them, O and l brought to them, P again.  Every wave
+      // comes here, or none.
+      auto settle = [&](int k, int slot) {
+        float x = -INFINITY, over = pmost;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(fmaxf(U[kt][0], U[kt][1]), fmaxf(U[kt][2], U[kt][3])));
-        x = fmaxf(x, __shfl_xor(x, 16));
-        x = fmaxf(x, __shfl_xor(x, 32));
-        if (KG > 1 && g == 0) stat[kg * BM + my_row] = x;
-        // the largest finite scale of the page's keys that some row sees
-        const float sk = __builtin_fabsf(reinterpret_cast<const float*>(smem + C::SCALE_OFF + slot * kKvPageKeys * 4)[lane]);
-        const bool use = (pg0 + k) * kKvPageKeys + lane < seen_last && sk < INFINITY && valid(id);
-        s_ref = fmaxf(s_ref, fmaxf(wave_max_f32(use ? sk : 0.f), 0x1p-100f));
-        __syncthreads();
-        if constexpr (KG > 1)
+        x = four_max(x);
+        if constexpr (KG > 1) {
+          if (g == 0) {
+            stat[kg * BM + my_row] = x;
+            stat[(KG + kg) * BM + my_row] = over;
+          }
+          __syncthreads();
 #pragma unroll
-          for (int i = 0; i < KG; ++i) x = fmaxf(x, stat[i * BM + my_row]);
-        const float was = mk, was_r = r;
-        const bool none = m == -INFINITY;
-        m = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
-        mk = m == -INFINITY ? -300.f : m;
-        // s_ref < 2^(e - 126), e its exponent's bits, 27 .. 254
-        const uint32_t e = __builtin_amdgcn_readfirstlane(__float_as_uint(s_ref) >> 23);
-        r = __uint_as_float((127 + kPLog + 126 - e) << 23);
+          for (int i = 0; i < KG; ++i) {
+            x = fmaxf(x, stat[i * BM + my_row]);
+            over = fmaxf(over, stat[(KG + i) * BM + my_row]);
+          }
+        }
+        const bool none = m == -INFINITY, set = none || over > kPMost;
+        const float was = mk;
+        if (set) {
+          m = fmaxf(m, x == -INFINITY ? -INFINITY : x * f);
+          mk = m == -INFINITY ? -300.f : m;
+        }
         const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(was - mk);
+        // the row's largest weight times scale on this page
+        float top = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const v4f sk = scale_seen(kt, slot);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(__builtin_amdgcn_exp2f(__builtin_fmaf(U[kt][i], f, -mk)) * sk[i]));
+        }
+        top = four_max(top);
+        if constexpr (KG > 1) {
+          if (g == 0) stat[(2 * KG + kg) * BM + my_row] = top;
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < KG; ++i) top = fmaxf(top, stat[(2 * KG + i) * BM + my_row]);
+        }
+        const float unit = one_over(r);
+        if (set) r = __uint_as_float((254u << 23) - min(max(__float_as_uint(fmaxf(top, alpha * unit)) & 0x7f800000u, 27u << 23), 253u << 23));
         l *= alpha;
-        if (kg == 0 && g == 0) alpha_l[my_row] = alpha * (r / was_r);
+        if (kg == 0 && g == 0) alpha_l[my_row] = alpha * r * unit;  // (in this order: no factor of it passes fp32's range)
         weights(k, slot);
         __syncthreads();
       };
@@ -681,7 +769,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         if (masked(0, id0)) clean(0);
         scores(0, 0, std::false_type{});
         if (masked(0, id0)) mask_scores(0, id0);
-        settle(0, 0, id0);
+        settle(0, 0);
         int next = 1, free = 2, slot = 0, id = id1, id_after = id_of(2);
         bool fresh = !valid(id0);  // no page so far had keys: nothing is set yet
 #pragma unroll 1
@@ -700,7 +788,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           if ((!fits || fresh) && lane == 0) flag[(k + 1) & 3] = 1;
           fresh = fresh && !valid(id);
           arrive();
-          if (flag[(k + 1) & 3]) settle(k + 1, next, id);
+          if (flag[(k + 1) & 3]) settle(k + 1, next);
           id = id_after;
           id_after = id_of(k + 3);
           const int was = slot;
@@ -712,12 +800,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       }
       // l over the lanes and waves of a row
       __syncthreads();
-      if (tid == 0) scan[0] = static_cast<int>(__float_as_uint(1.0f / r));
       l += __shfl_xor(l, 16);
       l += __shfl_xor(l, 32);
       if (g == 0) {
         stat[kg * BM + my_row] = l;
-        if (kg == 0) alpha_l[my_row] = m == -INFINITY ? -INFINITY : mk;
+        if (kg == 0) {
+          alpha_l[my_row] = m == -INFINITY ? -INFINITY : mk;
+          unit_l[my_row] = one_over(r);
+        }
       }
       __syncthreads();
       if (tid < BM) {
@@ -729,9 +819,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       __syncthreads();
     } else {
       const int dw = wave - 4;  // dims 128 dw ..
-      const int at_value = (32 * half + (n16 >> 1)) * kKvLatent + (dw & 2) * 128 + (lane & 1) * 8 +
-                           ((8 * (dw & 1) + (g & 1)) ^ (n16 & 14)) * 16;  // 32-dim tile d: ^ 32 d; keys 8 .. 15 and 24 .. 31: ^ 16
-      const int at_p = n32 * kPStride + half * 32;
+      const int at_value = (16 * half + (n16 >> 1)) * kKvLatent + (dw & 2) * 128 + (lane & 1) * 8 +
+                           ((8 * (dw & 1) + (g & 1)) ^ (n16 & 14)) * 16;  // 32-dim tile d: ^ 32 d; keys 8 .. 15 behind it: ^ 16
+      const int at_p = n32 * kPStride + half * 16;
+      const int at_pow = C::POW_OFF + (n32 * 2 + half) * 4;
       v16f o[RT2][DT];
 #pragma unroll
       for (int a = 0; a < RT2; ++a)
@@ -740,10 +831,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[a][d][i] = 0.f;
 
-      // O^T += latent^T P^T of page k: rows of A are dims, of B the tile's rows, 64 keys in one MFMA.  The operand lane
-      // (dim n32, half) needs 32 keys of its dim, a column of the key-major codes: ds_read_b64_tr_b8 gives lane i of a
-      // 16-lane group byte i % 8 of the 8 bytes at lane 2 j + i / 8's address as its byte j, so lane i addresses key
-      // 32 half + 8 r + i / 2, half i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
+      // O^T += latent^T P^T of page k: rows of A are dims, of B the tile's rows, 64 keys in one MFMA, whose two scale blocks are
+      // the page's halves: lane (n32, half) holds keys 16 half .. +15 of the one and of the other.  A lane's dim is
+      // a column of the key-major codes: ds_read_b64_tr_b8 gives lane i of a 16-lane group byte i % 8 of the 8 bytes at
+      // lane 2 j + i / 8's address as its byte j, so lane i addresses key 32 (r / 2) + 16 half + 8 (r % 2) + i / 2, half
+      // i % 2 of the group's 16-dim chunk, and receives 8 keys of dim i.
       auto product = [&](int k, int slot) {
         const uint8_t* P = smem + C::P_OFF + (k & 1) * 2 * C::P_BYTES + at_p;
         const int at = slot * kSlotBytes + at_value;  // (a slot's place leaves bits 4 .. 8 alone)
@@ -751,7 +843,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           v8i v;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(smem + (at ^ (32 * d + 16 * (r & 1))) + r * 8 * kKvLatent));
+            const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(smem + (at ^ (32 * d + 16 * (r & 1))) + ((r >> 1) * 32 + (r & 1) * 8) * kKvLatent));
             v[2 * r] = x[0];
             v[2 * r + 1] = x[1];
           }
@@ -763,28 +855,33 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         for (int a = 0; a < RT2; ++a) {
           const v4i* hi = reinterpret_cast<const v4i*>(P + a * 32 * kPStride);
           const v4i* lo = reinterpret_cast<const v4i*>(P + a * 32 * kPStride + C::P_BYTES);
-          ph[a] = two_v4i(hi[0], hi[1]);
-          pl[a] = two_v4i(lo[0], lo[1]);
+          ph[a] = two_v4i(hi[0], hi[2]);
+          pl[a] = two_v4i(lo[0], lo[2]);
         }
+        const int pow = *reinterpret_cast<const int*>(smem + at_pow + (k & 1) * 256);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           if (d + 1 < DT) v[(d + 1) & 1] = load_value(d + 1);
           __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int a = 0; a < RT2; ++a) {
-            o[a][d] = mfma32_fp8(v[d & 1], ph[a], o[a][d], kScaleOne);
-            o[a][d] = mfma32_fp8(v[d & 1], pl[a], o[a][d], kScaleLo);
+          o[0][d] = mfma32_fp8<0>(v[d & 1], ph[0], o[0][d], pow);
+          o[0][d] = mfma32_fp8<1>(v[d & 1], pl[0], o[0][d], pow);
+          if constexpr (RT2 > 1) {
+            o[1][d] = mfma32_fp8<2>(v[d & 1], ph[1], o[1][d], pow);
+            o[1][d] = mfma32_fp8<3>(v[d & 1], pl[1], o[1][d], pow);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       };
       auto settle = [&](bool first) {
-        __syncthreads();
+        if constexpr (KG > 1) {
+          __syncthreads();
+          __syncthreads();
+        }
         __syncthreads();
         if (first) return;  // (nothing to bring along)
 #pragma unroll
         for (int a = 0; a < RT2; ++a) {
-          const float x = alpha_l[min(a * 32 + n32, BM - 1)];
+          const float x = alpha_l[(a * 32 + n32) & (BM - 1)];
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -812,11 +909,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           free = was;
         }
         product(n - 1, slot);
+        if constexpr (C::kTwoRows)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[0][d][i] = pair_sum(o[0][d][i]);
       }
       __syncthreads();
       __syncthreads();
       __syncthreads();
-      const float unit = __uint_as_float(scan[0]);  // 1 / r, a power of two
 
       // ---- the rows' results, or the tile's partial sums
       if (!A.split || (u == tile_u0 && u_end >= tile_u1)) {
@@ -826,7 +927,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         for (int a = 0; a < RT2; ++a) {
           const int r = a * 32 + n32;
           if (r < rows) {
-            const float L = rowl[r], x = L == 0.f ? 0.f : 1.0f / L * unit;
+            const float L = rowl[r], x = L == 0.f ? 0.f : 1.0f / L * unit_l[r];
             uint16_t* dst = A.out + (row0 + r) * kKvLatent + dw * 128 + 4 * half;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -843,6 +944,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 #pragma unroll
         for (int a = 0; a < RT2; ++a)
           if (a * 32 + n32 < rows) {
+            const float unit = unit_l[a * 32 + n32];
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
