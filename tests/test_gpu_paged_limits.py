@@ -1,0 +1,30 @@
+"""flash_paged_mla at the ends of its ranges: the widest tables, the smallest scales, the largest keys.  The tolerance is that of
+test_gpu_paged_weights."""
+import pytest
+import torch
+
+from oracle import paged
+from tests.test_gpu_paged_weights import close, put
+from tilert_amd.flash_paged_mla import flash_paged_mla
+
+pytestmark = pytest.mark.gpu
+ARCH = "deepseek_v3_2"
+BF16, I32 = torch.bfloat16, torch.int32
+
+
+@pytest.mark.parametrize("columns", [2 ** 20 - 11, 2 ** 20])
+def test_the_most_tiles_over_the_widest_table(cuda, columns):
+    """2048 row tiles: split with the one table, one workgroup a tile with the other."""
+    g = torch.Generator(device=cuda).manual_seed(3)
+    tokens, keys = 8188, 8300
+    n = -(-keys // 64)
+    pages = torch.empty(n, paged.PAGE_BYTES, dtype=torch.uint8, device=cuda)
+    ids = torch.full((columns,), -1, dtype=I32, device=cuda)
+    ids[:n] = torch.randperm(n, generator=g, device=cuda).to(I32)
+    put(pages, ids, torch.randn(keys, 512, generator=g, device=cuda), torch.randn(keys, 64, generator=g, device=cuda))
+    q, qp = ((torch.randn(tokens, 16, w, generator=g, device=cuda) * 0.3).to(BF16) for w in (512, 64))
+    out, lse = torch.full_like(q, 7.0), torch.full((tokens, 16), 7.0, device=cuda)
+    cu, lens = torch.tensor([0, tokens], dtype=I32, device=cuda), torch.tensor([keys], dtype=I32, device=cuda)
+    flash_paged_mla(q, qp, pages, ids[None], cu, lens, out, lse, model_arch=ARCH)
+    close(out, lse, q, qp, pages, ids, keys - tokens, [0, 1, 4000, tokens - 1])
+    assert not (lse == 7.0).any()

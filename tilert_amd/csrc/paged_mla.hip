@@ -1083,7 +1083,9 @@ inline PagedPlan paged_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads, int
   d.bm = each <= 16 ? 16 : (each <= 128 ? 32 : 64);
   d.pr = d.bm < 32 ? 32 : d.bm;
   d.tiles = rows / d.bm + (n_seqs < n_tokens ? n_seqs : n_tokens);
-  d.split = d.tiles <= kPagedMaxTiles && n_seqs <= kPagedMaxTiles && max_pages > kPagedFew;
+  // (units and the end of the last workgroup's share of them, up to kPagedWgs behind, are ints)
+  d.split = d.tiles <= kPagedMaxTiles && n_seqs <= kPagedMaxTiles && max_pages > kPagedFew &&
+            d.tiles * (max_pages + kPagedStart) <= INT32_MAX - kPagedWgs;
   if (d.split) {
     d.ml_at = kPagedWgs * sizeof(SplitTile);
     d.o_at = d.ml_at + static_cast<size_t>(2 * kPagedWgs) * d.pr * sizeof(float2);
