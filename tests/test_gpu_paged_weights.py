@@ -6,7 +6,8 @@ sum_j p_j |latent_j| for the weights; the scores' error) and what a weight much 
 32 keys loses.  x = p_j scale_j over the power of two that brings the largest of the 32 into [128, 256) is held as two e4m3
 numbers, hi + lo / 32, whose smallest steps are 2^-9 and 2^-9 / 32 = 2^-14: where x is too small for 2^-8 of it, it is off by
 half of the latter, 2^-15, at most, which is 2^-22 of the largest, 128 or more.  An output's sum of |code| times that, over
-the keys of each 32, is the term `beside`.
+the keys of each 32, is the term `beside`.  An exponential below 2^-126 of the row's largest is below fp32's normal numbers and
+may be 0: 2^-126 of sum_j |latent_j| over the keys.
 
 Every number of tokens per sequence runs in its own tile height (16, 32 and 64 rows)."""
 import math
@@ -50,7 +51,7 @@ def definition(q, qp, pages, ids, n, scale):
     top = torch.nn.functional.pad(w * s, (0, pad)).view(w.shape[0], -1, 32).amax(-1)
     beside = 2.0 ** -22 * top @ torch.nn.functional.pad(code.abs(), (0, 0, 0, pad)).view(-1, 32, 512).sum(1)
     out = w @ latent
-    tol = 2 ** -8 * out.abs() + (2 ** -8 + 2 * (slack[:, None] + 2 ** -18)) * (w @ latent.abs()) + beside
+    tol = 2 ** -8 * out.abs() + (2 ** -8 + 2 * (slack[:, None] + 2 ** -18)) * (w @ latent.abs()) + beside + 2.0 ** -126 * latent.abs().sum(0)
     return out, lse, tol, slack + 2 ** -20 * (1 + lse.abs())
 
 
@@ -172,3 +173,19 @@ def test_keys_of_very_different_sizes(cuda, new, heads, total, powers):
     scales = paged.views(case[2])[1]
     scales *= torch.pow(2.0, torch.randint(0, powers + 1, scales.shape, generator=g).float()).to(cuda)
     check_all(case, *run(cuda, *case))
+
+
+@pytest.mark.parametrize("new,heads", TILES)
+@pytest.mark.parametrize("first", [0, 64, 256])
+def test_keys_of_scale_zero_with_all_the_weight(cuda, new, heads, first):
+    """Keys without a latent, from page `first` / 64 on, whose rope parts outweigh the others' by e^200: zeros, and the lse."""
+    total = first + 100
+    case = _sized(cuda, new, total, heads, 113)
+    case[1].fill_(0.5)
+    codes, scales, ropes = paged.views(case[2])
+    p = torch.arange(first, total - new, device=cuda)
+    at = (case[3][0, p // 64].long(), p % 64)
+    codes.view(torch.uint8)[at], scales[at], ropes[at] = 0, 0.0, 46.0
+    out, lse = run(cuda, *case)
+    check_all(case, out, lse)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()

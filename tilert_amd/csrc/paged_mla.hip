@@ -53,8 +53,9 @@ constexpr int kPagedStart = 10;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
 constexpr int kPStride = 80;        // bytes of a P row of 64 codes: 8 rows' 16-byte pieces are in different banks
-// A weight times key scale, in units of 1 / r (the row's largest when m and r were set, below 2 then), until they are set
-// again: sums of 2^26 such times a code are far inside fp32's range.
+// A weight times key scale, in units of 1 / r (the row's largest when m and r were set, below 2 then), and a lane's sum of
+// weights on a page, until m and r are set again: sums of 2^26 such times a code are far inside fp32's range.  The second is
+// for keys whose scale is 0, or far below the row's others.
 constexpr float kPMost = 0x1p40f;
 constexpr int kScaleOne = 0x7f7f7f7f, kScaleLo = 0x7a7a7a7a;  // E8M0: 1, 2^-5
 
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       const int seen = my_row < rows ? s.seen(A, in_seq + my_row) : 0;
       // Weights are e = exp2(U * f - mk), mk = m: the row's largest U * f when it was last set (-300 where it has none).
       // P is e * scale * r; r = 1 / unit, a power of two of the row's largest e * scale when it was set.  l is the sum of such
-      // e, O of P times codes.  m and r are set where the row's first keys are, and where a P would pass kPMost: both follow
+      // e, O of P times codes.  m and r are set where the row's first keys are, and where a P or l would pass kPMost: both follow
       // from the row's own keys alone, and where they stay another row's change leaves the row's results as they were.
       float m = -INFINITY, mk = 0.f, l = f == f || seen == 0 ? 0.f : f, psum = 0.f, pmost = 0.f, r = 1.f;
       if (f != f) f = 0.f;
@@ -677,6 +678,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
             }
         }
         psum = sum;
+        pmost = fmaxf(pmost, sum);
         return !__any(pmost > kPMost);
       };
       // the scores of page k that the row does not see
@@ -711,6 +713,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           put_block(k, b, w, most);
         }
         psum = sum;
+        pmost = fmaxf(pmost, sum);
         return !__any(pmost > kPMost);
       };
 
@@ -718,7 +721,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       // New m and r from page k's scores and scales for the rows that need them, O and l brought to them, P again.  Every wave
       // comes here, or none.
       auto settle = [&](int k, int slot) {
-        float x = -INFINITY, over = pmost;
+        float x = -INFINITY, over = four_max(pmost);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) x = fmaxf(x, fmaxf(fmaxf(U[kt][0], U[kt][1]), fmaxf(U[kt][2], U[kt][3])));
         x = four_max(x);
