@@ -430,7 +430,8 @@ int tl_flash_sparse_mla(const void* q_nope_bf16, const void* q_pe_bf16, const vo
  * fp32 [dim], h = x + residual in fp32, sum_bf16 = bf16(h), n = gamma * h * 1/sqrt(mean(h^2) +
  * eps), y_bf16 = bf16(n), and per 1x128 group y_scale = the act_quant scale of max |n|
  * (scale_mode as tl_act_quant), y_fp8 = e4m3fn(clamp(n / y_scale)): norm and codes come from
- * unrounded values, where tl_rmsnorm_quant's codes are those of its bf16 output.  sum_bf16 may
+ * unrounded values, where tl_rmsnorm_quant's codes are those of its bf16 output.  y_scale is NaN
+ * for a group with a NaN or an infinity, whose codes are finite all the same.  sum_bf16 may
  * be x or residual itself; no other output may overlap an input.  Either y_bf16 or
  * (y_fp8, y_scale) may be null.  dim % 128 == 0, dim <= 16384; pointers 16-byte aligned. */
 int tl_add_rmsnorm_quant(const void* x_bf16, const void* residual_bf16, const float* gamma, float eps,

@@ -158,6 +158,14 @@ __device__ inline float row16_reduce(float v) {
   return dpp_combine<0x140, MAX>(v);  // row_mirror
 }
 
+// Max of a 32-bit unsigned value over each 16-lane row, in every lane of it.
+__device__ inline uint32_t row16_max_u32(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, false)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xf, 0xf, false)));
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xf, 0xf, false)));
+}
+
 // Max of a 32-bit unsigned value over the wave, wave-uniform (the same DPP scan).
 __device__ inline uint32_t wave_max_u32(uint32_t v) {
 #define TL_DPP_MAXU(ctrl, rmask) \

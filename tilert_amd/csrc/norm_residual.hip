@@ -4,7 +4,8 @@
 //   n = h * rsqrt(mean(h^2) + eps) * gamma, y = bf16(n)
 //   per 128 columns s = group_scale(max |n|), code = e4m3(clamp(n / s))
 // The norm is the unrounded sum's, and the codes are the unrounded norm's: one rounding each.  (rmsnorm_quant's codes
-// are those of its bf16 output.)
+// are those of its bf16 output.)  A group that holds a NaN or an infinity gets the scale NaN; its codes are finite
+// whatever it held.
 #include <type_traits>
 
 #include "common.h"
@@ -67,11 +68,12 @@ __global__ __launch_bounds__(NT) void add_rmsnorm_quant_kernel(const uint16_t* x
   for (int j = 0; j < NC; ++j) {
     const int c = tid + j * NT, cc = min(c, nch - 1);
     const v4f g0 = reinterpret_cast<const v4f*>(gamma)[2 * cc], g1 = reinterpret_cast<const v4f*>(gamma)[2 * cc + 1];
-    float n[8], amax = 0.f;
+    float n[8];
+    uint32_t most = 0;  // the largest magnitude's bits: a NaN's are above an infinity's
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       n[i] = h[j][i] * r * (i < 4 ? g0[i & 3] : g1[i & 3]);
-      amax = fmaxf(amax, __builtin_fabsf(n[i]));
+      most = max(most, __float_as_uint(n[i]) & 0x7fffffffu);
     }
     if (y && c < nch) {
       u32x4r v;
@@ -80,7 +82,8 @@ __global__ __launch_bounds__(NT) void add_rmsnorm_quant_kernel(const uint16_t* x
       reinterpret_cast<u32x4r*>(y + row)[c] = v;
     }
     if (y8) {
-      const float s = group_scale(row16_reduce<true>(amax), scale_mode);
+      most = row16_max_u32(most);
+      const float s = most < 0x7f800000u ? group_scale(__uint_as_float(most), scale_mode) : __builtin_nanf("");
       const uint2 code = quant8_e4m3(n, s);
       if (c < nch) {
         reinterpret_cast<uint2*>(y8 + row)[c] = code;

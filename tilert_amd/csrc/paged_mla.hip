@@ -205,14 +205,6 @@ __device__ inline bool block_scan2(int& a, int& b, bool no, int* part, int& tota
   return !bad;
 }
 
-// Max over each 16-lane row, in every lane of it.
-__device__ inline uint32_t row16_max_u32(uint32_t v) {
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, false)));
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, false)));
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xf, 0xf, false)));
-  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xf, 0xf, false)));
-}
-
 // The first index of an ascending array that is > x.
 __device__ inline int upper(const int* a, int n, int x) {
   int lo = 0;

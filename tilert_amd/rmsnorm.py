@@ -63,7 +63,8 @@ def add_rmsnorm_quant(hidden_in: torch.Tensor, residual_in: torch.Tensor, gamma_
     """``rmsnorm_quant`` behind a residual sum (RMSNorm.forward with a residual, tilert/models/common.py:92-133):
     residual_out = bf16(hidden_in + residual_in), and the norm of the unrounded sum to hidden_out (bf16) and, quantised
     per 1x128 group from its unrounded values, to quant_hidden_out (e4m3fn) with quant_hidden_scale_out (fp32
-    (..., dim // 128)).  hidden_out, or the two quantised outputs, may be left out.  residual_out may be
+    (..., dim // 128); NaN for a group that holds a NaN or an infinity, whose codes are finite all the same).
+    hidden_out, or the two quantised outputs, may be left out.  residual_out may be
     residual_in or hidden_in itself; no other output may share memory with an input."""
     if profile_logs is None:
         raise ValueError("profile_logs is required when calling add_rmsnorm_quant.")
