@@ -445,7 +445,7 @@ int tl_add_rmsnorm_quant(const void* x_bf16, const void* residual_bf16, const fl
  * 0), its cache holds seq_lens[b] keys with them, and its key at position p is row p % 64 of
  * page block_table[b, p / 64] (block_table [n_seqs, max_pages]): token t stands at position
  * seq_lens[b] - (cu_seqlens[b+1] - cu_seqlens[b]) + t - cu_seqlens[b].  n_tokens is the number
- * of rows of the call's tensors, fewer than 2^26: rows from cu_seqlens[n_seqs] on are left as they are.  No
+ * of rows of the call's tensors, at most 2^26 - 4: rows from cu_seqlens[n_seqs] on are left as they are.  No
  * metadata makes a kernel leave the pages: a position below 0 or past the table, and a page id
  * outside [0, n_pages), name no key. */
 

@@ -66,8 +66,8 @@ __device__ inline KeyPlace key_place(const PagedBatch& p, int b, int t) {
 // The host's checks of a batch; `who` names the entry point.
 inline int check_batch(const char* who, const void* pages, int64_t n_pages, const int32_t* table, int64_t max_pages,
                        const int32_t* cu, const int32_t* lens, int64_t n_seqs, int64_t n_tokens) {
-  // (a launch has fewer than 2^32 threads: a wave a token)
-  if (n_seqs < 0 || n_tokens < 0 || n_seqs >= (1ll << 24) || n_tokens >= (1ll << 26)) {
+  // (a launch has fewer than 2^32 threads: a wave a token, four tokens a workgroup)
+  if (n_seqs < 0 || n_tokens < 0 || n_seqs >= (1ll << 24) || n_tokens > (1ll << 26) - 4) {
     set_error("%s: %lld sequences, %lld tokens: out of range", who, (long long)n_seqs, (long long)n_tokens);
     return kErrArg;
   }
