@@ -4,7 +4,9 @@ import pytest
 import torch
 
 from oracle import paged
-from tests.test_gpu_paged_weights import close, put
+from tests import _paged
+from tests.test_gpu_flash_paged_mla import queries, run
+from tests.test_gpu_paged_weights import TILES, check_all, close, put
 from tilert_amd.flash_paged_mla import flash_paged_mla
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +30,25 @@ def test_the_most_tiles_over_the_widest_table(cuda, columns):
     flash_paged_mla(q, qp, pages, ids[None], cu, lens, out, lse, model_arch=ARCH)
     close(out, lse, q, qp, pages, ids, keys - tokens, [0, 1, 4000, tokens - 1])
     assert not (lse == 7.0).any()
+
+
+def _case(cuda, new, total, heads, seed):
+    pages, table, cu, lens, rows = _paged.batch([new], [total], seed=seed)
+    _paged.fill(pages, table, [total], seed=seed)
+    return list(_paged.to(cuda, *queries(rows, heads, seed + 1), pages, table, cu, lens))
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1e-12, 1e-30, 2.0 ** -126])
+@pytest.mark.parametrize("new,heads", TILES)
+@pytest.mark.parametrize("total", [90, 1000])
+def test_zero_queries_and_a_tiny_scale(cuda, new, heads, total, scale):
+    """All keys weigh alike, on whole and on masked pages: a score's factor, the row's power of two times the scale, may be
+    below fp32's numbers, and a masked score is still -inf."""
+    case = _case(cuda, new, total, heads, 5)
+    case[0][:, ::2] = 0
+    case[1][:, ::2] = 0
+    case[0][:, 1::4] *= 2.0 ** -100
+    case[1][:, 1::4] *= 2.0 ** -100
+    out, lse = run(cuda, *case, scale=scale)
+    check_all(case, out, lse, scale)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()

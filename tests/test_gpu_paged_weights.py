@@ -64,9 +64,9 @@ def close(out, lse, q, qp, pages, ids, first, tokens, scale=SCALE):
         assert torch.all((lse[t].double() - want_lse).abs() <= tol_lse), t
 
 
-def check_all(case, out, lse):
+def check_all(case, out, lse, scale=SCALE):
     new = case[0].shape[0]
-    close(out, lse, case[0], case[1], case[2], case[3][0], int(case[5][0]) - new, range(new))
+    close(out, lse, case[0], case[1], case[2], case[3][0], int(case[5][0]) - new, range(new), scale)
 
 
 def sink_case(cuda, keys, mass, mean, seed):

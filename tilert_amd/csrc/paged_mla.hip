@@ -551,8 +551,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         }
         *reinterpret_cast<u32x4p*>(to + kQueryRope + place * 128 + (n16 ^ (place & 7)) * 16) = x;
       }
-      // (a bad row's factor is NaN, which makes its sum NaN)
-      if (n16 == 0 && r < BM) rowl[r] = bad && live ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale;
+      // (A bad row's factor is NaN, which makes its sum NaN.  Another's is not 0, which would make a masked score, -inf, NaN:
+      // one below fp32's normal numbers stands for scores of 0, and 2^-126 does too.)
+      if (n16 == 0 && r < BM)
+        rowl[r] = bad && live ? __builtin_nanf("") : fmaxf(__uint_as_float(static_cast<uint32_t>(127 + e) << 23) * A.scale, 0x1p-126f);
       __syncthreads();
       if (wave < 4 && my_row / 32 == round) {
         const int q = my_row & 31;
