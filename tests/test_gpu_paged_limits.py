@@ -52,3 +52,18 @@ def test_zero_queries_and_a_tiny_scale(cuda, new, heads, total, scale):
     out, lse = run(cuda, *case, scale=scale)
     check_all(case, out, lse, scale)
     assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("size", [1e30, 1e38])
+@pytest.mark.parametrize("new,heads", TILES)
+@pytest.mark.parametrize("total", [300, 3000])  # one kernel; split and joined
+def test_keys_near_the_largest_numbers(cuda, new, heads, total, size):
+    """Latents of one sign whose sums pass fp32's range while their means do not; no part of the scores is theirs."""
+    g = torch.Generator().manual_seed(7)
+    case = _case(cuda, new, total, heads, 9)
+    case[0].zero_()
+    latent = (1 + 0.2 * torch.randn(total, 512, generator=g).clamp(-3, 3)) * size
+    put(case[2], case[3][0], latent.to(cuda), torch.randn(total, 64, generator=g).to(cuda))
+    out, lse = run(cuda, *case)
+    assert torch.isfinite(out).all()
+    check_all(case, out, lse)

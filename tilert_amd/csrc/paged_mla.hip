@@ -105,8 +105,8 @@ constexpr int kQueryLo = 32 * kKvLatent, kQueryRope = 2 * kQueryLo;
 static_assert(kQueryRope + 32 * kKvRope * 2 <= kSlotBytes, "");
 
 // What a split launch leaves for the combine kernel, in the workspace: for every workgroup the tile that it
-// continues, if it is the second on it; two slots of partial sums a workgroup (0: of the tile that it continues, 1: of
-// the tile that another one goes on with).
+// continues, if it is the second on it; two slots of partial results a workgroup (0: of the tile that it continues, 1: of
+// the tile that another one goes on with): (m, l) and the mean of the latents, whose sum may pass fp32's range.
 struct SplitTile {
   int64_t row0;
   int rows, parts;
@@ -916,7 +916,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       __syncthreads();
       __syncthreads();
 
-      // ---- the rows' results, or the tile's partial sums
+      // ---- the rows' results, or the tile's partial ones
       if (!A.split || (u == tile_u0 && u_end >= tile_u1)) {
         const int t = tid - 256;
         if (A.lse && t < rows) A.lse[row0 + t] = rowl[t] == 0.f ? -INFINITY : (alpha_l[t] + log2f(rowl[t])) * 0.6931471805599453f;
@@ -941,13 +941,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
 #pragma unroll
         for (int a = 0; a < RT2; ++a)
           if (a * 32 + n32 < rows) {
-            const float unit = unit_l[a * 32 + n32];
+            const float L = rowl[a * 32 + n32], x = L == 0.f ? 0.f : 1.0f / L * unit_l[a * 32 + n32];
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 dst[((a * 16 + dw * DT + d) * 4 + i) * 64 + lane] =
-                    v4f{o[a][d][4 * i], o[a][d][4 * i + 1], o[a][d][4 * i + 2], o[a][d][4 * i + 3]} * unit;
+                    v4f{o[a][d][4 * i], o[a][d][4 * i + 1], o[a][d][4 * i + 2], o[a][d][4 * i + 3]} * x;
           }
       }
     }
@@ -957,7 +957,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   }
 }
 
-// The split tiles' partial sums joined, in a fixed order.  An item is 32 rows x 64 / G dims of a tile: a thread takes one
+// The split tiles' partial means joined, in a fixed order, each weighted by its share of l.  An item is 32 rows x 64 / G dims of a tile: a thread takes one
 // row, 4 dims and every G'th part, so that it has few parts (up to eight, all their loads in flight together; a
 // context split over all workgroups: sixteen), and the G half-waves of the same dims are joined in LDS.  Bound by round
 // trips (the tiles, then the sums, which other XCDs wrote) where few tiles are split, and by the sums' bytes where many
@@ -990,8 +990,7 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
     return reinterpret_cast<const v4f*>(part_o + slot * (static_cast<int64_t>(PR) * kKvLatent))[((a * 16 + d4 / 8) * 4 + (d4 % 8) / 2) * 64 + (d4 & 1) * 32 + n32];
   };
   auto store = [&](int64_t row, int d4, const v4f& o, float l, float mx) {
-    const float x = l == 0.f ? 0.f : 1.0f / l;
-    *reinterpret_cast<u32x2p*>(out + row * kKvLatent + 4 * d4) = u32x2p{bf16x2_bits(v2f{o[0] * x, o[1] * x}), bf16x2_bits(v2f{o[2] * x, o[3] * x})};
+    *reinterpret_cast<u32x2p*>(out + row * kKvLatent + 4 * d4) = u32x2p{bf16x2_bits(v2f{o[0], o[1]}), bf16x2_bits(v2f{o[2], o[3]})};
     if (lse && d4 == 0) lse[row] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
   };
   // N parts i0, i0 + step, .. below `end`, added to (mx, l, o); their loads are all in flight together
@@ -1008,16 +1007,19 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
     float top = mx;
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, i0 + i * step < end ? ml[i].x : -INFINITY);
-    const float keep = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mx - top);  // (0, or a bad row's NaN, before the first)
-    l *= keep;
-    o *= keep;
+    const float kept = mx == -INFINITY ? l : l * __builtin_amdgcn_exp2f(mx - top);  // (0, or a bad row's NaN, before the first)
+    float share[N];
+    l = kept;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (i0 + i * step >= end) continue;
-      const float f = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - top);
-      l += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * f;
-      o += x[i] * f;
+      share[i] = i0 + i * step >= end ? 0.f : (ml[i].x == -INFINITY ? ml[i].y : ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - top));
+      l += share[i];
     }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    o *= kept * inv;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i0 + i * step < end) o += x[i] * (share[i] * inv);
     mx = top;
   };
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
@@ -1045,13 +1047,12 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
       __syncthreads();
       if (part0 == 0 && live) {
         for (int i = hw + dims; i < kHalfWaves; i += dims) mx = fmaxf(mx, top[i][n32]);
+        auto share = [&](int i) { return top[i][n32] == -INFINITY ? sums[i][n32] : sums[i][n32] * __builtin_amdgcn_exp2f(top[i][n32] - mx); };
         l = 0.f;
+        for (int i = hw; i < kHalfWaves; i += dims) l += share(i);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
         o = v4f{0.f, 0.f, 0.f, 0.f};
-        for (int i = hw; i < kHalfWaves; i += dims) {
-          const float f = top[i][n32] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[i][n32] - mx);
-          l += top[i][n32] == -INFINITY ? sums[i][n32] : sums[i][n32] * f;
-          o += acc[i][n32] * f;
-        }
+        for (int i = hw; i < kHalfWaves; i += dims) o += acc[i][n32] * (share(i) * inv);
       }
       __syncthreads();
     }
