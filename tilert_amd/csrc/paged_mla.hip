@@ -617,8 +617,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           *reinterpret_cast<int*>(P + (b * BT + i) * 16) = hi;
           *reinterpret_cast<int*>(P + (b * BT + i) * 16 + C::P_BYTES) = lo;
         }
-        const uint32_t e = top >> 23;
-        if (g == 0) *reinterpret_cast<uint16_t*>(smem + put_pow + b * 4 + (k & 1) * 256) = static_cast<uint16_t>(e - 7 | (e - 12) << 8);
+        const uint32_t e = top >> 23;  // (all four lanes of a row store it: a branch for one of them costs 2 % of a chunk's time)
+        *reinterpret_cast<uint16_t*>(smem + put_pow + b * 4 + (k & 1) * 256) = static_cast<uint16_t>(e - 7 | (e - 12) << 8);
       };
       // U of page k, and with WEIGH its weights, whose tile of 16 keys is one behind that of the products: the wave issues
       // the vector instructions of the one while the matrix pipe works on the other.  Whether all weights were <= kPMost.
