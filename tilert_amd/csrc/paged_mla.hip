@@ -216,16 +216,17 @@ __device__ inline int upper(const int* a, int n, int x) {
   return lo;
 }
 
-// Max over the lanes i, i ^ 16, i ^ 32, i ^ 48, in all of them; the sum with lane i ^ 16.
+// Max over the lanes i, i ^ 16, i ^ 32, i ^ 48, in all of them; the sums of lanes i and i ^ 16: a's in the lower of the two, b's
+// in the upper.
 __device__ inline float four_max(float v) {
   const u32x2p a = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
   const float x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const u32x2p b = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ inline float pair_sum(float v) {
-  const u32x2p a = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+__device__ inline float pair_sum(float a, float b) {
+  const u32x2p x = __builtin_bit_cast(u32x2p, __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
 __device__ inline v4f mfma16_fp8(const v8i& a, const v8i& b, v4f c, int scale_b) {
@@ -906,12 +907,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
           free = was;
         }
         product(n - 1, slot);
+        // P rows r and r + 16 together: groups of 8 dims 2 i in lanes n32 = r, 2 i + 1 in lanes r + 16
         if constexpr (C::kTwoRows)
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[0][d][i] = pair_sum(o[0][d][i]);
+            for (int i = 0; i < 8; ++i) o[0][d][i] = pair_sum(o[0][d][i / 4 * 8 + i % 4], o[0][d][i / 4 * 8 + 4 + i % 4]);
       }
+      constexpr int kGroups = C::kTwoRows ? 2 : 4;  // of a lane's groups of 8 dims in 32
+      const int row_in = C::kTwoRows ? n16 : n32;
+      auto group = [&](int i) { return C::kTwoRows ? 2 * i + (g & 1) : i; };
       __syncthreads();
       __syncthreads();
       __syncthreads();
@@ -922,15 +927,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         if (A.lse && t < rows) A.lse[row0 + t] = rowl[t] == 0.f ? -INFINITY : (alpha_l[t] + log2f(rowl[t])) * 0.6931471805599453f;
 #pragma unroll
         for (int a = 0; a < RT2; ++a) {
-          const int r = a * 32 + n32;
+          const int r = a * 32 + row_in;
           if (r < rows) {
             const float L = rowl[r], x = L == 0.f ? 0.f : 1.0f / L * unit_l[r];
             uint16_t* dst = A.out + (row0 + r) * kKvLatent + dw * 128 + 4 * half;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<u32x2p*>(dst + d * 32 + 8 * i) = u32x2p{bf16x2_bits(v2f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x}),
+              for (int i = 0; i < kGroups; ++i)
+                *reinterpret_cast<u32x2p*>(dst + d * 32 + 8 * group(i)) = u32x2p{bf16x2_bits(v2f{o[a][d][4 * i] * x, o[a][d][4 * i + 1] * x}),
                                                                          bf16x2_bits(v2f{o[a][d][4 * i + 2] * x, o[a][d][4 * i + 3] * x})};
           }
         }
@@ -940,13 +945,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
         v4f* dst = reinterpret_cast<v4f*>(A.part_o + static_cast<int64_t>(slot) * C::kPartFloats);
 #pragma unroll
         for (int a = 0; a < RT2; ++a)
-          if (a * 32 + n32 < rows) {
-            const float L = rowl[a * 32 + n32], x = L == 0.f ? 0.f : 1.0f / L * unit_l[a * 32 + n32];
+          if (a * 32 + row_in < rows) {
+            const float L = rowl[a * 32 + row_in], x = L == 0.f ? 0.f : 1.0f / L * unit_l[a * 32 + row_in];
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                dst[((a * 16 + dw * DT + d) * 4 + i) * 64 + lane] =
+              for (int i = 0; i < kGroups; ++i)
+                dst[((a * 16 + dw * DT + d) * 4 + group(i)) * 64 + half * 32 + row_in] =
                     v4f{o[a][d][4 * i], o[a][d][4 * i + 1], o[a][d][4 * i + 2], o[a][d][4 * i + 3]} * x;
           }
       }
