@@ -67,3 +67,17 @@ def test_keys_near_the_largest_numbers(cuda, new, heads, total, size):
     out, lse = run(cuda, *case)
     assert torch.isfinite(out).all()
     check_all(case, out, lse)
+
+
+@pytest.mark.parametrize("power", [5, 8])
+@pytest.mark.parametrize("new,heads", TILES)
+@pytest.mark.parametrize("total", [200, 1500])
+def test_one_dim_far_above_the_others(cuda, new, heads, total, power):
+    """A dim whose latents are 2^power times the others', of one sign: its products are most of every score, and alike."""
+    g = torch.Generator().manual_seed(11)
+    case = _case(cuda, new, total, heads, 13)
+    latent = torch.randn(total, 512, generator=g)
+    latent[:, 77] = 2.0 ** power * (1 + 0.01 * torch.randn(total, generator=g))
+    put(case[2], case[3][0], latent.to(cuda), torch.randn(total, 64, generator=g).to(cuda))
+    out, lse = run(cuda, *case)
+    check_all(case, out, lse, cut=True)
