@@ -19,10 +19,10 @@ constexpr int kAddNormMaxDim = 16384;
 
 // One workgroup a row, held in registers as h: thread t has the chunks (8 columns) t, t + NT, ...; 16 consecutive lanes
 // hold a 128-column group.  sum_out may be x's or the residual's memory: every thread reads its chunks before it
-// writes them, and no other thread reads them.
-// Bound by bytes, 9 an element, in large calls: 4096 x 7168, 265 MB, 41 us (6.4 TB/s) where the Infinity Cache holds
+// writes them, and no other thread uses them (those behind the row's end read its last chunk and drop it).
+// Bound by bytes, 9 an element, in large calls: 4096 x 7168, 265 MB, 40 us (6.6 TB/s) where the Infinity Cache holds
 // part of them, 50 us a call (5.3 TB/s) where it does not; by its two round trips and the reduction in small ones:
-// 4 x 7168 3.4 us.  One chunk a thread, up to 8192 columns of 1024 threads: a row is read in one round of loads (4 x 7168
+// 4 x 7168 3.5 us.  One chunk a thread, up to 8192 columns of 1024 threads: a row is read in one round of loads (4 x 7168
 // in a graph 3.0 us, 3.4 with 512 threads, 4.4 with 256; 4096 x 7168 49.2, 50.4, 52.7); up to 2048 columns 256
 // threads, where 1024 would leave three quarters of them without one (4096 x 2048 13.4 us, 22.8 with 1024).
 template <int NT, int NC>

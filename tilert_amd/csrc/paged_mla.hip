@@ -7,14 +7,17 @@
 // sequence's pages, 64 keys a step.  The latents go into both products as the codes they are stored as, on the fp8
 // MFMA; the other operand is split into two e4m3 numbers, x = hi + lo / 32:
 //   q / sigma (sigma: a power of two that brings the row's largest magnitude into [128, 256)): exact for
-//     values down to 2^-15 of the row's largest, below that within 2^-23 of it;
+//     values down to 2^-14 of the row's largest, below that within 2^-22 of it;
 //   p * scale_j over a power of two that brings the largest of the row's 32 keys (one half of a page) into [128, 256), the
-//     scale of that operand in the MFMA: within 2^-8 of the value, as bf16, down to 2^-15 of the largest, below that
+//     scale of that operand in the MFMA: within 2^-8 of the value, as bf16, down to 2^-14 of the largest, below that
 //     within 2^-22 of it.  Nothing else sets that power: not the row's other keys, and no other row.
 // Two fp8 products take the time of one in bf16, and no code is converted: with codes turned into bf16 the
 // conversions alone (64 a page and wave for each product and 32 rows) would take as long as the products.
 // Scores are U = scale_j * (codes . q / sigma) + (q_pe / sigma) . rope (bf16 MFMA), the exponent U * (sigma *
-// softmax_scale * log2 e) - m; all statistics and sums are fp32.
+// softmax_scale * log2 e) - m; maxima, l and O are fp32.  Inside one instruction the fp8 MFMA adds eight consecutive products
+// at a time, aligned to the largest and cut 13 bits below it, and those sums in fp32 (measured): a score's codes . q is
+// within 2^-10 of the sum of each eight's largest product (512 random codes: 2^-16 of all products' magnitudes, rms; the lse's
+// 1e-6 comes from it), and a page's part of O within 2^-10 of each eight keys' largest, beside the 2^-8 of P.
 #include <math.h>
 
 #include <type_traits>
@@ -34,21 +37,21 @@ typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar l
 
 constexpr int kPagedWgs = 256;        // workgroups of a split launch: one per CU
 // Tiles (and sequences) that a split launch plans in LDS; with more, a workgroup takes one and the last round of them is
-// short against the others.  273 tiles, ragged: 177 us split, 237 not; 512 tiles of 225 to 256 pages, two for every
-// workgroup: 966 split, 918 not; 1040 tiles (4160 tokens over 32768 keys), a few more than four: 3.77 ms split, 4.33 not.
+// short against the others.  273 tiles, ragged: 177 us split, 230 not; 512 tiles of 225 to 256 pages, two for every
+// workgroup: 979 split, 903 not; 1040 tiles (4160 tokens over 32768 keys), a few more than four: 3.97 ms split, 4.38 not.
 constexpr int kPagedMaxTiles = 2048;
 constexpr int64_t kPagedMaxRows = 1 << 27;  // (token, head) rows, fewer than this (PagedArgs::per_head)
-// Pages that a sequence can have (a table's width), up to which no tile is split: one token, 16 heads, 512 keys take
-// 14.2 us in one workgroup and 8.5 + 4.6 us over eight and with the join, and the second launch costs the caller 4 us
-// (10.1 against 14.5 us a call); from there on the page loop, 1.0 us a page, decides.
+// Pages that a sequence can have (a table's width), up to which no tile is split: one token, 16 heads, 500 keys take
+// 13.6 us in one workgroup and 8.6 + 5.3 us over eight and with the join (14.0 and 15.5 us a call, and the second launch
+// costs the host 4); from there on the page loop, 1.0 us a page, decides.
 constexpr int kPagedFew = 8;
 // Pages' time that a tile is counted for besides its pages, where a launch has many tiles: its queries' way into registers,
 // the first scores, its results (18 thousand cycles at 64 rows, a page 3.4 thousand), rounded up for the tile that is cut in
-// two.  Seven sequences of 2 to 700 new tokens, 273 tiles of 6 to 79 pages: 244 us without, 184 with 5, 173 with 9, 170
-// with 18.  32 tiles of 25 to 256 pages (1 token, 128 heads, 8 sequences): 36.2 without, 32.0 with 10; 60 tiles: 102 both
-// ways.  A launch of at most kPagedWgs / 16 tiles has few workgroups with two of them, and does without: 2 tiles of one
-// sequence (4 tokens over 131072 keys) are 38.9 us, 42.9 with it, as the workgroups on the same pages of both are then
-// no longer a multiple of 8, an XCD's L2, apart.
+// two.  Seven sequences of 2 to 700 new tokens, 273 tiles of 6 to 79 pages: 234 us without, 179 with 5, 175 with 10, 170
+// with 18.  32 tiles of 25 to 256 pages (1 token, 128 heads, 8 sequences): 36.3 without, 33.3, 31.8, 32.4; 60 tiles: 101.2,
+// 98.6, 101.7, 103.2.  A launch of at most kPagedWgs / 16 tiles has few workgroups with two of them, and does without: 2
+// tiles of one sequence (4 tokens over 131072 keys) are 39.7 us, 43.9 with it, as the workgroups on the same pages of both
+// are then no longer a multiple of 8, an XCD's L2, apart.
 constexpr int kPagedStart = 10;
 constexpr int kSlotBytes = kKvPageKeys * (kKvLatent + 2 * kKvRope);  // a page in LDS, its scales apart
 constexpr int kSlots = 3;
@@ -92,14 +95,14 @@ struct PagedCfg {
 };
 constexpr int kPagedThreads = 512;
 
-// What bounds it.  Decode: bytes; 60 sequences, 60 to 32768 keys, 447 MB of pages and rows: 102 us a call, 4.4 TB/s (a large
-// copy 4.7), 95 + 8.6 us in the two kernels.  Chunks: 2048 tokens, 16 heads over 16384 keys, 1.10 TFLOP: 0.94 to 0.99 ms,
-// 1.10 to 1.17 PFLOP/s; a large bf16 product of the library reaches 1.39.  A step of 64 rows x 64 keys takes 3750 cycles, in
-// which a SIMD's matrix pipe works for 2176; without the scoring waves' reads of the codes it takes 2980, without the
-// second product 3160, without writing P 3300, without fetches 3680, but then at 2.19 GHz instead of 1.95: the
-// clock gives way to the power drawn.  (Scoring waves of 32 rows would halve the reads; their queries' 144 registers leave
-// too few: with reloads from scratch memory 1.8 ms.)  Small calls: the latency of plan, queries, pages and join, one
-// behind another; 1 token over 500 keys 13.7 us in one kernel, of which seven pages' steps are 7.5.
+// What bounds it.  Decode: bytes; 60 sequences, 60 to 32768 keys, 447 MB of pages and rows: 101 us a call, 4.4 TB/s (a large
+// copy 4.7), 96 + 7.9 us in the two kernels.  Chunks: 2048 tokens, 16 heads over 16384 keys, 1.10 TFLOP: 0.95 to 0.98 ms,
+// 1.12 to 1.16 PFLOP/s; a large bf16 product of the library reaches 1.39.  A step of 64 rows x 64 keys takes 3900 cycles, in
+// which a SIMD's matrix pipe works for 2176.  Of 976 us a call 682 are left without the scoring waves' reads of the codes,
+// 769 without the second product, 936 without turning the weights into P, 925 without fetches, partly by a higher
+// clock, which gives way to the power drawn.  (Scoring waves of 32 rows would halve the reads; their queries' 144 registers
+// leave too few: with reloads from scratch memory 1.8 ms.)  Small calls: the latency of plan, queries, pages and join, one
+// behind another; 1 token over 500 keys 13.6 us in one kernel, of which seven pages' steps are 7.5.
 // 32 rows' queries on their way into registers, in slot 2: hi codes [32][512], lo codes, rope parts bf16 [32][64]
 constexpr int kQueryLo = 32 * kKvLatent, kQueryRope = 2 * kQueryLo;
 static_assert(kQueryRope + 32 * kKvRope * 2 <= kSlotBytes, "");
@@ -631,7 +634,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
       };
       auto scores = [&](int k, int slot, auto weigh_tag) {
         constexpr bool WEIGH = decltype(weigh_tag)::value;
-        constexpr int kItems = 4 * KT, kAhead = kItems < 4 ? kItems : 4;  // (8: 962 -> 979 us at 2048 tokens, 16 heads, 16384 keys; 6: 970)
+        constexpr int kItems = 4 * KT, kAhead = kItems < 4 ? kItems : 4;  // (6: 979 -> 990 us at 2048 tokens, 16 heads, 16384 keys)
         float most = 0.f, sum = 0.f;
         pmost = 0.f;
         float w[BT][4];
@@ -962,12 +965,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_mla_kernel(const Paged
   }
 }
 
-// The split tiles' partial means joined, in a fixed order, each weighted by its share of l.  An item is 32 rows x 64 / G dims of a tile: a thread takes one
-// row, 4 dims and every G'th part, so that it has few parts (up to eight, all their loads in flight together; a
-// context split over all workgroups: sixteen), and the G half-waves of the same dims are joined in LDS.  Bound by round
-// trips (the tiles, then the sums, which other XCDs wrote) where few tiles are split, and by the sums' bytes where many
-// are: 256 parts of 32 rows, 17 MB, 8 us; 495 of 64, 65 MB, 21 us.  Four workgroups a CU: 60 sequences 101.2 us a call, 102.6
-// with two; sixteen do no better.
+// The split tiles' partial means joined, in a fixed order, each weighted by its share of l.  An item is 32 rows x 64 / G
+// dims of a tile: a thread takes one row, 4 dims and every G'th part, so that it has few parts (up to eight, all their
+// loads in flight together; a context split over all workgroups: sixteen), and the G half-waves of the same dims are joined
+// in LDS.  Bound by round trips (the tiles, then the parts, which other XCDs wrote) where few tiles are split, and by the
+// parts' bytes where many are: 256 parts of 32 rows, 17 MB, 9 us; 495 of 64, 65 MB, 21 us.  Four workgroups a CU: 60
+// sequences 101.2 us a call, 102.6 with two; sixteen do no better.
 constexpr int kCombineWgs = 1024, kCombineThreads = 512, kHalfWaves = kCombineThreads / 32;
 __device__ inline int part_groups(int parts) { return parts <= 8 ? 1 : (parts <= 16 ? 2 : (parts <= 32 ? 4 : (parts <= 64 ? 8 : 16))); }
 template <int PR>
@@ -1069,11 +1072,11 @@ __global__ __launch_bounds__(kCombineThreads) void paged_mla_combine_kernel(cons
 // once, and for 64 rows both 32-row products of a multiplying wave share its read of the page; fewer rows have their
 // queries split and their sums written in less time and waste less where a sequence's rows end.  Measured, for the rows
 // that a sequence has on average, in us with 16 / 32 / 64 rows a tile:
-//   16 rows (1 sequence, 500 keys)                         13.8 / 14.7 / 22.6
-//   17 rows (60 sequences of 60 to 32768 keys, padded)     101.5 / 102.1 / 117.9
-//   64 rows (4 tokens, 16 heads, 131072 keys)              48.7 / 38.8 / 42.5
-//   128 rows (8 sequences of 1589 to 16384 keys)           42.2 / 32.2 / 38.4
-//   2471 rows (7 sequences of 2 to 700 new tokens)         305 / 181 / 171
+//   16 rows (1 sequence, 500 keys)                         13.9 / 14.7 / 21.7
+//   17 rows (60 sequences of 60 to 32768 keys, padded)     100.9 / 101.4 / 116.5
+//   64 rows (4 tokens, 16 heads, 131072 keys)              49.4 / 38.8 / 41.7
+//   128 rows (8 sequences of 1589 to 16384 keys)           40.6 / 31.5 / 35.5
+//   2471 rows (7 sequences of 2 to 700 new tokens)         322 / 181 / 175
 struct PagedPlan {
   int bm, pr;
   int64_t tiles;  // of a split launch, at most
