@@ -491,6 +491,76 @@ int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const voi
                        float softmax_scale, void* out_bf16, float* lse, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* ---- The paged per-head cache (grouped-query attention), its batch as above.  kv_pages u8
+ * [n_pages, kv_heads * 128 * head_dim + kv_heads * 8 rounded up to 128], 16-byte aligned: page p
+ * holds 64 keys, for each kv head 64 x head_dim e4m3fn key codes, then head_dim x 64 e4m3fn
+ * value codes (a dim is a row); behind all heads two fp32 scales a head, the keys' and the
+ * values', powers of two.  A key is code * its block's scale; a scale that is not positive and
+ * finite makes its block's keys NaN.  head_dim 64 or 128; heads <= 128, a multiple of kv_heads;
+ * query head h reads kv head h / (heads / kv_heads). */
+
+/* The new tokens' keys and values, and their queries: rows x of k and q bf16 [n_tokens, kv_heads
+ * or heads, head_dim] (a token's heads contiguous, tokens k_stride, q_stride elements apart,
+ * multiples of 8) become n = x / sqrt(mean(x^2) + eps) * gamma (gamma_k, gamma_q fp32 [head_dim];
+ * null: n = x), their first rope_dim dims (a multiple of 16) turned by the token's row of freqs
+ * fp32 [n_tokens, rope_dim] ((cos, sin) interleaved; null: not turned), dims (i, i + rope_dim / 2)
+ * paired, or (2i, 2i + 1) with interleaved = 1; v is taken as it is.  q_out bf16 [n_tokens, heads,
+ * head_dim] (q_bf16 null: none).  A block's scale (one page, one head) is the least power of two
+ * with max(amax, 1e-4) <= 448 scale over its new rows; where the page holds older keys of the
+ * sequence in front of them and their scale is larger, it stays, and where it is smaller their
+ * codes move to the new one, rounded where they become subnormal.  A key whose key or value row
+ * holds a NaN or an infinity gets NaN key codes and value codes 0 and does not count for the
+ * scales.  key_weights fp32 [n_pages, kv_heads, 64] (nullable): those of the written keys become
+ * 0.  Sequences must not share pages that are written to. */
+int tl_gqa_cache_write(const void* k_bf16, int64_t k_stride, const void* v_bf16, int64_t v_stride, void* kv_pages,
+                       int64_t n_pages, const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
+                       const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t kv_heads, int64_t head_dim,
+                       const float* gamma_k, const float* freqs, int64_t rope_dim, const void* q_bf16, int64_t q_stride,
+                       int64_t heads, const float* gamma_q, void* q_out_bf16, float* key_weights, float eps,
+                       int interleaved, void* stream);
+
+/* Causal attention of the batch's tokens: q bf16 [n_tokens, heads, head_dim] (tokens q_stride
+ * elements apart); token t at position p sees the keys 0 .. p of its sequence:
+ *   s[j] = q . k[j] * softmax_scale,  out = softmax(s) . v
+ * out bf16 [n_tokens, heads, head_dim], lse fp32 [n_tokens, heads] (nullable) = ln sum e^s; 0 and
+ * -inf where no key is seen.  Codes times scales are exact in bf16, statistics and sums fp32.  A row's
+ * result follows from the keys that it sees and from no other row's.  n_tokens * heads < 2^27, n_seqs
+ * <= 2^16, max_pages <= 2^20.  workspace: the bytes that tl_flash_paged_gqa_workspace_bytes names
+ * for these sizes (0: none), 16-byte aligned, its contents of no account before or after; calls
+ * that overlap in time need one each. */
+size_t tl_flash_paged_gqa_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads,
+                                          int64_t head_dim, int64_t max_pages);
+int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const void* kv_pages, int64_t n_pages,
+                       const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
+                       const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, float softmax_scale, void* out_bf16, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* The attention weights that the keys gather from the batch's tokens: with q and lse as
+ * tl_flash_paged_gqa took and gave them, key_weights fp32 [n_pages, kv_heads, 64] at the page and
+ * row of each key j of a sequence with new tokens, j below its last token's position,
+ *   key_weights (+)= sum of e^(s[j] - lse) over the tokens that see j and the heads of the group,
+ * added to what is there (accumulate = 1) or in its place (0); summed in fp32 in a fixed order.
+ * Sequences must not share pages.  Limits as tl_flash_paged_gqa's. */
+int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const float* lse, const void* kv_pages, int64_t n_pages,
+                         const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
+                         const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads,
+                         int64_t head_dim, float softmax_scale, int accumulate, float* key_weights, void* stream);
+
+/* Eviction by weight: of the seq_lens[b] keys of sequence b, for each kv head on its own, k =
+ * min(keep_lens[b], the keys there are, kept_pages * 64) stay: the last `recent` (at most k), and
+ * of the others those of the largest key_weights (equal ones: the lowest position; a NaN counts as
+ * the largest).  They go in ascending order into the pages kept_table [n_seqs, kept_pages] of the
+ * same pool, which must not be among the tables' own (a page outside the pool: dropped),
+ * their codes under the blocks' new scales (the least power of two, as above) and their weights with
+ * them; kept_lens int32 [n_seqs] = k, kept_slots int32 [n_seqs, kv_heads, kept_pages * 64] their
+ * positions, -1 behind the k-th.  block_table, seq_lens, keep_lens, kept_table: int32 on the
+ * device.  Keys of pages outside the pool are not there. */
+int tl_gqa_cache_evict(void* kv_pages, float* key_weights, int64_t n_pages, const int32_t* block_table, int64_t max_pages,
+                       const int32_t* seq_lens, const int32_t* keep_lens, int64_t n_seqs, int64_t kv_heads,
+                       int64_t head_dim, int64_t recent, const int32_t* kept_table, int64_t kept_pages,
+                       int32_t* kept_lens, int32_t* kept_slots, void* stream);
+
 /* Exact per-row top-k.  logits fp32 [rows, ld]; row i considers columns
  * [0, valid_base + 1 + i) (clamped to [0, ld]) -- topk_accurate's convention with
  * valid_base = seq_len - num_samples (ops/topk.py:77-80,101).  out int32 [rows, k]

@@ -1,0 +1,526 @@
+// The paged per-head cache (gqa.h): writing new tokens with their heads' norms and rotation, and eviction by weight.
+#include "gqa.h"
+#include "../../include/tilert_amd.h"
+
+namespace tl {
+
+// ------------------------------------------------------------------------------------------------------ writing
+// For a head's row x (a query, a key; a value is taken as it is):
+//   n = x * rsqrt(mean(x^2) + eps) * gamma        (fp32; n = x without gamma)
+//   y = n with its first `rope` dims turned pair by pair by the token's angles (n without)
+// A query row leaves as bf16(y).  Keys and values are quantised by block, the new rows of one page and head:
+//   s = the least power of two with max |y| <= 448 s; a block that holds older keys keeps its scale if it is larger, and
+//   if not its older codes are brought to the new one;  code = e4m3(y / s).
+// A key with a NaN or an infinity in its key or value row gets NaN key codes and value codes 0, and does not count for
+// the scales: its scores are NaN for the rows that see it, and nothing reaches a row that does not.
+struct GqaWriteArgs {
+  const uint16_t *k, *v, *q;
+  int64_t k_stride, v_stride, q_stride;
+  uint8_t* pages;
+  int64_t page_bytes;
+  PagedBatch p;
+  int kv_heads, heads, rope, interleaved, page_slots;
+  const float *gamma_k, *gamma_q, *freqs;
+  float eps;
+  uint16_t* q_out;
+  float* key_weights;
+};
+
+template <int LANES>  // sum / max over 8 or 16 consecutive lanes, in all of them
+__device__ inline float row_sum(float v) {
+  v = dpp_combine<0xb1, false>(v);
+  v = dpp_combine<0x4e, false>(v);
+  v = dpp_combine<0x141, false>(v);
+  return LANES == 16 ? dpp_combine<0x140, false>(v) : v;
+}
+
+__device__ inline void unpack8(u32x4g raw, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(raw[i] << 16);
+    x[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+  }
+}
+
+// The row's norm and rotation; lane `part` of the row's D / 8 holds dims 8 part .. + 7.  All lanes of a row call it together.
+template <int D>
+__device__ inline void norm_rope(float (&x)[8], int part, const float* gamma, const float* freqs, int rope, int interleaved, float eps) {
+  constexpr int LANES = D / 8;
+  if (gamma) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+    const float r = 1.0f / __builtin_sqrtf(row_sum<LANES>(ss) / D + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * gamma[part * 8 + i];
+  }
+  if (!freqs) return;
+  const bool turned = part * 8 < rope;
+  if (interleaved) {
+    if (!turned) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float c = freqs[part * 8 + 2 * i], s = freqs[part * 8 + 2 * i + 1], a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = a * c - b * s;
+      x[2 * i + 1] = a * s + b * c;
+    }
+    return;
+  }
+  const int half = rope / 16;  // lanes of half the turned dims
+  const bool upper = part >= half;
+  const int lane = threadIdx.x & 63, from = turned ? lane + (upper ? -half : half) : lane;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float other = __shfl(x[i], from);
+    if (turned) {
+      const int pair = (upper ? part - half : part) * 8 + i;
+      const float c = freqs[2 * pair], s = freqs[2 * pair + 1];
+      x[i] = upper ? other * s + x[i] * c : x[i] * c - other * s;
+    }
+  }
+}
+
+// A workgroup takes one page of a sequence's new keys and one kv head, or 8 D / 16 .. query rows (the workgroups behind).
+template <int D>
+__global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
+  constexpr int LANES = D / 8, ROWS = 256 / LANES, STEPS = kGqaKeys / ROWS;
+  __shared__ __attribute__((aligned(16))) uint8_t vt[D][kGqaKeys + 16];
+  __shared__ float amax_w[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int part = tid % LANES, sub = tid / LANES;
+  const PagedBatch& p = A.p;
+  const int page_wgs = A.page_slots * A.kv_heads;
+  if (static_cast<int>(blockIdx.x) >= page_wgs) {  // ---- query rows
+    const int64_t end = static_cast<int64_t>(min(max(p.cu[p.n_seqs], 0), p.n_tokens)) * A.heads;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x - page_wgs) * kGqaKeys;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int64_t row = row0 + i * ROWS + sub;
+      const bool live = row < end;
+      const int64_t r = live ? row : 0;
+      const int t = static_cast<int>(r / A.heads), h = static_cast<int>(r - static_cast<int64_t>(t) * A.heads);
+      float x[8];
+      unpack8(*reinterpret_cast<const u32x4g*>(A.q + t * A.q_stride + h * D + part * 8), x);
+      norm_rope<D>(x, part, A.gamma_q, A.freqs ? A.freqs + static_cast<int64_t>(t) * A.rope : nullptr, A.rope, A.interleaved, A.eps);
+      if (live) *reinterpret_cast<u32x4g*>(A.q_out + r * D + part * 8) = u32x4g{bf16x2_bits(v2f{x[0], x[1]}), bf16x2_bits(v2f{x[2], x[3]}),
+                                                                               bf16x2_bits(v2f{x[4], x[5]}), bf16x2_bits(v2f{x[6], x[7]})};
+    }
+    return;
+  }
+  // ---- a page: sequence b's are the slots from before(b) on, which leaves it as many as its tokens can touch
+  const int slot = blockIdx.x / A.kv_heads, head = blockIdx.x % A.kv_heads;
+  auto before = [&](int b) { return min(max(p.cu[b], 0), p.n_tokens) / kGqaKeys + 2 * b; };
+  const int b = last_seq(p.n_seqs, [&](int i) { return before(i) <= slot; });
+  if (b < 0 || b >= p.n_seqs) return;
+  const int c0 = p.cu[b], c1 = p.cu[b + 1];
+  const int first = min(max(c0, 0), p.n_tokens), n = min(max(c1, first), p.n_tokens) - first;
+  const int64_t base = static_cast<int64_t>(p.lens[b]) - c1 + first;  // position of the first token
+  if (n <= 0) return;
+  const int64_t pg = (base >> 6) + (slot - before(b));
+  if (pg < 0 || pg >= p.max_pages || pg > (base + n - 1) >> 6) return;
+  const int page = p.table[static_cast<int64_t>(b) * p.max_pages + pg];
+  if (page < 0 || page >= p.n_pages) return;
+  // rows r0 .. r1 - 1 of the page are tokens first + pg * 64 - base + row
+  const int64_t shift = pg * kGqaKeys - base;
+  const int r0 = static_cast<int>(shift < 0 ? -shift : 0), r1 = static_cast<int>(n - shift < kGqaKeys ? n - shift : kGqaKeys);
+  const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, head);
+  const float old_k = blk.scale[0], old_v = blk.scale[1];
+  float y[STEPS][8], z[STEPS][8];
+  bool fine[STEPS];
+  float amax_k = 0.f, amax_v = 0.f;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int row = i * ROWS + sub;
+    const bool live = row >= r0 && row < r1;
+    const int64_t t = first + shift + (live ? row : r0);
+    unpack8(*reinterpret_cast<const u32x4g*>(A.k + t * A.k_stride + head * D + part * 8), y[i]);
+    unpack8(*reinterpret_cast<const u32x4g*>(A.v + t * A.v_stride + head * D + part * 8), z[i]);
+    norm_rope<D>(y[i], part, A.gamma_k, A.freqs ? A.freqs + t * A.rope : nullptr, A.rope, A.interleaved, A.eps);
+    float bad = 0.f, mk = 0.f, mv = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bad = __builtin_fabsf(y[i][j]) < INFINITY && __builtin_fabsf(z[i][j]) < INFINITY ? bad : 1.f;
+      mk = fmaxf(mk, __builtin_fabsf(y[i][j]));
+      mv = fmaxf(mv, __builtin_fabsf(z[i][j]));
+    }
+    fine[i] = row_sum<LANES>(bad) == 0.f;
+    if (live && fine[i]) {
+      amax_k = fmaxf(amax_k, mk);
+      amax_v = fmaxf(amax_v, mv);
+    }
+  }
+  amax_k = wave_max_f32(amax_k);
+  amax_v = wave_max_f32(amax_v);
+  if (lane == 0) {
+    amax_w[0][wave] = amax_k;
+    amax_w[1][wave] = amax_v;
+  }
+  __syncthreads();
+  float s_k = gqa_scale(fmaxf(fmaxf(amax_w[0][0], amax_w[0][1]), fmaxf(amax_w[0][2], amax_w[0][3])));
+  float s_v = gqa_scale(fmaxf(fmaxf(amax_w[1][0], amax_w[1][1]), fmaxf(amax_w[1][2], amax_w[1][3])));
+  if (r0 > 0) {  // older keys in front
+    if (gqa_scale_ok(old_k)) {
+      if (old_k >= s_k) {
+        s_k = old_k;
+      } else {
+        const float ratio = old_k / s_k;
+        for (int i = tid; i < r0 * (D / 16); i += 256) {
+          u32x4g x = reinterpret_cast<u32x4g*>(blk.k)[i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = gqa_rescale4(x[j], ratio);
+          reinterpret_cast<u32x4g*>(blk.k)[i] = x;
+        }
+      }
+    }
+    if (gqa_scale_ok(old_v)) {
+      if (old_v >= s_v) {
+        s_v = old_v;
+      } else {
+        const float ratio = old_v / s_v;
+        for (int i = tid; i < D * kGqaKeys / 4; i += 256) {  // four keys of a dim; those behind r0 - 1 are written below
+          uint32_t* at = reinterpret_cast<uint32_t*>(blk.v) + i;
+          if (i % (kGqaKeys / 4) * 4 < r0) *at = gqa_rescale4(*at, ratio);
+        }
+      }
+    }
+  }
+  const float inv_k = 1.0f / s_k, inv_v = 1.0f / s_v, most_k = gqa_most(s_k), most_v = gqa_most(s_v);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int row = i * ROWS + sub;
+    if (row < r0 || row >= r1) continue;
+    u32x2g c = u32x2g{0x7f7f7f7fu, 0x7f7f7f7fu}, d = u32x2g{0, 0};
+    if (fine[i]) {
+      c = u32x2g{gqa_codes4(y[i][0], y[i][1], y[i][2], y[i][3], inv_k, most_k), gqa_codes4(y[i][4], y[i][5], y[i][6], y[i][7], inv_k, most_k)};
+      d = u32x2g{gqa_codes4(z[i][0], z[i][1], z[i][2], z[i][3], inv_v, most_v), gqa_codes4(z[i][4], z[i][5], z[i][6], z[i][7], inv_v, most_v)};
+    }
+    reinterpret_cast<u32x2g*>(blk.k + row * D)[part] = c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vt[part * 8 + j][row] = static_cast<uint8_t>(d[j / 4] >> (8 * (j % 4)));
+  }
+  __syncthreads();  // (and the older codes are where they go: the stores of this workgroup are in order from here)
+  for (int i = tid; i < D * 4; i += 256) {
+    const int dim = i >> 2, q = i & 3, lo = max(r0, 16 * q), hi = min(r1, 16 * q + 16);
+    uint8_t* to = blk.v + dim * kGqaKeys;
+    if (hi - lo == 16) *reinterpret_cast<u32x4g*>(to + 16 * q) = *reinterpret_cast<const u32x4g*>(&vt[dim][16 * q]);
+    else
+      for (int r = lo; r < hi; ++r) to[r] = vt[dim][r];
+  }
+  if (tid == 0) {
+    blk.scale[0] = s_k;
+    blk.scale[1] = s_v;
+  }
+  if (A.key_weights && tid >= r0 && tid < r1) A.key_weights[(static_cast<int64_t>(page) * A.kv_heads + head) * kGqaKeys + tid] = 0.f;
+}
+
+// ----------------------------------------------------------------------------------------------------- eviction
+struct GqaEvictArgs {
+  uint8_t* pages;
+  int64_t page_bytes;
+  float* weights;  // [n_pages][kv_heads][64]
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* keep;
+  int n_pages, max_pages, kv_heads, recent;
+  const int32_t* kept_table;
+  int kept_pages;
+  int32_t* kept_lens;
+  int32_t* slots;  // [n_seqs][kv_heads][kept_pages * 64]
+};
+
+// A weight as a number that ascends with it; -0 is 0 and a NaN the largest.
+__device__ inline uint32_t weight_key(float w) {
+  const uint32_t u = __float_as_uint(w + 0.f);
+  if (w != w) return 0xffffffffu;
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+// Which keys of one sequence and head stay: the last `recent`, and the heaviest of the others, k in all, in ascending
+// order; equal weights: the lowest position.  The k-th largest weight is found digit by digit (11, 11 and 10 bits) from
+// histograms in LDS, then every wave counts and writes its own stretch of the positions.
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
+__global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictArgs A) {
+  __shared__ int hist[kSelBins];
+  __shared__ int wave_sum[kSelWaves], wave_eq[kSelWaves];
+  __shared__ int found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x / A.kv_heads, h = blockIdx.x % A.kv_heads;
+  const int32_t* table = A.table + static_cast<int64_t>(b) * A.max_pages;
+  const int width = A.kept_pages * kGqaKeys;
+  int32_t* out = A.slots + (static_cast<int64_t>(b) * A.kv_heads + h) * width;
+  const int64_t most = static_cast<int64_t>(A.max_pages) * kGqaKeys;
+  const int n = static_cast<int>(min(static_cast<int64_t>(max(A.lens[b], 0)), most));
+  const int n_pages = (n + kGqaKeys - 1) / kGqaKeys;
+  auto there = [&](int pg) { const int id = table[pg]; return id >= 0 && id < A.n_pages; };
+  auto weight = [&](int pg, int row) { return A.weights[(static_cast<int64_t>(table[pg]) * A.kv_heads + h) * kGqaKeys + row]; };
+  // the keys that there are
+  int mine = 0;
+  for (int pg = tid; pg < n_pages; pg += kSelThreads) mine += there(pg) ? min(n - pg * kGqaKeys, kGqaKeys) : 0;
+  for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
+  if (lane == 0) wave_sum[wave] = mine;
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < kSelWaves; ++w) total += wave_sum[w];
+  const int k = min(min(max(A.keep[b], 0), total), width);
+  const int last0 = n - min(A.recent, k);  // positions from here on stay
+  mine = 0;
+  for (int pg = last0 / kGqaKeys + tid; pg < n_pages; pg += kSelThreads)
+    mine += there(pg) ? min(n - pg * kGqaKeys, kGqaKeys) - max(last0 - pg * kGqaKeys, 0) : 0;
+  for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
+  __syncthreads();
+  if (lane == 0) wave_sum[wave] = mine;
+  __syncthreads();
+  int need = k;  // of the others
+  for (int w = 0; w < kSelWaves; ++w) need -= wave_sum[w];
+  // the need-th largest key of the positions below last0, and how many equal to it stay
+  uint32_t prefix = 0, known = 0;
+  const int others = (last0 + kGqaKeys - 1) / kGqaKeys;
+  if (need > 0) {
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bins = digit == 2 ? 1024 : 2048;
+      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+      for (int pg = wave; pg < others; pg += kSelWaves) {
+        if (!there(pg) || pg * kGqaKeys + lane >= last0) continue;
+        const uint32_t key = weight_key(weight(pg, lane));
+        if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
+      }
+      __syncthreads();
+      // suffix sums: wave 0, 32 bins a lane
+      if (wave == 0) {
+        int sum = 0;
+        for (int i = 0; i < kSelBins / 64; ++i) sum += hist[lane * (kSelBins / 64) + i];
+        int above = sum;  // inclusive sum over the lanes behind
+        for (int o = 1; o < 64; o <<= 1) {
+          const int x = __shfl_down(above, o);
+          above += lane + o < 64 ? x : 0;
+        }
+        above -= sum;
+        if (above < need && above + sum >= need) {
+          for (int i = kSelBins / 64 - 1; i >= 0; --i) {
+            const int c = hist[lane * (kSelBins / 64) + i];
+            if (above + c >= need) {
+              found[0] = lane * (kSelBins / 64) + i;
+              found[1] = above;
+              break;
+            }
+            above += c;
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= static_cast<uint32_t>(found[0]) << shift;
+      known |= static_cast<uint32_t>(bins - 1) << shift;
+      need -= found[1];
+      __syncthreads();
+    }
+  } else {
+    prefix = 0xffffffffu;  // nothing above it, and none equal to it
+  }
+  // every wave's stretch of pages: how many it keeps above the threshold or as the last ones, and how many equal it
+  const int per = (n_pages + kSelWaves - 1) / kSelWaves, p0 = wave * per, p1 = min(p0 + per, n_pages);
+  auto kind = [&](int pg, bool& sure, bool& equal) {
+    const int pos = pg * kGqaKeys + lane;
+    sure = equal = false;
+    if (!there(pg) || pos >= n) return;
+    if (pos >= last0) { sure = true; return; }
+    const uint32_t key = weight_key(weight(pg, lane));
+    sure = key > prefix;
+    equal = key == prefix;
+  };
+  int sures = 0, equals = 0;
+  for (int pg = p0; pg < p1; ++pg) {
+    bool s, e;
+    kind(pg, s, e);
+    sures += __popcll(__ballot(s));
+    equals += __popcll(__ballot(e));
+  }
+  if (lane == 0) {
+    wave_sum[wave] = sures;
+    wave_eq[wave] = equals;
+  }
+  __syncthreads();
+  int eq = 0, at = 0;  // equal ones in front, kept ones in front
+  for (int w = 0; w < wave; ++w) {
+    at += wave_sum[w] + max(0, min(wave_eq[w], need - eq));
+    eq += wave_eq[w];
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  for (int pg = p0; pg < p1; ++pg) {
+    bool s, e;
+    kind(pg, s, e);
+    const uint64_t em = __ballot(e);
+    const bool stays = s || (e && eq + __popcll(em & below) < need);
+    const uint64_t m = __ballot(stays);
+    const int to = at + __popcll(m & below);
+    if (stays && to < width) out[to] = pg * kGqaKeys + lane;
+    at += __popcll(m);
+    eq += __popcll(em);
+  }
+  for (int i = k + tid; i < width; i += kSelThreads) out[i] = -1;
+  if (h == 0 && tid == 0) A.kept_lens[b] = k;
+}
+
+// A workgroup gathers the keys of one new page and head: their codes under the least common scale, and their weights.
+template <int D>
+__global__ __launch_bounds__(256) void gqa_gather_kernel(const GqaEvictArgs A) {
+  constexpr int CH = D / 16, ROWS = 256 / CH, STEPS = kGqaKeys / ROWS, DIMS = D / 4;
+  __shared__ int src_page[kGqaKeys], src_row[kGqaKeys];
+  __shared__ float src_k[kGqaKeys], src_v[kGqaKeys];
+  __shared__ float amax_w[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x % A.kv_heads, slot = blockIdx.x / A.kv_heads, b = slot / A.kept_pages, pg = slot % A.kept_pages;
+  const int to = A.kept_table[static_cast<int64_t>(b) * A.kept_pages + pg];
+  if (to < 0 || to >= A.n_pages) return;
+  const int32_t* list = A.slots + ((static_cast<int64_t>(b) * A.kv_heads + h) * A.kept_pages + pg) * kGqaKeys;
+  if (list[0] < 0) return;
+  if (tid < kGqaKeys) {
+    const int pos = list[tid];
+    int page = -1;
+    float sk = 0.f, sv = 0.f;
+    if (pos >= 0) {
+      page = A.table[static_cast<int64_t>(b) * A.max_pages + (pos >> 6)];
+      const GqaBlock s = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h);
+      sk = gqa_scale_ok(s.scale[0]) ? s.scale[0] : __builtin_nanf("");
+      sv = gqa_scale_ok(s.scale[1]) ? s.scale[1] : __builtin_nanf("");
+      A.weights[(static_cast<int64_t>(to) * A.kv_heads + h) * kGqaKeys + tid] = A.weights[(static_cast<int64_t>(page) * A.kv_heads + h) * kGqaKeys + (pos & 63)];
+    }
+    src_page[tid] = page;
+    src_row[tid] = pos & 63;
+    src_k[tid] = sk;
+    src_v[tid] = sv;
+  }
+  __syncthreads();
+  u32x4g kc[STEPS];
+  float amax_k = 0.f, amax_v = 0.f;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int row = i * ROWS + tid / CH, page = src_page[row];
+    kc[i] = u32x4g{0, 0, 0, 0};
+    if (page >= 0) {
+      kc[i] = reinterpret_cast<const u32x4g*>(gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h).k + src_row[row] * D)[tid % CH];
+      const float s = src_k[row];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(kc[i][j], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(kc[i][j], true);
+        amax_k = fmaxf(amax_k, fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1]))) * s);
+      }
+    }
+  }
+  // values: lane = key, a wave a quarter of the dims
+  uint32_t vc[DIMS / 4];
+  const int vpage = src_page[lane];
+  const float sv = src_v[lane];
+  if (vpage >= 0) {
+    const uint8_t* from = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, vpage, h).v + wave * DIMS * kGqaKeys + src_row[lane];
+#pragma unroll
+    for (int i = 0; i < DIMS / 4; ++i)
+      vc[i] = from[(4 * i) * kGqaKeys] | from[(4 * i + 1) * kGqaKeys] << 8 | from[(4 * i + 2) * kGqaKeys] << 16 |
+              static_cast<uint32_t>(from[(4 * i + 3) * kGqaKeys]) << 24;
+#pragma unroll
+    for (int i = 0; i < DIMS / 4; ++i) {
+      const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(vc[i], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(vc[i], true);
+      amax_v = fmaxf(amax_v, fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1]))) * sv);
+    }
+  }
+  amax_k = wave_max_f32(amax_k);
+  amax_v = wave_max_f32(amax_v);
+  if (lane == 0) {
+    amax_w[0][wave] = amax_k;
+    amax_w[1][wave] = amax_v;
+  }
+  __syncthreads();
+  const float s_k = gqa_scale(fmaxf(fmaxf(amax_w[0][0], amax_w[0][1]), fmaxf(amax_w[0][2], amax_w[0][3])));
+  const float s_v = gqa_scale(fmaxf(fmaxf(amax_w[1][0], amax_w[1][1]), fmaxf(amax_w[1][2], amax_w[1][3])));
+  const GqaBlock dst = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, to, h);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int row = i * ROWS + tid / CH;
+    if (src_page[row] < 0) continue;
+    const float ratio = src_k[row] / s_k;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kc[i][j] = gqa_rescale4(kc[i][j], ratio);
+    reinterpret_cast<u32x4g*>(dst.k + row * D)[tid % CH] = kc[i];
+  }
+  if (vpage >= 0) {
+    const float ratio = sv / s_v;
+    uint8_t* into = dst.v + wave * DIMS * kGqaKeys + lane;
+#pragma unroll
+    for (int i = 0; i < DIMS / 4; ++i) {
+      const uint32_t x = gqa_rescale4(vc[i], ratio);
+      into[(4 * i) * kGqaKeys] = static_cast<uint8_t>(x);
+      into[(4 * i + 1) * kGqaKeys] = static_cast<uint8_t>(x >> 8);
+      into[(4 * i + 2) * kGqaKeys] = static_cast<uint8_t>(x >> 16);
+      into[(4 * i + 3) * kGqaKeys] = static_cast<uint8_t>(x >> 24);
+    }
+  }
+  if (tid == 0) {
+    dst.scale[0] = s_k;
+    dst.scale[1] = s_v;
+  }
+}
+
+}  // namespace tl
+
+using namespace tl;
+
+extern "C" int tl_gqa_cache_write(const void* k_bf16, int64_t k_stride, const void* v_bf16, int64_t v_stride, void* kv_pages,
+                                  int64_t n_pages, const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
+                                  const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t kv_heads, int64_t head_dim,
+                                  const float* gamma_k, const float* freqs, int64_t rope_dim, const void* q_bf16, int64_t q_stride,
+                                  int64_t heads, const float* gamma_q, void* q_out_bf16, float* key_weights, float eps,
+                                  int interleaved, void* stream) {
+  const char* who = "gqa_cache_write";
+  if (int rc = check_batch(who, kv_pages, n_pages, block_table, max_pages, cu_seqlens, seq_lens, n_seqs, n_tokens)) return rc;
+  if (int rc = check_gqa(who, kv_heads, head_dim)) return rc;
+  if (freqs && (rope_dim < 16 || rope_dim > head_dim || rope_dim % 16)) {
+    set_error("%s: rope_dim=%lld must be a multiple of 16 in [16, %lld]", who, (long long)rope_dim, (long long)head_dim);
+    return kErrUnsupported;
+  }
+  if (q_bf16)
+    if (int rc = check_gqa_heads(who, heads, kv_heads)) return rc;
+  if (n_seqs == 0 || n_tokens == 0) return kOk;
+  if (int rc = check_gqa_rows(who, "key", k_bf16, k_stride, kv_heads, head_dim)) return rc;
+  if (int rc = check_gqa_rows(who, "value", v_bf16, v_stride, kv_heads, head_dim)) return rc;
+  if (q_bf16) {
+    if (int rc = check_gqa_rows(who, "query", q_bf16, q_stride, heads, head_dim)) return rc;
+    if (int rc = check_gqa_rows(who, "query_out", q_out_bf16, heads * head_dim, heads, head_dim)) return rc;
+  }
+  const int64_t slots = n_tokens / kGqaKeys + 2 * n_seqs;
+  const int64_t wgs = slots * kv_heads + (q_bf16 ? cdiv(n_tokens * heads, kGqaKeys) : 0);
+  if (wgs >= (1ll << 24)) {  // 256 threads each, fewer than 2^32
+    set_error("%s: %lld tokens, %lld sequences: more than a launch has room for", who, (long long)n_tokens, (long long)n_seqs);
+    return kErrUnsupported;
+  }
+  const GqaWriteArgs args{(const uint16_t*)k_bf16, (const uint16_t*)v_bf16, (const uint16_t*)q_bf16, k_stride, v_stride, q_stride,
+                          (uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
+                          PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
+                          (int)kv_heads, (int)heads, (int)rope_dim, interleaved, (int)slots, gamma_k, gamma_q, freqs, eps,
+                          (uint16_t*)q_out_bf16, key_weights};
+  hipLaunchKernelGGL(head_dim == 64 ? gqa_write_kernel<64> : gqa_write_kernel<128>, dim3(wgs), dim3(256), 0, (hipStream_t)stream, args);
+  return check_launch(who);
+}
+
+extern "C" int tl_gqa_cache_evict(void* kv_pages, float* key_weights, int64_t n_pages, const int32_t* block_table, int64_t max_pages,
+                                  const int32_t* seq_lens, const int32_t* keep_lens, int64_t n_seqs, int64_t kv_heads,
+                                  int64_t head_dim, int64_t recent, const int32_t* kept_table, int64_t kept_pages,
+                                  int32_t* kept_lens, int32_t* kept_slots, void* stream) {
+  const char* who = "gqa_cache_evict";
+  if (int rc = check_batch(who, kv_pages, n_pages, block_table, max_pages, keep_lens, seq_lens, n_seqs, n_seqs)) return rc;
+  if (int rc = check_gqa(who, kv_heads, head_dim)) return rc;
+  if (recent < 0 || recent > INT32_MAX) { set_error("%s: recent=%lld is out of range", who, (long long)recent); return kErrArg; }
+  if (n_seqs == 0) return kOk;
+  if (kept_pages < 1 || kept_pages > (1ll << 25) - 1) { set_error("%s: kept_pages=%lld must be in [1, 2^25)", who, (long long)kept_pages); return kErrArg; }
+  if (!key_weights || !kept_table || !kept_lens || !kept_slots) { set_error("%s: null pointer", who); return kErrArg; }
+  if (n_seqs * kv_heads * kept_pages >= (1ll << 24) || n_seqs * kv_heads >= (1ll << 22)) {  // 256 and 1024 threads each, fewer than 2^32
+    set_error("%s: %lld sequences of %lld kept pages: more than a launch has room for", who, (long long)n_seqs, (long long)kept_pages);
+    return kErrUnsupported;
+  }
+  const GqaEvictArgs args{(uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim), key_weights, block_table, seq_lens, keep_lens,
+                          (int)n_pages, (int)max_pages, (int)kv_heads, (int)recent, kept_table, (int)kept_pages, kept_lens, kept_slots};
+  hipLaunchKernelGGL(gqa_select_kernel, dim3(n_seqs * kv_heads), dim3(kSelThreads), 0, (hipStream_t)stream, args);
+  if (int rc = check_launch(who)) return rc;
+  hipLaunchKernelGGL(head_dim == 64 ? gqa_gather_kernel<64> : gqa_gather_kernel<128>, dim3(n_seqs * kv_heads * kept_pages), dim3(256), 0,
+                     (hipStream_t)stream, args);
+  return check_launch(who);
+}
