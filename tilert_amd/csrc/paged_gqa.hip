@@ -17,6 +17,10 @@
 #include "gqa.h"
 #include "../../include/tilert_amd.h"
 
+#ifndef GQA_RW
+#define GQA_RW 2
+#define GQA_NW 8
+#endif
 namespace tl {
 
 typedef const __attribute__((address_space(4))) int32_t* gqa_const_i32;  // scalar loads
@@ -31,9 +35,10 @@ struct GqaArgs {
   float scale;  // softmax_scale * log2 e
   uint16_t* out;
   float* lse;
-  int chunk, splits;  // pages a workgroup, workgroups a tile
-  float2* part_ml;    // [tile slots][kv_heads][splits][BM]
-  float* part_o;      // [tile slots][kv_heads][splits][BM * D]
+  int target;       // workgroups that the pages of all tiles are cut for; 0: one workgroup a tile
+  int2* tile_parts;  // [tile slots]: a tile's first part and its parts (heads: `kv_heads` of them side by side)
+  float2* part_ml;   // [parts][BM]
+  float* part_o;     // [parts][BM * D]
 };
 
 // A sequence's rows of one kv head and what they see, from untrusted metadata.
@@ -47,23 +52,148 @@ struct GqaSeq {
     base = static_cast<int64_t>(p.lens[b]) - c1 + first;
     most = static_cast<int64_t>(p.max_pages) * kGqaKeys;
   }
-  // keys that a row sees
+  __device__ inline GqaSeq(const PagedBatch& p, int group_, int first_, int rows_, int64_t base_)
+      : first(first_), rows(rows_), group(group_), base(base_), most(static_cast<int64_t>(p.max_pages) * kGqaKeys) {}
+  // keys that a row sees, and their pages
   __device__ inline int seen(int row) const {
     const int64_t n = base + row / group + 1;
     return static_cast<int>(n < 0 ? 0 : (n > most ? most : n));
   }
+  __device__ inline int pages(int row) const { return (seen(row) + kGqaKeys - 1) / kGqaKeys; }
 };
 
-// Tiles of BM rows: sequence b's are the slots from before(b) on, which leaves it as many as it can have.
-template <int BM>
-__device__ inline bool gqa_tile(const PagedBatch& p, int group, int slot, int& b, int& tile) {
-  auto before = [&](int i) { return min(max(p.cu[i], 0), p.n_tokens) * group / BM + i; };
-  b = last_seq(p.n_seqs, [&](int i) { return before(i) <= slot; });
+// Tiles of BM rows: sequence b's have the slots from gqa_slot0(b) on, which leaves it as many as it can have.
+__device__ inline int gqa_slot0(const PagedBatch& p, int group, int b, int bm) { return min(max(p.cu[b], 0), p.n_tokens) * group / bm + b; }
+__device__ inline bool gqa_tile(const PagedBatch& p, int group, int slot, int bm, int& b, int& tile) {
+  b = __builtin_amdgcn_readfirstlane(last_seq(p.n_seqs, [&](int i) { return gqa_slot0(p, group, i, bm) <= slot; }));
   if (b < 0 || b >= p.n_seqs) return false;
-  tile = slot - before(b);
+  tile = slot - gqa_slot0(p, group, b, bm);
   return tile >= 0;
 }
 inline int64_t gqa_slots(int64_t n_tokens, int64_t group, int64_t n_seqs, int bm) { return n_tokens * group / bm + n_seqs; }
+
+// What a workgroup works on: a tile of one kv head, and its pages pg0 .. pg1 - 1; the tile's parts and which of them this is.
+struct GqaItem {
+  int b, tile, pg0, pg1, parts;
+  int64_t part;
+};
+// Every workgroup plans the launch for itself, from the metadata on the device: the pages of all tiles are cut into pieces of
+// at most `chunk`, about `target` of them in all and at least kGqaFew pages each; a tile's pieces are of one size.  Where a tile
+// has several, they have a place each in the workspace: at most 2 * target of them, as such a tile has more than `chunk`
+// pages.
+constexpr int kGqaPlanSeqs = 512;  // sequences that a launch plans for; with more, a workgroup takes a tile
+constexpr int kGqaFew = 8;         // pages that are not cut
+struct GqaPlanLds {
+  int end[kGqaPlanSeqs];   // pieces up to sequence b and with it
+  int part[kGqaPlanSeqs];  // of them, those of tiles with several, before sequence b
+  int splits[kGqaPlanSeqs], rows[kGqaPlanSeqs], first[kGqaPlanSeqs];
+  int64_t base[kGqaPlanSeqs];
+  int scan[2][8];
+  float sum[8];
+};
+__device__ inline int gqa_wave_scan(int v) {  // inclusive sum over the wave
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
+template <int THREADS, int BM>
+__device__ inline bool gqa_plan_item(const GqaArgs& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
+  constexpr int WAVES = THREADS / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float units = 0.f;
+  for (int b = tid; b < A.p.n_seqs; b += THREADS) {
+    const GqaSeq s(A.p, A.group, b);
+    const int n = s.rows > 0 ? s.pages(s.rows - 1) : 0, tiles = (s.rows + BM - 1) / BM;
+    L.first[b] = s.first;
+    L.rows[b] = s.rows;
+    L.base[b] = s.base;
+    L.splits[b] = n;
+    units += static_cast<float>(tiles) * static_cast<float>(n);
+  }
+  units = wave_sum_f32(units);
+  if (lane == 0) L.sum[wave] = units;
+  __syncthreads();
+  units = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) units += L.sum[w];
+  // (a little more than their share, so that the sum's rounding leaves no piece over)
+  const int chunk = max(kGqaFew, static_cast<int>(fminf(units * A.kv_heads / A.target * 1.001f, 2e6f)) + 1);  // (2^20 pages a sequence at most)
+  int ends = 0, parts = 0;
+  for (int b0 = 0; b0 < A.p.n_seqs; b0 += THREADS) {
+    const int b = b0 + tid;
+    int pieces = 0, cut = 0;
+    if (b < A.p.n_seqs) {
+      const int tiles = (L.rows[b] + BM - 1) / BM, n = max(1, (L.splits[b] + chunk - 1) / chunk);
+      L.splits[b] = n;
+      pieces = tiles * n;
+      cut = n > 1 ? pieces : 0;
+    }
+    const int e = gqa_wave_scan(pieces), p = gqa_wave_scan(cut);
+    if (lane == 63) {
+      L.scan[0][wave] = e;
+      L.scan[1][wave] = p;
+    }
+    __syncthreads();
+    int before_e = ends, before_p = parts;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const int x = L.scan[0][w], y = L.scan[1][w];
+      before_e += w < wave ? x : 0;
+      before_p += w < wave ? y : 0;
+      ends += x;
+      parts += y;
+    }
+    if (b < A.p.n_seqs) {
+      L.end[b] = before_e + e;
+      L.part[b] = before_p + p - cut;
+    }
+    __syncthreads();
+  }
+  if (v >= ends) return false;
+  const int b = __builtin_amdgcn_readfirstlane(last_seq(A.p.n_seqs, [&](int i) { return (i ? L.end[i - 1] : 0) <= v; }));
+  if (b < 0 || b >= A.p.n_seqs) return false;
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  first = uniform(L.first[b]);
+  rows = uniform(L.rows[b]);
+  base = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(L.base[b] >> 32)))) << 32 |
+                              static_cast<uint32_t>(uniform(static_cast<int>(L.base[b]))));
+  const int at = uniform(v - (b ? L.end[b - 1] : 0));
+  it.b = b;
+  it.parts = uniform(L.splits[b]);
+  it.tile = at / it.parts;
+  it.part = static_cast<int64_t>(uniform(L.part[b])) + at;
+  it.pg0 = at % it.parts;  // (in pieces yet)
+  return at >= 0 && it.tile < (rows + BM - 1) / BM;  // (cu_seqlens that does not ascend)
+}
+
+// The workgroup's item; false: it has none.
+template <int THREADS, int BM>
+__device__ inline bool gqa_item(const GqaArgs& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
+  if (A.target) {
+    if (!gqa_plan_item<THREADS, BM>(A, L, v, it, first, rows, base)) return false;
+  } else {
+    if (!gqa_tile(A.p, A.group, v, BM, it.b, it.tile)) return false;
+    const GqaSeq s(A.p, A.group, it.b);
+    first = s.first;
+    rows = s.rows;
+    base = s.base;
+    if (it.tile >= (rows + BM - 1) / BM) return false;
+    it.parts = 1;
+    it.pg0 = 0;
+    it.part = 0;
+  }
+  const GqaSeq s(A.p, A.group, first, rows, base);
+  const int n = s.pages(min((it.tile + 1) * BM, rows) - 1), each = (n + it.parts - 1) / it.parts, piece = it.pg0;
+  it.pg0 = piece * each;
+  it.pg1 = min(it.pg0 + each, n);
+  // (tile_parts: by slot, as a join's workgroups find their tiles)
+  if (A.target && piece == 0 && threadIdx.x == 0 && blockIdx.x % A.kv_heads == 0)
+    A.tile_parts[gqa_slot0(A.p, A.group, it.b, BM) + it.tile] = int2{static_cast<int>(it.part), it.parts};
+  return true;
+}
 
 __device__ inline v8bf bf16_of(u32x4g x) { return __builtin_bit_cast(v8bf, x); }
 // Eight codes times a power of two.
@@ -133,14 +263,19 @@ __device__ inline GqaKeys<D> load_keys(const uint8_t* k, int lane) {
     for (int i = 0; i < D / 64; ++i) r.k[t][i] = *reinterpret_cast<const u32x4g*>(from + 4 * t * D + 64 * i);
   return r;
 }
-template <int D>
+template <int D, bool ONCE>  // ONCE: no other wave reads them
 __device__ inline GqaValues<D> load_values(const uint8_t* v, int lane) {
   GqaValues<D> r;
   const uint8_t* from = v + (lane & 15) * kGqaKeys + 16 * (lane >> 4);
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) r.v[d] = *reinterpret_cast<const u32x4g*>(from + d * 16 * kGqaKeys);
+  for (int d = 0; d < D / 16; ++d) {
+    const u32x4g* at = reinterpret_cast<const u32x4g*>(from + d * 16 * kGqaKeys);
+    r.v[d] = ONCE ? __builtin_nontemporal_load(at) : *at;
+  }
   return r;
 }
+
+__device__ inline float2 load_scales(const float* s) { return float2{load_f32_vector(s), load_f32_vector(s + 1)}; }
 
 // One tile of 16 RT rows and one kv head over `chunk` pages; the four waves take every fourth of them, each with its own
 // statistics, and are joined in LDS.  Weights go into the second product as hi + lo in bf16, 16 bits of them.
@@ -148,272 +283,509 @@ __device__ inline GqaValues<D> load_values(const uint8_t* v, int lane) {
 constexpr float kGqaHead = 24.f;
 template <int D, int RT>
 __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
-  constexpr int BM = 16 * RT, DT = D / 16, KI = D / 64;
-  __shared__ v4f sum_o[4][DT][64];
-  __shared__ float sum_m[4][BM], sum_l[4][BM];
+  constexpr int BM = 16 * RT, DT = D / 16, KI = D / 64, PW = 4 / RT;  // PW: waves that share the pages of 16 rows
+  __shared__ union {
+    GqaPlanLds plan;
+    v4f sum_o[4][DT][64];
+  } L;
+  __shared__ float sum_m[4][16], sum_l[4][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int slot = blockIdx.x / A.kv_heads, head = blockIdx.x % A.kv_heads, split = blockIdx.y;
-  int b, tile;
-  if (!gqa_tile<BM>(A.p, A.group, slot, b, tile)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  const GqaSeq s(A.p, A.group, b);
-  const int row0 = tile * BM, rows = min(s.rows - row0, BM);
-  if (rows <= 0) return;
-  const int least = s.seen(row0), n_pages = (s.seen(row0 + rows - 1) + kGqaKeys - 1) / kGqaKeys;
-  const int pg0 = split * A.chunk, pg1 = min(pg0 + A.chunk, n_pages);
-  if (split > 0 && pg0 >= n_pages) return;
-  const gqa_const_i32 table = (gqa_const_i32)(A.p.table + static_cast<int64_t>(b) * A.p.max_pages);
-  GqaQuery<D> q[RT];
-  int seen[RT];
-  float m[RT], l[RT];
-  v4f o[RT][DT];
+  const int c = lane & 15, g = lane >> 4, rt = wave % RT, pw = wave / RT;
+  const int head = blockIdx.x % A.kv_heads;
+  GqaItem it;
+  int first, rows_all;
+  int64_t base;
+  if (!gqa_item<256, BM>(A, L.plan, blockIdx.x / A.kv_heads, it, first, rows_all, base)) return;
+  const GqaSeq s(A.p, A.group, first, rows_all, base);
+  const int row0 = it.tile * BM, rows = min(s.rows - row0, BM);
+  const int least = s.seen(row0 + min(16 * rt, rows - 1));
+  const gqa_const_i32 table = (gqa_const_i32)(A.p.table + static_cast<int64_t>(it.b) * A.p.max_pages);
+  const GqaQuery<D> q = load_query<D>(A.q, A.q_stride, s, head * A.group, row0 + rt * 16 + c, g);
+  const int seen = s.seen(row0 + min(rt * 16 + c, rows - 1));
+  float m = -INFINITY, l = 0.f;
+  v4f o[DT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    q[r] = load_query<D>(A.q, A.q_stride, s, head * A.group, row0 + r * 16 + c, g);
-    seen[r] = s.seen(row0 + min(r * 16 + c, rows - 1));
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
-  for (int pg = pg0 + wave; pg < pg1; pg += 4) {
-    const int id = __builtin_amdgcn_readfirstlane(table[pg]);
-    if (id < 0 || id >= A.p.n_pages) continue;
-    const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, id, head);
-    const GqaKeys<D> kc = load_keys<D>(blk.k, lane);
-    GqaValues<D> vc = load_values<D>(blk.v, lane);
-    const bool ok = gqa_scale_ok(blk.scale[0]) && gqa_scale_ok(blk.scale[1]);
-    const float sk = ok ? blk.scale[0] : 1.f, sv = ok ? blk.scale[1] : 1.f, unit = ok ? A.scale : __builtin_nanf("");
+  for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
+  // A page's scores, weights and sums.  Its keys are there already; its values are under way while the scores are made, and
+  // the next page's keys behind them.
+  auto step = [&](int pg, bool there, const GqaKeys<D>& kc, GqaValues<D>& vc, float2 scales) {
+    const bool ok = gqa_scale_ok(scales.x) && gqa_scale_ok(scales.y);
+    const float sk = ok ? scales.x : 1.f, sv = ok ? scales.y : 1.f;
     const int key0 = pg * kGqaKeys;
-    const bool masked = key0 + kGqaKeys > least;
+    const bool masked = !there || !__all(ok) || key0 + kGqaKeys > least;
     // ---- scores
-    v4f x[RT][4];
+    v4f x[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r) x[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+      x[t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KI; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const v8bf a = codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], sk);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) x[r][t] = mfma_bf16(a, q[r].x[i][e], x[r][t]);
-        }
+        for (int e = 0; e < 2; ++e) x[t] = mfma_bf16(codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], sk), q.x[i][e], x[t]);
     }
     // ---- weights
-    v8bf hi[RT][2], lo[RT][2];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int my = seen[r] - key0 - 16 * g;  // of this lane's 16 keys, the row sees this many
-      float top = -INFINITY;
+    const int my = there ? seen - key0 - 16 * g : 0;  // of this lane's 16 keys, the row sees this many
+    if (masked) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[r][t][j] *= unit;
-          if (masked && 4 * t + j >= my) x[r][t][j] = -INFINITY;
-          top = fmaxf(top, x[r][t][j]);
-        }
-      top = fmaxf(m[r], four_lanes<true>(top));
-      if (__any(top > m[r])) {
-        const float by = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - top);  // (before the first key all is 0, or NaN)
-        m[r] = top;
-        l[r] *= by;
+        for (int j = 0; j < 4; ++j) x[t][j] = 4 * t + j >= my ? -INFINITY : (ok ? x[t][j] : __builtin_nanf(""));
+    }
+    float top = x[0][0];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] *= by;
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, x[t][j]);
+    top = fmaxf(m, four_lanes<true>(top) * A.scale);
+    if (__any(top > m)) {
+      const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);  // (before the first key all is 0, or NaN)
+      m = top;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= by;
+    }
+    const float from = m == -INFINITY ? 0.f : m + kGqaHead;
+    v8bf hi[2], lo[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      u32x4g h, w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v4f y = x[2 * e + i / 2];
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1)], A.scale, -from));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1) + 1], A.scale, -from));
+        l += p0 + p1;
+        h[i] = bf16x2_bits(v2f{p0, p1});
+        w[i] = bf16x2_bits(v2f{p0 - __uint_as_float(h[i] << 16), p1 - __uint_as_float(h[i] & 0xffff0000u)});
       }
-      const float from = m[r] == -INFINITY ? 0.f : m[r] + kGqaHead;
-      float p[16];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          p[4 * t + j] = __builtin_amdgcn_exp2f(x[r][t][j] - from);
-          l[r] += p[4 * t + j];
-        }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        u32x4g h, w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p0 = p[8 * e + 2 * i], p1 = p[8 * e + 2 * i + 1];
-          h[i] = bf16x2_bits(v2f{p0, p1});
-          w[i] = bf16x2_bits(v2f{p0 - __uint_as_float(h[i] << 16), p1 - __uint_as_float(h[i] & 0xffff0000u)});
-        }
-        hi[r][e] = bf16_of(h);
-        lo[r][e] = bf16_of(w);
-      }
+      hi[e] = bf16_of(h);
+      lo[e] = bf16_of(w);
     }
     // ---- values; on a page with keys that some row does not see, codes that are NaN are taken apart
-    uint32_t bad[DT][4] = {};
-    bool any_bad = false;
     if (masked) {
       uint32_t all = 0;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t n = nan_codes(vc.v[d][i]);
-          all |= n;
-          bad[d][i] = n;
-          vc.v[d][i] &= ~(n | (n - (n >> 7)));
+        for (int i = 0; i < 4; ++i) all |= nan_codes(vc.v[d][i]);
+      if (__any(all != 0)) {  // how many NaN values a row sees
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          v4f n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            u32x4g w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (8 * e + 2 * i < my ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my ? 0x3f800000u : 0u);
+            n = mfma_bf16(codes8_bf16(nan_codes(vc.v[d][2 * e]) >> 1, nan_codes(vc.v[d][2 * e + 1]) >> 1, 1.f), bf16_of(w), n);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[d][j] = n[j] > 0.f ? __builtin_nanf("") : o[d][j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t bad = nan_codes(vc.v[d][i]);
+            vc.v[d][i] &= ~(bad | (bad - (bad >> 7)));
+          }
         }
-      any_bad = __any(all != 0);
+      }
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const v8bf a = codes8_bf16(vc.v[d][2 * e], vc.v[d][2 * e + 1], sv);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          o[r][d] = mfma_bf16(a, hi[r][e], o[r][d]);
-          o[r][d] = mfma_bf16(a, lo[r][e], o[r][d]);
-        }
+        o[d] = mfma_bf16(a, hi[e], o[d]);
+        o[d] = mfma_bf16(a, lo[e], o[d]);
       }
-    if (any_bad) {  // how many NaN values a row sees
+  };
+  // pages pg0 + pw, + PW, ..; one outside the pool is read as page 0 and seen by no row
+  auto page_id = [&](int pg) { return __builtin_amdgcn_readfirstlane(table[min(pg, it.pg1 - 1)]); };
+  auto there = [&](int id) { return id >= 0 && id < A.p.n_pages; };
+  auto block = [&](int id) { return gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there(id) ? id : 0, head); };
+  int pg = it.pg0 + pw;
+  if (pg < it.pg1 && rt * 16 < rows) {
+    GqaKeys<D> ka, kb;
+    GqaValues<D> va, vb;
+    float2 sa, sb;
+    int id = page_id(pg), next = page_id(pg + PW);
+    ka = load_keys<D>(block(id).k, lane);
+    va = load_values<D, RT == 1>(block(id).v, lane);
+    sa = load_scales(block(id).scale);
+    // (two buffers by turns: one copied into the other would wait for its loads)
+    auto half = [&](const GqaKeys<D>& k_now, GqaValues<D>& v_now, float2 s_now, GqaKeys<D>& k_then, GqaValues<D>& v_then, float2& s_then) {
+      k_then = load_keys<D>(block(next).k, lane);
+      v_then = load_values<D, RT == 1>(block(next).v, lane);
+      s_then = load_scales(block(next).scale);
+      const bool is = there(id);
+      id = next;
+      next = page_id(pg + 2 * PW);
+      step(pg, is, k_now, v_now, s_now);
+      pg += PW;
+    };
+    while (true) {
+      half(ka, va, sa, kb, vb, sb);
+      if (pg >= it.pg1) break;
+      half(kb, vb, sb, ka, va, sa);
+      if (pg >= it.pg1) break;
+    }
+  }
+  // ---- the waves of the same rows together
+  l = four_lanes<false>(l);
+  if (g == 0) {
+    sum_m[wave][c] = m;
+    sum_l[wave][c] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY, total = 0.f;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int my = seen[r] - key0 - 16 * g;
-        v8bf sees[2];
+  for (int w = 0; w < PW; ++w) top = fmaxf(top, sum_m[rt + RT * w][c]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          u32x4g w;
+  for (int w = 0; w < PW; ++w) {
+    const float mw = sum_m[rt + RT * w][c];
+    total += sum_l[rt + RT * w][c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - top));
+  }
+  if constexpr (PW > 1) {
+    const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = (8 * e + 2 * i < my ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my ? 0x3f800000u : 0u);
-          sees[e] = bf16_of(w);
+    for (int d = 0; d < DT; ++d) L.sum_o[wave][d][lane] = o[d] * by;
+    __syncthreads();
+  }
+  const bool live = rt * 16 + c < rows, whole = it.parts == 1;
+  const int row = row0 + rt * 16 + c;
+  const int64_t at = static_cast<int64_t>(s.first + row / A.group) * A.heads + head * A.group + row % A.group;
+  const int64_t part = it.part * A.kv_heads + head;
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+#pragma unroll
+  for (int i = 0; i < DT / PW; ++i) {
+    const int d = PW * i + pw;
+    v4f v;
+    if constexpr (PW > 1) {
+      v = L.sum_o[rt][d][lane];
+#pragma unroll
+      for (int w = 1; w < PW; ++w) v += L.sum_o[rt + RT * w][d][lane];
+    } else {
+      v = o[i];
+    }
+    if (!live) continue;
+    if (whole) *reinterpret_cast<u32x2g*>(A.out + at * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
+    else reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[(rt * DT + d) * 64 + lane] = v;
+  }
+  if (pw == 0 && g == 0 && live) {
+    if (!whole) A.part_ml[part * BM + rt * 16 + c] = float2{top, total};
+    else if (A.lse) A.lse[at] = total == 0.f ? -INFINITY : (top + kGqaHead + log2f(total)) * kLn2;
+  }
+}
+
+// ---- many rows: the waves of a workgroup go through the pages together
+// A page's codes are turned into bf16 once, by the wave that loaded them, and lie in LDS as the products' operands, fragment
+// by fragment in lane order; each wave multiplies them with its own 16 RW rows.  Weights go into the second product in
+// bf16, 8 bits.  A row's reference m is set anew only where a score passes it by 2^8: hardly a page rescales anything.
+constexpr float kGqaLag = 8.f;
+template <int D>
+constexpr int gqa_chunk_lds() { return 2 * (2 * (4 * (D / 64) + D / 16) + D / 16) * 1024 + 16; }
+template <int D, int RW, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void gqa_chunk_kernel(const GqaArgs A) {
+  constexpr int BM = 16 * RW * NW, DT = D / 16, KI = D / 64, KP = 4 * KI, PIECES = KP + DT, MINE = PIECES / NW, FRAG = 2 * PIECES;
+  extern __shared__ __attribute__((aligned(16))) uint8_t gqa_smem[];
+  struct Lds {
+    union {
+      GqaPlanLds plan;
+      u32x4g frag[2][FRAG][64];  // keys [t][i][e], then values [d][e]
+    };
+    u32x4g bad[2][DT][64];  // where those of a page are NaN that is not seen by all rows
+    int odd[2];             // the page of a buffer that has such values
+  };
+  static_assert(sizeof(Lds) <= gqa_chunk_lds<D>(), "");
+  Lds& L = *reinterpret_cast<Lds*>(gqa_smem);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x % A.kv_heads;
+  GqaItem it;
+  int first, rows_all;
+  int64_t base;
+  if (!gqa_item<64 * NW, BM>(A, L.plan, blockIdx.x / A.kv_heads, it, first, rows_all, base)) return;
+  const GqaSeq s(A.p, A.group, first, rows_all, base);
+  const int row0 = it.tile * BM + wave * 16 * RW, rows = min(s.rows - it.tile * BM, BM) - wave * 16 * RW;  // this wave's
+  const int last = s.rows - 1;
+  const int least = s.seen(min(row0, last)), least_all = s.seen(it.tile * BM);
+  const gqa_const_i32 table = (gqa_const_i32)(A.p.table + static_cast<int64_t>(it.b) * A.p.max_pages);
+  GqaQuery<D> q[RW];
+  int seen[RW];
+  float m[RW], l[RW];
+  v4f o[RW][DT];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    q[r] = load_query<D>(A.q, A.q_stride, s, head * A.group, row0 + r * 16 + c, g);
+    seen[r] = s.seen(min(row0 + r * 16 + c, last));
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  auto page_id = [&](int pg) { return __builtin_amdgcn_readfirstlane(table[min(pg, it.pg1 - 1)]); };
+  auto there = [&](int id) { return id >= 0 && id < A.p.n_pages; };
+  struct Codes {
+    u32x4g x[MINE];
+    float2 s;
+  };
+  auto fetch = [&](int id) {  // this wave's pieces of a page
+    const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there(id) ? id : 0, head);
+    Codes r;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int piece = wave + NW * j;
+      const uint8_t* k = blk.k + (16 * (c >> 2) + (c & 3) + 4 * (piece / KI)) * D + 64 * (piece % KI) + 16 * g;
+      const uint8_t* v = blk.v + ((piece - KP) * 16 + c) * kGqaKeys + 16 * g;
+      r.x[j] = *reinterpret_cast<const u32x4g*>(piece < KP ? k : v);
+    }
+    r.s = load_scales(blk.scale);
+    return r;
+  };
+  auto stage = [&](const Codes& r, int buf, int pg, bool masked) {
+    const bool ok = gqa_scale_ok(r.s.x) && gqa_scale_ok(r.s.y);
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+      const int piece = wave + NW * j;
+      const float by = ok ? (piece < KP ? r.s.x : r.s.y) : 1.f;
+      u32x4g x = r.x[j];
+      if (masked && piece >= KP) {  // on a page with keys that some row does not see, values that are NaN are taken apart
+        u32x4g bad;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad[i] = nan_codes(x[i]);
+        if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0) && lane == 0) L.odd[buf] = pg;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] &= ~(bad[i] | (bad[i] - (bad[i] >> 7)));
+          bad[i] >>= 1;  // the code of 2
         }
+        L.bad[buf][piece - KP][lane] = bad;
+      }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
+      for (int e = 0; e < 2; ++e) L.frag[buf][2 * piece + e][lane] = __builtin_bit_cast(u32x4g, codes8_bf16(x[2 * e], x[2 * e + 1], by));
+    }
+  };
+  auto frag = [&](int buf, int f) { return bf16_of(L.frag[buf][f][lane]); };
+  auto step = [&](int pg, bool is, bool ok, int buf) {
+    const int key0 = pg * kGqaKeys;
+    const bool masked = !is || !ok || key0 + kGqaKeys > least;
+    v4f x[RW][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) x[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 2 * KI; ++i) {
+        const v8bf a = frag(buf, t * 2 * KI + i);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) x[r][t] = mfma_bf16(a, q[r].x[i / 2][i % 2], x[r][t]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (masked)
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        const int my = is ? seen[r] - key0 - 16 * g : 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[r][t][j] = 4 * t + j >= my ? -INFINITY : (ok ? x[r][t][j] : __builtin_nanf(""));
+      }
+    float top[RW];
+    bool grows = false;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      top[r] = x[r][0][0];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[r] = fmaxf(top[r], x[r][t][j]);
+      top[r] *= A.scale;
+      grows = grows || top[r] > m[r] + kGqaLag;
+    }
+    if (__any(grows))
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        const float now = fmaxf(m[r], four_lanes<true>(top[r]));
+        const float by = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - now);
+        m[r] = now;
+        l[r] *= by;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] *= by;
+      }
+    v8bf p[RW][2];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const float from = m[r] == -INFINITY ? 0.f : m[r] + kGqaHead;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        u32x4g h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f y = x[r][2 * e + i / 2];
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1)], A.scale, -from));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1) + 1], A.scale, -from));
+          l[r] += p0 + p1;
+          h[i] = bf16x2_bits(v2f{p0, p1});
+        }
+        p[r][e] = bf16_of(h);
+      }
+    }
+    if (masked && L.odd[buf] == pg)  // how many NaN values a row sees
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const u32x4g w = L.bad[buf][d][lane];
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          const int my = is ? seen[r] - key0 - 16 * g : 0;
           v4f n = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) n = mfma_bf16(codes8_bf16(bad[d][2 * e] >> 1, bad[d][2 * e + 1] >> 1, 1.f), sees[e], n);
+          for (int e = 0; e < 2; ++e) {
+            u32x4g sees;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sees[i] = (8 * e + 2 * i < my ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my ? 0x3f800000u : 0u);
+            n = mfma_bf16(codes8_bf16(w[2 * e], w[2 * e + 1], 1.f), bf16_of(sees), n);
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[r][d][j] = n[j] > 0.f ? __builtin_nanf("") : o[r][d][j];
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-  }
-  // ---- the four waves together
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    l[r] = four_lanes<false>(l[r]);
-    if (g == 0) {
-      sum_m[wave][r * 16 + c] = m[r];
-      sum_l[wave][r * 16 + c] = l[r];
-    }
-  }
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const v8bf a = frag(buf, 2 * (KP + d) + e);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) o[r][d] = mfma_bf16(a, p[r][e], o[r][d]);
+        if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  const int n = it.pg1 - it.pg0;
+  __syncthreads();  // (the plan's memory is free)
+  if (tid < 2) L.odd[tid] = -1;
   __syncthreads();
-  const bool whole = n_pages <= A.chunk;
-  const int64_t part = (static_cast<int64_t>(slot) * A.kv_heads + head) * A.splits + split;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    float top = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sum_m[w][r * 16 + c]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = sum_m[w][r * 16 + c];
-      total += sum_l[w][r * 16 + c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - top));
-    }
-    const float by = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - top);
-    if (r) __syncthreads();
-#pragma unroll
-    for (int d = 0; d < DT; ++d) sum_o[wave][d][lane] = o[r][d] * by;
+  if (n > 0) {
+    auto unseen = [&](int pg) { return (pg + 1) * kGqaKeys > least_all; };  // some row of the tile does not see all of the page
+    auto fine = [&](const Codes& r) { return static_cast<bool>(__all(gqa_scale_ok(r.s.x) && gqa_scale_ok(r.s.y))); };
+    int id = page_id(it.pg0), id1 = page_id(it.pg0 + 1), id2 = page_id(it.pg0 + 2);
+    Codes ca = fetch(id), cb = fetch(id1);
+    stage(ca, 0, it.pg0, unseen(it.pg0));
+    bool ok = fine(ca);
     __syncthreads();
-    const int row = row0 + r * 16 + c;
-    const int64_t at = (static_cast<int64_t>(s.first + row / A.group) * A.heads + head * A.group + row % A.group);
-    const bool live = r * 16 + c < rows;
-    const float inv = total == 0.f ? 0.f : 1.0f / total;
-#pragma unroll
-    for (int i = 0; i < DT / 4; ++i) {
-      const int d = 4 * i + wave;
-      const v4f v = sum_o[0][d][lane] + sum_o[1][d][lane] + sum_o[2][d][lane] + sum_o[3][d][lane];
-      if (whole) {
-        if (live) *reinterpret_cast<u32x2g*>(A.out + at * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
-      } else if (live) {
-        reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[(r * DT + d) * 64 + lane] = v;
-      }
+    // page k from its buffer; page k + 1's codes, loaded a page ago, go into the other one; page k + 2's are fetched
+    auto half = [&](int k, int buf, Codes& next, Codes& then) {
+      then = fetch(id2);
+      const bool is = there(id);
+      if (rows > 0) step(it.pg0 + k, is, ok, buf);
+      id = id1;
+      id1 = id2;
+      id2 = page_id(it.pg0 + k + 3);
+      if (k + 1 < n) stage(next, buf ^ 1, it.pg0 + k + 1, unseen(it.pg0 + k + 1));
+      ok = fine(next);
+      __syncthreads();
+    };
+    for (int k = 0; k < n; k += 2) {
+      half(k, 0, cb, ca);
+      if (k + 1 >= n) break;
+      half(k + 1, 1, ca, cb);
     }
-    if (wave == 0 && g == 0 && live) {
-      if (!whole) A.part_ml[part * BM + r * 16 + c] = float2{top, total};
-      else if (A.lse) A.lse[at] = total == 0.f ? -INFINITY : (top + kGqaHead + log2f(total)) * kLn2;
+  }
+  const bool whole = it.parts == 1;
+  const int64_t part = it.part * A.kv_heads + head;
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    l[r] = four_lanes<false>(l[r]);
+    if (r * 16 + c >= rows) continue;
+    const int row = row0 + r * 16 + c;
+    const int64_t at = static_cast<int64_t>(s.first + row / A.group) * A.heads + head * A.group + row % A.group;
+    const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const v4f v = o[r][d];
+      if (whole) *reinterpret_cast<u32x2g*>(A.out + at * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
+      else reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[((wave * RW + r) * DT + d) * 64 + lane] = v;
+    }
+    if (g == 0) {
+      if (!whole) A.part_ml[part * BM + (wave * RW + r) * 16 + c] = float2{m[r], l[r]};
+      else if (A.lse) A.lse[at] = l[r] == 0.f ? -INFINITY : (m[r] + kGqaHead + log2f(l[r])) * kLn2;
     }
   }
 }
 
-// The parts of split tiles joined in a fixed order: a workgroup takes 16 rows x 16 dims of a tile, its eight waves every eighth
-// part, joined in LDS.
-template <int D, int RT>
-__global__ __launch_bounds__(512) void gqa_join_kernel(const GqaArgs A) {
-  constexpr int BM = 16 * RT, DT = D / 16, WAVES = 8;
-  __shared__ v4f sum_o[WAVES][64];
-  __shared__ float sum_l[WAVES][16];
+// The parts of cut tiles joined in a fixed order, 16 rows of a tile at a time.  DEEP: a workgroup takes 16 dims of them, its eight
+// waves every eighth part, joined in LDS (few tiles of many parts); else its waves take 16 dims each.
+constexpr int kJoinWaves = 8;
+template <int D, int BM, bool DEEP>
+__global__ __launch_bounds__(64 * kJoinWaves) void gqa_join_kernel(const GqaArgs A) {
+  constexpr int DT = D / 16, PER = DEEP ? DT : (DT + kJoinWaves - 1) / kJoinWaves, STEP = DEEP ? kJoinWaves : 1;
+  __shared__ v4f sum_o[kJoinWaves][64];
+  __shared__ float sum_l[kJoinWaves][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int slot = blockIdx.x / A.kv_heads, head = blockIdx.x % A.kv_heads, r = blockIdx.y / DT, d = blockIdx.y % DT;
+  const int slot = blockIdx.x / A.kv_heads, head = blockIdx.x % A.kv_heads, r = blockIdx.y / PER;
+  const int d = DEEP ? blockIdx.y % PER : blockIdx.y % PER * kJoinWaves + wave;
+  if (!DEEP && d >= DT) return;
   int b, tile;
-  if (!gqa_tile<BM>(A.p, A.group, slot, b, tile)) return;
+  const int2 mine = A.tile_parts[slot];
+  if (!gqa_tile(A.p, A.group, slot, BM, b, tile)) return;
   const GqaSeq s(A.p, A.group, b);
-  const int row0 = tile * BM, rows = min(s.rows - row0, BM);
-  if (rows <= r * 16) return;
-  const int n_pages = (s.seen(row0 + rows - 1) + kGqaKeys - 1) / kGqaKeys, parts = (n_pages + A.chunk - 1) / A.chunk;
-  if (parts <= 1) return;
-  const int64_t part0 = (static_cast<int64_t>(slot) * A.kv_heads + head) * A.splits;
+  const int row0 = tile * BM, rows = min(s.rows - row0, BM), parts = mine.y;
+  if (rows <= r * 16 || parts <= 1) return;  // (a tile that is there has told its parts)
   const bool live = r * 16 + c < rows;
   const int row = r * 16 + (live ? c : 0);  // (rows that are not there have no parts)
   const int at = (r * DT + d) * 64 + (live ? lane : 16 * g);
+  auto part = [&](int i) { return static_cast<int64_t>(mine.x + i) * A.kv_heads + head; };
   float top = -INFINITY;
-  for (int i = g; i < parts; i += 4) top = fmaxf(top, A.part_ml[(part0 + i) * BM + row].x);
+  for (int i = g; i < parts; i += 4) top = fmaxf(top, A.part_ml[part(i) * BM + row].x);
   top = four_lanes<true>(top);
   float l = 0.f;
   v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = wave; i < parts; i += WAVES) {
-    const float2 ml = A.part_ml[(part0 + i) * BM + row];
-    const v4f x = reinterpret_cast<const v4f*>(A.part_o + (part0 + i) * (BM * D))[at];
+#pragma unroll 8
+  for (int i = DEEP ? wave : 0; i < parts; i += STEP) {
+    const float2 ml = A.part_ml[part(i) * BM + row];
+    const v4f x = reinterpret_cast<const v4f*>(A.part_o + part(i) * (BM * D))[at];
     const float by = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
     l += ml.y * by;
     o += x * by;
   }
-  sum_o[wave][lane] = o;
-  if (g == 0) sum_l[wave][c] = l;
-  __syncthreads();
-  if (wave > 0 || !live) return;
-  l = sum_l[0][c];
-  for (int w = 1; w < WAVES; ++w) {
-    o += sum_o[w][lane];
-    l += sum_l[w][c];
+  if constexpr (DEEP) {
+    sum_o[wave][lane] = o;
+    if (g == 0) sum_l[wave][c] = l;
+    __syncthreads();
+    if (wave > 0) return;
+    l = sum_l[0][c];
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) {
+      o += sum_o[w][lane];
+      l += sum_l[w][c];
+    }
   }
+  if (!live) return;
   const int64_t to = static_cast<int64_t>(s.first + (row0 + row) / A.group) * A.heads + head * A.group + (row0 + row) % A.group;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   *reinterpret_cast<u32x2g*>(A.out + to * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{o[0] * inv, o[1] * inv}), bf16x2_bits(v2f{o[2] * inv, o[3] * inv})};
   if (A.lse && d == 0 && g == 0) A.lse[to] = l == 0.f ? -INFINITY : (top + kGqaHead + log2f(l)) * kLn2;
 }
 
-// The launch: rows a tile, pages a workgroup, and the workspace.
-struct GqaPlan {
-  int rt;
-  int64_t slots, chunk, splits;
-  size_t o_at, bytes;
+// The launch: rows a tile, workgroups, and the workspace.
+struct GqaLaunch {
+  int bm;
+  bool deep;  // the join's form
+  int64_t slots, target, wgs;
+  size_t ml_at, o_at, bytes;
 };
-constexpr int kGqaChunks = 2048;  // workgroups of a split launch, about
-constexpr int kGqaFew = 8;        // pages that are not split
-inline GqaPlan gqa_plan(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_pages) {
-  GqaPlan d{};
+inline GqaLaunch gqa_launch(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_pages) {
+  GqaLaunch d{};
   const int64_t group = heads / kv_heads, each = cdiv(n_tokens * group, n_seqs);
-  d.rt = each <= 16 ? 1 : 2;
-  d.slots = gqa_slots(n_tokens, group, n_seqs, 16 * d.rt);
-  const int64_t tiles = d.slots * kv_heads;
-  d.chunk = cdiv(tiles * max_pages, kGqaChunks);
-  if (d.chunk < kGqaFew) d.chunk = kGqaFew;
-  if (d.chunk > max_pages) d.chunk = max_pages;
-  d.splits = cdiv(max_pages, d.chunk);
-  if (d.splits > 1) {
-    d.o_at = static_cast<size_t>((tiles * d.splits * 16 * d.rt * sizeof(float2) + 255) / 256 * 256);
-    d.bytes = d.o_at + static_cast<size_t>(tiles * d.splits) * 16 * d.rt * head_dim * sizeof(float);
+  d.bm = each <= 16 ? 16 : (each <= 32 ? 32 : (each <= 64 ? 64 : 256));
+  d.slots = gqa_slots(n_tokens, group, n_seqs, d.bm);
+  d.deep = d.bm <= 64;
+  d.target = n_seqs > kGqaPlanSeqs || max_pages <= kGqaFew ? 0 : (d.bm > 64 ? 256 : (d.slots * kv_heads <= 128 ? 512 : 1024));
+  d.wgs = d.slots * kv_heads + d.target;
+  if (d.target) {
+    d.ml_at = (d.slots * sizeof(int2) + 255) / 256 * 256;
+    d.o_at = d.ml_at + static_cast<size_t>(2 * d.target) * d.bm * sizeof(float2);
+    d.bytes = d.o_at + static_cast<size_t>(2 * d.target) * d.bm * head_dim * sizeof(float);
   }
   return d;
 }
@@ -532,7 +904,7 @@ extern "C" size_t tl_flash_paged_gqa_workspace_bytes(int64_t n_seqs, int64_t n_t
                                                      int64_t head_dim, int64_t max_pages) {
   if (n_seqs < 1 || n_tokens < 1 || kv_heads < 1 || heads < 1 || heads > 128 || heads % kv_heads || max_pages < 1 || n_seqs > (1ll << 16) ||
       max_pages > (1ll << 20) || n_tokens * heads >= kGqaMaxRows || (head_dim != 64 && head_dim != 128)) return 0;
-  return gqa_plan(n_seqs, n_tokens, heads, kv_heads, head_dim, max_pages).bytes;
+  return gqa_launch(n_seqs, n_tokens, heads, kv_heads, head_dim, max_pages).bytes;
 }
 
 extern "C" int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const void* kv_pages, int64_t n_pages,
@@ -548,12 +920,12 @@ extern "C" int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const vo
   if (int rc = check_gqa_batch(who, n_seqs, n_tokens, heads, max_pages, softmax_scale)) return rc;
   if (int rc = check_gqa_rows(who, "query", q_bf16, q_stride, heads, head_dim)) return rc;
   if (int rc = check_gqa_rows(who, "output", out_bf16, heads * head_dim, heads, head_dim)) return rc;
-  const GqaPlan d = gqa_plan(n_seqs, n_tokens, heads, kv_heads, head_dim, max_pages);
+  const GqaLaunch d = gqa_launch(n_seqs, n_tokens, heads, kv_heads, head_dim, max_pages);
   if (d.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < d.bytes)) {
     set_error("%s: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", who, d.bytes, workspace_bytes);
     return kErrArg;
   }
-  if (d.slots * kv_heads * d.splits >= (1ll << 24)) {
+  if (d.wgs >= (1ll << 24)) {
     set_error("%s: %lld tokens, %lld sequences: more than a launch has room for", who, (long long)n_tokens, (long long)n_seqs);
     return kErrUnsupported;
   }
@@ -561,19 +933,35 @@ extern "C" int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const vo
   const GqaArgs args{(const uint16_t*)q_bf16, q_stride, (const uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
                      PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
                      (int)heads, (int)kv_heads, (int)(heads / kv_heads), softmax_scale * kLog2e, (uint16_t*)out_bf16, lse,
-                     (int)d.chunk, (int)d.splits, reinterpret_cast<float2*>(ws), reinterpret_cast<float*>(ws + d.o_at)};
+                     (int)d.target, reinterpret_cast<int2*>(ws), reinterpret_cast<float2*>(ws + d.ml_at), reinterpret_cast<float*>(ws + d.o_at)};
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto dim, auto rt) -> int {
-    constexpr int D = decltype(dim)::value, RT = decltype(rt)::value;
-    hipLaunchKernelGGL((gqa_attend_kernel<D, RT>), dim3(d.slots * kv_heads, d.splits), dim3(256), 0, st, args);
-    if (int rc = check_launch(who)) return rc;
-    if (d.splits == 1) return kOk;
-    hipLaunchKernelGGL((gqa_join_kernel<D, RT>), dim3(d.slots * kv_heads, RT * D / 16), dim3(512), 0, st, args);
+  auto join = [&](auto dim, auto bm, auto deep) -> int {
+    constexpr int D = decltype(dim)::value, BM = decltype(bm)::value, DT = D / 16;
+    if (!d.target) return kOk;
+    hipLaunchKernelGGL((gqa_join_kernel<D, BM, decltype(deep)::value>), dim3(d.slots * kv_heads, BM / 16 * (decltype(deep)::value ? DT : cdiv(DT, kJoinWaves))),
+                       dim3(64 * kJoinWaves), 0, st, args);
     return check_launch(who);
   };
   using std::integral_constant;
-  if (head_dim == 64) return d.rt == 1 ? launch(integral_constant<int, 64>{}, integral_constant<int, 1>{}) : launch(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  return d.rt == 1 ? launch(integral_constant<int, 128>{}, integral_constant<int, 1>{}) : launch(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+  auto few = [&](auto dim, auto rt) -> int {
+    constexpr int D = decltype(dim)::value, RT = decltype(rt)::value;
+    hipLaunchKernelGGL((gqa_attend_kernel<D, RT>), dim3(d.wgs), dim3(256), 0, st, args);
+    if (int rc = check_launch(who)) return rc;
+    return join(dim, integral_constant<int, 16 * RT>{}, std::true_type{});
+  };
+  auto many = [&](auto dim, auto rw, auto nw) -> int {
+    constexpr int D = decltype(dim)::value, RW = decltype(rw)::value, NW = decltype(nw)::value;
+    const auto kern = gqa_chunk_kernel<D, RW, NW>;
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), gqa_chunk_lds<D>(), who)) return rc;
+    hipLaunchKernelGGL(kern, dim3(d.wgs), dim3(64 * NW), gqa_chunk_lds<D>(), st, args);
+    if (int rc = check_launch(who)) return rc;
+    return join(dim, integral_constant<int, 16 * RW * NW>{}, std::false_type{});
+  };
+  auto by_rows = [&](auto dim) -> int {
+    return d.bm == 16 ? few(dim, integral_constant<int, 1>{}) : (d.bm == 32 ? few(dim, integral_constant<int, 2>{}) :
+           (d.bm == 64 ? few(dim, integral_constant<int, 4>{}) : many(dim, integral_constant<int, GQA_RW>{}, integral_constant<int, GQA_NW>{})));
+  };
+  return head_dim == 64 ? by_rows(std::integral_constant<int, 64>{}) : by_rows(std::integral_constant<int, 128>{});
 }
 
 extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const float* lse, const void* kv_pages, int64_t n_pages,
