@@ -162,9 +162,10 @@ def test_bad_pages_among_many(cuda, new):
     for b, n in enumerate(total):
         need = -(-n // 64)
         bad = torch.randperm(need, generator=g)[:need // 3]
-        table[b, bad] = torch.where(bad % 2 == 0, -1, pages.shape[0]).to(torch.int32)
-        table[b, :4] = -1
+        table[b, bad] = torch.where(bad % 2 == 0, -2, pages.shape[0]).to(torch.int32)
+        table[b, :4] = -2
     table[2, :-(-total[2] // 64) - 1] = -3  # one page is left, the last
+    pages, table = torch.cat([torch.full_like(pages[:1], 0xff), pages]), table + 1  # page 0 is nobody's, and NaN
     q = _gqa.queries(rows, 8, 64, 63)
     out, lse = run(cuda, q, pages, table, cu, lens, 2)
     check(cuda, q, pages, table, cu, lens, 2, out, lse)
@@ -183,15 +184,15 @@ def test_a_cache_longer_than_its_table(cuda, new):
 
 
 @pytest.mark.parametrize("what", ["key", "value", "key scale", "value scale", "infinite scale", "negative scale"])
-@pytest.mark.parametrize("new,total", [(50, 250), (300, 430)])
-def test_a_bad_key_reaches_only_the_tokens_that_see_it(cuda, what, new, total):
+@pytest.mark.parametrize("new,total,back", [(50, 250, 30), (300, 430, 30), (300, 430, 100), (300, 430, 50)])
+def test_a_bad_key_reaches_only_the_tokens_that_see_it(cuda, what, new, total, back):
     """A NaN in a key's or value's codes, or a scale that is none: tokens before it are as without it, bit for bit, and
     those from it on are NaN where the definition is."""
     pages, table, cu, lens, rows = _gqa.batch([new], [total], 2, 128, seed=39)
     _gqa.fill(pages, table, [total], 2, 128)
     q = _gqa.queries(rows, 8, 128, 41)
     clean, clean_lse = run(cuda, q, pages, table, cu, lens, 2)
-    at = total - 30
+    at = total - back
     page, row, first = int(table[0, at // 64]), at % 64, at - (total - new)
     k, v, scales = gqa.views(pages, 2, 128)
     if what == "key":

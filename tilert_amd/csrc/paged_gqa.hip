@@ -17,12 +17,9 @@
 #include "gqa.h"
 #include "../../include/tilert_amd.h"
 
-#ifndef GQA_RW
-#define GQA_RW 2
-#define GQA_NW 8
-#endif
 namespace tl {
 
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef const __attribute__((address_space(4))) int32_t* gqa_const_i32;  // scalar loads
 
 struct GqaArgs {
@@ -478,237 +475,320 @@ __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
 
 // ---- many rows: the waves of a workgroup go through the pages together
 // A page's codes are turned into bf16 once, by the wave that loaded them, and lie in LDS as the products' operands, fragment
-// by fragment in lane order; each wave multiplies them with its own 16 RW rows.  Weights go into the second product in
+// by fragment in lane order; each wave multiplies them with its own 32 rows.  Weights go into the second product in
 // bf16, 8 bits.  A row's reference m is set anew only where a score passes it by 2^8: hardly a page rescales anything.
+//
+// The two waves of a SIMD are a third of a page apart: between two barriers waves 0 .. 3 make scores, weights and sums of page k,
+// waves 4 .. 7 weights and sums of page k - 1 and scores of page k, so that one's products run while the other makes
+// weights.  (At the same place of the page, 532 us for 2048 tokens over 16384 keys.)  Values are multiplied up to a page
+// later than keys, so they have three buffers and keys two.
 constexpr float kGqaLag = 8.f;
+constexpr int kChunkWaves = 8, kChunkRows = 32 * kChunkWaves;
 template <int D>
-constexpr int gqa_chunk_lds() { return 2 * (2 * (4 * (D / 64) + D / 16) + D / 16) * 1024 + 16; }
-template <int D, int RW, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void gqa_chunk_kernel(const GqaArgs A) {
-  constexpr int BM = 16 * RW * NW, DT = D / 16, KI = D / 64, KP = 4 * KI, PIECES = KP + DT, MINE = PIECES / NW, FRAG = 2 * PIECES;
-  extern __shared__ __attribute__((aligned(16))) uint8_t gqa_smem[];
-  struct Lds {
-    union {
-      GqaPlanLds plan;
-      u32x4g frag[2][FRAG][64];  // keys [t][i][e], then values [d][e]
+struct GqaChunkLds {
+  static constexpr int KF = D / 16, VT = D / 32;  // fragments of 32 keys; 32-dim tiles of the values
+  union {
+    GqaPlanLds plan;
+    struct {
+      u32x4g k[2][2][KF][64];     // [t][f]: 32 keys x 16 dims
+      u32x4g v[3][VT][2][2][64];  // [d][t][e]: 32 dims x 16 keys
+      u32x4g bad[3][VT][2][64];   // [d][t]: where values of a page are NaN that is not seen by all rows
     };
-    u32x4g bad[2][DT][64];  // where those of a page are NaN that is not seen by all rows
-    int odd[2];             // the page of a buffer that has such values
   };
-  static_assert(sizeof(Lds) <= gqa_chunk_lds<D>(), "");
-  Lds& L = *reinterpret_cast<Lds*>(gqa_smem);
+  int odd[3];  // the page of a buffer that has such values
+};
+__device__ inline v16f mfma32_bf16(v8bf a, v8bf b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+template <bool MAX>
+__device__ inline float two_halves(float v) {  // of lanes i, i ^ 32, in both
+  const u32x2g b = __builtin_bit_cast(u32x2g, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  const float b0 = __uint_as_float(b[0]), b1 = __uint_as_float(b[1]);
+  return MAX ? fmaxf(b0, b1) : b0 + b1;
+}
+// Row i of a 32-key fragment of tile t is the page's key 32 (i / 4 % 2) + 16 t + 4 (i / 8) + i % 4, so that a lane's sixteen
+// results are the keys 32 h + 16 t .. + 15 of its row, as a 16-byte load of a dim's values has them (h: the lane's half).
+template <int D>
+__global__ __launch_bounds__(64 * kChunkWaves, 2) void gqa_chunk_kernel(const GqaArgs A) {
+  constexpr int NW = kChunkWaves, BM = kChunkRows, KI = D / 64, KP = 4 * KI, MINE = (KP + D / 16) / NW, KF = D / 16, VT = D / 32;
+  extern __shared__ __attribute__((aligned(16))) uint8_t gqa_smem[];
+  GqaChunkLds<D>& L = *reinterpret_cast<GqaChunkLds<D>*>(gqa_smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
+  const int c = lane & 31, h = lane >> 5, late = wave >> 2;
   const int head = blockIdx.x % A.kv_heads;
   GqaItem it;
   int first, rows_all;
   int64_t base;
   if (!gqa_item<64 * NW, BM>(A, L.plan, blockIdx.x / A.kv_heads, it, first, rows_all, base)) return;
   const GqaSeq s(A.p, A.group, first, rows_all, base);
-  const int row0 = it.tile * BM + wave * 16 * RW, rows = min(s.rows - it.tile * BM, BM) - wave * 16 * RW;  // this wave's
-  const int last = s.rows - 1;
+  const int row0 = it.tile * BM + wave * 32, last = s.rows - 1;  // this wave's rows
+  const bool any = row0 <= last;
   const int least = s.seen(min(row0, last)), least_all = s.seen(it.tile * BM);
   const gqa_const_i32 table = (gqa_const_i32)(A.p.table + static_cast<int64_t>(it.b) * A.p.max_pages);
-  GqaQuery<D> q[RW];
-  int seen[RW];
-  float m[RW], l[RW];
-  v4f o[RW][DT];
+  // the query rows as the first product's B operand: lane (c, h) has of row c the dims 64 i + 32 j + 16 h + 8 e .. + 7 for
+  // fragment 4 i + 2 j + e, as a 16-byte load gives it a key's codes
+  v8bf q[KF];
+  {
+    const bool live = row0 + c <= last;
+    const int at = live ? row0 + c : 0;
+    const uint16_t* from = A.q + (s.first + at / A.group) * A.q_stride + (head * A.group + at % A.group) * D + 16 * h;
 #pragma unroll
-  for (int r = 0; r < RW; ++r) {
-    q[r] = load_query<D>(A.q, A.q_stride, s, head * A.group, row0 + r * 16 + c, g);
-    seen[r] = s.seen(min(row0 + r * 16 + c, last));
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < KF; ++f) {
+      u32x4g v = *reinterpret_cast<const u32x4g*>(from + 32 * (f / 2) + 8 * (f % 2));
+      if (!live) v = u32x4g{0, 0, 0, 0};
+      q[f] = bf16_of(v);
+    }
   }
-  auto page_id = [&](int pg) { return __builtin_amdgcn_readfirstlane(table[min(pg, it.pg1 - 1)]); };
+  const int seen = s.seen(min(row0 + c, last));
+  float m = -INFINITY, l = 0.f;
+  v16f o[VT], x[2];
+  v8bf p[2][2];
+#pragma unroll
+  for (int d = 0; d < VT; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[d][j] = 0.f;
+  const int n = it.pg1 - it.pg0;
+  auto page_id = [&](int k) { return __builtin_amdgcn_readfirstlane(table[it.pg0 + min(k, n - 1)]); };
   auto there = [&](int id) { return id >= 0 && id < A.p.n_pages; };
+  auto unseen = [&](int k) { return (it.pg0 + k + 1) * kGqaKeys > least_all; };  // some row of the tile does not see all of the page
+  auto fine = [&](float2 v) { return static_cast<bool>(__all(gqa_scale_ok(v.x) && gqa_scale_ok(v.y))); };
   struct Codes {
     u32x4g x[MINE];
     float2 s;
+    bool is;
   };
-  auto fetch = [&](int id) {  // this wave's pieces of a page
+  // This wave's pieces of a page, 1 KB each: 16 keys x 64 dims, then 16 dims x 64 keys; lane (r, b) has 16 bytes b of row r
+  const int r16 = lane & 15, b16 = lane >> 4;
+  auto fetch = [&](int id) __attribute__((always_inline)) {
     const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there(id) ? id : 0, head);
     Codes r;
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
-      const int piece = wave + NW * j;
-      const uint8_t* k = blk.k + (16 * (c >> 2) + (c & 3) + 4 * (piece / KI)) * D + 64 * (piece % KI) + 16 * g;
-      const uint8_t* v = blk.v + ((piece - KP) * 16 + c) * kGqaKeys + 16 * g;
+      const int piece = wave + NW * j, rows = piece / KI;  // of keys: t = rows / 2, fragment rows 16 (rows % 2) ..
+      const int i = 16 * (rows & 1) + r16;
+      const uint8_t* k = blk.k + (32 * (i >> 2 & 1) + 16 * (rows >> 1) + 4 * (i >> 3) + (i & 3)) * D + 64 * (piece % KI) + 16 * b16;
+      const uint8_t* v = blk.v + ((piece - KP) * 16 + r16) * kGqaKeys + 16 * b16;
       r.x[j] = *reinterpret_cast<const u32x4g*>(piece < KP ? k : v);
     }
     r.s = load_scales(blk.scale);
+    r.is = there(id);
     return r;
   };
-  auto stage = [&](const Codes& r, int buf, int pg, bool masked) {
-    const bool ok = gqa_scale_ok(r.s.x) && gqa_scale_ok(r.s.y);
+  auto stage = [&](const Codes& r, bool ok, int k, int kb, int vb) __attribute__((always_inline)) {
+    const bool masked = unseen(k) || !r.is;
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
       const int piece = wave + NW * j;
       const float by = ok ? (piece < KP ? r.s.x : r.s.y) : 1.f;
       u32x4g x = r.x[j];
-      if (masked && piece >= KP) {  // on a page with keys that some row does not see, values that are NaN are taken apart
-        u32x4g bad;
+      u32x4g* to;  // the fragment of the piece's even 8 bytes; that of the odd ones is the next
+      if (piece < KP) {
+        const int rows = piece / KI;
+        to = &L.k[kb][rows >> 1][4 * (piece % KI) + 2 * (b16 >> 1)][32 * (b16 & 1) + 16 * (rows & 1) + r16];
+      } else {
+        const int d = piece - KP, at = 32 * (b16 >> 1) + 16 * (d & 1) + r16;
+        if (masked) {  // on a page with keys that some row does not see, values that are NaN are taken apart
+          u32x4g bad;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad[i] = nan_codes(x[i]);
-        if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0) && lane == 0) L.odd[buf] = pg;
+          for (int i = 0; i < 4; ++i) bad[i] = nan_codes(x[i]);
+          if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0) && lane == 0) L.odd[vb] = it.pg0 + k;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] &= ~(bad[i] | (bad[i] - (bad[i] >> 7)));
-          bad[i] >>= 1;  // the code of 2
+          for (int i = 0; i < 4; ++i) {
+            x[i] &= ~(bad[i] | (bad[i] - (bad[i] >> 7)));
+            bad[i] >>= 1;  // the code of 2
+          }
+          L.bad[vb][d >> 1][b16 & 1][at] = bad;
         }
-        L.bad[buf][piece - KP][lane] = bad;
+        to = &L.v[vb][d >> 1][b16 & 1][0][at];
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) L.frag[buf][2 * piece + e][lane] = __builtin_bit_cast(u32x4g, codes8_bf16(x[2 * e], x[2 * e + 1], by));
+      for (int e = 0; e < 2; ++e) to[64 * e] = __builtin_bit_cast(u32x4g, codes8_bf16(x[2 * e], x[2 * e + 1], by));
     }
   };
-  auto frag = [&](int buf, int f) { return bf16_of(L.frag[buf][f][lane]); };
-  auto step = [&](int pg, bool is, bool ok, int buf) {
-    const int key0 = pg * kGqaKeys;
-    const bool masked = !is || !ok || key0 + kGqaKeys > least;
-    v4f x[RW][4];
+  // (operands are read four fragments ahead of the products, by hand: left to itself the compiler waits for each)
+  auto scores = [&](int kb) __attribute__((always_inline)) {
+    if (!any) return;
+    v8bf f[2][4];
+    auto load = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+      for (int j = 0; j < 4; ++j) f[i & 1][j] = bf16_of(L.k[kb][i / (KF / 4)][i % (KF / 4) * 4 + j][lane]);
+    };
+    load(0);
 #pragma unroll
-      for (int r = 0; r < RW; ++r) x[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < KF / 2; ++i) {
+      const int t = i / (KF / 4);
+      if (i + 1 < KF / 2) load(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i % (KF / 4) == 0)
 #pragma unroll
-      for (int i = 0; i < 2 * KI; ++i) {
-        const v8bf a = frag(buf, t * 2 * KI + i);
+        for (int j = 0; j < 16; ++j) x[t][j] = 0.f;
 #pragma unroll
-        for (int r = 0; r < RW; ++r) x[r][t] = mfma_bf16(a, q[r].x[i / 2][i % 2], x[r][t]);
-      }
+      for (int j = 0; j < 4; ++j) x[t] = mfma32_bf16(f[i & 1][j], q[i % (KF / 4) * 4 + j], x[t]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (masked)
+  };
+  auto values = [&](int k, bool is, int vb) __attribute__((always_inline)) {
+    if ((unseen(k) || !is) && L.odd[vb] == it.pg0 + k) {  // how many NaN values a row sees
+      const int my = is ? seen - (it.pg0 + k) * kGqaKeys - 32 * h : 0;
 #pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        const int my = is ? seen[r] - key0 - 16 * g : 0;
+      for (int d = 0; d < VT; ++d) {
+        v16f z;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int j = 0; j < 16; ++j) z[j] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[r][t][j] = 4 * t + j >= my ? -INFINITY : (ok ? x[r][t][j] : __builtin_nanf(""));
-      }
-    float top[RW];
-    bool grows = false;
-#pragma unroll
-    for (int r = 0; r < RW; ++r) {
-      top[r] = x[r][0][0];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top[r] = fmaxf(top[r], x[r][t][j]);
-      top[r] *= A.scale;
-      grows = grows || top[r] > m[r] + kGqaLag;
-    }
-    if (__any(grows))
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        const float now = fmaxf(m[r], four_lanes<true>(top[r]));
-        const float by = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - now);
-        m[r] = now;
-        l[r] *= by;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] *= by;
-      }
-    v8bf p[RW][2];
-#pragma unroll
-    for (int r = 0; r < RW; ++r) {
-      const float from = m[r] == -INFINITY ? 0.f : m[r] + kGqaHead;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        u32x4g h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4f y = x[r][2 * e + i / 2];
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1)], A.scale, -from));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1) + 1], A.scale, -from));
-          l[r] += p0 + p1;
-          h[i] = bf16x2_bits(v2f{p0, p1});
-        }
-        p[r][e] = bf16_of(h);
-      }
-    }
-    if (masked && L.odd[buf] == pg)  // how many NaN values a row sees
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const u32x4g w = L.bad[buf][d][lane];
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          const int my = is ? seen[r] - key0 - 16 * g : 0;
-          v4f n = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 2; ++t) {
+          const u32x4g w = L.bad[vb][d][t][lane];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             u32x4g sees;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sees[i] = (8 * e + 2 * i < my ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my ? 0x3f800000u : 0u);
-            n = mfma_bf16(codes8_bf16(w[2 * e], w[2 * e + 1], 1.f), bf16_of(sees), n);
+            for (int i = 0; i < 4; ++i) sees[i] = (16 * t + 8 * e + 2 * i < my ? 0x3f80u : 0u) | (16 * t + 8 * e + 2 * i + 1 < my ? 0x3f800000u : 0u);
+            z = mfma32_bf16(codes8_bf16(w[2 * e], w[2 * e + 1], 1.f), bf16_of(sees), z);
           }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[r][d][j] = n[j] > 0.f ? __builtin_nanf("") : o[r][d][j];
         }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[d][j] = z[j] > 0.f ? __builtin_nanf("") : o[d][j];
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    v8bf f[2][VT];
+    auto load = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+      for (int d = 0; d < VT; ++d) f[i & 1][d] = bf16_of(L.v[vb][d][i >> 1][i & 1][lane]);
+    };
+    load(0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const v8bf a = frag(buf, 2 * (KP + d) + e);
+    for (int i = 0; i < 4; ++i) {
+      if (i < 3) load(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < RW; ++r) o[r][d] = mfma_bf16(a, p[r][e], o[r][d]);
-        if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      for (int d = 0; d < VT; ++d) o[d] = mfma32_bf16(f[i & 1][d], p[i >> 1][i & 1], o[d]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto weights = [&](int pg, bool is, bool ok) __attribute__((always_inline)) {
+    const int key0 = pg * kGqaKeys;
+    if (!is || !ok || key0 + kGqaKeys > least) {
+      const int my = is ? seen - key0 - 32 * h : 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[t][j] = 16 * t + j >= my ? -INFINITY : (ok ? x[t][j] : __builtin_nanf(""));
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
+    top *= A.scale;
+    if (__any(top > m + kGqaLag)) {
+      const float now = fmaxf(m, two_halves<true>(top));
+      const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < VT; ++d) o[d] *= by;
+    }
+    const float from = m == -INFINITY ? 0.f : m + kGqaHead;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        u32x4g w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][8 * e + 2 * i], A.scale, -from));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][8 * e + 2 * i + 1], A.scale, -from));
+          l += p0 + p1;
+          w[i] = bf16x2_bits(v2f{p0, p1});
+        }
+        p[t][e] = bf16_of(w);
       }
   };
-  const int n = it.pg1 - it.pg0;
+  // Of two waves that could issue, the hardware takes the older one, and waves 4 .. 7, with their weights first and both
+  // products behind, would come last to every barrier: 510 us, 482 with their priority raised.
+  if (late) __builtin_amdgcn_s_setprio(1);
   __syncthreads();  // (the plan's memory is free)
-  if (tid < 2) L.odd[tid] = -1;
+  if (tid < 3) L.odd[tid] = -1;
   __syncthreads();
   if (n > 0) {
-    auto unseen = [&](int pg) { return (pg + 1) * kGqaKeys > least_all; };  // some row of the tile does not see all of the page
-    auto fine = [&](const Codes& r) { return static_cast<bool>(__all(gqa_scale_ok(r.s.x) && gqa_scale_ok(r.s.y))); };
-    int id = page_id(it.pg0), id1 = page_id(it.pg0 + 1), id2 = page_id(it.pg0 + 2);
-    Codes ca = fetch(id), cb = fetch(id1);
-    stage(ca, 0, it.pg0, unseen(it.pg0));
-    bool ok = fine(ca);
+    // of page k and the one before: whether its scales are fine, and whether it is there; the codes of the two pages behind it,
+    // by turns in ca and cb
+    int vb = 0;
+    Codes ca = fetch(page_id(0)), cb;
+    bool ok = fine(ca.s), is = ca.is, ok_before = ok, was = is;
+    stage(ca, ok, 0, 0, 0);
+    cb = fetch(page_id(1));
+    ca = fetch(page_id(2));
     __syncthreads();
-    // page k from its buffer; page k + 1's codes, loaded a page ago, go into the other one; page k + 2's are fetched
-    auto half = [&](int k, int buf, Codes& next, Codes& then) {
-      then = fetch(id2);
-      const bool is = there(id);
-      if (rows > 0) step(it.pg0 + k, is, ok, buf);
-      id = id1;
-      id1 = id2;
-      id2 = page_id(it.pg0 + k + 3);
-      if (k + 1 < n) stage(next, buf ^ 1, it.pg0 + k + 1, unseen(it.pg0 + k + 1));
-      ok = fine(next);
+    auto ahead = [&](int k, int kb, Codes& codes) __attribute__((always_inline)) {  // page k + 1 into its buffers, page k + 3 on its way
+      const int to = vb == 2 ? 0 : vb + 1;
+      ok_before = ok;
+      was = is;
+      ok = fine(codes.s);
+      is = codes.is;
+      if (k + 1 < n) stage(codes, ok, k + 1, kb ^ 1, to);
+      codes = fetch(page_id(k + 3));
+      vb = to;
       __syncthreads();
     };
-    for (int k = 0; k < n; k += 2) {
-      half(k, 0, cb, ca);
-      if (k + 1 >= n) break;
-      half(k + 1, 1, ca, cb);
+    auto earlier = [&](int k) __attribute__((always_inline)) {
+      if (!any) return;
+      weights(it.pg0 + k - 1, was, ok_before);
+      values(k - 1, was, vb == 0 ? 2 : vb - 1);
+    };
+    if (late) {
+      scores(0);
+      ahead(0, 0, cb);
+      int k = 1;
+#pragma unroll 1
+      for (; k + 1 < n; k += 2) {
+        earlier(k);
+        scores(1);
+        ahead(k, 1, ca);
+        earlier(k + 1);
+        scores(0);
+        ahead(k + 1, 0, cb);
+      }
+      if (k < n) {
+        earlier(k);
+        scores(1);
+        ahead(k, 1, ca);
+      }
+      earlier(n);
+    } else {
+      auto page = [&](int k, int kb, Codes& codes) __attribute__((always_inline)) {
+        scores(kb);
+        if (any) {
+          weights(it.pg0 + k, is, ok);
+          values(k, is, vb);
+        }
+        ahead(k, kb, codes);
+      };
+      int k = 0;
+#pragma unroll 1
+      for (; k + 1 < n; k += 2) {
+        page(k, 0, cb);
+        page(k + 1, 1, ca);
+      }
+      if (k < n) page(k, 0, cb);
     }
   }
+  l = two_halves<false>(l);
+  if (row0 + c > last) return;
   const bool whole = it.parts == 1;
   const int64_t part = it.part * A.kv_heads + head;
+  const int64_t at = static_cast<int64_t>(s.first + (row0 + c) / A.group) * A.heads + head * A.group + (row0 + c) % A.group;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-  for (int r = 0; r < RW; ++r) {
-    l[r] = four_lanes<false>(l[r]);
-    if (r * 16 + c >= rows) continue;
-    const int row = row0 + r * 16 + c;
-    const int64_t at = static_cast<int64_t>(s.first + row / A.group) * A.heads + head * A.group + row % A.group;
-    const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
+  for (int d = 0; d < VT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const v4f v = o[r][d];
-      if (whole) *reinterpret_cast<u32x2g*>(A.out + at * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
-      else reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[((wave * RW + r) * DT + d) * 64 + lane] = v;
+    for (int j = 0; j < 4; ++j) {  // dims 32 d + 8 j + 4 h .. + 3
+      const v4f v = {o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+      if (whole) *reinterpret_cast<u32x2g*>(A.out + at * D + 32 * d + 8 * j + 4 * h) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
+      else reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[((wave * 2 + (c >> 4)) * (D / 16) + 2 * d + (j >> 1)) * 64 + (2 * (j & 1) + h) * 16 + (c & 15)] = v;
     }
-    if (g == 0) {
-      if (!whole) A.part_ml[part * BM + (wave * RW + r) * 16 + c] = float2{m[r], l[r]};
-      else if (A.lse) A.lse[at] = l[r] == 0.f ? -INFINITY : (m[r] + kGqaHead + log2f(l[r])) * kLn2;
-    }
+  if (h == 0) {
+    if (!whole) A.part_ml[part * BM + wave * 32 + c] = float2{m, l};
+    else if (A.lse) A.lse[at] = l == 0.f ? -INFINITY : (m + kGqaHead + log2f(l)) * kLn2;
   }
 }
 
@@ -777,10 +857,18 @@ struct GqaLaunch {
 inline GqaLaunch gqa_launch(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_pages) {
   GqaLaunch d{};
   const int64_t group = heads / kv_heads, each = cdiv(n_tokens * group, n_seqs);
-  d.bm = each <= 16 ? 16 : (each <= 32 ? 32 : (each <= 64 ? 64 : 256));
+  // In us with 64-row / kChunkRows tiles, rows a sequence and head: 48 rows of 1 sequence over 16384 keys 24 / 31, 64 rows 26 / 31, 96
+  // 36 / 33; of 8 sequences over 4096, 64 heads' tiles, 64 rows 48 / 45; of 32 over 1024, 256 tiles, 16 rows 31 / 35, 24
+  // rows 37 / 36, 32 rows 43 / 35, 64 rows 72 / 37: with a tile for every CU a page is better read by one workgroup.
+  d.bm = each > (n_seqs * kv_heads >= 256 ? 24 : 64) ? kChunkRows : (each <= 16 ? 16 : (each <= 32 ? 32 : 64));
   d.slots = gqa_slots(n_tokens, group, n_seqs, d.bm);
   d.deep = d.bm <= 64;
-  d.target = n_seqs > kGqaPlanSeqs || max_pages <= kGqaFew ? 0 : (d.bm > 64 ? 256 : (d.slots * kv_heads <= 128 ? 512 : 1024));
+  const int64_t tiles = d.slots * kv_heads;
+  // In us: 60 sequences of 2048 to 32768 keys, 1 token (480 tiles of 16 rows) 282 with 512 pieces, 273 with 1024, 277 with 2048; 4
+  // tokens over 131072 keys (8 tiles of 32 rows) 76, 86, 104: there a piece is a workgroup's all, and fewer are less to
+  // join.  Tiles of kChunkRows, a workgroup a CU: 7 sequences of 2 to 700 new tokens 60 with 256, 49 with 384, 58 with
+  // 512; 256 tiles that see 14336 to 16384 keys 484, 491, 491.
+  if (n_seqs <= kGqaPlanSeqs && max_pages > kGqaFew) d.target = d.bm == kChunkRows ? (tiles < 256 ? 384 : 256) : (tiles <= 128 ? 512 : 1024);
   d.wgs = d.slots * kv_heads + d.target;
   if (d.target) {
     d.ml_at = (d.slots * sizeof(int2) + 255) / 256 * 256;
@@ -949,17 +1037,17 @@ extern "C" int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const vo
     if (int rc = check_launch(who)) return rc;
     return join(dim, integral_constant<int, 16 * RT>{}, std::true_type{});
   };
-  auto many = [&](auto dim, auto rw, auto nw) -> int {
-    constexpr int D = decltype(dim)::value, RW = decltype(rw)::value, NW = decltype(nw)::value;
-    const auto kern = gqa_chunk_kernel<D, RW, NW>;
-    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), gqa_chunk_lds<D>(), who)) return rc;
-    hipLaunchKernelGGL(kern, dim3(d.wgs), dim3(64 * NW), gqa_chunk_lds<D>(), st, args);
+  auto many = [&](auto dim) -> int {
+    constexpr int D = decltype(dim)::value, bytes = sizeof(GqaChunkLds<D>);
+    const auto kern = gqa_chunk_kernel<D>;
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, who)) return rc;
+    hipLaunchKernelGGL(kern, dim3(d.wgs), dim3(64 * kChunkWaves), bytes, st, args);
     if (int rc = check_launch(who)) return rc;
-    return join(dim, integral_constant<int, 16 * RW * NW>{}, std::false_type{});
+    return join(dim, integral_constant<int, kChunkRows>{}, std::false_type{});
   };
   auto by_rows = [&](auto dim) -> int {
     return d.bm == 16 ? few(dim, integral_constant<int, 1>{}) : (d.bm == 32 ? few(dim, integral_constant<int, 2>{}) :
-           (d.bm == 64 ? few(dim, integral_constant<int, 4>{}) : many(dim, integral_constant<int, GQA_RW>{}, integral_constant<int, GQA_NW>{})));
+           (d.bm == 64 ? few(dim, integral_constant<int, 4>{}) : many(dim)));
   };
   return head_dim == 64 ? by_rows(std::integral_constant<int, 64>{}) : by_rows(std::integral_constant<int, 128>{});
 }
