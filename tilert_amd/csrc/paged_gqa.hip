@@ -96,8 +96,8 @@ __device__ inline int gqa_wave_scan(int v) {  // inclusive sum over the wave
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
   return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
-template <int THREADS, int BM>
-__device__ inline bool gqa_plan_item(const GqaArgs& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
+template <int THREADS, int BM, class Args>
+__device__ inline bool gqa_plan_item(const Args& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
   constexpr int WAVES = THREADS / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float units = 0.f;
@@ -889,86 +889,302 @@ struct GqaSumArgs {
   int heads, kv_heads, group, accumulate;
   float scale;  // softmax_scale * log2 e
   float* weights;
-  int64_t units;  // sequences x groups of pages x kv heads
-  int page_groups;
+  int target;       // few rows: as in GqaArgs
+  int64_t units;    // sequences x groups of pages x kv heads
+  int page_groups;  // of a sequence
+  uint64_t per_group;  // ceil(2^34 / group): x / group = x * per_group >> 34 for x < 2^27, group <= 128
+};
+// Unit u: its kv head, sequence and group of pages (a head's units are kv_heads apart: with 8 heads, on one XCD and its L2).
+struct GqaUnit {
+  int head, b, pages;
+  __device__ inline GqaUnit(const GqaSumArgs& A, int64_t u) {
+    head = static_cast<int>(u % A.kv_heads);
+    const int64_t v = u / A.kv_heads;
+    b = static_cast<int>(v / A.page_groups);
+    pages = static_cast<int>(v % A.page_groups);
+  }
 };
 
-// One page and kv head at a time: its keys stay in registers, the rows that see them come by in tiles of 16, and every lane
-// sums its keys' weights over its column of rows.  SPLIT: the four waves of a workgroup share a page, each with every
-// fourth tile of rows, and are joined in LDS; else each has a page of its own.
-template <int D, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void gqa_sum_kernel(const GqaSumArgs A) {
-  constexpr int KI = D / 64;
-  __shared__ float part[4][kGqaKeys];
+// Few rows (a decode step): a wave takes every fourth page of a piece, one behind another, the next one's keys on their way;
+// their rows, one tile of 16 as a rule, stay in registers.  Scores as in the attention's first product, S^T = K Q^T: a
+// lane sums its keys' weights over its column of rows.  Bound by bytes.  Pieces as the attention plans them (in groups of
+// kSumPages pages by the table's width, 60 sequences of 2048 to 32768 keys took 170 us).
+constexpr int kSumPages = 32;  // pages of a piece where nothing is planned
+constexpr int kSumTarget = 1536;
+template <int D>
+__global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A) {
+  __shared__ GqaPlanLds plan;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   for (int64_t u = blockIdx.x; u < A.units; u += gridDim.x) {
-    const int head = static_cast<int>(u % A.kv_heads);
-    const int64_t v = u / A.kv_heads;
-    const int b = static_cast<int>(v / A.page_groups), pg = static_cast<int>(v % A.page_groups) * (SPLIT ? 1 : 4) + (SPLIT ? 0 : wave);
-    const GqaSeq s(A.p, A.group, b);
-    const int n_keys = s.rows > 0 ? s.seen(s.rows - 1) : 0, key0 = pg * kGqaKeys;
-    int id = -1;
-    if (key0 < n_keys) id = A.p.table[static_cast<int64_t>(b) * A.p.max_pages + pg];
-    id = __builtin_amdgcn_readfirstlane(id);
-    const bool there = id >= 0 && id < A.p.n_pages;
-    float w[4][4] = {};
-    if (there) {
-      const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, id, head);
-      const GqaKeys<D> kc = load_keys<D>(blk.k, lane);
-      const bool ok = gqa_scale_ok(blk.scale[0]);
-      const float sk = ok ? blk.scale[0] : 1.f, unit = ok ? A.scale : __builtin_nanf("");
-      v8bf k[4][KI][2];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < KI; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) k[t][i][e] = codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], sk);
-      // the first row that sees a key of the page
-      const int64_t row_first = max(static_cast<int64_t>(0), key0 - s.base) * A.group;
-      for (int row0 = static_cast<int>(row_first / 16) * 16 + (SPLIT ? 16 * wave : 0); row0 < s.rows; row0 += SPLIT ? 64 : 16) {
-        const int row = row0 + c;
-        const GqaQuery<D> q = load_query<D>(A.q, A.q_stride, s, head * A.group, row, g);
-        const int at = min(row, s.rows - 1);
-        const float lse2 = A.lse[(static_cast<int64_t>(s.first) + at / A.group) * A.heads + head * A.group + at % A.group] * kLog2e;
-        const int my = row < s.rows ? s.seen(row) - key0 - 16 * g : 0;
+    GqaUnit unit(A, u);
+    int pg0, pg1, first, rows_all;
+    int64_t base;
+    if (A.target) {  // (one unit a workgroup)
+      GqaItem it;
+      if (!gqa_plan_item<256, 1 << 30>(A, plan, static_cast<int>(u / A.kv_heads), it, first, rows_all, base)) return;
+      unit.b = it.b;
+      unit.pages = it.pg0;
+      pg0 = it.parts;
+    } else {
+      const GqaSeq s(A.p, A.group, unit.b);
+      first = s.first;
+      rows_all = s.rows;
+      base = s.base;
+      pg0 = 0;
+    }
+    const GqaSeq s(A.p, A.group, first, rows_all, base);
+    const int n_keys = s.rows > 0 ? s.seen(s.rows - 1) : 0, n_pages = (n_keys + kGqaKeys - 1) / kGqaKeys;
+    const int each = A.target ? (n_pages + pg0 - 1) / pg0 : kSumPages;
+    pg0 = unit.pages * each + wave;
+    pg1 = min((unit.pages + 1) * each, n_pages);
+    if (pg0 >= pg1) continue;
+    const gqa_const_i32 table = (gqa_const_i32)(A.p.table + static_cast<int64_t>(unit.b) * A.p.max_pages);
+    auto page_id = [&](int pg) { return __builtin_amdgcn_readfirstlane(table[min(pg, pg1 - 1)]); };
+    auto there = [&](int id) { return id >= 0 && id < A.p.n_pages; };
+    auto block = [&](int id) { return gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there(id) ? id : 0, unit.head); };
+    GqaQuery<D> q;
+    float lse2;
+    int seen;
+    auto rows = [&](int row0) {
+      const int row = row0 + c, at = min(row, s.rows - 1);
+      q = load_query<D>(A.q, A.q_stride, s, unit.head * A.group, row, g);
+      lse2 = A.lse[(static_cast<int64_t>(s.first) + at / A.group) * A.heads + unit.head * A.group + at % A.group] * kLog2e;
+      seen = row < s.rows ? s.seen(row) : 0;
+    };
+    rows(0);
+    int pg = pg0;
+    auto page = [&](const GqaKeys<D>& kc, float sk, bool is, int id) __attribute__((always_inline)) {
+      const bool ok = gqa_scale_ok(sk);
+      const float by = ok ? sk : 1.f, scale = ok ? A.scale : __builtin_nanf("");
+      const int key0 = pg * kGqaKeys;
+      float w[4][4] = {};
+      for (int row0 = 0; row0 < s.rows; row0 += 16) {
+        if (s.rows > 16) rows(row0);
+        const int my = seen - key0 - 16 * g;
         const bool masked = __any(my < 16);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < KI; ++i)
+          for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) x = mfma_bf16(k[t][i][e], q.x[i][e], x);
+            for (int e = 0; e < 2; ++e) x = mfma_bf16(codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], by), q.x[i][e], x);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], unit, -lse2));
-            if (masked && 4 * t + j >= my) p = 0.f;
-            w[t][j] += p;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], scale, -lse2));
+            w[t][j] += masked && 4 * t + j >= my ? 0.f : p;
           }
         }
       }
+      float mine = 0.f;  // over the 16 rows of a column: lane (c, g) keeps key 16 g + c
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = row16_reduce<false>(w[t][j]);
+          mine = c == 4 * t + j ? x : mine;
+        }
+      if (is && key0 + lane < n_keys) {
+        float* to = A.weights + (static_cast<int64_t>(id) * A.kv_heads + unit.head) * kGqaKeys + lane;
+        *to = A.accumulate ? *to + mine : mine;
+      }
+    };
+    // Two pages' keys on their way behind the one at work, 128 KB a CU.  (Three buffers by turns: one copied into another would
+    // wait for its loads.)
+    GqaKeys<D> k0, k1, k2;
+    float s0, s1, s2;
+    int id = page_id(pg), id1 = page_id(pg + 4), id2 = page_id(pg + 8);
+    k0 = load_keys<D>(block(id).k, lane);
+    s0 = load_f32_vector(block(id).scale);
+    k1 = load_keys<D>(block(id1).k, lane);
+    s1 = load_f32_vector(block(id1).scale);
+    auto turn = [&](const GqaKeys<D>& now, float s_now, GqaKeys<D>& then, float& s_then) __attribute__((always_inline)) {
+      then = load_keys<D>(block(id2).k, lane);
+      s_then = load_f32_vector(block(id2).scale);
+      page(now, s_now, there(id), id);
+      id = id1;
+      id1 = id2;
+      id2 = page_id(pg + 12);
+      pg += 4;
+      return pg < pg1;
+    };
+    while (turn(k0, s0, k2, s2) && turn(k1, s1, k0, s0) && turn(k2, s2, k1, s1)) {
     }
-    // over the 16 rows of a column: lane (c, g) keeps key 16 g + c
+  }
+}
+
+// Many rows: eight waves share PW pages of a head, each with a page's keys in registers as bf16, and 8 / PW tiles of 32 rows a
+// step, which go through LDS as the product's operand (32 x 32 scores an instruction).  Waves of the same page are added
+// at the end, in a fixed order.  Bound by vector instructions: a score takes a multiply-add, an exponential and a sum,
+// 21 cycles a wave of 64 lanes, and 8 of the matrix pipe's.
+constexpr int kSumWaves = 8;
+template <int D, int PW>
+struct GqaSumLds {
+  static constexpr int KF = D / 16, RS = kSumWaves / PW;
+  u32x4g q[2][RS][KF][64];
+  float lse[2][RS][32];
+  float part[kSumWaves][kGqaKeys];
+};
+template <int D, int PW>
+__global__ __launch_bounds__(64 * kSumWaves, 2) void gqa_sum_kernel(const GqaSumArgs A) {
+  constexpr int KF = D / 16, RS = kSumWaves / PW, CH = D / 8, ALL = RS * 32 * CH;      // 16-byte pieces of a row, and of a step
+  constexpr int PIECES = (ALL + 64 * kSumWaves - 1) / (64 * kSumWaves);                // that a thread loads
+  extern __shared__ __attribute__((aligned(16))) uint8_t gqa_smem[];
+  GqaSumLds<D, PW>& L = *reinterpret_cast<GqaSumLds<D, PW>*>(gqa_smem);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5, pw = wave % PW, rs = wave / PW;
+  for (int64_t u = blockIdx.x; u < A.units; u += gridDim.x) {
+    const GqaUnit unit(A, u);
+    const GqaSeq s(A.p, A.group, unit.b);
+    const int n_keys = s.rows > 0 ? s.seen(s.rows - 1) : 0, first = unit.pages * PW * kGqaKeys;
+    if (first >= n_keys) continue;  // (the whole workgroup)
+    const int pg = unit.pages * PW + pw, key0 = pg * kGqaKeys;
+    int id = -1;
+    if (key0 < n_keys) id = __builtin_amdgcn_readfirstlane(A.p.table[static_cast<int64_t>(unit.b) * A.p.max_pages + pg]);
+    const bool there = id >= 0 && id < A.p.n_pages;
+    const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there ? id : 0, unit.head);
+    const bool ok = gqa_scale_ok(blk.scale[0]);
+    const float sk = ok ? blk.scale[0] : 1.f, scale = ok ? A.scale : __builtin_nanf("");
+    // keys: fragment f of tile t, row c of it the key 32 (c / 4 % 2) + 16 t + 4 (c / 8) + c % 4, dims 64 i + 32 j + 16 h + 8 e .. + 7
+    // for f = 4 i + 2 j + e; the queries' fragments are the same
+    v8bf k[2][KF];
+    {
+      const uint8_t* from = blk.k + (32 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3)) * D + 16 * h;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int f = 0; f < KF / 2; ++f) {
+          const u32x4g x = *reinterpret_cast<const u32x4g*>(from + 16 * t * D + 32 * f);
+          k[t][2 * f] = codes8_bf16(x[0], x[1], sk);
+          k[t][2 * f + 1] = codes8_bf16(x[2], x[3], sk);
+        }
+    }
+    // rows below `none` see none of this wave's page, rows from `full` on all of it
+    auto row_of = [&](int64_t pos) { const int64_t n = pos - s.base; return static_cast<int>(n <= 0 ? 0 : (n * s.group < s.rows ? n * s.group : s.rows)); };
+    const int none = there ? row_of(key0) : s.rows, full = row_of(static_cast<int64_t>(key0) + kGqaKeys - 1);
+    const int start = row_of(first) / (32 * RS) * (32 * RS), steps = (s.rows - start + 32 * RS - 1) / (32 * RS);
+    auto token_of = [&](int row) { return static_cast<int>(row * A.per_group >> 34); };  // (a division is 30 instructions)
+    struct Rows {
+      u32x4g x[PIECES];
+      float lse;
+    };
+    auto fetch = [&](int step) __attribute__((always_inline)) {
+      Rows r;
+      const int row0 = start + min(step, steps - 1) * 32 * RS;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int piece = i * 64 * kSumWaves + tid, at = min(row0 + piece / CH, s.rows - 1), t = token_of(at);
+        r.x[i] = *reinterpret_cast<const u32x4g*>(A.q + (s.first + t) * A.q_stride + (unit.head * s.group + at - t * s.group) * D + piece % CH * 8);
+      }
+      r.lse = 0.f;
+      if (tid < 32 * RS) {
+        const int at = min(row0 + tid, s.rows - 1), t = token_of(at);
+        r.lse = A.lse[(static_cast<int64_t>(s.first) + t) * A.heads + unit.head * s.group + at - t * s.group];
+      }
+      return r;
+    };
+    // (a piece's place is its row, turned by its fragment and half, so that a row's pieces are in different banks)
+    auto stage = [&](const Rows& r, int buf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int piece = i * 64 * kSumWaves + tid, row = piece / CH, j = piece % CH, f = 2 * (j >> 2) + (j & 1), half = j >> 1 & 1;
+        if (ALL % (64 * kSumWaves) == 0 || piece < ALL) L.q[buf][row >> 5][f][32 * half + ((row & 31) ^ (2 * f + half))] = r.x[i];
+      }
+      if (tid < 32 * RS) L.lse[buf][tid >> 5][tid & 31] = r.lse * kLog2e;
+    };
+    float w[2][16] = {}, lse2 = 0.f;
+    v16f x[2];
+    auto row_at = [&](int step) { return start + step * 32 * RS + 32 * rs; };
+    auto idle = [&](int row0) { return row0 + 32 <= none || row0 >= s.rows; };
+    auto scores = [&](int step, int buf) __attribute__((always_inline)) {
+      if (idle(row_at(step))) return;
+      lse2 = L.lse[buf][rs][c];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[0][j] = x[1][j] = 0.f;
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        const v8bf q = bf16_of(L.q[buf][rs][f][32 * h + (c ^ (2 * f + h))]);
+        x[0] = mfma32_bf16(k[0][f], q, x[0]);
+        x[1] = mfma32_bf16(k[1][f], q, x[1]);
+      }
+    };
+    auto weights = [&](int step) __attribute__((always_inline)) {
+      const int row0 = row_at(step);
+      if (idle(row0)) return;
+      if (row0 < full || row0 + 32 > s.rows) {
+        const int row = row0 + c, my = row < s.rows ? s.seen(row) - key0 - 32 * h : 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j], scale, -lse2));
+            w[t][j] += 16 * t + j >= my ? 0.f : p;
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[t][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j], scale, -lse2));
+      }
+    };
+    auto tile = [&](int step, int buf) __attribute__((always_inline)) {
+      scores(step, buf);
+      weights(step);
+    };
+    // rows on their way for two steps (281 us for 2048 tokens over 16384 keys, 295 with one), or, where a step's take many
+    // registers, for one
+    Rows ra = fetch(0), rb;
+    stage(ra, 0);
+    if constexpr (RS <= 2) {
+      rb = fetch(1);
+      ra = fetch(2);
+      __syncthreads();
+#pragma unroll 1
+      for (int step = 0; step < steps; step += 2) {
+        tile(step, 0);
+        stage(rb, 1);
+        rb = fetch(step + 3);
+        __syncthreads();
+        if (step + 1 < steps) tile(step + 1, 1);
+        stage(ra, 0);
+        ra = fetch(step + 4);
+        __syncthreads();
+      }
+    } else {
+      ra = fetch(1);
+      __syncthreads();
+#pragma unroll 1
+      for (int step = 0; step < steps; ++step) {
+        tile(step, step & 1);
+        stage(ra, (step & 1) ^ 1);
+        ra = fetch(step + 2);
+        __syncthreads();
+      }
+    }
+    // over a half's 32 rows: lane (c, h) keeps key 32 h + c
     float mine = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = row16_reduce<false>(w[t][j]);
-        mine = c == 4 * t + j ? x : mine;
+      for (int j = 0; j < 16; ++j) {
+        const float y = row16_reduce<false>(w[t][j]);
+        const u32x2g z = __builtin_bit_cast(u32x2g, __builtin_amdgcn_permlane16_swap(__float_as_uint(y), __float_as_uint(y), false, false));
+        const float sum = __uint_as_float(z[0]) + __uint_as_float(z[1]);
+        mine = c == 16 * t + j ? sum : mine;
       }
-    if constexpr (SPLIT) {
-      part[wave][lane] = mine;
+    if constexpr (RS > 1) {
+      L.part[wave][lane] = mine;
       __syncthreads();
-      mine = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-      __syncthreads();
+      mine = L.part[pw][lane];
+#pragma unroll
+      for (int i = 1; i < RS; ++i) mine += L.part[pw + PW * i][lane];
     }
-    if (there && (!SPLIT || wave == 0) && key0 + lane < n_keys) {
-      float* to = A.weights + (static_cast<int64_t>(id) * A.kv_heads + head) * kGqaKeys + lane;
+    if (there && rs == 0 && key0 + lane < n_keys) {
+      float* to = A.weights + (static_cast<int64_t>(id) * A.kv_heads + unit.head) * kGqaKeys + lane;
       *to = A.accumulate ? *to + mine : mine;
     }
+    __syncthreads();  // (the next unit's rows)
   }
 }
 
@@ -1064,13 +1280,32 @@ extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const 
   if (int rc = check_gqa_batch(who, n_seqs, n_tokens, heads, max_pages, softmax_scale)) return rc;
   if (int rc = check_gqa_rows(who, "query", q_bf16, q_stride, heads, head_dim)) return rc;
   if (!lse || !key_weights) { set_error("%s: null pointer", who); return kErrArg; }
-  const bool split = n_tokens * (heads / kv_heads) >= 64 * n_seqs;
-  const int64_t groups = split ? max_pages : cdiv(max_pages, 4), units = n_seqs * groups * kv_heads;
+  const int64_t each = cdiv(n_tokens * (heads / kv_heads), n_seqs);
+  const bool few = each <= 16;
+  int pw = 8;  // pages a workgroup: as many as leave a workgroup for every CU
+  while (pw > 1 && cdiv(max_pages, pw) * kv_heads * n_seqs < 256) pw /= 2;
+  const int64_t target = few && n_seqs <= kGqaPlanSeqs ? kSumTarget : 0;
+  const int64_t groups = cdiv(max_pages, few ? kSumPages : pw), units = target ? target + n_seqs * kv_heads : n_seqs * groups * kv_heads;
   const GqaSumArgs args{(const uint16_t*)q_bf16, q_stride, lse, (const uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
                         PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
-                        (int)heads, (int)kv_heads, (int)(heads / kv_heads), accumulate, softmax_scale * kLog2e, key_weights, units, (int)groups};
-  const auto kern = head_dim == 64 ? (split ? gqa_sum_kernel<64, true> : gqa_sum_kernel<64, false>)
-                                   : (split ? gqa_sum_kernel<128, true> : gqa_sum_kernel<128, false>);
-  hipLaunchKernelGGL(kern, dim3(units < (1 << 16) ? units : (1 << 16)), dim3(256), 0, (hipStream_t)stream, args);
-  return check_launch(who);
+                        (int)heads, (int)kv_heads, (int)(heads / kv_heads), accumulate, softmax_scale * kLog2e, key_weights, (int)target, units, (int)groups, ((1ull << 34) + heads / kv_heads - 1) / (heads / kv_heads)};
+  const dim3 grid(target || units < (1 << 16) ? units : (1 << 16));  // (a workgroup goes on with another unit)
+  const hipStream_t st = (hipStream_t)stream;
+  if (few) {
+    hipLaunchKernelGGL(head_dim == 64 ? gqa_sum_few_kernel<64> : gqa_sum_few_kernel<128>, grid, dim3(256), 0, st, args);
+    return check_launch(who);
+  }
+  auto many = [&](auto dim, auto pages) -> int {
+    constexpr int D = decltype(dim)::value, PW = decltype(pages)::value, bytes = sizeof(GqaSumLds<D, PW>);
+    const auto kern = gqa_sum_kernel<D, PW>;
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, who)) return rc;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * kSumWaves), bytes, st, args);
+    return check_launch(who);
+  };
+  using std::integral_constant;
+  auto by_pages = [&](auto dim) -> int {
+    return pw == 8 ? many(dim, integral_constant<int, 8>{}) : (pw == 4 ? many(dim, integral_constant<int, 4>{}) :
+           (pw == 2 ? many(dim, integral_constant<int, 2>{}) : many(dim, integral_constant<int, 1>{})));
+  };
+  return head_dim == 64 ? by_pages(integral_constant<int, 64>{}) : by_pages(integral_constant<int, 128>{});
 }
