@@ -238,75 +238,95 @@ __device__ inline uint32_t weight_key(float w) {
 // Which keys of one sequence and head stay: the last `recent`, and the heaviest of the others, k in all, in ascending
 // order; equal weights: the lowest position.  The k-th largest weight is found digit by digit (11, 11 and 10 bits) from
 // histograms in LDS, then every wave counts and writes its own stretch of the positions.
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
+// A workgroup a head; each of its 16 waves goes through its own stretch of pages, four pages at a time, four keys a lane, once
+// for each digit and once to mark the keys that stay, two bits each in LDS, from which their places are counted.  Bound by
+// vector instructions, some 15 a key and pass: 65536 keys 115 us with a page at a time and the marking done twice.
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048, kSelBatch = 4;
+constexpr int kSelBlock = 1024;  // pages that are marked at a time
 __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictArgs A) {
   __shared__ int hist[kSelBins];
+  __shared__ uint8_t marks[kSelBlock * kGqaKeys / 4];  // of four keys: bits 0 .. 3, which stay; 4 .. 7, which equal the threshold
   __shared__ int wave_sum[kSelWaves], wave_eq[kSelWaves];
   __shared__ int found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / A.kv_heads, h = blockIdx.x % A.kv_heads;
   const int32_t* table = A.table + static_cast<int64_t>(b) * A.max_pages;
   const int width = A.kept_pages * kGqaKeys;
   int32_t* out = A.slots + (static_cast<int64_t>(b) * A.kv_heads + h) * width;
   const int64_t most = static_cast<int64_t>(A.max_pages) * kGqaKeys;
-  const int n = static_cast<int>(min(static_cast<int64_t>(max(A.lens[b], 0)), most));
+  const int n = static_cast<int>(A.lens[b] < 0 ? 0 : (A.lens[b] < most ? A.lens[b] : most));
   const int n_pages = (n + kGqaKeys - 1) / kGqaKeys;
-  auto there = [&](int pg) { const int id = table[pg]; return id >= 0 && id < A.n_pages; };
-  auto weight = [&](int pg, int row) { return A.weights[(static_cast<int64_t>(table[pg]) * A.kv_heads + h) * kGqaKeys + row]; };
-  // the keys that there are
-  int mine = 0;
-  for (int pg = tid; pg < n_pages; pg += kSelThreads) mine += there(pg) ? min(n - pg * kGqaKeys, kGqaKeys) : 0;
-  for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
-  if (lane == 0) wave_sum[wave] = mine;
-  __syncthreads();
-  int total = 0;
-  for (int w = 0; w < kSelWaves; ++w) total += wave_sum[w];
-  const int k = min(min(max(A.keep[b], 0), total), width);
+  auto there = [&](int id) { return id >= 0 && id < A.n_pages; };
+  auto all_waves = [&](int mine) {  // a sum over the workgroup
+    for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
+    __syncthreads();
+    if (lane == 0) wave_sum[wave] = mine;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < kSelWaves; ++w) total += wave_sum[w];
+    return total;
+  };
+  // keys that there are from position `from` on
+  auto count = [&](int from) {
+    int mine = 0;
+    for (int pg = from / kGqaKeys + tid; pg < n_pages; pg += kSelThreads)
+      mine += there(table[pg]) ? min(n - pg * kGqaKeys, kGqaKeys) - max(from - pg * kGqaKeys, 0) : 0;
+    return all_waves(mine);
+  };
+  const int total = count(0), k = min(min(max(A.keep[b], 0), total), width);
   const int last0 = n - min(A.recent, k);  // positions from here on stay
-  mine = 0;
-  for (int pg = last0 / kGqaKeys + tid; pg < n_pages; pg += kSelThreads)
-    mine += there(pg) ? min(n - pg * kGqaKeys, kGqaKeys) - max(last0 - pg * kGqaKeys, 0) : 0;
-  for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
-  __syncthreads();
-  if (lane == 0) wave_sum[wave] = mine;
-  __syncthreads();
-  int need = k;  // of the others
-  for (int w = 0; w < kSelWaves; ++w) need -= wave_sum[w];
+  int need = k - count(last0);             // of the others
+  // f(position of a lane's four keys, their sort keys) for the wave's stretch of pages page0 .. page1 - 1, in order; sort key 0,
+  // which no weight has: none is there
+  auto pages = [&](int page0, int page1, auto f) __attribute__((always_inline)) {
+    const int quads = (page1 - page0 + 3) / 4, per = (quads + kSelWaves - 1) / kSelWaves;
+    const int q0 = wave * per, q1 = min(q0 + per, quads);
+    for (int first = q0; first < q1; first += kSelBatch) {
+      float4 w[kSelBatch];
+      int id[kSelBatch];
+#pragma unroll
+      for (int i = 0; i < kSelBatch; ++i) id[i] = table[min(page0 + 4 * min(first + i, q1 - 1) + (lane >> 4), page1 - 1)];
+#pragma unroll
+      for (int i = 0; i < kSelBatch; ++i)
+        w[i] = reinterpret_cast<const float4*>(A.weights + (static_cast<int64_t>(there(id[i]) ? id[i] : 0) * A.kv_heads + h) * kGqaKeys)[lane & 15];
+#pragma unroll
+      for (int i = 0; i < kSelBatch; ++i) {
+        if (first + i >= q1) break;
+        const int pos = (page0 + 4 * (first + i)) * kGqaKeys + 4 * lane, here = there(id[i]) ? n - pos : 0;
+        const uint32_t key[4] = {here > 0 ? weight_key(w[i].x) : 0u, here > 1 ? weight_key(w[i].y) : 0u,
+                                 here > 2 ? weight_key(w[i].z) : 0u, here > 3 ? weight_key(w[i].w) : 0u};
+        f(pos, key);
+      }
+    }
+  };
   // the need-th largest key of the positions below last0, and how many equal to it stay
   uint32_t prefix = 0, known = 0;
-  const int others = (last0 + kGqaKeys - 1) / kGqaKeys;
   if (need > 0) {
     for (int digit = 0; digit < 3; ++digit) {
       const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bins = digit == 2 ? 1024 : 2048;
       for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int pg = wave; pg < others; pg += kSelWaves) {
-        if (!there(pg) || pg * kGqaKeys + lane >= last0) continue;
-        const uint32_t key = weight_key(weight(pg, lane));
-        if ((key & known) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
-      }
+      pages(0, n_pages, [&](int pos, const uint32_t (&key)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (key[j] != 0 && pos + j < last0 && (key[j] & known) == prefix) atomicAdd(&hist[(key[j] >> shift) & (bins - 1)], 1);
+      });
       __syncthreads();
-      // suffix sums: wave 0, 32 bins a lane
-      if (wave == 0) {
-        int sum = 0;
-        for (int i = 0; i < kSelBins / 64; ++i) sum += hist[lane * (kSelBins / 64) + i];
-        int above = sum;  // inclusive sum over the lanes behind
-        for (int o = 1; o < 64; o <<= 1) {
-          const int x = __shfl_down(above, o);
-          above += lane + o < 64 ? x : 0;
-        }
-        above -= sum;
-        if (above < need && above + sum >= need) {
-          for (int i = kSelBins / 64 - 1; i >= 0; --i) {
-            const int c = hist[lane * (kSelBins / 64) + i];
-            if (above + c >= need) {
-              found[0] = lane * (kSelBins / 64) + i;
-              found[1] = above;
-              break;
-            }
-            above += c;
-          }
-        }
+      // from the largest digit down: thread t has the bins 2047 - 2 t and 2046 - 2 t
+      const int hi = hist[kSelBins - 1 - 2 * tid], lo = hist[kSelBins - 2 - 2 * tid];
+      int up = hi + lo;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(up, o);
+        up += lane >= o ? x : 0;
+      }
+      if (lane == 63) wave_sum[wave] = up;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) up += wave_sum[w];
+      const int above = up - hi - lo;
+      if (above < need && up >= need) {
+        found[0] = above + hi >= need ? kSelBins - 1 - 2 * tid : kSelBins - 2 - 2 * tid;
+        found[1] = above + hi >= need ? above : above + hi;
       }
       __syncthreads();
       prefix |= static_cast<uint32_t>(found[0]) << shift;
@@ -314,145 +334,203 @@ __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictA
       need -= found[1];
       __syncthreads();
     }
-  } else {
-    prefix = 0xffffffffu;  // nothing above it, and none equal to it
-  }
-  // every wave's stretch of pages: how many it keeps above the threshold or as the last ones, and how many equal it
-  const int per = (n_pages + kSelWaves - 1) / kSelWaves, p0 = wave * per, p1 = min(p0 + per, n_pages);
-  auto kind = [&](int pg, bool& sure, bool& equal) {
-    const int pos = pg * kGqaKeys + lane;
-    sure = equal = false;
-    if (!there(pg) || pos >= n) return;
-    if (pos >= last0) { sure = true; return; }
-    const uint32_t key = weight_key(weight(pg, lane));
-    sure = key > prefix;
-    equal = key == prefix;
-  };
-  int sures = 0, equals = 0;
-  for (int pg = p0; pg < p1; ++pg) {
-    bool s, e;
-    kind(pg, s, e);
-    sures += __popcll(__ballot(s));
-    equals += __popcll(__ballot(e));
-  }
-  if (lane == 0) {
-    wave_sum[wave] = sures;
-    wave_eq[wave] = equals;
-  }
-  __syncthreads();
-  int eq = 0, at = 0;  // equal ones in front, kept ones in front
-  for (int w = 0; w < wave; ++w) {
-    at += wave_sum[w] + max(0, min(wave_eq[w], need - eq));
-    eq += wave_eq[w];
   }
   const uint64_t below = (1ull << lane) - 1;
-  for (int pg = p0; pg < p1; ++pg) {
-    bool s, e;
-    kind(pg, s, e);
-    const uint64_t em = __ballot(e);
-    const bool stays = s || (e && eq + __popcll(em & below) < need);
-    const uint64_t m = __ballot(stays);
-    const int to = at + __popcll(m & below);
-    if (stays && to < width) out[to] = pg * kGqaKeys + lane;
-    at += __popcll(m);
-    eq += __popcll(em);
+  int at0 = 0, eq0 = 0;  // kept ones, and equal ones, in the blocks in front
+  for (int page0 = 0; page0 < n_pages; page0 += kSelBlock) {
+    const int page1 = min(page0 + kSelBlock, n_pages), pos0 = page0 * kGqaKeys;
+    int sures = 0, equals = 0;
+    pages(page0, page1, [&](int pos, const uint32_t (&key)[4]) {
+      int sure = 0, equal = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool last = pos + j >= last0;
+        sure |= key[j] != 0 && (last || (need > 0 && key[j] > prefix)) ? 1 << j : 0;
+        equal |= key[j] != 0 && !last && need > 0 && key[j] == prefix ? 1 << j : 0;
+      }
+      sures += __popc(sure);
+      equals += __popc(equal);
+      marks[(pos - pos0) / 4] = static_cast<uint8_t>(sure | equal << 4);
+    });
+    for (int o = 32; o; o >>= 1) {
+      sures += __shfl_xor(sures, o);
+      equals += __shfl_xor(equals, o);
+    }
+    __syncthreads();
+    if (lane == 0) {
+      wave_sum[wave] = sures;
+      wave_eq[wave] = equals;
+    }
+    __syncthreads();
+    int at = at0, eq = eq0;
+    for (int w = 0; w < kSelWaves; ++w) {
+      if (w == wave) {
+        at = at0;
+        eq = eq0;
+      }
+      at0 += wave_sum[w] + max(0, min(wave_eq[w], need - eq0));
+      eq0 += wave_eq[w];
+    }
+    // (the stretch that this wave has marked)
+    const int quads = (page1 - page0 + 3) / 4, per = (quads + kSelWaves - 1) / kSelWaves, q1 = min((wave + 1) * per, quads);
+    for (int q = wave * per; q < q1; ++q) {
+      const int mark = marks[q * 64 + lane], equal = mark >> 4;
+      int e_before = 0, before = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e_before += __popcll(__ballot(equal >> j & 1) & below);
+      int stays = mark & 15, e = eq + e_before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (equal >> j & 1) stays |= e++ < need ? 1 << j : 0;
+      int all = 0, all_eq = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t m = __ballot(stays >> j & 1);
+        before += __popcll(m & below);
+        all += __popcll(m);
+        all_eq += __popcll(__ballot(equal >> j & 1));
+      }
+      int to = at + before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (stays >> j & 1) {
+          if (to < width) out[to] = pos0 + q * 256 + 4 * lane + j;
+          ++to;
+        }
+      at += all;
+      eq += all_eq;
+    }
+    __syncthreads();  // (the next block's marks)
   }
   for (int i = k + tid; i < width; i += kSelThreads) out[i] = -1;
   if (h == 0 && tid == 0) A.kept_lens[b] = k;
 }
 
-// A workgroup gathers the keys of one new page and head: their codes under the least common scale, and their weights.
+// A workgroup gathers the keys of one new page and head: their codes under the least common scale, and their weights.  A key's
+// row is a load; a value is a column of its page's block, so the blocks of the pages that hold the kept keys, which ascend,
+// come through LDS four at a time, whole (a byte a lane from memory, 122 us for 9 sequences brought down to 8192 keys), and
+// the new block goes out through LDS too.  Bound by bytes: those of all pages with a kept key.
 template <int D>
 __global__ __launch_bounds__(256) void gqa_gather_kernel(const GqaEvictArgs A) {
-  constexpr int CH = D / 16, ROWS = 256 / CH, STEPS = kGqaKeys / ROWS, DIMS = D / 4;
+  constexpr int CH = D / 16, ROWS = 256 / CH, STEPS = kGqaKeys / ROWS, DIMS = D / 4, BATCH = 4, BLK = D * kGqaKeys / 16 / 256;
+  __shared__ u32x4g blocks[BATCH][D * kGqaKeys / 16];
+  __shared__ float src_k[kGqaKeys];
   __shared__ int src_page[kGqaKeys], src_row[kGqaKeys];
-  __shared__ float src_k[kGqaKeys], src_v[kGqaKeys];
   __shared__ float amax_w[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.x % A.kv_heads, slot = blockIdx.x / A.kv_heads, b = slot / A.kept_pages, pg = slot % A.kept_pages;
   const int to = A.kept_table[static_cast<int64_t>(b) * A.kept_pages + pg];
   if (to < 0 || to >= A.n_pages) return;
   const int32_t* list = A.slots + ((static_cast<int64_t>(b) * A.kv_heads + h) * A.kept_pages + pg) * kGqaKeys;
-  if (list[0] < 0) return;
-  if (tid < kGqaKeys) {
-    const int pos = list[tid];
-    int page = -1;
-    float sk = 0.f, sv = 0.f;
-    if (pos >= 0) {
-      page = A.table[static_cast<int64_t>(b) * A.max_pages + (pos >> 6)];
-      const GqaBlock s = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h);
-      sk = gqa_scale_ok(s.scale[0]) ? s.scale[0] : __builtin_nanf("");
-      sv = gqa_scale_ok(s.scale[1]) ? s.scale[1] : __builtin_nanf("");
-      A.weights[(static_cast<int64_t>(to) * A.kv_heads + h) * kGqaKeys + tid] = A.weights[(static_cast<int64_t>(page) * A.kv_heads + h) * kGqaKeys + (pos & 63)];
-    }
-    src_page[tid] = page;
-    src_row[tid] = pos & 63;
-    src_k[tid] = sk;
-    src_v[tid] = sv;
+  const int pos = list[lane];  // (each wave for itself: lane = key)
+  const int kept = __popcll(__ballot(pos >= 0));
+  if (kept == 0) return;
+  const int page = pos >= 0 ? A.table[static_cast<int64_t>(b) * A.max_pages + (pos >> 6)] : -1;
+  auto block = [&](int p) { return gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, p, h); };
+  // the distinct pages: those of the lanes in `heads`, in order; this lane's is the mine-th
+  const int before = __shfl_up(pos >> 6, 1);
+  const uint64_t heads = __ballot(pos >= 0 && (lane == 0 || before != pos >> 6));
+  const int mine = __popcll(heads & (2ull << lane) - 1) - 1, pages = __popcll(heads);
+  float sk = 0.f, sv = 0.f;
+  if (pos >= 0) {
+    const float* s = block(page).scale;
+    sk = gqa_scale_ok(s[0]) ? s[0] : __builtin_nanf("");
+    sv = gqa_scale_ok(s[1]) ? s[1] : __builtin_nanf("");
+    if (wave == 0) A.weights[(static_cast<int64_t>(to) * A.kv_heads + h) * kGqaKeys + lane] = A.weights[(static_cast<int64_t>(page) * A.kv_heads + h) * kGqaKeys + (pos & 63)];
+  }
+  if (wave == 0) {
+    src_page[lane] = page;
+    src_row[lane] = pos & 63;
+    src_k[lane] = sk;
   }
   __syncthreads();
   u32x4g kc[STEPS];
-  float amax_k = 0.f, amax_v = 0.f;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int row = i * ROWS + tid / CH, page = src_page[row];
+    const int row = i * ROWS + tid / CH;
     kc[i] = u32x4g{0, 0, 0, 0};
-    if (page >= 0) {
-      kc[i] = reinterpret_cast<const u32x4g*>(gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h).k + src_row[row] * D)[tid % CH];
-      const float s = src_k[row];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(kc[i][j], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(kc[i][j], true);
-        amax_k = fmaxf(amax_k, fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1]))) * s);
-      }
-    }
+    if (row < kept) kc[i] = reinterpret_cast<const u32x4g*>(block(src_page[row]).k + src_row[row] * D)[tid % CH];
   }
   // values: lane = key, a wave a quarter of the dims
   uint32_t vc[DIMS / 4];
-  const int vpage = src_page[lane];
-  const float sv = src_v[lane];
-  if (vpage >= 0) {
-    const uint8_t* from = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, vpage, h).v + wave * DIMS * kGqaKeys + src_row[lane];
 #pragma unroll
-    for (int i = 0; i < DIMS / 4; ++i)
-      vc[i] = from[(4 * i) * kGqaKeys] | from[(4 * i + 1) * kGqaKeys] << 8 | from[(4 * i + 2) * kGqaKeys] << 16 |
-              static_cast<uint32_t>(from[(4 * i + 3) * kGqaKeys]) << 24;
+  for (int i = 0; i < DIMS / 4; ++i) vc[i] = 0;
+  u32x4g next[BATCH][BLK];
+  uint64_t left = heads;
+  auto fetch = [&]() __attribute__((always_inline)) {  // the next four blocks (the last one again where there are fewer)
 #pragma unroll
-    for (int i = 0; i < DIMS / 4; ++i) {
-      const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(vc[i], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(vc[i], true);
-      amax_v = fmaxf(amax_v, fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1]))) * sv);
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = left ? __builtin_ctzll(left) : 63 - __builtin_clzll(heads);
+      left &= left - 1;
+      const u32x4g* from = reinterpret_cast<const u32x4g*>(block(__builtin_amdgcn_readlane(page, at)).v);
+#pragma unroll
+      for (int j = 0; j < BLK; ++j) next[i][j] = __builtin_nontemporal_load(from + j * 256 + tid);
+    }
+  };
+  fetch();
+  for (int first = 0; first < pages; first += BATCH) {
+    if (first) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+      for (int j = 0; j < BLK; ++j) blocks[i][j * 256 + tid] = next[i][j];
+    __syncthreads();
+    if (first + BATCH < pages) fetch();
+    const int in = mine - first;
+    if (pos >= 0 && in >= 0 && in < BATCH) {
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(blocks[in]) + wave * DIMS * kGqaKeys + (pos & 63);
+#pragma unroll
+      for (int i = 0; i < DIMS / 4; ++i)
+        vc[i] = from[(4 * i) * kGqaKeys] | from[(4 * i + 1) * kGqaKeys] << 8 | from[(4 * i + 2) * kGqaKeys] << 16 |
+                static_cast<uint32_t>(from[(4 * i + 3) * kGqaKeys]) << 24;
     }
   }
+  auto largest = [&](uint32_t x) {
+    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), c = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
+    return fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1])));
+  };
+  float amax_k = 0.f, amax_v = 0.f;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const float s = src_k[i * ROWS + tid / CH];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) amax_k = fmaxf(amax_k, largest(kc[i][j]) * s);
+  }
+#pragma unroll
+  for (int i = 0; i < DIMS / 4; ++i) amax_v = fmaxf(amax_v, largest(vc[i]) * sv);
   amax_k = wave_max_f32(amax_k);
   amax_v = wave_max_f32(amax_v);
   if (lane == 0) {
     amax_w[0][wave] = amax_k;
     amax_w[1][wave] = amax_v;
   }
-  __syncthreads();
+  __syncthreads();  // (and the blocks are read)
   const float s_k = gqa_scale(fmaxf(fmaxf(amax_w[0][0], amax_w[0][1]), fmaxf(amax_w[0][2], amax_w[0][3])));
   const float s_v = gqa_scale(fmaxf(fmaxf(amax_w[1][0], amax_w[1][1]), fmaxf(amax_w[1][2], amax_w[1][3])));
-  const GqaBlock dst = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, to, h);
+  const GqaBlock dst = block(to);
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int row = i * ROWS + tid / CH;
-    if (src_page[row] < 0) continue;
     const float ratio = src_k[row] / s_k;
 #pragma unroll
     for (int j = 0; j < 4; ++j) kc[i][j] = gqa_rescale4(kc[i][j], ratio);
-    reinterpret_cast<u32x4g*>(dst.k + row * D)[tid % CH] = kc[i];
+    if (row < kept) reinterpret_cast<u32x4g*>(dst.k + row * D)[tid % CH] = kc[i];
   }
-  if (vpage >= 0) {
-    const float ratio = sv / s_v;
-    uint8_t* into = dst.v + wave * DIMS * kGqaKeys + lane;
+  const float ratio = sv / s_v;
+  uint8_t* out = reinterpret_cast<uint8_t*>(blocks[0]);
 #pragma unroll
-    for (int i = 0; i < DIMS / 4; ++i) {
-      const uint32_t x = gqa_rescale4(vc[i], ratio);
-      into[(4 * i) * kGqaKeys] = static_cast<uint8_t>(x);
-      into[(4 * i + 1) * kGqaKeys] = static_cast<uint8_t>(x >> 8);
-      into[(4 * i + 2) * kGqaKeys] = static_cast<uint8_t>(x >> 16);
-      into[(4 * i + 3) * kGqaKeys] = static_cast<uint8_t>(x >> 24);
-    }
+  for (int i = 0; i < DIMS / 4; ++i) {
+    const uint32_t x = gqa_rescale4(vc[i], ratio);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[(wave * DIMS + 4 * i + j) * kGqaKeys + lane] = static_cast<uint8_t>(x >> (8 * j));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < BLK; ++j) {
+    const int at = j * 256 + tid, key0 = at % 4 * 16;
+    if (key0 + 16 <= kept) reinterpret_cast<u32x4g*>(dst.v)[at] = blocks[0][at];
+    else
+      for (int i = 0; key0 + i < kept; ++i) dst.v[at * 16 + i] = out[at * 16 + i];
   }
   if (tid == 0) {
     dst.scale[0] = s_k;
