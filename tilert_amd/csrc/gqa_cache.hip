@@ -24,6 +24,7 @@ struct GqaWriteArgs {
   float eps;
   uint16_t* q_out;
   float* key_weights;
+  uint64_t per_heads;  // ceil(2^34 / heads): x / heads = x * per_heads >> 34 for x < 2^27, heads <= 128
 };
 
 template <int LANES>  // sum / max over 8 or 16 consecutive lanes, in all of them
@@ -42,17 +43,47 @@ __device__ inline void unpack8(u32x4g raw, float (&x)[8]) {
   }
 }
 
-// The row's norm and rotation; lane `part` of the row's D / 8 holds dims 8 part .. + 7.  All lanes of a row call it together.
+// Eight floats, for which 16-byte alignment is not known, in as few loads as there can be.
+__device__ inline void load8(const float* p, float (&x)[8]) {
+  typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
+  const v4u a = *reinterpret_cast<const v4u*>(p), b = *reinterpret_cast<const v4u*>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = a[i];
+    x[4 + i] = b[i];
+  }
+}
+
+// A lane's angles for a row of its token, cosines and sines of its dims' pairs: lane `part` of the row's D / 8 has the dims 8
+// part .. + 7, so eight pairs, or four where a pair's dims are neighbours.
+struct Angles {
+  float x[8], y[8];
+};
+__device__ inline Angles load_angles(const float* freqs, int part, int rope, int interleaved) {
+  Angles r;
+  const bool turned = part * 8 < rope;
+  if (interleaved) {
+    load8(freqs + (turned ? part * 8 : 0), r.x);
+  } else {
+    const int half = rope / 16, pair = turned ? (part >= half ? part - half : part) : 0;
+    load8(freqs + pair * 16, r.x);
+    load8(freqs + pair * 16 + 8, r.y);
+  }
+  return r;
+}
+
+// The row's norm and rotation, all lanes of a row together.
 template <int D>
-__device__ inline void norm_rope(float (&x)[8], int part, const float* gamma, const float* freqs, int rope, int interleaved, float eps) {
+__device__ inline void norm_rope(float (&x)[8], int part, bool norm, const float (&gamma)[8], const float* freqs, const Angles& w,
+                                 int rope, int interleaved, float eps) {
   constexpr int LANES = D / 8;
-  if (gamma) {
+  if (norm) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
     const float r = 1.0f / __builtin_sqrtf(row_sum<LANES>(ss) / D + eps);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * gamma[part * 8 + i];
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * gamma[i];
   }
   if (!freqs) return;
   const bool turned = part * 8 < rope;
@@ -60,7 +91,7 @@ __device__ inline void norm_rope(float (&x)[8], int part, const float* gamma, co
     if (!turned) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float c = freqs[part * 8 + 2 * i], s = freqs[part * 8 + 2 * i + 1], a = x[2 * i], b = x[2 * i + 1];
+      const float c = w.x[2 * i], s = w.x[2 * i + 1], a = x[2 * i], b = x[2 * i + 1];
       x[2 * i] = a * c - b * s;
       x[2 * i + 1] = a * s + b * c;
     }
@@ -72,11 +103,8 @@ __device__ inline void norm_rope(float (&x)[8], int part, const float* gamma, co
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float other = __shfl(x[i], from);
-    if (turned) {
-      const int pair = (upper ? part - half : part) * 8 + i;
-      const float c = freqs[2 * pair], s = freqs[2 * pair + 1];
-      x[i] = upper ? other * s + x[i] * c : x[i] * c - other * s;
-    }
+    const float c = i < 4 ? w.x[2 * i] : w.y[2 * i - 8], s = i < 4 ? w.x[2 * i + 1] : w.y[2 * i - 7];
+    if (turned) x[i] = upper ? other * s + x[i] * c : x[i] * c - other * s;
   }
 }
 
@@ -90,20 +118,32 @@ __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
   const int part = tid % LANES, sub = tid / LANES;
   const PagedBatch& p = A.p;
   const int page_wgs = A.page_slots * A.kv_heads;
-  if (static_cast<int>(blockIdx.x) >= page_wgs) {  // ---- query rows
+  const bool query = static_cast<int>(blockIdx.x) >= page_wgs;
+  const float* gamma_at = query ? A.gamma_q : A.gamma_k;
+  float gamma[8] = {};
+  if (gamma_at) load8(gamma_at + part * 8, gamma);
+  auto angles = [&](int64_t t) { return A.freqs ? load_angles(A.freqs + t * A.rope, part, A.rope, A.interleaved) : Angles{}; };
+  if (query) {  // ---- query rows; all loads first
     const int64_t end = static_cast<int64_t>(min(max(p.cu[p.n_seqs], 0), p.n_tokens)) * A.heads;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x - page_wgs) * kGqaKeys;
+    if (row0 >= end) return;
+    u32x4g raw[STEPS];
+    Angles w[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int64_t row = row0 + i * ROWS + sub, r = row < end ? row : end - 1;
+      const int t = static_cast<int>(static_cast<uint64_t>(r) * A.per_heads >> 34), h = static_cast<int>(r - static_cast<int64_t>(t) * A.heads);
+      raw[i] = *reinterpret_cast<const u32x4g*>(A.q + t * A.q_stride + h * D + part * 8);
+      w[i] = angles(t);
+    }
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int64_t row = row0 + i * ROWS + sub;
-      const bool live = row < end;
-      const int64_t r = live ? row : 0;
-      const int t = static_cast<int>(r / A.heads), h = static_cast<int>(r - static_cast<int64_t>(t) * A.heads);
       float x[8];
-      unpack8(*reinterpret_cast<const u32x4g*>(A.q + t * A.q_stride + h * D + part * 8), x);
-      norm_rope<D>(x, part, A.gamma_q, A.freqs ? A.freqs + static_cast<int64_t>(t) * A.rope : nullptr, A.rope, A.interleaved, A.eps);
-      if (live) *reinterpret_cast<u32x4g*>(A.q_out + r * D + part * 8) = u32x4g{bf16x2_bits(v2f{x[0], x[1]}), bf16x2_bits(v2f{x[2], x[3]}),
-                                                                               bf16x2_bits(v2f{x[4], x[5]}), bf16x2_bits(v2f{x[6], x[7]})};
+      unpack8(raw[i], x);
+      norm_rope<D>(x, part, gamma_at != nullptr, gamma, A.freqs, w[i], A.rope, A.interleaved, A.eps);
+      if (row < end) *reinterpret_cast<u32x4g*>(A.q_out + row * D + part * 8) = u32x4g{bf16x2_bits(v2f{x[0], x[1]}), bf16x2_bits(v2f{x[2], x[3]}),
+                                                                                     bf16x2_bits(v2f{x[4], x[5]}), bf16x2_bits(v2f{x[6], x[7]})};
     }
     return;
   }
@@ -135,7 +175,7 @@ __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
     const int64_t t = first + shift + (live ? row : r0);
     unpack8(*reinterpret_cast<const u32x4g*>(A.k + t * A.k_stride + head * D + part * 8), y[i]);
     unpack8(*reinterpret_cast<const u32x4g*>(A.v + t * A.v_stride + head * D + part * 8), z[i]);
-    norm_rope<D>(y[i], part, A.gamma_k, A.freqs ? A.freqs + t * A.rope : nullptr, A.rope, A.interleaved, A.eps);
+    norm_rope<D>(y[i], part, gamma_at != nullptr, gamma, A.freqs, angles(t), A.rope, A.interleaved, A.eps);
     float bad = 0.f, mk = 0.f, mv = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -555,8 +595,10 @@ extern "C" int tl_gqa_cache_write(const void* k_bf16, int64_t k_stride, const vo
     set_error("%s: rope_dim=%lld must be a multiple of 16 in [16, %lld]", who, (long long)rope_dim, (long long)head_dim);
     return kErrUnsupported;
   }
-  if (q_bf16)
+  if (q_bf16) {
     if (int rc = check_gqa_heads(who, heads, kv_heads)) return rc;
+    if (n_tokens * heads >= (1ll << 27)) { set_error("%s: %lld tokens x %lld heads: fewer than 2^27 rows", who, (long long)n_tokens, (long long)heads); return kErrUnsupported; }
+  }
   if (n_seqs == 0 || n_tokens == 0) return kOk;
   if (int rc = check_gqa_rows(who, "key", k_bf16, k_stride, kv_heads, head_dim)) return rc;
   if (int rc = check_gqa_rows(who, "value", v_bf16, v_stride, kv_heads, head_dim)) return rc;
@@ -574,7 +616,7 @@ extern "C" int tl_gqa_cache_write(const void* k_bf16, int64_t k_stride, const vo
                           (uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
                           PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
                           (int)kv_heads, (int)heads, (int)rope_dim, interleaved, (int)slots, gamma_k, gamma_q, freqs, eps,
-                          (uint16_t*)q_out_bf16, key_weights};
+                          (uint16_t*)q_out_bf16, key_weights, q_bf16 ? ((1ull << 34) + heads - 1) / heads : 0};
   hipLaunchKernelGGL(head_dim == 64 ? gqa_write_kernel<64> : gqa_write_kernel<128>, dim3(wgs), dim3(256), 0, (hipStream_t)stream, args);
   return check_launch(who);
 }
