@@ -44,8 +44,8 @@ __device__ inline void unpack8(u32x4g raw, float (&x)[8]) {
 }
 
 // Eight floats, for which 16-byte alignment is not known, in as few loads as there can be.
+typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
 __device__ inline void load8(const float* p, float (&x)[8]) {
-  typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
   const v4u a = *reinterpret_cast<const v4u*>(p), b = *reinterpret_cast<const v4u*>(p + 4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
   const int slot = blockIdx.x / A.kv_heads, head = blockIdx.x % A.kv_heads;
   auto before = [&](int b) { return min(max(p.cu[b], 0), p.n_tokens) / kGqaKeys + 2 * b; };
   const int b = last_seq(p.n_seqs, [&](int i) { return before(i) <= slot; });
-  if (b < 0 || b >= p.n_seqs) return;
+  if (b < 0 || b >= p.n_seqs || slot < before(b)) return;  // (below it where cu_seqlens does not ascend)
   const int c0 = p.cu[b], c1 = p.cu[b + 1];
   const int first = min(max(c0, 0), p.n_tokens), n = min(max(c1, first), p.n_tokens) - first;
   const int64_t base = static_cast<int64_t>(p.lens[b]) - c1 + first;  // position of the first token
@@ -322,13 +322,13 @@ __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictA
     const int quads = (page1 - page0 + 3) / 4, per = (quads + kSelWaves - 1) / kSelWaves;
     const int q0 = wave * per, q1 = min(q0 + per, quads);
     for (int first = q0; first < q1; first += kSelBatch) {
-      float4 w[kSelBatch];
+      v4u w[kSelBatch];
       int id[kSelBatch];
 #pragma unroll
       for (int i = 0; i < kSelBatch; ++i) id[i] = table[min(page0 + 4 * min(first + i, q1 - 1) + (lane >> 4), page1 - 1)];
 #pragma unroll
       for (int i = 0; i < kSelBatch; ++i)
-        w[i] = reinterpret_cast<const float4*>(A.weights + (static_cast<int64_t>(there(id[i]) ? id[i] : 0) * A.kv_heads + h) * kGqaKeys)[lane & 15];
+        w[i] = reinterpret_cast<const v4u*>(A.weights + (static_cast<int64_t>(there(id[i]) ? id[i] : 0) * A.kv_heads + h) * kGqaKeys)[lane & 15];
 #pragma unroll
       for (int i = 0; i < kSelBatch; ++i) {
         if (first + i >= q1) break;

@@ -810,7 +810,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void gqa_join_kernel(const GqaArgs
   if (!gqa_tile(A.p, A.group, slot, BM, b, tile)) return;
   const GqaSeq s(A.p, A.group, b);
   const int row0 = tile * BM, rows = min(s.rows - row0, BM), parts = mine.y;
-  if (rows <= r * 16 || parts <= 1) return;  // (a tile that is there has told its parts)
+  // A tile that is there has told its parts; where cu_seqlens does not ascend, one may be found here that has not, and
+  // nothing outside the workspace is read for it.
+  if (rows <= r * 16 || parts <= 1 || parts > 2 * A.target || mine.x < 0 || mine.x > 2 * A.target) return;
+  if ((static_cast<int64_t>(mine.x) + parts) * A.kv_heads > 2 * A.target) return;
   const bool live = r * 16 + c < rows;
   const int row = r * 16 + (live ? c : 0);  // (rows that are not there have no parts)
   const int at = (r * DT + d) * 64 + (live ? lane : 16 * g);
@@ -850,7 +853,6 @@ __global__ __launch_bounds__(64 * kJoinWaves) void gqa_join_kernel(const GqaArgs
 // The launch: rows a tile, workgroups, and the workspace.
 struct GqaLaunch {
   int bm;
-  bool deep;  // the join's form
   int64_t slots, target, wgs;
   size_t ml_at, o_at, bytes;
 };
@@ -862,7 +864,6 @@ inline GqaLaunch gqa_launch(int64_t n_seqs, int64_t n_tokens, int64_t heads, int
   // rows 37 / 36, 32 rows 43 / 35, 64 rows 72 / 37: with a tile for every CU a page is better read by one workgroup.
   d.bm = each > (n_seqs * kv_heads >= 256 ? 24 : 64) ? kChunkRows : (each <= 16 ? 16 : (each <= 32 ? 32 : 64));
   d.slots = gqa_slots(n_tokens, group, n_seqs, d.bm);
-  d.deep = d.bm <= 64;
   const int64_t tiles = d.slots * kv_heads;
   // In us: 60 sequences of 2048 to 32768 keys, 1 token (480 tiles of 16 rows) 282 with 512 pieces, 273 with 1024, 277 with 2048; 4
   // tokens over 131072 keys (8 tiles of 32 rows) 76, 86, 104: there a piece is a workgroup's all, and fewer are less to
