@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .gqa_cache import _check_metadata, _check_pages, _check_rows, _token_stride
+from .gqa_cache import _check_metadata, _check_pages, _check_rows
 from .kernel import _call, _require_cuda, _stream
 
 
@@ -19,21 +19,21 @@ def flash_paged_gqa(query: torch.Tensor, kv_pages: torch.Tensor, block_table: to
     the sum of exp of its scores) are filled, with 0 and -inf for a token that sees no key.  ``scale`` is the softmax
     scale, head_dim ** -0.5 unless given."""
     name = "flash_paged_gqa"
-    _check_rows(name, "query", query)
+    query_stride = _check_rows(name, "query", query)
     tokens, heads, head_dim = query.shape
-    _check_pages(name, kv_pages, kv_heads, head_dim)
+    n_pages = _check_pages(name, kv_pages, kv_heads, head_dim)
     if not 1 <= heads <= 128 or heads % kv_heads:
         raise ValueError(f"{name}: unsupported heads {heads} over kv_heads {kv_heads}")
-    n = _check_metadata(name, block_table, seq_lens, cu_seqlens)
+    n, max_pages = _check_metadata(name, block_table, seq_lens, cu_seqlens)
     if output.dtype != torch.bfloat16 or output.shape != query.shape or not output.is_contiguous():
         raise ValueError(f"{name}: output must be a contiguous bfloat16 tensor of query's shape")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous()):
         raise ValueError(f"{name}: lse must be a contiguous float32 [{tokens}, {heads}] tensor")
     _require_cuda(name, query, kv_pages, block_table, cu_seqlens, seq_lens, output, lse)
-    nbytes = _lib.query("tl_flash_paged_gqa_workspace_bytes", n, tokens, heads, kv_heads, head_dim, block_table.shape[1])
+    nbytes = _lib.query("tl_flash_paged_gqa_workspace_bytes", n, tokens, heads, kv_heads, head_dim, max_pages)
     # taken from the allocator call by call: its memory is ordered on the stream, and a captured graph's is its own
     ws = query.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _call(query, "tl_flash_paged_gqa", query.data_ptr(), _token_stride(query), kv_pages.data_ptr(), kv_pages.shape[0],
-          block_table.data_ptr(), block_table.shape[1], cu_seqlens.data_ptr(), seq_lens.data_ptr(), n, tokens, heads, kv_heads, head_dim,
+    _call(query, "tl_flash_paged_gqa", query.data_ptr(), query_stride, kv_pages.data_ptr(), n_pages,
+          block_table.data_ptr(), max_pages, cu_seqlens.data_ptr(), seq_lens.data_ptr(), n, tokens, heads, kv_heads, head_dim,
           float(head_dim ** -0.5 if scale is None else scale), output.data_ptr(), lse.data_ptr() if lse is not None else None,
           ws.data_ptr() if ws is not None else None, nbytes, _stream(query))

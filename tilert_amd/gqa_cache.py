@@ -27,47 +27,51 @@ def gqa_page_bytes(kv_heads: int, head_dim: int) -> int:
     return kv_heads * 2 * GQA_PAGE_KEYS * head_dim + -(-kv_heads * 8 // 128) * 128
 
 
-def _check_pages(name: str, kv_pages, kv_heads: int, head_dim: int) -> None:
+def _check_pages(name: str, kv_pages, kv_heads: int, head_dim: int) -> int:
+    """The number of pages."""
     if head_dim not in GQA_HEAD_DIMS:
         raise ValueError(f"{name}: unsupported head_dim {head_dim} (one of {GQA_HEAD_DIMS})")
     if not 1 <= kv_heads <= 128:
         raise ValueError(f"{name}: unsupported kv_heads {kv_heads}")
-    size = gqa_page_bytes(kv_heads, head_dim)
-    if kv_pages.dtype != torch.uint8 or kv_pages.dim() != 2 or kv_pages.shape[1] != size or not kv_pages.is_contiguous():
+    size, shape = gqa_page_bytes(kv_heads, head_dim), kv_pages.shape
+    if kv_pages.dtype != torch.uint8 or len(shape) != 2 or shape[1] != size or not kv_pages.is_contiguous():
         raise ValueError(f"{name}: kv_pages must be a contiguous uint8 [n_pages, {size}] tensor")
+    return shape[0]
 
 
-def _check_metadata(name: str, block_table, seq_lens, cu_seqlens=None) -> int:
-    """The number of sequences."""
-    for t in (block_table, seq_lens, cu_seqlens):
-        if t is not None and t.dtype != torch.int32:
-            raise ValueError(f"{name}: block_table, cu_seqlens and seq_lens must be int32 tensors")
-    if block_table.dim() != 2 or not block_table.is_contiguous() or not seq_lens.is_contiguous() \
+def _check_metadata(name: str, block_table, seq_lens, cu_seqlens=None) -> tuple[int, int]:
+    """The numbers of sequences and of a table's pages."""
+    i32 = torch.int32
+    if block_table.dtype != i32 or seq_lens.dtype != i32 or (cu_seqlens is not None and cu_seqlens.dtype != i32):
+        raise ValueError(f"{name}: block_table, cu_seqlens and seq_lens must be int32 tensors")
+    shape = block_table.shape
+    if len(shape) != 2 or not block_table.is_contiguous() or not seq_lens.is_contiguous() \
             or (cu_seqlens is not None and not cu_seqlens.is_contiguous()):
         raise ValueError(f"{name}: block_table must be a contiguous [sequences, max_pages] tensor, cu_seqlens and seq_lens "
                          "contiguous")
-    n = block_table.shape[0]
+    n = shape[0]
     if seq_lens.numel() != n or (cu_seqlens is not None and cu_seqlens.numel() != n + 1):
         raise ValueError(f"{name}: {n} sequences take {n + 1} cu_seqlens and {n} seq_lens")
-    return n
+    return n, shape[1]
 
 
-def _check_rows(name: str, what: str, t, tokens: int | None = None, heads: int | None = None, head_dim: int | None = None) -> None:
-    """bf16 [tokens, heads, head_dim] whose heads are contiguous; tokens may be further apart (views of a joint projection)."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3:
+def _check_rows(name: str, what: str, t, tokens: int | None = None, heads: int | None = None, head_dim: int | None = None) -> int:
+    """bf16 [tokens, heads, head_dim] whose heads are contiguous; tokens may be further apart (views of a joint projection).
+    Returns a token's stride."""
+    shape = t.shape
+    if t.dtype != torch.bfloat16 or len(shape) != 3:
         raise ValueError(f"{name}: {what} must be a bfloat16 [tokens, heads, head_dim] tensor")
-    if (tokens is not None and t.shape[0] != tokens) or (heads is not None and t.shape[1] != heads) \
-            or (head_dim is not None and t.shape[2] != head_dim):
-        raise ValueError(f"{name}: {what} is {tuple(t.shape)}, not "
+    n, h, d = shape
+    if (tokens is not None and n != tokens) or (heads is not None and h != heads) or (head_dim is not None and d != head_dim):
+        raise ValueError(f"{name}: {what} is {tuple(shape)}, not "
                          f"[{tokens}, {'heads' if heads is None else heads}, {'head_dim' if head_dim is None else head_dim}]")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or
-                      (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1] * t.shape[2]))):
+    per_token, per_head, per_dim = t.stride()
+    if n <= 1:
+        per_token = h * d
+    if n * h * d and (per_dim != 1 or (h > 1 and per_head != d) or per_token % 8 or per_token < h * d):
         raise ValueError(f"{name}: a token's heads in {what} must be contiguous, and tokens a multiple of 8 elements apart "
                          f"(strides {t.stride()})")
-
-
-def _token_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return per_token
 
 
 def _check_key_weights(name: str, key_weights, n_pages: int, kv_heads: int) -> None:
@@ -93,16 +97,16 @@ def gqa_cache_write(key: torch.Tensor, value: torch.Tensor, kv_pages: torch.Tens
     in its key or its value row, is NaN to the rows that see it and touches nothing else.  ``key_weights`` (fp32 [n_pages,
     kv_heads, 64]) is set to 0 for the keys written.  Sequences must not share the pages that are written to."""
     name = "gqa_cache_write"
-    _check_rows(name, "key", key)
+    key_stride = _check_rows(name, "key", key)
     tokens, kv_heads, head_dim = key.shape
-    _check_rows(name, "value", value, tokens, kv_heads, head_dim)
-    _check_pages(name, kv_pages, kv_heads, head_dim)
-    n = _check_metadata(name, block_table, seq_lens, cu_seqlens)
+    value_stride = _check_rows(name, "value", value, tokens, kv_heads, head_dim)
+    n_pages = _check_pages(name, kv_pages, kv_heads, head_dim)
+    n, max_pages = _check_metadata(name, block_table, seq_lens, cu_seqlens)
     if (query is None) != (query_out is None) or (query is None and gamma_q is not None):
         raise ValueError(f"{name}: query and query_out go together, and gamma_q with them")
-    heads = 0
+    heads = query_stride = 0
     if query is not None:
-        _check_rows(name, "query", query, tokens, None, head_dim)
+        query_stride = _check_rows(name, "query", query, tokens, None, head_dim)
         heads = query.shape[1]
         if not 1 <= heads <= 128 or heads % kv_heads:
             raise ValueError(f"{name}: unsupported heads {heads} over kv_heads {kv_heads}")
@@ -119,14 +123,13 @@ def gqa_cache_write(key: torch.Tensor, value: torch.Tensor, kv_pages: torch.Tens
         if t is not None and (t.dtype != torch.float32 or t.numel() != head_dim or not t.is_contiguous()):
             raise ValueError(f"{name}: {what} must be a contiguous float32 tensor of {head_dim} values")
     if key_weights is not None:
-        _check_key_weights(name, key_weights, kv_pages.shape[0], kv_heads)
+        _check_key_weights(name, key_weights, n_pages, kv_heads)
     _require_cuda(name, key, value, kv_pages, block_table, cu_seqlens, seq_lens, gamma_k, freqs_cis, query, gamma_q, query_out,
                   key_weights)
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    _call(key, "tl_gqa_cache_write", key.data_ptr(), _token_stride(key), value.data_ptr(), _token_stride(value), kv_pages.data_ptr(),
-          kv_pages.shape[0], block_table.data_ptr(), block_table.shape[1], cu_seqlens.data_ptr(), seq_lens.data_ptr(), n, tokens,
-          kv_heads, head_dim, ptr(gamma_k), ptr(freqs_cis), rope_dim, ptr(query), _token_stride(query) if query is not None else 0,
-          heads, ptr(gamma_q), ptr(query_out), ptr(key_weights), float(eps), int(interleaved), _stream(key))
+    _call(key, "tl_gqa_cache_write", key.data_ptr(), key_stride, value.data_ptr(), value_stride, kv_pages.data_ptr(),
+          n_pages, block_table.data_ptr(), max_pages, cu_seqlens.data_ptr(), seq_lens.data_ptr(), n, tokens,
+          kv_heads, head_dim, ptr(gamma_k), ptr(freqs_cis), rope_dim, ptr(query), query_stride, heads, ptr(gamma_q), ptr(query_out), ptr(key_weights), float(eps), int(interleaved), _stream(key))
 
 
 def gqa_cache_weights(query: torch.Tensor, lse: torch.Tensor, kv_pages: torch.Tensor, block_table: torch.Tensor,
@@ -138,19 +141,19 @@ def gqa_cache_weights(query: torch.Tensor, lse: torch.Tensor, kv_pages: torch.Te
     (fp32 [n_pages, kv_heads, 64], at the key's page and row), or takes its place with ``accumulate=False``.  A batch of a
     prompt's last tokens alone (their own cu_seqlens) gives the weights of that window.  Sequences must not share pages."""
     name = "gqa_cache_weights"
-    _check_rows(name, "query", query)
+    query_stride = _check_rows(name, "query", query)
     tokens, heads, head_dim = query.shape
     kv_heads = key_weights.shape[1] if key_weights.dim() == 3 else 0
     if not 1 <= kv_heads <= 128 or not 1 <= heads <= 128 or heads % kv_heads:
         raise ValueError(f"{name}: unsupported heads {heads} over kv_heads {kv_heads}")
-    _check_pages(name, kv_pages, kv_heads, head_dim)
-    _check_key_weights(name, key_weights, kv_pages.shape[0], kv_heads)
-    n = _check_metadata(name, block_table, seq_lens, cu_seqlens)
+    n_pages = _check_pages(name, kv_pages, kv_heads, head_dim)
+    _check_key_weights(name, key_weights, n_pages, kv_heads)
+    n, max_pages = _check_metadata(name, block_table, seq_lens, cu_seqlens)
     if lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous():
         raise ValueError(f"{name}: lse must be a contiguous float32 [{tokens}, {heads}] tensor")
     _require_cuda(name, query, lse, kv_pages, block_table, cu_seqlens, seq_lens, key_weights)
-    _call(query, "tl_gqa_cache_weights", query.data_ptr(), _token_stride(query), lse.data_ptr(), kv_pages.data_ptr(), kv_pages.shape[0],
-          block_table.data_ptr(), block_table.shape[1], cu_seqlens.data_ptr(), seq_lens.data_ptr(), n, tokens, heads, kv_heads, head_dim,
+    _call(query, "tl_gqa_cache_weights", query.data_ptr(), query_stride, lse.data_ptr(), kv_pages.data_ptr(), n_pages,
+          block_table.data_ptr(), max_pages, cu_seqlens.data_ptr(), seq_lens.data_ptr(), n, tokens, heads, kv_heads, head_dim,
           float(head_dim ** -0.5 if scale is None else scale), int(accumulate), key_weights.data_ptr(), _stream(query))
 
 
@@ -166,9 +169,9 @@ def gqa_cache_evict(kv_pages: torch.Tensor, key_weights: torch.Tensor, block_tab
     one of the tables'; one outside the pool is not written."""
     name = "gqa_cache_evict"
     kv_heads = key_weights.shape[1] if key_weights.dim() == 3 else 0
-    _check_pages(name, kv_pages, kv_heads, head_dim)
-    _check_key_weights(name, key_weights, kv_pages.shape[0], kv_heads)
-    n = _check_metadata(name, block_table, seq_lens)
+    n_pages = _check_pages(name, kv_pages, kv_heads, head_dim)
+    _check_key_weights(name, key_weights, n_pages, kv_heads)
+    n, max_pages = _check_metadata(name, block_table, seq_lens)
     for what, t in (("keep_lens", keep_lens), ("kept_lens", kept_lens)):
         if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{name}: {what} must be a contiguous int32 tensor of {n} values")
@@ -183,6 +186,6 @@ def gqa_cache_evict(kv_pages: torch.Tensor, key_weights: torch.Tensor, block_tab
     _require_cuda(name, kv_pages, key_weights, block_table, seq_lens, keep_lens, kept_table, kept_lens, kept_slots)
     if kept_slots is None:
         kept_slots = kept_table.new_empty(n, kv_heads, pages * GQA_PAGE_KEYS)
-    _call(kv_pages, "tl_gqa_cache_evict", kv_pages.data_ptr(), key_weights.data_ptr(), kv_pages.shape[0], block_table.data_ptr(),
-          block_table.shape[1], seq_lens.data_ptr(), keep_lens.data_ptr(), n, kv_heads, head_dim, recent, kept_table.data_ptr(), pages,
+    _call(kv_pages, "tl_gqa_cache_evict", kv_pages.data_ptr(), key_weights.data_ptr(), n_pages, block_table.data_ptr(),
+          max_pages, seq_lens.data_ptr(), keep_lens.data_ptr(), n, kv_heads, head_dim, recent, kept_table.data_ptr(), pages,
           kept_lens.data_ptr(), kept_slots.data_ptr(), _stream(kv_pages))
