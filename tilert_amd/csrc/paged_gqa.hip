@@ -32,7 +32,8 @@ struct GqaArgs {
   float scale;  // softmax_scale * log2 e
   uint16_t* out;
   float* lse;
-  int target;       // workgroups that the pages of all tiles are cut for; 0: one workgroup a tile
+  int target;       // pieces that the pages of all tiles are cut into at most, about; 0: one workgroup a tile
+  int at_once;      // workgroups that run at a time
   int2* tile_parts;  // [tile slots]: a tile's first part and its parts (heads: `kv_heads` of them side by side)
   float2* part_ml;   // [parts][BM]
   float* part_o;     // [parts][BM * D]
@@ -69,17 +70,34 @@ __device__ inline bool gqa_tile(const PagedBatch& p, int group, int slot, int bm
 }
 inline int64_t gqa_slots(int64_t n_tokens, int64_t group, int64_t n_seqs, int bm) { return n_tokens * group / bm + n_seqs; }
 
+// Max / sum over the lanes i, i ^ 16, i ^ 32, i ^ 48, in all of them.
+template <bool MAX>
+__device__ inline float four_lanes(float v) {
+  const u32x2g a = __builtin_bit_cast(u32x2g, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  const float a0 = __uint_as_float(a[0]), a1 = __uint_as_float(a[1]), x = MAX ? fmaxf(a0, a1) : a0 + a1;
+  const u32x2g b = __builtin_bit_cast(u32x2g, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  const float b0 = __uint_as_float(b[0]), b1 = __uint_as_float(b[1]);
+  return MAX ? fmaxf(b0, b1) : b0 + b1;
+}
+
 // What a workgroup works on: a tile of one kv head, and its pages pg0 .. pg1 - 1; the tile's parts and which of them this is.
 struct GqaItem {
   int b, tile, pg0, pg1, parts;
   int64_t part;
 };
 // Every workgroup plans the launch for itself, from the metadata on the device: the pages of all tiles are cut into pieces of
-// at most `chunk`, about `target` of them in all and at least kGqaFew pages each; a tile's pieces are of one size.  Where a tile
-// has several, they have a place each in the workspace: at most 2 * target of them, as such a tile has more than `chunk`
-// pages.
+// at most `chunk`, at least kGqaFew; a tile's pieces are of one size.  Where a tile has several, they have a place each in
+// the workspace: at most 2 * target of them, as such a tile has more than `chunk` pages, and `chunk` is no less than the
+// target-th part of all.
+// SEARCH: of kGqaPlans sizes from that part on, up to four times of it, the one that should be done first.  Pieces that run all at
+// once are done with the longest; where they are more, they follow one another as workgroups end: all of them, and half of the
+// longest.  A piece costs kGqaPiece pages beside its own.  (With a fixed number of pieces wanted, 7 sequences of 2 to 700 new
+// tokens over 324 to 5000 keys took 57 us with 120, 53 with 330, 50 with 384 and 55 with 780; with the search 45.  32 sequences of
+// 1024 keys, 256 tiles of 32 rows: 33 uncut, as the search has it, and 52 with 512 pieces.)
 constexpr int kGqaPlanSeqs = 512;  // sequences that a launch plans for; with more, a workgroup takes a tile
 constexpr int kGqaFew = 8;         // pages that are not cut
+constexpr int kGqaPlans = 16;
+constexpr float kGqaPiece = 9.f;
 struct GqaPlanLds {
   int end[kGqaPlanSeqs];   // pieces up to sequence b and with it
   int part[kGqaPlanSeqs];  // of them, those of tiles with several, before sequence b
@@ -87,6 +105,7 @@ struct GqaPlanLds {
   int64_t base[kGqaPlanSeqs];
   int scan[2][8];
   float sum[8];
+  float pieces[8][kGqaPlans], longest[8][kGqaPlans];
 };
 __device__ inline int gqa_wave_scan(int v) {  // inclusive sum over the wave
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
@@ -96,7 +115,7 @@ __device__ inline int gqa_wave_scan(int v) {  // inclusive sum over the wave
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
   return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
-template <int THREADS, int BM, class Args>
+template <int THREADS, int BM, bool SEARCH, class Args>
 __device__ inline bool gqa_plan_item(const Args& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
   constexpr int WAVES = THREADS / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -117,7 +136,43 @@ __device__ inline bool gqa_plan_item(const Args& A, GqaPlanLds& L, int v, GqaIte
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) units += L.sum[w];
   // (a little more than their share, so that the sum's rounding leaves no piece over)
-  const int chunk = max(kGqaFew, static_cast<int>(fminf(units * A.kv_heads / A.target * 1.001f, 2e6f)) + 1);  // (2^20 pages a sequence at most)
+  units *= A.kv_heads;
+  auto size = [&](float by) { return max(kGqaFew, static_cast<int>(fminf(units / A.target * 1.001f * by, 2e6f)) + 1); };  // (2^20 pages a sequence at most)
+  int chunk = size(1.f);
+  if constexpr (SEARCH) {
+    auto plan = [](int i) { return __builtin_amdgcn_exp2f(2.f / (kGqaPlans - 1) * i); };
+    static_assert(kGqaPlans == 16, "a plan is a lane of 16");
+    const int mine = lane & 15;
+    const float by = 1.0f / size(plan(mine));
+    float pieces = 0.f, longest = 0.f;
+    for (int b = tid >> 4; b < A.p.n_seqs; b += THREADS / 16) {
+      const int tiles = (L.rows[b] + BM - 1) / BM;
+      const float n = static_cast<float>(L.splits[b]), cut = fmaxf(1.f, __builtin_ceilf(n * by));
+      pieces += tiles * cut;
+      longest = fmaxf(longest, tiles ? n / cut : 0.f);
+    }
+    pieces = four_lanes<false>(pieces);
+    longest = four_lanes<true>(longest);
+    if (lane < 16) {
+      L.pieces[wave][lane] = pieces;
+      L.longest[wave][lane] = longest;
+    }
+    __syncthreads();
+    pieces = longest = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      pieces += L.pieces[w][mine];
+      longest = fmaxf(longest, L.longest[w][mine]);
+    }
+    pieces *= A.kv_heads;
+    longest += kGqaPiece;
+    const float time = pieces <= A.at_once ? longest : (units + pieces * kGqaPiece) / A.at_once + 0.5f * longest;
+    float best = time;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) best = fminf(best, __shfl_xor(best, o));
+    chunk = size(plan(63 - __builtin_clzll(__ballot(lane < 16 && time == best) | 1)));
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+  }
   int ends = 0, parts = 0;
   for (int b0 = 0; b0 < A.p.n_seqs; b0 += THREADS) {
     const int b = b0 + tid;
@@ -170,7 +225,7 @@ __device__ inline bool gqa_plan_item(const Args& A, GqaPlanLds& L, int v, GqaIte
 template <int THREADS, int BM>
 __device__ inline bool gqa_item(const GqaArgs& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
   if (A.target) {
-    if (!gqa_plan_item<THREADS, BM>(A, L, v, it, first, rows, base)) return false;
+    if (!gqa_plan_item<THREADS, BM, true>(A, L, v, it, first, rows, base)) return false;
   } else {
     if (!gqa_tile(A.p, A.group, v, BM, it.b, it.tile)) return false;
     const GqaSeq s(A.p, A.group, it.b);
@@ -203,16 +258,6 @@ __device__ inline v8bf codes8_bf16(uint32_t a, uint32_t b, float scale) {
   return bf16_of(r);
 }
 __device__ inline v4f mfma_bf16(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-
-// Max / sum over the lanes i, i ^ 16, i ^ 32, i ^ 48, in all of them.
-template <bool MAX>
-__device__ inline float four_lanes(float v) {
-  const u32x2g a = __builtin_bit_cast(u32x2g, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
-  const float a0 = __uint_as_float(a[0]), a1 = __uint_as_float(a[1]), x = MAX ? fmaxf(a0, a1) : a0 + a1;
-  const u32x2g b = __builtin_bit_cast(u32x2g, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
-  const float b0 = __uint_as_float(b[0]), b1 = __uint_as_float(b[1]);
-  return MAX ? fmaxf(b0, b1) : b0 + b1;
-}
 
 // Bytes that are a NaN code, as 0x80 each.
 __device__ inline uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
@@ -274,20 +319,24 @@ __device__ inline GqaValues<D> load_values(const uint8_t* v, int lane) {
 
 __device__ inline float2 load_scales(const float* s) { return float2{load_f32_vector(s), load_f32_vector(s + 1)}; }
 
-// One tile of 16 RT rows and one kv head over `chunk` pages; the four waves take every fourth of them, each with its own
-// statistics, and are joined in LDS.  Weights go into the second product as hi + lo in bf16, 16 bits of them.
+// One tile of 16 RT rows and one kv head over a piece's pages; the four waves take every fourth of them (RT = 4: two by two every
+// second), each with its own statistics, and are joined in LDS.  A wave has up to 32 rows, so that the codes, 128 conversions
+// of two a page and lane, are turned for all of them (16 rows a wave, two waves on the same pages: 4 tokens of 8 heads over
+// 131072 keys 76 us, 59 so).  Weights go into the second product as hi + lo in bf16, 16 bits of them.
 // Weights are relative to 2^24 times the row's largest: their sums of values then stay inside fp32 whatever the values.
+// Bound by bytes, two pages a wave on their way: 60 sequences of 2048 to 32768 keys, 1.42 GB, 238 us, 6.0 TB/s; 131072 keys, 268 MB,
+// 51 us and 8 to join, where a copy's rate takes 52.
 constexpr float kGqaHead = 24.f;
 template <int D, int RT>
-__global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
-  constexpr int BM = 16 * RT, DT = D / 16, KI = D / 64, PW = 4 / RT;  // PW: waves that share the pages of 16 rows
+__global__ __launch_bounds__(256, D * RT > 128 ? 1 : 2) void gqa_attend_kernel(const GqaArgs A) {
+  constexpr int BM = 16 * RT, DT = D / 16, KI = D / 64, TW = RT < 2 ? 1 : 2, RG = RT / TW, PW = 4 / RG;  // TW: row tiles of a wave; PW: waves that share their pages
   __shared__ union {
     GqaPlanLds plan;
     v4f sum_o[4][DT][64];
   } L;
-  __shared__ float sum_m[4][16], sum_l[4][16];
+  __shared__ float sum_m[TW][4][16], sum_l[TW][4][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4, rt = wave % RT, pw = wave / RT;
+  const int c = lane & 15, g = lane >> 4, rg = wave % RG, pw = wave / RG, rt0 = rg * TW;
   const int head = blockIdx.x % A.kv_heads;
   GqaItem it;
   int first, rows_all;
@@ -295,68 +344,84 @@ __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
   if (!gqa_item<256, BM>(A, L.plan, blockIdx.x / A.kv_heads, it, first, rows_all, base)) return;
   const GqaSeq s(A.p, A.group, first, rows_all, base);
   const int row0 = it.tile * BM, rows = min(s.rows - row0, BM);
-  const int least = s.seen(row0 + min(16 * rt, rows - 1));
+  const int least = s.seen(row0 + min(16 * rt0, rows - 1));
   const gqa_const_i32 table = (gqa_const_i32)(A.p.table + static_cast<int64_t>(it.b) * A.p.max_pages);
-  const GqaQuery<D> q = load_query<D>(A.q, A.q_stride, s, head * A.group, row0 + rt * 16 + c, g);
-  const int seen = s.seen(row0 + min(rt * 16 + c, rows - 1));
-  float m = -INFINITY, l = 0.f;
-  v4f o[DT];
+  GqaQuery<D> q[TW];
+  int seen[TW];
+  float m[TW], l[TW];
+  v4f o[TW][DT];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < TW; ++r) {
+    q[r] = load_query<D>(A.q, A.q_stride, s, head * A.group, row0 + (rt0 + r) * 16 + c, g);
+    seen[r] = s.seen(row0 + min((rt0 + r) * 16 + c, rows - 1));
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
   // A page's scores, weights and sums.  Its keys are there already; its values are under way while the scores are made, and
   // the next page's keys behind them.
-  auto step = [&](int pg, bool there, const GqaKeys<D>& kc, GqaValues<D>& vc, float2 scales) {
+  auto step = [&](int pg, bool there, const GqaKeys<D>& kc, GqaValues<D>& vc, float2 scales) __attribute__((always_inline)) {
     const bool ok = gqa_scale_ok(scales.x) && gqa_scale_ok(scales.y);
     const float sk = ok ? scales.x : 1.f, sv = ok ? scales.y : 1.f;
     const int key0 = pg * kGqaKeys;
     const bool masked = !there || !__all(ok) || key0 + kGqaKeys > least;
     // ---- scores
-    v4f x[4];
+    v4f x[TW][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      x[t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < TW; ++r) x[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KI; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) x[t] = mfma_bf16(codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], sk), q.x[i][e], x[t]);
+        for (int e = 0; e < 2; ++e) {
+          const v8bf k = codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], sk);
+#pragma unroll
+          for (int r = 0; r < TW; ++r) x[r][t] = mfma_bf16(k, q[r].x[i][e], x[r][t]);
+        }
     }
     // ---- weights
-    const int my = there ? seen - key0 - 16 * g : 0;  // of this lane's 16 keys, the row sees this many
-    if (masked) {
+    v8bf hi[TW][2], lo[TW][2];
+    int my[TW];  // of this lane's 16 keys, the row sees this many
+#pragma unroll
+    for (int r = 0; r < TW; ++r) {
+      my[r] = there ? seen[r] - key0 - 16 * g : 0;
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[r][t][j] = 4 * t + j >= my[r] ? -INFINITY : (ok ? x[r][t][j] : __builtin_nanf(""));
+      }
+      float top = x[r][0][0];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[t][j] = 4 * t + j >= my ? -INFINITY : (ok ? x[t][j] : __builtin_nanf(""));
-    }
-    float top = x[0][0];
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, x[r][t][j]);
+      top = fmaxf(m[r], four_lanes<true>(top) * A.scale);
+      if (__any(top > m[r])) {
+        const float by = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - top);  // (before the first key all is 0, or NaN)
+        m[r] = top;
+        l[r] *= by;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = fmaxf(top, x[t][j]);
-    top = fmaxf(m, four_lanes<true>(top) * A.scale);
-    if (__any(top > m)) {
-      const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);  // (before the first key all is 0, or NaN)
-      m = top;
-      l *= by;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= by;
-    }
-    const float from = m == -INFINITY ? 0.f : m + kGqaHead;
-    v8bf hi[2], lo[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      u32x4g h, w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v4f y = x[2 * e + i / 2];
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1)], A.scale, -from));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1) + 1], A.scale, -from));
-        l += p0 + p1;
-        h[i] = bf16x2_bits(v2f{p0, p1});
-        w[i] = bf16x2_bits(v2f{p0 - __uint_as_float(h[i] << 16), p1 - __uint_as_float(h[i] & 0xffff0000u)});
+        for (int d = 0; d < DT; ++d) o[r][d] *= by;
       }
-      hi[e] = bf16_of(h);
-      lo[e] = bf16_of(w);
+      const float from = m[r] == -INFINITY ? 0.f : m[r] + kGqaHead;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        u32x4g h, w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f y = x[r][2 * e + i / 2];
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1)], A.scale, -from));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * (i & 1) + 1], A.scale, -from));
+          l[r] += p0 + p1;
+          h[i] = bf16x2_bits(v2f{p0, p1});
+          w[i] = bf16x2_bits(v2f{p0 - __uint_as_float(h[i] << 16), p1 - __uint_as_float(h[i] & 0xffff0000u)});
+        }
+        hi[r][e] = bf16_of(h);
+        lo[r][e] = bf16_of(w);
+      }
     }
     // ---- values; on a page with keys that some row does not see, codes that are NaN are taken apart
     if (masked) {
@@ -368,16 +433,19 @@ __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
       if (__any(all != 0)) {  // how many NaN values a row sees
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          v4f n = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            u32x4g w;
+          for (int r = 0; r < TW; ++r) {
+            v4f n = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (8 * e + 2 * i < my ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my ? 0x3f800000u : 0u);
-            n = mfma_bf16(codes8_bf16(nan_codes(vc.v[d][2 * e]) >> 1, nan_codes(vc.v[d][2 * e + 1]) >> 1, 1.f), bf16_of(w), n);
+            for (int e = 0; e < 2; ++e) {
+              u32x4g w;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = (8 * e + 2 * i < my[r] ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my[r] ? 0x3f800000u : 0u);
+              n = mfma_bf16(codes8_bf16(nan_codes(vc.v[d][2 * e]) >> 1, nan_codes(vc.v[d][2 * e + 1]) >> 1, 1.f), bf16_of(w), n);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[r][d][j] = n[j] > 0.f ? __builtin_nanf("") : o[r][d][j];
           }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d][j] = n[j] > 0.f ? __builtin_nanf("") : o[d][j];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t bad = nan_codes(vc.v[d][i]);
@@ -391,8 +459,11 @@ __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const v8bf a = codes8_bf16(vc.v[d][2 * e], vc.v[d][2 * e + 1], sv);
-        o[d] = mfma_bf16(a, hi[e], o[d]);
-        o[d] = mfma_bf16(a, lo[e], o[d]);
+#pragma unroll
+        for (int r = 0; r < TW; ++r) {
+          o[r][d] = mfma_bf16(a, hi[r][e], o[r][d]);
+          o[r][d] = mfma_bf16(a, lo[r][e], o[r][d]);
+        }
       }
   };
   // pages pg0 + pw, + PW, ..; one outside the pool is read as page 0 and seen by no row
@@ -400,18 +471,18 @@ __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
   auto there = [&](int id) { return id >= 0 && id < A.p.n_pages; };
   auto block = [&](int id) { return gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there(id) ? id : 0, head); };
   int pg = it.pg0 + pw;
-  if (pg < it.pg1 && rt * 16 < rows) {
+  if (pg < it.pg1 && rt0 * 16 < rows) {
     GqaKeys<D> ka, kb;
     GqaValues<D> va, vb;
     float2 sa, sb;
     int id = page_id(pg), next = page_id(pg + PW);
     ka = load_keys<D>(block(id).k, lane);
-    va = load_values<D, RT == 1>(block(id).v, lane);
+    va = load_values<D, RG == 1>(block(id).v, lane);
     sa = load_scales(block(id).scale);
     // (two buffers by turns: one copied into the other would wait for its loads)
-    auto half = [&](const GqaKeys<D>& k_now, GqaValues<D>& v_now, float2 s_now, GqaKeys<D>& k_then, GqaValues<D>& v_then, float2& s_then) {
+    auto half = [&](const GqaKeys<D>& k_now, GqaValues<D>& v_now, float2 s_now, GqaKeys<D>& k_then, GqaValues<D>& v_then, float2& s_then) __attribute__((always_inline)) {
       k_then = load_keys<D>(block(next).k, lane);
-      v_then = load_values<D, RT == 1>(block(next).v, lane);
+      v_then = load_values<D, RG == 1>(block(next).v, lane);
       s_then = load_scales(block(next).scale);
       const bool is = there(id);
       id = next;
@@ -427,49 +498,56 @@ __global__ __launch_bounds__(256, 2) void gqa_attend_kernel(const GqaArgs A) {
     }
   }
   // ---- the waves of the same rows together
-  l = four_lanes<false>(l);
-  if (g == 0) {
-    sum_m[wave][c] = m;
-    sum_l[wave][c] = l;
+  float top[TW], total[TW];
+#pragma unroll
+  for (int r = 0; r < TW; ++r) {
+    l[r] = four_lanes<false>(l[r]);
+    if (g == 0) {
+      sum_m[r][wave][c] = m[r];
+      sum_l[r][wave][c] = l[r];
+    }
   }
   __syncthreads();
-  float top = -INFINITY, total = 0.f;
 #pragma unroll
-  for (int w = 0; w < PW; ++w) top = fmaxf(top, sum_m[rt + RT * w][c]);
+  for (int r = 0; r < TW; ++r) {
+    top[r] = -INFINITY;
+    total[r] = 0.f;
 #pragma unroll
-  for (int w = 0; w < PW; ++w) {
-    const float mw = sum_m[rt + RT * w][c];
-    total += sum_l[rt + RT * w][c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - top));
-  }
-  if constexpr (PW > 1) {
-    const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    for (int w = 0; w < PW; ++w) top[r] = fmaxf(top[r], sum_m[r][rg + RG * w][c]);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) L.sum_o[wave][d][lane] = o[d] * by;
-    __syncthreads();
-  }
-  const bool live = rt * 16 + c < rows, whole = it.parts == 1;
-  const int row = row0 + rt * 16 + c;
-  const int64_t at = static_cast<int64_t>(s.first + row / A.group) * A.heads + head * A.group + row % A.group;
-  const int64_t part = it.part * A.kv_heads + head;
-  const float inv = total == 0.f ? 0.f : 1.0f / total;
-#pragma unroll
-  for (int i = 0; i < DT / PW; ++i) {
-    const int d = PW * i + pw;
-    v4f v;
-    if constexpr (PW > 1) {
-      v = L.sum_o[rt][d][lane];
-#pragma unroll
-      for (int w = 1; w < PW; ++w) v += L.sum_o[rt + RT * w][d][lane];
-    } else {
-      v = o[i];
+    for (int w = 0; w < PW; ++w) {
+      const float mw = sum_m[r][rg + RG * w][c];
+      total[r] += sum_l[r][rg + RG * w][c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - top[r]));
     }
-    if (!live) continue;
-    if (whole) *reinterpret_cast<u32x2g*>(A.out + at * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
-    else reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[(rt * DT + d) * 64 + lane] = v;
   }
-  if (pw == 0 && g == 0 && live) {
-    if (!whole) A.part_ml[part * BM + rt * 16 + c] = float2{top, total};
-    else if (A.lse) A.lse[at] = total == 0.f ? -INFINITY : (top + kGqaHead + log2f(total)) * kLn2;
+  const bool whole = it.parts == 1;
+  const int64_t part = it.part * A.kv_heads + head;
+#pragma unroll
+  for (int r = 0; r < TW; ++r) {
+    const int rt = rt0 + r;
+    const float by = m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - top[r]);
+    if (r) __syncthreads();  // (the tile in front is read)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) L.sum_o[wave][d][lane] = o[r][d] * by;
+    __syncthreads();
+    const bool live = rt * 16 + c < rows;
+    const int row = row0 + rt * 16 + c;
+    const int64_t at = static_cast<int64_t>(s.first + row / A.group) * A.heads + head * A.group + row % A.group;
+    const float inv = total[r] == 0.f ? 0.f : 1.0f / total[r];
+#pragma unroll
+    for (int i = 0; i < DT / PW; ++i) {
+      const int d = PW * i + pw;
+      v4f v = L.sum_o[rg][d][lane];
+#pragma unroll
+      for (int w = 1; w < PW; ++w) v += L.sum_o[rg + RG * w][d][lane];
+      if (!live) continue;
+      if (whole) *reinterpret_cast<u32x2g*>(A.out + at * D + 16 * d + 4 * g) = u32x2g{bf16x2_bits(v2f{v[0] * inv, v[1] * inv}), bf16x2_bits(v2f{v[2] * inv, v[3] * inv})};
+      else reinterpret_cast<v4f*>(A.part_o + part * (BM * D))[(rt * DT + d) * 64 + lane] = v;
+    }
+    if (pw == 0 && g == 0 && live) {
+      if (!whole) A.part_ml[part * BM + rt * 16 + c] = float2{top[r], total[r]};
+      else if (A.lse) A.lse[at] = total[r] == 0.f ? -INFINITY : (top[r] + kGqaHead + log2f(total[r])) * kLn2;
+    }
   }
 }
 
@@ -853,23 +931,24 @@ __global__ __launch_bounds__(64 * kJoinWaves) void gqa_join_kernel(const GqaArgs
 // The launch: rows a tile, workgroups, and the workspace.
 struct GqaLaunch {
   int bm;
-  int64_t slots, target, wgs;
+  int64_t slots, target, at_once, wgs;
   size_t ml_at, o_at, bytes;
 };
 inline GqaLaunch gqa_launch(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_pages) {
   GqaLaunch d{};
   const int64_t group = heads / kv_heads, each = cdiv(n_tokens * group, n_seqs);
-  // In us with 64-row / kChunkRows tiles, rows a sequence and head: 48 rows of 1 sequence over 16384 keys 24 / 31, 64 rows 26 / 31, 96
-  // 36 / 33; of 8 sequences over 4096, 64 heads' tiles, 64 rows 48 / 45; of 32 over 1024, 256 tiles, 16 rows 31 / 35, 24
-  // rows 37 / 36, 32 rows 43 / 35, 64 rows 72 / 37: with a tile for every CU a page is better read by one workgroup.
-  d.bm = each > (n_seqs * kv_heads >= 256 ? 24 : 64) ? kChunkRows : (each <= 16 ? 16 : (each <= 32 ? 32 : 64));
+  // Tiles of 16 rows a wave, or 32 (64 in two waves where a head's 64 dims leave the registers), and beyond them kChunkRows.  In
+  // us with 32-row, 64-row / kChunkRows tiles, 64 heads over 8, head_dim 128: 32 rows of 1 sequence over 131072 keys 66 / 95, of 8
+  // over 4096 29 / 32, of 64 over 4096 142 / 184; 64 rows 91 / 98, 42 / 34, 204 / 191.  head_dim 64: 32 rows 35 / 73, 18 / 26,
+  // 66 / 140; 64 rows 55 / 76, 26 / 27, 105 / 147; 96 rows of 8 over 4096 34 / 27.
+  d.bm = each <= 16 ? 16 : (each <= 32 ? 32 : (each <= 64 && head_dim == 64 ? 64 : kChunkRows));
   d.slots = gqa_slots(n_tokens, group, n_seqs, d.bm);
+  d.at_once = d.bm == kChunkRows || (head_dim == 128 && d.bm > 16) ? 256 : 512;  // (by registers one workgroup a CU, or two)
+  // More pieces than run at once even out tiles of unlike lengths where those are about as many; elsewhere they are work to join,
+  // and workgroups without any.  In us with at_once / 2 at_once: 60 sequences of 2048 to 32768 keys (480 tiles) 282 / 273; 200 of 94 to
+  // 1500 (1600) 90 / 95; 4 tokens over 131072 (8) 66 / 75.
   const int64_t tiles = d.slots * kv_heads;
-  // In us: 60 sequences of 2048 to 32768 keys, 1 token (480 tiles of 16 rows) 282 with 512 pieces, 273 with 1024, 277 with 2048; 4
-  // tokens over 131072 keys (8 tiles of 32 rows) 76, 86, 104: there a piece is a workgroup's all, and fewer are less to
-  // join.  Tiles of kChunkRows, a workgroup a CU: 7 sequences of 2 to 700 new tokens 60 with 256, 49 with 384, 58 with
-  // 512; 256 tiles that see 14336 to 16384 keys 484, 491, 491.
-  if (n_seqs <= kGqaPlanSeqs && max_pages > kGqaFew) d.target = d.bm == kChunkRows ? (tiles < 256 ? 384 : 256) : (tiles <= 128 ? 512 : 1024);
+  if (n_seqs <= kGqaPlanSeqs && max_pages > kGqaFew) d.target = 2 * tiles <= d.at_once || tiles >= 2 * d.at_once ? d.at_once : d.at_once * 2;
   d.wgs = d.slots * kv_heads + d.target;
   if (d.target) {
     d.ml_at = (d.slots * sizeof(int2) + 255) / 256 * 256;
@@ -923,7 +1002,7 @@ __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A)
     int64_t base;
     if (A.target) {  // (one unit a workgroup)
       GqaItem it;
-      if (!gqa_plan_item<256, 1 << 30>(A, plan, static_cast<int>(u / A.kv_heads), it, first, rows_all, base)) return;
+      if (!gqa_plan_item<256, 1 << 30, false>(A, plan, static_cast<int>(u / A.kv_heads), it, first, rows_all, base)) return;
       unit.b = it.b;
       unit.pages = it.pg0;
       pg0 = it.parts;
@@ -1238,7 +1317,7 @@ extern "C" int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const vo
   const GqaArgs args{(const uint16_t*)q_bf16, q_stride, (const uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
                      PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
                      (int)heads, (int)kv_heads, (int)(heads / kv_heads), softmax_scale * kLog2e, (uint16_t*)out_bf16, lse,
-                     (int)d.target, reinterpret_cast<int2*>(ws), reinterpret_cast<float2*>(ws + d.ml_at), reinterpret_cast<float*>(ws + d.o_at)};
+                     (int)d.target, (int)d.at_once, reinterpret_cast<int2*>(ws), reinterpret_cast<float2*>(ws + d.ml_at), reinterpret_cast<float*>(ws + d.o_at)};
   const hipStream_t st = (hipStream_t)stream;
   auto join = [&](auto dim, auto bm, auto deep) -> int {
     constexpr int D = decltype(dim)::value, BM = decltype(bm)::value, DT = D / 16;
@@ -1263,8 +1342,9 @@ extern "C" int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const vo
     return join(dim, integral_constant<int, kChunkRows>{}, std::false_type{});
   };
   auto by_rows = [&](auto dim) -> int {
-    return d.bm == 16 ? few(dim, integral_constant<int, 1>{}) : (d.bm == 32 ? few(dim, integral_constant<int, 2>{}) :
-           (d.bm == 64 ? few(dim, integral_constant<int, 4>{}) : many(dim)));
+    if constexpr (decltype(dim)::value == 64)
+      if (d.bm == 64) return few(dim, integral_constant<int, 4>{});
+    return d.bm == 16 ? few(dim, integral_constant<int, 1>{}) : (d.bm == 32 ? few(dim, integral_constant<int, 2>{}) : many(dim));
   };
   return head_dim == 64 ? by_rows(std::integral_constant<int, 64>{}) : by_rows(std::integral_constant<int, 128>{});
 }
