@@ -985,13 +985,15 @@ struct GqaUnit {
   }
 };
 
-// Few rows (a decode step): a wave takes every fourth page of a piece, one behind another, the next one's keys on their way;
-// their rows, one tile of 16 as a rule, stay in registers.  Scores as in the attention's first product, S^T = K Q^T: a
-// lane sums its keys' weights over its column of rows.  Bound by bytes.  Pieces as the attention plans them (in groups of
-// kSumPages pages by the table's width, 60 sequences of 2048 to 32768 keys took 170 us).
+// Few rows (a decode step): a wave takes every fourth page of a piece, one behind another, the next two's keys on their way;
+// their rows, RT tiles of 16 as a rule, stay in registers (more of them are loaded page by page).  Scores as in the
+// attention's first product, S^T = K Q^T: a lane sums its keys' weights over its column of rows.  Bound by bytes: 60
+// sequences of 2048 to 32768 keys, 730 MB, 153 us, 4.8 TB/s.  Pieces as the attention plans them (in groups of kSumPages
+// pages by the table's width they took 170 us).  Two tiles against the kernel for many rows below: 4 tokens of 8 heads over
+// 131072 keys 44 / 59 us, over 8192 keys of 40 sequences 90 / 147; four tiles, 8 tokens, 75 / 66.
 constexpr int kSumPages = 32;  // pages of a piece where nothing is planned
 constexpr int kSumTarget = 1536;
-template <int D>
+template <int D, int RT>
 __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A) {
   __shared__ GqaPlanLds plan;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1023,14 +1025,17 @@ __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A)
     auto page_id = [&](int pg) { return __builtin_amdgcn_readfirstlane(table[min(pg, pg1 - 1)]); };
     auto there = [&](int id) { return id >= 0 && id < A.p.n_pages; };
     auto block = [&](int id) { return gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there(id) ? id : 0, unit.head); };
-    GqaQuery<D> q;
-    float lse2;
-    int seen;
+    GqaQuery<D> q[RT];
+    float lse2[RT];
+    int seen[RT];
     auto rows = [&](int row0) {
-      const int row = row0 + c, at = min(row, s.rows - 1);
-      q = load_query<D>(A.q, A.q_stride, s, unit.head * A.group, row, g);
-      lse2 = A.lse[(static_cast<int64_t>(s.first) + at / A.group) * A.heads + unit.head * A.group + at % A.group] * kLog2e;
-      seen = row < s.rows ? s.seen(row) : 0;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int row = row0 + 16 * r + c, at = min(row, s.rows - 1);
+        q[r] = load_query<D>(A.q, A.q_stride, s, unit.head * A.group, row, g);
+        lse2[r] = A.lse[(static_cast<int64_t>(s.first) + at / A.group) * A.heads + unit.head * A.group + at % A.group] * kLog2e;
+        seen[r] = row < s.rows ? s.seen(row) : 0;
+      }
     };
     rows(0);
     int pg = pg0;
@@ -1039,22 +1044,29 @@ __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A)
       const float by = ok ? sk : 1.f, scale = ok ? A.scale : __builtin_nanf("");
       const int key0 = pg * kGqaKeys;
       float w[4][4] = {};
-      for (int row0 = 0; row0 < s.rows; row0 += 16) {
-        if (s.rows > 16) rows(row0);
-        const int my = seen - key0 - 16 * g;
-        const bool masked = __any(my < 16);
+      for (int row0 = 0; row0 < s.rows; row0 += 16 * RT) {
+        if (s.rows > 16 * RT) rows(row0);
+        bool masked[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) masked[r] = __any(seen[r] - key0 - 16 * g < 16);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          v4f x = {0.f, 0.f, 0.f, 0.f};
+          v4f x[RT] = {};
 #pragma unroll
           for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) x = mfma_bf16(codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], by), q.x[i][e], x);
+            for (int e = 0; e < 2; ++e) {
+              const v8bf k = codes8_bf16(kc.k[t][i][2 * e], kc.k[t][i][2 * e + 1], by);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], scale, -lse2));
-            w[t][j] += masked && 4 * t + j >= my ? 0.f : p;
-          }
+              for (int r = 0; r < RT; ++r) x[r] = mfma_bf16(k, q[r].x[i][e], x[r]);
+            }
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][j], scale, -lse2[r]));
+              w[t][j] += masked[r] && 4 * t + j >= seen[r] - key0 - 16 * g ? 0.f : p;
+            }
         }
       }
       float mine = 0.f;  // over the 16 rows of a column: lane (c, g) keeps key 16 g + c
@@ -1362,7 +1374,7 @@ extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const 
   if (int rc = check_gqa_rows(who, "query", q_bf16, q_stride, heads, head_dim)) return rc;
   if (!lse || !key_weights) { set_error("%s: null pointer", who); return kErrArg; }
   const int64_t each = cdiv(n_tokens * (heads / kv_heads), n_seqs);
-  const bool few = each <= 16;
+  const bool few = each <= 32;
   int pw = 8;  // pages a workgroup: as many as leave a workgroup for every CU
   while (pw > 1 && cdiv(max_pages, pw) * kv_heads * n_seqs < 256) pw /= 2;
   const int64_t target = few && n_seqs <= kGqaPlanSeqs ? kSumTarget : 0;
@@ -1373,7 +1385,9 @@ extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const 
   const dim3 grid(target || units < (1 << 16) ? units : (1 << 16));  // (a workgroup goes on with another unit)
   const hipStream_t st = (hipStream_t)stream;
   if (few) {
-    hipLaunchKernelGGL(head_dim == 64 ? gqa_sum_few_kernel<64> : gqa_sum_few_kernel<128>, grid, dim3(256), 0, st, args);
+    const auto kern = head_dim == 64 ? (each <= 16 ? gqa_sum_few_kernel<64, 1> : gqa_sum_few_kernel<64, 2>) :
+                                       (each <= 16 ? gqa_sum_few_kernel<128, 1> : gqa_sum_few_kernel<128, 2>);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, args);
     return check_launch(who);
   }
   auto many = [&](auto dim, auto pages) -> int {
