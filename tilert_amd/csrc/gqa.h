@@ -63,6 +63,15 @@ __device__ inline uint32_t gqa_rescale4(uint32_t x, float ratio) {
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(b[0] * ratio, b[1] * ratio, r, true));
 }
 
+__device__ inline int gqa_wave_scan(int v) {  // inclusive sum over the wave
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
+
 // The host's checks of heads and dims; `who` names the entry point.
 inline int check_gqa(const char* who, int64_t kv_heads, int64_t head_dim) {
   if (head_dim != 64 && head_dim != 128) { set_error("%s: head_dim=%lld must be 64 or 128", who, (long long)head_dim); return kErrUnsupported; }

@@ -1,4 +1,6 @@
 // The paged per-head cache (gqa.h): writing new tokens with their heads' norms and rotation, and eviction by weight.
+#include <type_traits>
+
 #include "gqa.h"
 #include "../../include/tilert_amd.h"
 
@@ -280,7 +282,9 @@ __device__ inline uint32_t weight_key(float w) {
 // histograms in LDS, then every wave counts and writes its own stretch of the positions.
 // A workgroup a head; each of its 16 waves goes through its own stretch of pages, four pages at a time, four keys a lane, once
 // for each digit and once to mark the keys that stay, two bits each in LDS, from which their places are counted.  Bound by
-// vector instructions, some 15 a key and pass: 65536 keys 115 us with a page at a time and the marking done twice.
+// vector instructions, some 10 a key and pass: 65536 keys 55 us, 64 with every key's place looked at and 115 with a page at a
+// time and the marking done twice; 4000 keys 12.6 us.  (The keys kept in LDS, or only those of the first digit's bin, were no
+// faster: 68 and 13.0; nor the histogram in four or eight copies, 64 and 67.)
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048, kSelBatch = 4;
 constexpr int kSelBlock = 1024;  // pages that are marked at a time
 __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictArgs A) {
@@ -316,8 +320,8 @@ __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictA
   const int total = count(0), k = min(min(max(A.keep[b], 0), total), width);
   const int last0 = n - min(A.recent, k);  // positions from here on stay
   int need = k - count(last0);             // of the others
-  // f(position of a lane's four keys, their sort keys) for the wave's stretch of pages page0 .. page1 - 1, in order; sort key 0,
-  // which no weight has: none is there
+  // f(position of a lane's four keys, their sort keys, low) for the wave's stretch of pages page0 .. page1 - 1, in order; sort
+  // key 0, which no weight has: none is there; low: the wave's keys are all there and below last0
   auto pages = [&](int page0, int page1, auto f) __attribute__((always_inline)) {
     const int quads = (page1 - page0 + 3) / 4, per = (quads + kSelWaves - 1) / kSelWaves;
     const int q0 = wave * per, q1 = min(q0 + per, quads);
@@ -333,60 +337,80 @@ __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictA
       for (int i = 0; i < kSelBatch; ++i) {
         if (first + i >= q1) break;
         const int pos = (page0 + 4 * (first + i)) * kGqaKeys + 4 * lane, here = there(id[i]) ? n - pos : 0;
-        const uint32_t key[4] = {here > 0 ? weight_key(w[i].x) : 0u, here > 1 ? weight_key(w[i].y) : 0u,
-                                 here > 2 ? weight_key(w[i].z) : 0u, here > 3 ? weight_key(w[i].w) : 0u};
-        f(pos, key);
+        uint32_t key[4] = {weight_key(w[i].x), weight_key(w[i].y), weight_key(w[i].z), weight_key(w[i].w)};
+        const bool low = __all(here > 3) && (page0 + 4 * (first + i) + 4) * kGqaKeys <= last0;
+        if (!low)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) key[j] = here > j ? key[j] : 0u;
+        f(pos, key, low);
       }
     }
   };
   // the need-th largest key of the positions below last0, and how many equal to it stay
-  uint32_t prefix = 0, known = 0;
-  if (need > 0) {
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bins = digit == 2 ? 1024 : 2048;
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      pages(0, n_pages, [&](int pos, const uint32_t (&key)[4]) {
+  uint32_t prefix = 0;
+  auto digit = [&](auto high, auto bits) __attribute__((always_inline)) {  // the digit of `bits` bits below bit `high`
+    constexpr int HIGH = decltype(high)::value, SHIFT = HIGH - decltype(bits)::value, BINS = 1 << decltype(bits)::value;
+    for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    auto add = [&](uint32_t key) __attribute__((always_inline)) {
+      if (HIGH == 32 || (key ^ prefix) >> (HIGH % 32) == 0) atomicAdd(&hist[(key >> SHIFT) & (BINS - 1)], 1);
+    };
+    pages(0, n_pages, [&](int pos, const uint32_t (&key)[4], bool low) __attribute__((always_inline)) {
+      if (low) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) add(key[j]);
+      } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (key[j] != 0 && pos + j < last0 && (key[j] & known) == prefix) atomicAdd(&hist[(key[j] >> shift) & (bins - 1)], 1);
-      });
-      __syncthreads();
-      // from the largest digit down: thread t has the bins 2047 - 2 t and 2046 - 2 t
-      const int hi = hist[kSelBins - 1 - 2 * tid], lo = hist[kSelBins - 2 - 2 * tid];
-      int up = hi + lo;
+          if (key[j] != 0 && pos + j < last0) add(key[j]);
+      }
+    });
+    __syncthreads();
+    // from the largest digit down: thread t has the bins 2047 - 2 t and 2046 - 2 t
+    const int hi = hist[kSelBins - 1 - 2 * tid], lo = hist[kSelBins - 2 - 2 * tid];
+    int up = gqa_wave_scan(hi + lo);
+    if (lane == 63) wave_sum[wave] = up;
+    __syncthreads();
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(up, o);
-        up += lane >= o ? x : 0;
-      }
-      if (lane == 63) wave_sum[wave] = up;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) up += wave_sum[w];
-      const int above = up - hi - lo;
-      if (above < need && up >= need) {
-        found[0] = above + hi >= need ? kSelBins - 1 - 2 * tid : kSelBins - 2 - 2 * tid;
-        found[1] = above + hi >= need ? above : above + hi;
-      }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(found[0]) << shift;
-      known |= static_cast<uint32_t>(bins - 1) << shift;
-      need -= found[1];
-      __syncthreads();
+    for (int w = 0; w < kSelWaves; ++w) up += w < wave ? wave_sum[w] : 0;
+    const int above = up - hi - lo;
+    if (above < need && up >= need) {
+      found[0] = above + hi >= need ? kSelBins - 1 - 2 * tid : kSelBins - 2 - 2 * tid;
+      found[1] = above + hi >= need ? above : above + hi;
     }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(found[0]) << SHIFT;
+    need -= found[1];
+    __syncthreads();
+  };
+  if (need > 0) {
+    using std::integral_constant;
+    digit(integral_constant<int, 32>{}, integral_constant<int, 11>{});
+    digit(integral_constant<int, 21>{}, integral_constant<int, 11>{});
+    digit(integral_constant<int, 10>{}, integral_constant<int, 10>{});
   }
   const uint64_t below = (1ull << lane) - 1;
   int at0 = 0, eq0 = 0;  // kept ones, and equal ones, in the blocks in front
   for (int page0 = 0; page0 < n_pages; page0 += kSelBlock) {
     const int page1 = min(page0 + kSelBlock, n_pages), pos0 = page0 * kGqaKeys;
     int sures = 0, equals = 0;
-    pages(page0, page1, [&](int pos, const uint32_t (&key)[4]) {
+    const uint32_t over = need > 0 ? prefix : 0xffffffffu;  // (without a threshold nothing is over it)
+    pages(page0, page1, [&](int pos, const uint32_t (&key)[4], bool low) __attribute__((always_inline)) {
       int sure = 0, equal = 0;
+      if (low) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool last = pos + j >= last0;
-        sure |= key[j] != 0 && (last || (need > 0 && key[j] > prefix)) ? 1 << j : 0;
-        equal |= key[j] != 0 && !last && need > 0 && key[j] == prefix ? 1 << j : 0;
+        for (int j = 0; j < 4; ++j) {
+          sure |= key[j] > over ? 1 << j : 0;
+          equal |= key[j] == over ? 1 << j : 0;
+        }
+        equal = need > 0 ? equal : 0;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool last = pos + j >= last0;
+          sure |= key[j] != 0 && (last || key[j] > over) ? 1 << j : 0;
+          equal |= key[j] != 0 && !last && need > 0 && key[j] == over ? 1 << j : 0;
+        }
       }
       sures += __popc(sure);
       equals += __popc(equal);

@@ -107,14 +107,6 @@ struct GqaPlanLds {
   float sum[8];
   float pieces[8][kGqaPlans], longest[8][kGqaPlans];
 };
-__device__ inline int gqa_wave_scan(int v) {  // inclusive sum over the wave
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-}
 template <int THREADS, int BM, bool SEARCH, class Args>
 __device__ inline bool gqa_plan_item(const Args& A, GqaPlanLds& L, int v, GqaItem& it, int& first, int& rows, int64_t& base) {
   constexpr int WAVES = THREADS / 64;
