@@ -110,7 +110,9 @@ __device__ inline void norm_rope(float (&x)[8], int part, bool norm, const float
   }
 }
 
-// A workgroup takes one page of a sequence's new keys and one kv head, or 8 D / 16 .. query rows (the workgroups behind).
+// A workgroup takes one page of a sequence's new keys and one kv head (its scales need all of the block's rows), or, behind
+// those, 64 query rows; 8 or 16 lanes a row, 16 bytes each.  Values are transposed through LDS.  Bound by bytes and the loads'
+// latency, as a workgroup's work is one round of them: 4000 tokens, 32 heads over 8 of 128 dims, 92 MB, 27 us, 3.4 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES, STEPS = kGqaKeys / ROWS;
@@ -471,130 +473,100 @@ __global__ __launch_bounds__(kSelThreads) void gqa_select_kernel(const GqaEvictA
 }
 
 // A workgroup gathers the keys of one new page and head: their codes under the least common scale, and their weights.  A key's
-// row is a load; a value is a column of its page's block, so the blocks of the pages that hold the kept keys, which ascend,
-// come through LDS four at a time, whole (a byte a lane from memory, 122 us for 9 sequences brought down to 8192 keys), and
-// the new block goes out through LDS too.  Bound by bytes: those of all pages with a kept key.
+// row is loads of 16 bytes; a value is a column of its page's block, a byte a lane, so that the blocks of all pages with a
+// kept key come whole.  Bound by those bytes: 9 sequences of up to 65536 keys brought down to 8192, 594 MB, 122 us, 4.9 TB/s
+// (the blocks through LDS by loads of 16 bytes: 125).
 template <int D>
 __global__ __launch_bounds__(256) void gqa_gather_kernel(const GqaEvictArgs A) {
-  constexpr int CH = D / 16, ROWS = 256 / CH, STEPS = kGqaKeys / ROWS, DIMS = D / 4, BATCH = 4, BLK = D * kGqaKeys / 16 / 256;
-  __shared__ u32x4g blocks[BATCH][D * kGqaKeys / 16];
-  __shared__ float src_k[kGqaKeys];
+  constexpr int CH = D / 16, ROWS = 256 / CH, STEPS = kGqaKeys / ROWS, DIMS = D / 4;
   __shared__ int src_page[kGqaKeys], src_row[kGqaKeys];
+  __shared__ float src_k[kGqaKeys], src_v[kGqaKeys];
   __shared__ float amax_w[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x % A.kv_heads, slot = blockIdx.x / A.kv_heads, b = slot / A.kept_pages, pg = slot % A.kept_pages;
   const int to = A.kept_table[static_cast<int64_t>(b) * A.kept_pages + pg];
   if (to < 0 || to >= A.n_pages) return;
   const int32_t* list = A.slots + ((static_cast<int64_t>(b) * A.kv_heads + h) * A.kept_pages + pg) * kGqaKeys;
-  const int pos = list[lane];  // (each wave for itself: lane = key)
-  const int kept = __popcll(__ballot(pos >= 0));
-  if (kept == 0) return;
-  const int page = pos >= 0 ? A.table[static_cast<int64_t>(b) * A.max_pages + (pos >> 6)] : -1;
-  auto block = [&](int p) { return gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, p, h); };
-  // the distinct pages: those of the lanes in `heads`, in order; this lane's is the mine-th
-  const int before = __shfl_up(pos >> 6, 1);
-  const uint64_t heads = __ballot(pos >= 0 && (lane == 0 || before != pos >> 6));
-  const int mine = __popcll(heads & (2ull << lane) - 1) - 1, pages = __popcll(heads);
-  float sk = 0.f, sv = 0.f;
-  if (pos >= 0) {
-    const float* s = block(page).scale;
-    sk = gqa_scale_ok(s[0]) ? s[0] : __builtin_nanf("");
-    sv = gqa_scale_ok(s[1]) ? s[1] : __builtin_nanf("");
-    if (wave == 0) A.weights[(static_cast<int64_t>(to) * A.kv_heads + h) * kGqaKeys + lane] = A.weights[(static_cast<int64_t>(page) * A.kv_heads + h) * kGqaKeys + (pos & 63)];
-  }
-  if (wave == 0) {
-    src_page[lane] = page;
-    src_row[lane] = pos & 63;
-    src_k[lane] = sk;
+  if (list[0] < 0) return;
+  if (tid < kGqaKeys) {
+    const int pos = list[tid];
+    int page = -1;
+    float sk = 0.f, sv = 0.f;
+    if (pos >= 0) {
+      page = A.table[static_cast<int64_t>(b) * A.max_pages + (pos >> 6)];
+      const GqaBlock s = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h);
+      sk = gqa_scale_ok(s.scale[0]) ? s.scale[0] : __builtin_nanf("");
+      sv = gqa_scale_ok(s.scale[1]) ? s.scale[1] : __builtin_nanf("");
+      A.weights[(static_cast<int64_t>(to) * A.kv_heads + h) * kGqaKeys + tid] = A.weights[(static_cast<int64_t>(page) * A.kv_heads + h) * kGqaKeys + (pos & 63)];
+    }
+    src_page[tid] = page;
+    src_row[tid] = pos & 63;
+    src_k[tid] = sk;
+    src_v[tid] = sv;
   }
   __syncthreads();
   u32x4g kc[STEPS];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int row = i * ROWS + tid / CH;
-    kc[i] = u32x4g{0, 0, 0, 0};
-    if (row < kept) kc[i] = reinterpret_cast<const u32x4g*>(block(src_page[row]).k + src_row[row] * D)[tid % CH];
-  }
-  // values: lane = key, a wave a quarter of the dims
-  uint32_t vc[DIMS / 4];
-#pragma unroll
-  for (int i = 0; i < DIMS / 4; ++i) vc[i] = 0;
-  u32x4g next[BATCH][BLK];
-  uint64_t left = heads;
-  auto fetch = [&]() __attribute__((always_inline)) {  // the next four blocks (the last one again where there are fewer)
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int at = left ? __builtin_ctzll(left) : 63 - __builtin_clzll(heads);
-      left &= left - 1;
-      const u32x4g* from = reinterpret_cast<const u32x4g*>(block(__builtin_amdgcn_readlane(page, at)).v);
-#pragma unroll
-      for (int j = 0; j < BLK; ++j) next[i][j] = __builtin_nontemporal_load(from + j * 256 + tid);
-    }
-  };
-  fetch();
-  for (int first = 0; first < pages; first += BATCH) {
-    if (first) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-#pragma unroll
-      for (int j = 0; j < BLK; ++j) blocks[i][j * 256 + tid] = next[i][j];
-    __syncthreads();
-    if (first + BATCH < pages) fetch();
-    const int in = mine - first;
-    if (pos >= 0 && in >= 0 && in < BATCH) {
-      const uint8_t* from = reinterpret_cast<const uint8_t*>(blocks[in]) + wave * DIMS * kGqaKeys + (pos & 63);
-#pragma unroll
-      for (int i = 0; i < DIMS / 4; ++i)
-        vc[i] = from[(4 * i) * kGqaKeys] | from[(4 * i + 1) * kGqaKeys] << 8 | from[(4 * i + 2) * kGqaKeys] << 16 |
-                static_cast<uint32_t>(from[(4 * i + 3) * kGqaKeys]) << 24;
-    }
-  }
-  auto largest = [&](uint32_t x) {
-    const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), c = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
-    return fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1])));
-  };
   float amax_k = 0.f, amax_v = 0.f;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const float s = src_k[i * ROWS + tid / CH];
+    const int row = i * ROWS + tid / CH, page = src_page[row];
+    kc[i] = u32x4g{0, 0, 0, 0};
+    if (page >= 0) {
+      kc[i] = reinterpret_cast<const u32x4g*>(gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h).k + src_row[row] * D)[tid % CH];
+      const float s = src_k[row];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) amax_k = fmaxf(amax_k, largest(kc[i][j]) * s);
+      for (int j = 0; j < 4; ++j) {
+        const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(kc[i][j], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(kc[i][j], true);
+        amax_k = fmaxf(amax_k, fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1]))) * s);
+      }
+    }
   }
+  // values: lane = key, a wave a quarter of the dims
+  uint32_t vc[DIMS / 4];
+  const int vpage = src_page[lane];
+  const float sv = src_v[lane];
+  if (vpage >= 0) {
+    const uint8_t* from = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, vpage, h).v + wave * DIMS * kGqaKeys + src_row[lane];
 #pragma unroll
-  for (int i = 0; i < DIMS / 4; ++i) amax_v = fmaxf(amax_v, largest(vc[i]) * sv);
+    for (int i = 0; i < DIMS / 4; ++i)
+      vc[i] = from[(4 * i) * kGqaKeys] | from[(4 * i + 1) * kGqaKeys] << 8 | from[(4 * i + 2) * kGqaKeys] << 16 |
+              static_cast<uint32_t>(from[(4 * i + 3) * kGqaKeys]) << 24;
+#pragma unroll
+    for (int i = 0; i < DIMS / 4; ++i) {
+      const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(vc[i], false), c = __builtin_amdgcn_cvt_pk_f32_fp8(vc[i], true);
+      amax_v = fmaxf(amax_v, fmaxf(fmaxf(__builtin_fabsf(a[0]), __builtin_fabsf(a[1])), fmaxf(__builtin_fabsf(c[0]), __builtin_fabsf(c[1]))) * sv);
+    }
+  }
   amax_k = wave_max_f32(amax_k);
   amax_v = wave_max_f32(amax_v);
   if (lane == 0) {
     amax_w[0][wave] = amax_k;
     amax_w[1][wave] = amax_v;
   }
-  __syncthreads();  // (and the blocks are read)
+  __syncthreads();
   const float s_k = gqa_scale(fmaxf(fmaxf(amax_w[0][0], amax_w[0][1]), fmaxf(amax_w[0][2], amax_w[0][3])));
   const float s_v = gqa_scale(fmaxf(fmaxf(amax_w[1][0], amax_w[1][1]), fmaxf(amax_w[1][2], amax_w[1][3])));
-  const GqaBlock dst = block(to);
+  const GqaBlock dst = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, to, h);
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int row = i * ROWS + tid / CH;
+    if (src_page[row] < 0) continue;
     const float ratio = src_k[row] / s_k;
 #pragma unroll
     for (int j = 0; j < 4; ++j) kc[i][j] = gqa_rescale4(kc[i][j], ratio);
-    if (row < kept) reinterpret_cast<u32x4g*>(dst.k + row * D)[tid % CH] = kc[i];
+    reinterpret_cast<u32x4g*>(dst.k + row * D)[tid % CH] = kc[i];
   }
-  const float ratio = sv / s_v;
-  uint8_t* out = reinterpret_cast<uint8_t*>(blocks[0]);
+  if (vpage >= 0) {
+    const float ratio = sv / s_v;
+    uint8_t* into = dst.v + wave * DIMS * kGqaKeys + lane;
 #pragma unroll
-  for (int i = 0; i < DIMS / 4; ++i) {
-    const uint32_t x = gqa_rescale4(vc[i], ratio);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[(wave * DIMS + 4 * i + j) * kGqaKeys + lane] = static_cast<uint8_t>(x >> (8 * j));
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < BLK; ++j) {
-    const int at = j * 256 + tid, key0 = at % 4 * 16;
-    if (key0 + 16 <= kept) reinterpret_cast<u32x4g*>(dst.v)[at] = blocks[0][at];
-    else
-      for (int i = 0; key0 + i < kept; ++i) dst.v[at * 16 + i] = out[at * 16 + i];
+    for (int i = 0; i < DIMS / 4; ++i) {
+      const uint32_t x = gqa_rescale4(vc[i], ratio);
+      into[(4 * i) * kGqaKeys] = static_cast<uint8_t>(x);
+      into[(4 * i + 1) * kGqaKeys] = static_cast<uint8_t>(x >> 8);
+      into[(4 * i + 2) * kGqaKeys] = static_cast<uint8_t>(x >> 16);
+      into[(4 * i + 3) * kGqaKeys] = static_cast<uint8_t>(x >> 24);
+    }
   }
   if (tid == 0) {
     dst.scale[0] = s_k;

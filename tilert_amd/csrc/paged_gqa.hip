@@ -317,7 +317,7 @@ __device__ inline float2 load_scales(const float* s) { return float2{load_f32_ve
 // 131072 keys 76 us, 59 so).  Weights go into the second product as hi + lo in bf16, 16 bits of them.
 // Weights are relative to 2^24 times the row's largest: their sums of values then stay inside fp32 whatever the values.
 // Bound by bytes, two pages a wave on their way: 60 sequences of 2048 to 32768 keys, 1.42 GB, 238 us, 6.0 TB/s; 131072 keys, 268 MB,
-// 51 us and 8 to join, where a copy's rate takes 52.
+// 55 us and 6 to join, where a copy's rate takes 52.
 constexpr float kGqaHead = 24.f;
 template <int D, int RT>
 __global__ __launch_bounds__(256, D * RT > 128 ? 1 : 2) void gqa_attend_kernel(const GqaArgs A) {
@@ -550,7 +550,8 @@ __global__ __launch_bounds__(256, D * RT > 128 ? 1 : 2) void gqa_attend_kernel(c
 //
 // The two waves of a SIMD are a third of a page apart: between two barriers waves 0 .. 3 make scores, weights and sums of page k,
 // waves 4 .. 7 weights and sums of page k - 1 and scores of page k, so that one's products run while the other makes
-// weights.  (At the same place of the page, 532 us for 2048 tokens over 16384 keys.)  Values are multiplied up to a page
+// weights.  (At the same place of the page, 532 us for 2048 tokens over 16384 keys, 482 so: 1.07 PFLOP/s, the matrix pipe busy
+// 53 % of the cycles at 2.15 GHz; bound by the issue of vector instructions beside it.)  Values are multiplied up to a page
 // later than keys, so they have three buffers and keys two.
 constexpr float kGqaLag = 8.f;
 constexpr int kChunkWaves = 8, kChunkRows = 32 * kChunkWaves;
@@ -863,7 +864,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void gqa_chunk_kernel(const Gq
 }
 
 // The parts of cut tiles joined in a fixed order, 16 rows of a tile at a time.  DEEP: a workgroup takes 16 dims of them, its eight
-// waves every eighth part, joined in LDS (few tiles of many parts); else its waves take 16 dims each.
+// waves every eighth part, joined in LDS (few tiles of many parts); else its waves take 16 dims each.  Bound by latency: 8 tiles of
+// 32 parts, 8 MB in all, 5.9 us.
 constexpr int kJoinWaves = 8;
 template <int D, int BM, bool DEEP>
 __global__ __launch_bounds__(64 * kJoinWaves) void gqa_join_kernel(const GqaArgs A) {
@@ -980,7 +982,7 @@ struct GqaUnit {
 // Few rows (a decode step): a wave takes every fourth page of a piece, one behind another, the next two's keys on their way;
 // their rows, RT tiles of 16 as a rule, stay in registers (more of them are loaded page by page).  Scores as in the
 // attention's first product, S^T = K Q^T: a lane sums its keys' weights over its column of rows.  Bound by bytes: 60
-// sequences of 2048 to 32768 keys, 730 MB, 153 us, 4.8 TB/s.  Pieces as the attention plans them (in groups of kSumPages
+// sequences of 2048 to 32768 keys, 730 MB, 157 us, 4.6 TB/s.  Pieces as the attention plans them (in groups of kSumPages
 // pages by the table's width they took 170 us).  Two tiles against the kernel for many rows below: 4 tokens of 8 heads over
 // 131072 keys 44 / 59 us, over 8192 keys of 40 sequences 90 / 147; four tiles, 8 tokens, 75 / 66.
 constexpr int kSumPages = 32;  // pages of a piece where nothing is planned
@@ -1101,7 +1103,7 @@ __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A)
 // Many rows: eight waves share PW pages of a head, each with a page's keys in registers as bf16, and 8 / PW tiles of 32 rows a
 // step, which go through LDS as the product's operand (32 x 32 scores an instruction).  Waves of the same page are added
 // at the end, in a fixed order.  Bound by vector instructions: a score takes a multiply-add, an exponential and a sum,
-// 21 cycles a wave of 64 lanes, and 8 of the matrix pipe's.
+// 21 cycles a wave of 64 lanes, and 8 of the matrix pipe's: 2048 tokens over 16384 keys, 32 heads over 8 of 128 dims, 272 us.
 constexpr int kSumWaves = 8;
 template <int D, int PW>
 struct GqaSumLds {
