@@ -50,6 +50,8 @@
  *   tl_mla_cache_write     rmsnorm_kv_op, the key half of qkv_rope_op  .../ops/rmsnorm_kv.py:20-43, qkv_rope.py:42-50
  *   tl_mla_cache_read      the cache's bf16 form (MlaNsaProfile.convert)  pd_vllm/profiles/mla_nsa.py:150-185
  *   tl_flash_paged_mla     the dense form of flash_sparse_mla_op over those pages
+ *   tl_gqa_cache_write, tl_flash_paged_gqa, tl_gqa_cache_weights, tl_gqa_cache_evict
+ *                          no counterpart: a paged cache of grouped-query heads
  *   tl_add_rmsnorm_quant   rmsnorm_quant_op behind a residual sum  tilert/models/common.py:92-133
  *   tl_topk_rows           topk_accurate_op               .../ops/topk.py:62-109
  *   tl_indexer_fp8_topk    sparse_index_topk_dsv32_op (fp8 cache)  .../ops/sparse_index.py:72-128
