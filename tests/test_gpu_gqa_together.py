@@ -386,6 +386,27 @@ def test_evictions_in_the_widest_table(cuda):
     check_evict(*args, 2, 128, 40, *evict(cuda, *args, 2, 128, 40))
 
 
+def test_an_eviction_that_updates_keep_lens_in_place(cuda):
+    args = evict_case([900, 300, 64], [400, 500, 64], 4, 64, 111)
+    pages, w, table, lens, keep, to = (t.to(cuda) for t in args)
+    slots = torch.zeros(3, 4, 64 * to.shape[1], dtype=I32, device=cuda)
+    gqa_cache_evict(pages, w, table, lens, keep, to, keep, slots, head_dim=64, recent=7)
+    assert keep.tolist() == [400, 300, 64]
+    check_evict(*args, 4, 64, 7, pages.cpu(), w.cpu(), keep.cpu(), slots.cpu())
+
+
+def test_rows_turned_in_place(cuda):
+    """query_out may be the queries' own memory: a row's lanes have read it all before one of them writes."""
+    joint, gq, gk, freqs = inputs(150, 8, 2, 128, 128, 113)
+    pages, table, cu, lens, _ = _gqa.batch([150], [200], 2, 128, seed=115)
+    q, k, v = (t.contiguous() for t in split(joint.to(cuda), 8, 2))
+    args = _gqa.to(cuda, table, cu, lens, gk, freqs)
+    want, out = torch.zeros_like(q), [pages.to(cuda), pages.to(cuda)]
+    gqa_cache_write(k, v, out[0], *args, query=q, gamma_q=gq.to(cuda), query_out=want)
+    gqa_cache_write(k, v, out[1], *args, query=q, gamma_q=gq.to(cuda), query_out=q)
+    assert torch.equal(q, want) and torch.equal(out[0], out[1])
+
+
 def test_weights_and_angles_that_are_aligned_to_their_elements_only(cuda):
     args = evict_case([900], [400], 2, 64, 105)
     want = evict(cuda, *args, 2, 64, 30)

@@ -251,3 +251,9 @@ def test_the_oracle_reads_what_the_page_layout_says():
                                         (3.3895e38, 2.0 ** 120), (1e-4, 2.0 ** -22)])
 def test_the_least_scale(amax, scale):
     assert gqa.scale_of(amax) == scale and max(amax, 1e-4) <= 448 * scale
+
+
+@pytest.mark.parametrize("off", [0, 4, -4])
+def test_eviction_refuses_new_lengths_in_the_old_ones_place(off):
+    """A head's workgroup may still read a length when another one's has written the new one."""
+    _refused("tl_gqa_cache_evict", _evict_c(n_seqs=2, lens=P, kept=P + off), 1, "kept_lens")

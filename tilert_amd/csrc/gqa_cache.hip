@@ -632,6 +632,12 @@ extern "C" int tl_gqa_cache_evict(void* kv_pages, float* key_weights, int64_t n_
     set_error("%s: %lld sequences of %lld kept pages: more than a launch has room for", who, (long long)n_seqs, (long long)kept_pages);
     return kErrUnsupported;
   }
+  // (a head's workgroup may read its sequence's length when another's has written the new one)
+  const uintptr_t from = reinterpret_cast<uintptr_t>(seq_lens), to = reinterpret_cast<uintptr_t>(kept_lens);
+  if ((from < to ? to - from : from - to) < static_cast<uintptr_t>(n_seqs) * 4) {
+    set_error("%s: kept_lens must not be the memory of seq_lens", who);
+    return kErrArg;
+  }
   const GqaEvictArgs args{(uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim), key_weights, block_table, seq_lens, keep_lens,
                           (int)n_pages, (int)max_pages, (int)kv_heads, (int)recent, kept_table, (int)kept_pages, kept_lens, kept_slots};
   hipLaunchKernelGGL(gqa_select_kernel, dim3(n_seqs * kv_heads), dim3(kSelThreads), 0, (hipStream_t)stream, args);

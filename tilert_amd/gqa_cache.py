@@ -95,7 +95,7 @@ def gqa_cache_write(key: torch.Tensor, value: torch.Tensor, kv_pages: torch.Tens
     Keys and values are quantised by page and head, with the least power of two that holds the block's new rows; a block with
     older keys keeps a larger scale, or moves their codes to the larger new one.  A key that holds a NaN or an infinity,
     in its key or its value row, is NaN to the rows that see it and touches nothing else.  ``key_weights`` (fp32 [n_pages,
-    kv_heads, 64]) is set to 0 for the keys written.  Sequences must not share the pages that are written to."""
+    kv_heads, 64]) is set to 0 for the keys written.  A page that is written to belongs to one place of one sequence."""
     name = "gqa_cache_write"
     key_stride = _check_rows(name, "key", key)
     tokens, kv_heads, head_dim = key.shape
@@ -163,10 +163,10 @@ def gqa_cache_evict(kv_pages: torch.Tensor, key_weights: torch.Tensor, block_tab
     """Bring each sequence down to its keep_lens[b] keys, for each kv head on its own: the last ``recent`` positions stay, and
     of the others those of the largest ``key_weights`` (equal ones: the lowest position; NaN counts as the largest).  They
     go in ascending order, codes, scales and weights, into the pages of ``kept_table`` (int32 [sequences, pages], of the
-    same pool); the sequences' own pages are left as they are, and may be given back afterwards.  ``kept_lens`` (int32 [sequences])
-    receives the new lengths -- keep_lens, but no more than there are keys or kept_table has room for -- and ``kept_slots``
-    (int32 [sequences, kv_heads, 64 * pages]) the positions that were kept, -1 behind them.  No page of kept_table may be
-    one of the tables'; one outside the pool is not written."""
+    same pool); the sequences' own pages are left as they are, and may be given back afterwards.  ``kept_lens`` (int32
+    [sequences], not seq_lens itself; keep_lens may be it) receives the new lengths -- keep_lens, but no more than there are keys
+    or kept_table has room for -- and ``kept_slots`` (int32 [sequences, kv_heads, 64 * pages]) the positions that were kept,
+    -1 behind them.  kept_table names a page once, and none of the tables'; one outside the pool is not written."""
     name = "gqa_cache_evict"
     kv_heads = key_weights.shape[1] if key_weights.dim() == 3 else 0
     n_pages = _check_pages(name, kv_pages, kv_heads, head_dim)
