@@ -62,12 +62,12 @@ struct Angles {
   float x[8], y[8];
 };
 __device__ inline Angles load_angles(const float* freqs, int part, int rope, int interleaved) {
-  Angles r;
-  const bool turned = part * 8 < rope;
+  Angles r = {};
+  if (part * 8 >= rope) return r;
   if (interleaved) {
-    load8(freqs + (turned ? part * 8 : 0), r.x);
+    load8(freqs + part * 8, r.x);
   } else {
-    const int half = rope / 16, pair = turned ? (part >= half ? part - half : part) : 0;
+    const int half = rope / 16, pair = part >= half ? part - half : part;
     load8(freqs + pair * 16, r.x);
     load8(freqs + pair * 16 + 8, r.y);
   }
@@ -83,7 +83,9 @@ __device__ inline void norm_rope(float (&x)[8], int part, bool norm, const float
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-    const float r = 1.0f / __builtin_sqrtf(row_sum<LANES>(ss) / D + eps);
+    const float mean = row_sum<LANES>(ss) * (1.0f / D) + eps;
+    float r = __builtin_amdgcn_rsqf(mean);  // (within 2^-23; it takes a subnormal for 0)
+    if (mean < 0x1p-126f) r = 1.0f / __builtin_sqrtf(mean);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * r * gamma[i];
   }
@@ -101,18 +103,20 @@ __device__ inline void norm_rope(float (&x)[8], int part, bool norm, const float
   }
   const int half = rope / 16;  // lanes of half the turned dims
   const bool upper = part >= half;
-  const int lane = threadIdx.x & 63, from = turned ? lane + (upper ? -half : half) : lane;
+  const int lane = threadIdx.x & 63, from = 4 * (turned ? lane + (upper ? -half : half) : lane);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float other = __shfl(x[i], from);
+    const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(x[i])));
     const float c = i < 4 ? w.x[2 * i] : w.y[2 * i - 8], s = i < 4 ? w.x[2 * i + 1] : w.y[2 * i - 7];
-    if (turned) x[i] = upper ? other * s + x[i] * c : x[i] * c - other * s;
+    const float y = x[i] * c + other * (upper ? s : -s);
+    x[i] = turned ? y : x[i];
   }
 }
 
 // A workgroup takes one page of a sequence's new keys and one kv head (its scales need all of the block's rows), or, behind
 // those, 64 query rows; 8 or 16 lanes a row, 16 bytes each.  Values are transposed through LDS.  Bound by bytes and the loads'
-// latency, as a workgroup's work is one round of them: 4000 tokens, 32 heads over 8 of 128 dims, 92 MB, 27 us, 3.4 TB/s.
+// latency, as a workgroup's work is one round of them: 4000 tokens, 32 heads over 8 of 128 dims, 92 MB, 25 us, 3.7 TB/s,
+// vector instructions busy for 60 % of it (27 us with angles loaded row by row and for dims that are not turned).
 template <int D>
 __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES, STEPS = kGqaKeys / ROWS;
@@ -133,12 +137,15 @@ __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
     if (row0 >= end) return;
     u32x4g raw[STEPS];
     Angles w[STEPS];
+    int before = -1;  // (heads of one token have its angles in common)
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int64_t row = row0 + i * ROWS + sub, r = row < end ? row : end - 1;
       const int t = static_cast<int>(static_cast<uint64_t>(r) * A.per_heads >> 34), h = static_cast<int>(r - static_cast<int64_t>(t) * A.heads);
       raw[i] = *reinterpret_cast<const u32x4g*>(A.q + t * A.q_stride + h * D + part * 8);
-      w[i] = angles(t);
+      if (i > 0 && __all(t == before)) w[i] = w[i - 1];
+      else w[i] = angles(t);
+      before = t;
     }
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -183,7 +190,7 @@ __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
     float bad = 0.f, mk = 0.f, mv = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      bad = __builtin_fabsf(y[i][j]) < INFINITY && __builtin_fabsf(z[i][j]) < INFINITY ? bad : 1.f;
+      bad = __builtin_fmaf(z[i][j], 0.f, __builtin_fmaf(y[i][j], 0.f, bad));  // (NaN where one is not finite)
       mk = fmaxf(mk, __builtin_fabsf(y[i][j]));
       mv = fmaxf(mv, __builtin_fabsf(z[i][j]));
     }
