@@ -984,9 +984,8 @@ struct GqaUnit {
 // attention's first product, S^T = K Q^T: a lane sums its keys' weights over its column of rows.  Bound by bytes: 60
 // sequences of 2048 to 32768 keys, 730 MB, 157 us, 4.6 TB/s.  Pieces as the attention plans them (in groups of kSumPages
 // pages by the table's width they took 170 us).  Two tiles against the kernel for many rows below: 4 tokens of 8 heads over
-// 131072 keys 44 / 59 us, over 8192 keys of 40 sequences 90 / 147; four tiles, 8 tokens, 75 / 66.
+// 131072 keys 34 / 59 us, over 8192 keys of 40 sequences 90 / 147; four tiles, 8 tokens, 75 / 66.
 constexpr int kSumPages = 32;  // pages of a piece where nothing is planned
-constexpr int kSumTarget = 1536;
 template <int D, int RT>
 __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A) {
   __shared__ GqaPlanLds plan;
@@ -1364,9 +1363,15 @@ extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const 
   if (!lse || !key_weights) { set_error("%s: null pointer", who); return kErrArg; }
   const int64_t each = cdiv(n_tokens * (heads / kv_heads), n_seqs);
   const bool few = each <= 32;
-  int pw = 8;  // pages a workgroup: as many as leave a workgroup for every CU
-  while (pw > 1 && cdiv(max_pages, pw) * kv_heads * n_seqs < 256) pw /= 2;
-  const int64_t target = few && n_seqs <= kGqaPlanSeqs ? kSumTarget : 0;
+  // Pages a workgroup: as many as leave most CUs one, by the table's width, which of many sequences fewer fill.  In us with 1, 2, 4
+  // and 8: 32 tokens of 2 sequences of 1500 keys, 8 heads of 128 dims, 19 11 12 17; 2048 of 1 of 16384 928 709 575 528; 1000 of 1
+  // of 1000 63 93 152 264; 9 to 300 of 16 of 125 to 2000 98 68 72 91.
+  int pw = 8;
+  while (pw > 1 && cdiv(max_pages, pw) * kv_heads * n_seqs < std::min<int64_t>(128 + 32 * n_seqs, 768)) pw /= 2;
+  // Pieces that few rows' pages are cut into: as many as run at once, or, where more than a few tiles may be of unlike
+  // lengths, more.  In us with 512 / 1536: 1 sequence of 131072 keys 30 / 39, 8 of 4096 15 / 17, 16 of 1024 to 16384 33 / 38; 60 of 2048 to
+  // 32768 183 / 161, with 4 heads of 64 dims 56 / 50.
+  const int64_t target = few && n_seqs <= kGqaPlanSeqs ? (n_seqs * kv_heads <= 128 ? 512 : 1536) : 0;
   const int64_t groups = cdiv(max_pages, few ? kSumPages : pw), units = target ? target + n_seqs * kv_heads : n_seqs * groups * kv_heads;
   const GqaSumArgs args{(const uint16_t*)q_bf16, q_stride, lse, (const uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
                         PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
