@@ -497,3 +497,45 @@ def test_metadata_that_does_not_make_sense_stays_inside(cuda, seed):
         for t, value in ((out[0], 7), (lse[0], 7), (query[0], 7), (w[0], 7), (kept[0], 7), (slots[0], 7), (pool, 0x55)):
             assert torch.all(t[:4] == value) and torch.all(t[-4:] == value)
     check(cuda, good[0], pages, table, cu, lens, kv, *_attend(good, kv))
+
+
+@pytest.mark.parametrize("what", ["key", "value", "key scale", "value scale"])
+@pytest.mark.parametrize("new,dim,back", [(3, 128, 1), (4, 64, 2), (7, 128, 3), (8, 64, 5), (15, 64, 6), (16, 64, 1)])
+def test_a_bad_key_among_few_rows(cuda, what, new, dim, back):
+    """Tiles of 16, 32 and 64 rows: the tokens before a key that is NaN are as without it, bit for bit, also where they share its
+    page, and those from it on are NaN where the definition is; so are the weights that it gathers."""
+    total = 700
+    pages, table, cu, lens, rows = _gqa.batch([new], [total], 2, dim, seed=117)
+    _gqa.fill(pages, table, [total], 2, dim)
+    q = _gqa.queries(rows, 8, dim, 119)
+    clean, clean_lse = _attend(_gqa.to(cuda, q, pages, table, cu, lens), 2)
+    at = total - back
+    page, row, first = int(table[0, at // 64]), at % 64, at - (total - new)
+    k, v, scales = gqa.views(pages, 2, dim)
+    if what == "key":
+        k[page, 1, row, dim - 3] = 0xff
+    elif what == "value":
+        v[page, 1, dim - 5, row] = 0x7f
+    else:
+        scales[page, 1, 0 if what == "key scale" else 1] = math.nan
+        first = max(first - row, 0)
+    case = _gqa.to(cuda, q, pages, table, cu, lens)
+    out, lse = _attend(case, 2)
+    assert torch.equal(out[:first], clean[:first]) and torch.equal(lse[:first], clean_lse[:first])
+    assert torch.equal(out[:, :4], clean[:, :4])  # the other kv head
+    check(cuda, q, pages, table, cu, lens, 2, out, lse)
+    assert torch.isnan(out[first:, 4:, dim - 5]).all()
+    if what != "value":
+        w = _sums(case, clean_lse, 2)
+        check_sums(cuda, q, clean_lse, pages, table, cu, lens, 2, torch.zeros(w.shape), w, True)
+
+
+@pytest.mark.parametrize("new,total,heads,kv,dim", [([3], [70], 128, 128, 64), ([40, 1], [90, 200], 128, 128, 128), ([2], [300], 126, 63, 64),
+                                                    ([9], [100], 128, 16, 128), ([5, 2], [400, 30], 100, 20, 64)])
+def test_up_to_128_heads(cuda, new, total, heads, kv, dim):
+    pages, table, cu, lens, rows = _gqa.batch(new, total, kv, dim, seed=121)
+    _gqa.fill(pages, table, total, kv, dim)
+    case = _gqa.to(cuda, _gqa.queries(rows, heads, dim, 123), pages, table, cu, lens)
+    out, lse = _attend(case, kv)
+    check(cuda, case[0], pages, table, cu, lens, kv, out, lse)
+    check_sums(cuda, case[0], lse, pages, table, cu, lens, kv, torch.zeros(pages.shape[0], kv, 64), _sums(case, lse, kv), True)

@@ -1032,9 +1032,9 @@ __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A)
     };
     rows(0);
     int pg = pg0;
-    auto page = [&](const GqaKeys<D>& kc, float sk, bool is, int id) __attribute__((always_inline)) {
-      const bool ok = gqa_scale_ok(sk);
-      const float by = ok ? sk : 1.f, scale = ok ? A.scale : __builtin_nanf("");
+    auto page = [&](const GqaKeys<D>& kc, float2 scales, bool is, int id) __attribute__((always_inline)) {
+      const bool ok = gqa_scale_ok(scales.x) && gqa_scale_ok(scales.y);
+      const float by = ok ? scales.x : 1.f, scale = ok ? A.scale : __builtin_nanf("");
       const int key0 = pg * kGqaKeys;
       float w[4][4] = {};
       for (int row0 = 0; row0 < s.rows; row0 += 16 * RT) {
@@ -1078,15 +1078,15 @@ __global__ __launch_bounds__(256, 2) void gqa_sum_few_kernel(const GqaSumArgs A)
     // Two pages' keys on their way behind the one at work, 128 KB a CU.  (Three buffers by turns: one copied into another would
     // wait for its loads.)
     GqaKeys<D> k0, k1, k2;
-    float s0, s1, s2;
+    float2 s0, s1, s2;
     int id = page_id(pg), id1 = page_id(pg + 4), id2 = page_id(pg + 8);
     k0 = load_keys<D>(block(id).k, lane);
-    s0 = load_f32_vector(block(id).scale);
+    s0 = load_scales(block(id).scale);
     k1 = load_keys<D>(block(id1).k, lane);
-    s1 = load_f32_vector(block(id1).scale);
-    auto turn = [&](const GqaKeys<D>& now, float s_now, GqaKeys<D>& then, float& s_then) __attribute__((always_inline)) {
+    s1 = load_scales(block(id1).scale);
+    auto turn = [&](const GqaKeys<D>& now, float2 s_now, GqaKeys<D>& then, float2& s_then) __attribute__((always_inline)) {
       then = load_keys<D>(block(id2).k, lane);
-      s_then = load_f32_vector(block(id2).scale);
+      s_then = load_scales(block(id2).scale);
       page(now, s_now, there(id), id);
       id = id1;
       id1 = id2;
@@ -1129,7 +1129,7 @@ __global__ __launch_bounds__(64 * kSumWaves, 2) void gqa_sum_kernel(const GqaSum
     if (key0 < n_keys) id = __builtin_amdgcn_readfirstlane(A.p.table[static_cast<int64_t>(unit.b) * A.p.max_pages + pg]);
     const bool there = id >= 0 && id < A.p.n_pages;
     const GqaBlock blk = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, there ? id : 0, unit.head);
-    const bool ok = gqa_scale_ok(blk.scale[0]);
+    const bool ok = gqa_scale_ok(blk.scale[0]) && gqa_scale_ok(blk.scale[1]);
     const float sk = ok ? blk.scale[0] : 1.f, scale = ok ? A.scale : __builtin_nanf("");
     // keys: fragment f of tile t, row c of it the key 32 (c / 4 % 2) + 16 t + 4 (c / 8) + c % 4, dims 64 i + 32 j + 16 h + 8 e .. + 7
     // for f = 4 i + 2 j + e; the queries' fragments are the same
