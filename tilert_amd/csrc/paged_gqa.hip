@@ -320,7 +320,7 @@ __device__ inline float2 load_scales(const float* s) { return float2{load_f32_ve
 // 55 us and 6 to join, where a copy's rate takes 52.
 constexpr float kGqaHead = 24.f;
 template <int D, int RT>
-__global__ __launch_bounds__(256, D * RT > 128 ? 1 : 2) void gqa_attend_kernel(const GqaArgs A) {
+__global__ __launch_bounds__(256, D == 128 && RT > 1 ? 1 : 2) void gqa_attend_kernel(const GqaArgs A) {
   constexpr int BM = 16 * RT, DT = D / 16, KI = D / 64, TW = RT < 2 ? 1 : 2, RG = RT / TW, PW = 4 / RG;  // TW: row tiles of a wave; PW: waves that share their pages
   __shared__ union {
     GqaPlanLds plan;
@@ -1375,7 +1375,8 @@ extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const 
   const int64_t groups = cdiv(max_pages, few ? kSumPages : pw), units = target ? target + n_seqs * kv_heads : n_seqs * groups * kv_heads;
   const GqaSumArgs args{(const uint16_t*)q_bf16, q_stride, lse, (const uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim),
                         PagedBatch{block_table, cu_seqlens, seq_lens, (int)n_seqs, (int)max_pages, (int)n_pages, (int)n_tokens},
-                        (int)heads, (int)kv_heads, (int)(heads / kv_heads), accumulate, softmax_scale * kLog2e, key_weights, (int)target, units, (int)groups, ((1ull << 34) + heads / kv_heads - 1) / (heads / kv_heads)};
+                        (int)heads, (int)kv_heads, (int)(heads / kv_heads), accumulate, softmax_scale * kLog2e, key_weights, (int)target, units, (int)groups,
+                        ((1ull << 34) + heads / kv_heads - 1) / (heads / kv_heads)};
   const dim3 grid(target || units < (1 << 16) ? units : (1 << 16));  // (a workgroup goes on with another unit)
   const hipStream_t st = (hipStream_t)stream;
   if (few) {
