@@ -750,8 +750,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void gqa_chunk_kernel(const Gq
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, x[t][j]);
     top *= A.scale;
-    if (__any(top > m + kGqaLag)) {
-      const float now = fmaxf(m, two_halves<true>(top));
+    if (__any(top > m + kGqaLag)) {  // (row by row: one that stays is multiplied by 1, and owes nothing to its neighbours)
+      const float high = two_halves<true>(top), now = high > m + kGqaLag ? high : m;
       const float by = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= by;
