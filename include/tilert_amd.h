@@ -510,7 +510,8 @@ int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const voi
  * head_dim] (q_bf16 null: none).  A block's scale (one page, one head) is the least power of two
  * with max(amax, 1e-4) <= 448 scale over its new rows; where the page holds older keys of the
  * sequence in front of them and their scale is larger, it stays, and where it is smaller their
- * codes move to the new one, rounded where they become subnormal.  A key whose key or value row
+ * codes move to the new one, rounded where they become subnormal; where one of the block's two
+ * scales is none, the older keys stay NaN, in their codes.  A key whose key or value row
  * holds a NaN or an infinity gets NaN key codes and value codes 0 and does not count for the
  * scales.  key_weights fp32 [n_pages, kv_heads, 64] (nullable): those of the written keys become
  * 0.  Sequences must not share pages that are written to. */

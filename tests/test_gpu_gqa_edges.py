@@ -1,13 +1,16 @@
 """The paged per-head cache's operators where rows, blocks and sizes meet their ends."""
+import math
+
 import pytest
 import torch
 
 from oracle import gqa
 from tests import _gqa
 from tests.test_gpu_flash_paged_gqa import check, run
+from tilert_amd.gqa_cache import gqa_cache_write
 
 pytestmark = pytest.mark.gpu
-U8 = torch.uint8
+BF16, I32, U8 = torch.bfloat16, torch.int32, torch.uint8
 
 
 @pytest.mark.parametrize("dim", [64, 128])
@@ -32,3 +35,47 @@ def test_a_row_follows_from_what_it_sees_alone(cuda, what, new, total, dim):
     out, lse = run(cuda, q, pages, table, cu, lens, 2)
     assert torch.equal(out[other], clean[other]) and torch.equal(lse[other], clean_lse[other])
     check(cuda, q, pages, table, cu, lens, 2, out, lse)
+
+
+def append(cuda, pages, table, lens, key, value, n):
+    """The pages after a write of key and value behind the first n keys."""
+    p = pages.to(cuda)
+    cu = torch.tensor([0, key.shape[0]], dtype=I32)
+    gqa_cache_write(*_gqa.to(cuda, key, value), p, *_gqa.to(cuda, table, cu, lens))
+    return p.cpu()
+
+
+@pytest.mark.parametrize("side", ["key", "value", "both"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -1.0, 0.0, 2.0 ** -127])
+@pytest.mark.parametrize("old,new,dim,size", [(37, 3, 128, 1.0), (5, 1, 64, 100.0), (62, 2, 64, 0.01), (130, 70, 128, 1.0)])
+def test_older_keys_under_no_scale_stay_nan(cuda, side, bad, old, new, dim, size):
+    """New keys in a page whose older ones are NaN for a scale that is none: those stay NaN, keys and values, and the new ones are the
+    block's only ones for its new scales; the other head's block and other pages are as they were."""
+    pages, table, _, _, _ = _gqa.batch([new], [old + new], 2, dim, seed=141)
+    _gqa.fill(pages, table, [old], 2, dim)
+    lens = torch.tensor([old + new], dtype=I32)
+    g = torch.Generator().manual_seed(143)
+    key, value = ((torch.randn(new, 2, dim, generator=g) * size).to(BF16) for _ in range(2))
+    clean = append(cuda, pages, table, lens, key, value, old)
+    page, r0 = int(table[0, old // 64]), old % 64
+    r1 = min(64, r0 + new)
+    _, _, scales = gqa.views(pages, 2, dim)
+    for i, name in enumerate(("key", "value")):
+        if side in (name, "both"):
+            scales[page, 1, i] = bad
+    after = append(cuda, pages, table, lens, key, value, old)
+    for got, want, x in zip(gqa.views(after, 2, dim), gqa.views(clean, 2, dim), (key, value, None)):
+        same = torch.ones(pages.shape[0], 2, dtype=torch.bool)
+        same[page, 1] = False
+        assert torch.equal(got[same].view(U8), want[same].view(U8))
+        if x is None:
+            continue
+        codes, i = (got[page, 1], 0) if x is key else (got[page, 1].T, 1)
+        s = gqa.views(after, 2, dim)[2][page, 1, i]
+        assert torch.isnan(gqa.value_of(codes[:r0])).all()
+        assert float(s) == gqa.scale_of(float(x[:r1 - r0, 1].float().abs().max()))
+        assert torch.equal(codes[r0:r1], _gqa.codes_of(x[:r1 - r0, 1].float(), s))
+    q, cu = _gqa.queries(new, 4, dim, 145), torch.tensor([0, new], dtype=I32)
+    out, lse = run(cuda, q, after, table, cu, lens, 2)
+    check(cuda, q, after, table, cu, lens, 2, out, lse)
+    assert torch.isnan(out[:, 2:]).all() and torch.isnan(lse[:, 2:]).all() and torch.isfinite(out[:, :2]).all()

@@ -12,7 +12,8 @@ namespace tl {
 //   y = n with its first `rope` dims turned pair by pair by the token's angles (n without)
 // A query row leaves as bf16(y).  Keys and values are quantised by block, the new rows of one page and head:
 //   s = the least power of two with max |y| <= 448 s; a block that holds older keys keeps its scale if it is larger, and
-//   if not its older codes are brought to the new one;  code = e4m3(y / s).
+//   if not its older codes are brought to the new one;  code = e4m3(y / s).  Older keys of a block of which a scale is none
+//   are NaN; they become NaN codes.
 // A key with a NaN or an infinity in its key or value row gets NaN key codes and value codes 0, and does not count for
 // the scales: its scores are NaN for the rows that see it, and nothing reaches a row that does not.
 struct GqaWriteArgs {
@@ -209,31 +210,31 @@ __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {
   __syncthreads();
   float s_k = gqa_scale(fmaxf(fmaxf(amax_w[0][0], amax_w[0][1]), fmaxf(amax_w[0][2], amax_w[0][3])));
   float s_v = gqa_scale(fmaxf(fmaxf(amax_w[1][0], amax_w[1][1]), fmaxf(amax_w[1][2], amax_w[1][3])));
-  if (r0 > 0) {  // older keys in front
-    if (gqa_scale_ok(old_k)) {
-      if (old_k >= s_k) {
-        s_k = old_k;
-      } else {
-        const float ratio = old_k / s_k;
-        for (int i = tid; i < r0 * (D / 16); i += 256) {
-          u32x4g x = reinterpret_cast<u32x4g*>(blk.k)[i];
+  if (r0 > 0 && gqa_scale_ok(old_k) && gqa_scale_ok(old_v)) {  // older keys in front
+    if (old_k >= s_k) {
+      s_k = old_k;
+    } else {
+      const float ratio = old_k / s_k;
+      for (int i = tid; i < r0 * (D / 16); i += 256) {
+        u32x4g x = reinterpret_cast<u32x4g*>(blk.k)[i];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = gqa_rescale4(x[j], ratio);
-          reinterpret_cast<u32x4g*>(blk.k)[i] = x;
-        }
+        for (int j = 0; j < 4; ++j) x[j] = gqa_rescale4(x[j], ratio);
+        reinterpret_cast<u32x4g*>(blk.k)[i] = x;
       }
     }
-    if (gqa_scale_ok(old_v)) {
-      if (old_v >= s_v) {
-        s_v = old_v;
-      } else {
-        const float ratio = old_v / s_v;
-        for (int i = tid; i < D * kGqaKeys / 4; i += 256) {  // four keys of a dim; those behind r0 - 1 are written below
-          uint32_t* at = reinterpret_cast<uint32_t*>(blk.v) + i;
-          if (i % (kGqaKeys / 4) * 4 < r0) *at = gqa_rescale4(*at, ratio);
-        }
+    if (old_v >= s_v) {
+      s_v = old_v;
+    } else {
+      const float ratio = old_v / s_v;
+      for (int i = tid; i < D * kGqaKeys / 4; i += 256) {  // four keys of a dim; those behind r0 - 1 are written below
+        uint32_t* at = reinterpret_cast<uint32_t*>(blk.v) + i;
+        if (i % (kGqaKeys / 4) * 4 < r0) *at = gqa_rescale4(*at, ratio);
       }
     }
+  } else if (r0 > 0) {  // older keys that are NaN, as one of their scales is none: under the new scales their codes say so
+    for (int i = tid; i < r0 * (D / 16); i += 256) reinterpret_cast<u32x4g*>(blk.k)[i] = u32x4g{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+    for (int i = tid; i < D * kGqaKeys / 4; i += 256)
+      if (i % (kGqaKeys / 4) * 4 < r0) reinterpret_cast<uint32_t*>(blk.v)[i] = 0x7f7f7f7fu;
   }
   const float inv_k = 1.0f / s_k, inv_v = 1.0f / s_v, most_k = gqa_most(s_k), most_v = gqa_most(s_v);
 #pragma unroll

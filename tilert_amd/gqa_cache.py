@@ -93,7 +93,8 @@ def gqa_cache_write(key: torch.Tensor, value: torch.Tensor, kv_pages: torch.Tens
     it is given: dims i and i + rope_dim / 2 are a pair, or 2i and 2i + 1 with ``interleaved``.
 
     Keys and values are quantised by page and head, with the least power of two that holds the block's new rows; a block with
-    older keys keeps a larger scale, or moves their codes to the larger new one.  A key that holds a NaN or an infinity,
+    older keys keeps a larger scale, or moves their codes to the larger new one, and older keys under a scale that is none
+    (NaN to all that see them) stay NaN.  A key that holds a NaN or an infinity,
     in its key or its value row, is NaN to the rows that see it and touches nothing else.  ``key_weights`` (fp32 [n_pages,
     kv_heads, 64]) is set to 0 for the keys written.  A page that is written to belongs to one place of one sequence."""
     name = "gqa_cache_write"
