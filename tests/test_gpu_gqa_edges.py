@@ -7,10 +7,11 @@ import torch
 from oracle import gqa
 from tests import _gqa
 from tests.test_gpu_flash_paged_gqa import check, run
+from tests.test_gpu_gqa_cache import check_write, inputs, write
 from tilert_amd.gqa_cache import gqa_cache_write
 
 pytestmark = pytest.mark.gpu
-BF16, I32, U8 = torch.bfloat16, torch.int32, torch.uint8
+BF16, F32, I32, U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
 @pytest.mark.parametrize("dim", [64, 128])
@@ -79,3 +80,51 @@ def test_older_keys_under_no_scale_stay_nan(cuda, side, bad, old, new, dim, size
     out, lse = run(cuda, q, after, table, cu, lens, 2)
     check(cuda, q, after, table, cu, lens, 2, out, lse)
     assert torch.isnan(out[:, 2:]).all() and torch.isnan(lse[:, 2:]).all() and torch.isfinite(out[:, :2]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("std", [1e18, 1e19, 1e30, 3e38])
+@pytest.mark.parametrize("turn", [False, True])
+def test_norms_of_rows_whose_squares_pass_fp32(cuda, turn, std, dim):
+    new, total, kv = [70, 3], [100, 64], 2
+    pages, table, cu, lens, rows = _gqa.batch(new, total, kv, dim, seed=151)
+    _gqa.fill(pages, table, [t - n for n, t in zip(new, total)], kv, dim)
+    joint, gq, gk, freqs = inputs(rows, 4, kv, dim, 64, 153, 0.0)
+    g = torch.Generator().manual_seed(155)
+    joint = ((torch.rand(joint.shape, generator=g) * 2 - 1) * std).to(BF16)
+    joint[1::3] = (joint[1::3].float() / std).to(BF16)  # every third token of ordinary rows
+    joint[:, 4 + kv:] = torch.randn(rows, kv, dim, generator=g).to(BF16)
+    freqs = freqs if turn else None
+    after, out = write(cuda, joint, 4, kv, pages, table, cu, lens, gq, gk, freqs)
+    check_write(pages, after, joint, 4, kv, dim, table, cu, lens, gq, gk, freqs, False, out)
+
+
+@pytest.mark.parametrize("std,eps", [(1e-16, 0.0), (1e-30, 0.0), (1e-38, 0.0), (1e-38, 1e-38), (1e-30, 1e-45), (1e-20, 1e-12), (3e38, 0.0), (3e38, 1e30)])
+def test_norms_with_a_small_or_large_eps(cuda, std, eps):
+    """Rows of sizes whose squares fall below fp32 or pass it, with an eps that is as small, nothing, or far larger: within the
+    roundings of a norm, 2^-20 (the writer's tests say of what), and of bf16."""
+    dim, rows = 128, 40
+    g = torch.Generator().manual_seed(157)
+    q = ((torch.rand(rows, 4, dim, generator=g) * 2 - 1) * std).to(BF16)
+    pages, table, cu, lens, _ = _gqa.batch([rows], [rows], 4, dim, seed=159)
+    gamma, out = torch.rand(dim, generator=g) + 0.5, torch.zeros(rows, 4, dim, dtype=BF16, device=cuda)
+    gqa_cache_write(*_gqa.to(cuda, q, q, pages, table, cu, lens), gamma.to(cuda), query=q.to(cuda), gamma_q=gamma.to(cuda), query_out=out, eps=eps)
+    want = gqa.turned(q, gamma, None, False, float(torch.tensor(eps, dtype=F32)))
+    assert torch.all((out.cpu().double() - want).abs() <= (2 ** -8 + 2 ** -19) * want.abs() + 2.0 ** -134)  # (bf16's least step, 2^-133)
+
+
+def test_a_row_of_zeros_and_rows_that_are_not_finite(cuda):
+    """0 / sqrt(eps) is 0; a NaN or an infinity makes a query's row what the formula gives, and a key NaN."""
+    dim = 64
+    q = torch.randn(8, 1, dim, generator=torch.Generator().manual_seed(161)).to(BF16)
+    q[0], q[1, 0, 3], q[2, 0, 5], q[3, 0, 7] = 0, math.nan, math.inf, -math.inf
+    q[3, 0, 9:] = 3e38
+    pages, table, cu, lens, _ = _gqa.batch([8], [8], 1, dim, seed=163)
+    gamma, out, p = torch.ones(dim), torch.zeros(8, 1, dim, dtype=BF16, device=cuda), pages.to(cuda)
+    gqa_cache_write(*_gqa.to(cuda, q, q.nan_to_num(1.0, 1.0, 1.0)), p, *_gqa.to(cuda, table, cu, lens, gamma), query=q.to(cuda), gamma_q=gamma.to(cuda), query_out=out)
+    want = gqa.turned(q, gamma, None, False, 1e-6)
+    assert torch.equal(torch.isnan(out.cpu()), torch.isnan(want))
+    fine = ~torch.isnan(want)
+    assert torch.all((out.cpu().double() - want).abs()[fine] <= ((2 ** -8 + 2 ** -19) * want.abs())[fine])
+    keys = gqa.value_of(gqa.views(p.cpu(), 1, dim)[0][int(table[0, 0]), 0, :8])
+    assert torch.all(keys[0] == 0) and torch.isnan(keys[1:4]).all() and torch.isfinite(keys[4:]).all()

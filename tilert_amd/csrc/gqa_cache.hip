@@ -30,12 +30,12 @@ struct GqaWriteArgs {
   uint64_t per_heads;  // ceil(2^34 / heads): x / heads = x * per_heads >> 34 for x < 2^27, heads <= 128
 };
 
-template <int LANES>  // sum / max over 8 or 16 consecutive lanes, in all of them
+template <int LANES, bool MAX = false>  // sum / max over 8 or 16 consecutive lanes, in all of them
 __device__ inline float row_sum(float v) {
-  v = dpp_combine<0xb1, false>(v);
-  v = dpp_combine<0x4e, false>(v);
-  v = dpp_combine<0x141, false>(v);
-  return LANES == 16 ? dpp_combine<0x140, false>(v) : v;
+  v = dpp_combine<0xb1, MAX>(v);
+  v = dpp_combine<0x4e, MAX>(v);
+  v = dpp_combine<0x141, MAX>(v);
+  return LANES == 16 ? dpp_combine<0x140, MAX>(v) : v;
 }
 
 __device__ inline void unpack8(u32x4g raw, float (&x)[8]) {
@@ -84,9 +84,26 @@ __device__ inline void norm_rope(float (&x)[8], int part, bool norm, const float
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-    const float mean = row_sum<LANES>(ss) * (1.0f / D) + eps;
-    float r = __builtin_amdgcn_rsqf(mean);  // (within 2^-23; it takes a subnormal for 0)
-    if (mean < 0x1p-126f) r = 1.0f / __builtin_sqrtf(mean);
+    float mean = row_sum<LANES>(ss) * (1.0f / D) + eps;
+    // Where the squares pass fp32 (elements from some 2^60 on) or are lost below it (with an eps that is as small), the row and
+    // eps are brought by a power of two to where the larger of them, the row's largest or sqrt(eps), is in [1, 2).
+    const bool far = !(mean >= 0x1p-100f && mean < INFINITY);
+    if (__any(far)) {
+      float top = __builtin_sqrtf(eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf(x[i]));
+      top = row_sum<LANES, true>(top);
+      const int by = far && top > 0.f && top < INFINITY ? 1 - __builtin_amdgcn_frexp_expf(top) : 0;
+      ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_ldexpf(x[i], by);
+        ss = __builtin_fmaf(x[i], x[i], ss);
+      }
+      const float scaled = row_sum<LANES>(ss) * (1.0f / D) + __builtin_ldexpf(eps, 2 * by);
+      mean = far ? scaled : mean;
+    }
+    const float r = __builtin_amdgcn_rsqf(mean);  // (within 2^-23)
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * r * gamma[i];
   }
