@@ -128,3 +128,46 @@ def test_a_row_of_zeros_and_rows_that_are_not_finite(cuda):
     assert torch.all((out.cpu().double() - want).abs()[fine] <= ((2 ** -8 + 2 ** -19) * want.abs())[fine])
     keys = gqa.value_of(gqa.views(p.cpu(), 1, dim)[0][int(table[0, 0]), 0, :8])
     assert torch.all(keys[0] == 0) and torch.isnan(keys[1:4]).all() and torch.isfinite(keys[4:]).all()
+
+
+@pytest.mark.parametrize("new,total", [(1, 1), (3, 70), (16, 700), (100, 100), (100, 700)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_codes_of_a_page_s_earlier_use(cuda, dim, new, total):
+    """A reused page's codes of 448 behind the last key, under the scale of the largest values, which takes them past bf16: no row
+    sees them, and none is changed by them."""
+    pages, table, cu, lens, rows = _gqa.batch([new], [total], 2, dim, seed=171)
+    pages.fill_(0x7e)
+    _gqa.fill(pages, table, [total - new], 2, dim)
+    g = torch.Generator().manual_seed(173)
+    key, value = torch.randn(new, 2, dim, generator=g).to(BF16), torch.randn(new, 2, dim, generator=g).to(BF16)
+    value[:, 1] = torch.where(value[:, 1] < 0, -1, 1) * 3.3e38
+    after = append(cuda, pages, table, lens, key, value, total - new)
+    assert float(gqa.views(after, 2, dim)[2][int(table[0, (total - 1) // 64]), 1, 1]) == 2.0 ** 120
+    q = _gqa.queries(rows, 8, dim, 175)
+    out, lse = run(cuda, q, after, table, cu, lens, 2)
+    check(cuda, q, after, table, cu, lens, 2, out, lse)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("new", [3, 100])
+@pytest.mark.parametrize("power,most,code", [(120, 0x77, 0x78), (121, 0x6f, 0x70), (124, 0x57, 0x58), (127, 0x3f, 0x40), (127, 0x3f, 0x7e)])
+def test_a_value_past_bf16_reaches_only_the_tokens_that_see_it(cuda, power, most, code, new):
+    """A code that a scale takes past bf16 (the least: `most` is the last that stays inside), in the page of the newest tokens: rows before it are as without it, bit for bit, rows from
+    it on are not finite in its dim."""
+    total, dim = 200, 64
+    pages, table, cu, lens, rows = _gqa.batch([new], [total], 2, dim, seed=177)
+    _gqa.fill(pages, table, [total], 2, dim)
+    q = _gqa.queries(rows, 8, dim, 179)
+    _, v, scales = gqa.views(pages, 2, dim)
+    page, row = int(table[0, (total - 2) // 64]), (total - 2) % 64
+    scales[page, 1, 1] = 2.0 ** power
+    v[page, 1] &= 0x83  # (subnormal codes)
+    v[page, 1, 5, row] = most
+    clean, clean_lse = run(cuda, q, pages, table, cu, lens, 2)
+    assert torch.isfinite(clean).all()
+    v[page, 1, 5, row] = code
+    out, lse = run(cuda, q, pages, table, cu, lens, 2)
+    assert torch.equal(lse, clean_lse) and torch.equal(out[:-2], clean[:-2]) and torch.equal(out[:, :4], clean[:, :4])
+    assert not torch.isfinite(out[-2:, 4:, 5]).any()
+    out[-2:, 4:, 5] = clean[-2:, 4:, 5]
+    assert torch.equal(out, clean)

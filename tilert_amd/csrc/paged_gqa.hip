@@ -251,8 +251,13 @@ __device__ inline v8bf codes8_bf16(uint32_t a, uint32_t b, float scale) {
 }
 __device__ inline v4f mfma_bf16(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// Bytes that are a NaN code, as 0x80 each.
-__device__ inline uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// Bytes that are no number in bf16 under a block's scale, as 0x80 each: NaN codes, and from 2^120 on those that it takes past the
+// largest (a page's earlier use may have left them behind its last key; a key that a row does not see has weight 0, and 0 times an
+// infinity is NaN).  `from`, of the scale: what brings the least of them to 0x80.
+__device__ inline uint32_t bad_codes_from(float scale) {
+  return 0x01010101u * static_cast<uint32_t>(max(1, (static_cast<int>(__float_as_uint(scale) >> 23) - 246) * 8));
+}
+__device__ inline uint32_t bad_codes(uint32_t x, uint32_t from) { return ((x & 0x7f7f7f7fu) + from) & 0x80808080u; }
 
 // The query rows of a tile as the first product's B operand: lane (c, g) holds of row c the dims 64 i + 16 g + 8 e .. + 7, the
 // order in which a 16-byte load gives it a key's codes.
@@ -415,14 +420,15 @@ __global__ __launch_bounds__(256, D == 128 && RT > 1 ? 1 : 2) void gqa_attend_ke
         lo[r][e] = bf16_of(w);
       }
     }
-    // ---- values; on a page with keys that some row does not see, codes that are NaN are taken apart
+    // ---- values; on a page with keys that some row does not see, codes that are no number are taken apart
     if (masked) {
+      const uint32_t bad_from = bad_codes_from(sv);
       uint32_t all = 0;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) all |= nan_codes(vc.v[d][i]);
-      if (__any(all != 0)) {  // how many NaN values a row sees
+        for (int i = 0; i < 4; ++i) all |= bad_codes(vc.v[d][i], bad_from);
+      if (__any(all != 0)) {  // how many of them a row sees
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll
@@ -433,14 +439,14 @@ __global__ __launch_bounds__(256, D == 128 && RT > 1 ? 1 : 2) void gqa_attend_ke
               u32x4g w;
 #pragma unroll
               for (int i = 0; i < 4; ++i) w[i] = (8 * e + 2 * i < my[r] ? 0x3f80u : 0u) | (8 * e + 2 * i + 1 < my[r] ? 0x3f800000u : 0u);
-              n = mfma_bf16(codes8_bf16(nan_codes(vc.v[d][2 * e]) >> 1, nan_codes(vc.v[d][2 * e + 1]) >> 1, 1.f), bf16_of(w), n);
+              n = mfma_bf16(codes8_bf16(bad_codes(vc.v[d][2 * e], bad_from) >> 1, bad_codes(vc.v[d][2 * e + 1], bad_from) >> 1, 1.f), bf16_of(w), n);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[r][d][j] = n[j] > 0.f ? __builtin_nanf("") : o[r][d][j];
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t bad = nan_codes(vc.v[d][i]);
+            const uint32_t bad = bad_codes(vc.v[d][i], bad_from);
             vc.v[d][i] &= ~(bad | (bad - (bad >> 7)));
           }
         }
@@ -563,7 +569,7 @@ struct GqaChunkLds {
     struct {
       u32x4g k[2][2][KF][64];     // [t][f]: 32 keys x 16 dims
       u32x4g v[3][VT][2][2][64];  // [d][t][e]: 32 dims x 16 keys
-      u32x4g bad[3][VT][2][64];   // [d][t]: where values of a page are NaN that is not seen by all rows
+      u32x4g bad[3][VT][2][64];   // [d][t]: where values of a page that is not seen by all rows are no number
     };
   };
   int odd[3];  // the page of a buffer that has such values
@@ -656,10 +662,11 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void gqa_chunk_kernel(const Gq
         to = &L.k[kb][rows >> 1][4 * (piece % KI) + 2 * (b16 >> 1)][32 * (b16 & 1) + 16 * (rows & 1) + r16];
       } else {
         const int d = piece - KP, at = 32 * (b16 >> 1) + 16 * (d & 1) + r16;
-        if (masked) {  // on a page with keys that some row does not see, values that are NaN are taken apart
+        if (masked) {  // on a page with keys that some row does not see, values that are no number are taken apart
+          const uint32_t bad_from = bad_codes_from(by);
           u32x4g bad;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) bad[i] = nan_codes(x[i]);
+          for (int i = 0; i < 4; ++i) bad[i] = bad_codes(x[i], bad_from);
           if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0) && lane == 0) L.odd[vb] = it.pg0 + k;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -697,7 +704,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void gqa_chunk_kernel(const Gq
     }
   };
   auto values = [&](int k, bool is, int vb) __attribute__((always_inline)) {
-    if ((unseen(k) || !is) && L.odd[vb] == it.pg0 + k) {  // how many NaN values a row sees
+    if ((unseen(k) || !is) && L.odd[vb] == it.pg0 + k) {  // how many of them a row sees
       const int my = is ? seen - (it.pg0 + k) * kGqaKeys - 32 * h : 0;
 #pragma unroll
       for (int d = 0; d < VT; ++d) {
