@@ -497,8 +497,8 @@ int tl_flash_paged_mla(const void* q_nope_bf16, const void* q_pe_bf16, const voi
  * [n_pages, kv_heads * 128 * head_dim + kv_heads * 8 rounded up to 128], 16-byte aligned: page p
  * holds 64 keys, for each kv head 64 x head_dim e4m3fn key codes, then head_dim x 64 e4m3fn
  * value codes (a dim is a row); behind all heads two fp32 scales a head, the keys' and the
- * values', powers of two.  A key is code * its block's scale; a scale that is not positive and
- * finite makes its block's keys NaN.  head_dim 64 or 128; heads <= 128, a multiple of kv_heads;
+ * values', powers of two.  A key is code * its block's scale; where either of a block's two scales
+ * is not positive, normal and finite, its keys and values are NaN.  head_dim 64 or 128; heads <= 128, a multiple of kv_heads;
  * query head h reads kv head h / (heads / kv_heads). */
 
 /* The new tokens' keys and values, and their queries: rows x of k and q bf16 [n_tokens, kv_heads

@@ -7,8 +7,8 @@ import torch
 from oracle import gqa
 from tests import _gqa
 from tests.test_gpu_flash_paged_gqa import check, run
-from tests.test_gpu_gqa_cache import check_write, inputs, write
-from tilert_amd.gqa_cache import gqa_cache_write
+from tests.test_gpu_gqa_cache import check_sums, check_write, evict, evict_case, inputs, write
+from tilert_amd.gqa_cache import gqa_cache_weights, gqa_cache_write
 
 pytestmark = pytest.mark.gpu
 BF16, F32, I32, U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
@@ -171,3 +171,34 @@ def test_a_value_past_bf16_reaches_only_the_tokens_that_see_it(cuda, power, most
     assert not torch.isfinite(out[-2:, 4:, 5]).any()
     out[-2:, 4:, 5] = clean[-2:, 4:, 5]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_under_no_scale_are_nan_after_an_eviction(cuda, dim, side):
+    """One of a block's two scales is none: its keys are NaN in the attention and in the key weights, before an eviction and after it."""
+    args = evict_case([300], [130], 2, dim, 181)
+    pages, w, table, lens, keep, to = args
+    bad = int(table[0, 1])
+    gqa.views(pages, 2, dim)[2][bad, 1, side] = math.nan
+    w[bad, 1, 5:20] = 1e9  # some of them stay
+    after, _, kept, slots = evict(cuda, *args, 2, dim, 30)
+    mine = slots[0, 1]
+    from_bad = (mine >= 64) & (mine < 128)
+    assert from_bad.sum() >= 15 and kept.tolist() == [130]
+    k, v, _ = gqa.views(after, 2, dim)
+    for c in range(3):
+        page, at = int(to[0, c]), from_bad[64 * c:64 * c + 64]
+        there = mine[64 * c:64 * c + 64] >= 0
+        for codes in (k[page, 1], v[page, 1].T):
+            assert torch.equal(torch.isnan(gqa.value_of(codes)).all(-1)[there], at[there])
+            assert torch.isfinite(gqa.value_of(codes))[there & ~at].all()
+    q, cu = _gqa.queries(1, 8, dim, 183), torch.tensor([0, 1], dtype=I32)
+    for p, tab, n in ((pages, table, lens), (after, to, kept)):
+        out, lse = run(cuda, q, p, tab, cu, n, 2)
+        check(cuda, q, p, tab, cu, n, 2, out, lse)
+        assert torch.isnan(out[:, 4:]).all() and torch.isnan(lse[:, 4:]).all() and torch.isfinite(out[:, :4]).all()
+        got = torch.zeros(pages.shape[0], 2, 64, device=cuda)
+        finite = torch.nan_to_num(lse, nan=1.0)
+        gqa_cache_weights(*_gqa.to(cuda, q), finite, *_gqa.to(cuda, p, tab, cu, n), got)
+        check_sums(cuda, q, finite, p, tab, cu, n, 2, torch.zeros(got.shape), got, True)

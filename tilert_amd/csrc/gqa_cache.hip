@@ -520,8 +520,9 @@ __global__ __launch_bounds__(256) void gqa_gather_kernel(const GqaEvictArgs A) {
     if (pos >= 0) {
       page = A.table[static_cast<int64_t>(b) * A.max_pages + (pos >> 6)];
       const GqaBlock s = gqa_block<D>(A.pages, A.page_bytes, A.kv_heads, page, h);
-      sk = gqa_scale_ok(s.scale[0]) ? s.scale[0] : __builtin_nanf("");
-      sv = gqa_scale_ok(s.scale[1]) ? s.scale[1] : __builtin_nanf("");
+      sk = s.scale[0];
+      sv = s.scale[1];
+      if (!gqa_scale_ok(sk) || !gqa_scale_ok(sv)) sk = sv = __builtin_nanf("");  // (either: its keys are NaN, and their codes will say so)
       A.weights[(static_cast<int64_t>(to) * A.kv_heads + h) * kGqaKeys + tid] = A.weights[(static_cast<int64_t>(page) * A.kv_heads + h) * kGqaKeys + (pos & 63)];
     }
     src_page[tid] = page;
