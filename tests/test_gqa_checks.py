@@ -257,3 +257,10 @@ def test_the_least_scale(amax, scale):
 def test_eviction_refuses_new_lengths_in_the_old_ones_place(off):
     """A head's workgroup may still read a length when another one's has written the new one."""
     _refused("tl_gqa_cache_evict", _evict_c(n_seqs=2, lens=P, kept=P + off), 1, "kept_lens")
+
+
+@pytest.mark.parametrize("name,args", [("tl_flash_paged_gqa", _attend_c), ("tl_gqa_cache_weights", _sum_c)])
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38, float("inf")])
+def test_a_softmax_scale_that_passes_fp32_times_log2_e(name, args, scale):
+    """The exponents are powers of two: an infinite factor would make the scores of zero queries NaN."""
+    _refused(name, args(scale=scale), 1, "softmax_scale")

@@ -1287,7 +1287,10 @@ static int check_gqa_batch(const char* who, int64_t n_seqs, int64_t n_tokens, in
               "2^20 pages", who, (long long)n_tokens, (long long)heads, (long long)n_seqs, (long long)max_pages);
     return kErrUnsupported;
   }
-  if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) { set_error("%s: softmax_scale must be positive and finite", who); return kErrArg; }
+  if (!(softmax_scale > 0.f) || !(softmax_scale * kLog2e < INFINITY)) {  // (the kernels take it times log2 e; infinite, it makes a score of 0 NaN)
+    set_error("%s: softmax_scale must be positive, and finite times log2(e)", who);
+    return kErrArg;
+  }
   return kOk;
 }
 
