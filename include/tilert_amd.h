@@ -556,7 +556,8 @@ int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const float* lse,
  * the largest).  They go in ascending order into the pages kept_table [n_seqs, kept_pages] of the
  * same pool, which must not be among the tables' own (a page outside the pool: dropped),
  * their codes under the blocks' new scales (the least power of two, as above) and their weights with
- * them; kept_lens int32 [n_seqs] (not seq_lens' memory) = k, kept_slots int32 [n_seqs, kv_heads, kept_pages * 64] their
+ * them; kept_lens int32 [n_seqs] (not in seq_lens'
+ * memory; keep_lens itself or apart from it) = k, kept_slots int32 [n_seqs, kv_heads, kept_pages * 64] their
  * positions, -1 behind the k-th.  block_table, seq_lens, keep_lens, kept_table: int32 on the
  * device.  Keys of pages outside the pool are not there. */
 int tl_gqa_cache_evict(void* kv_pages, float* key_weights, int64_t n_pages, const int32_t* block_table, int64_t max_pages,

@@ -264,3 +264,9 @@ def test_eviction_refuses_new_lengths_in_the_old_ones_place(off):
 def test_a_softmax_scale_that_passes_fp32_times_log2_e(name, args, scale):
     """The exponents are powers of two: an infinite factor would make the scores of zero queries NaN."""
     _refused(name, args(scale=scale), 1, "softmax_scale")
+
+
+@pytest.mark.parametrize("off", [4, -4])
+def test_eviction_refuses_new_lengths_that_overlap_the_counts_of_others(off):
+    """The counts' own place is fine: a length in its sequence's count's place brings out itself.  One further, it is another's count."""
+    _refused("tl_gqa_cache_evict", _evict_c(n_seqs=2, lens=P + 4096, cu=P, kept=P + off), 1, "kept_lens")

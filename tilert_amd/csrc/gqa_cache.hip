@@ -658,10 +658,15 @@ extern "C" int tl_gqa_cache_evict(void* kv_pages, float* key_weights, int64_t n_
     set_error("%s: %lld sequences of %lld kept pages: more than a launch has room for", who, (long long)n_seqs, (long long)kept_pages);
     return kErrUnsupported;
   }
-  // (a head's workgroup may read its sequence's length when another's has written the new one)
-  const uintptr_t from = reinterpret_cast<uintptr_t>(seq_lens), to = reinterpret_cast<uintptr_t>(kept_lens);
-  if ((from < to ? to - from : from - to) < static_cast<uintptr_t>(n_seqs) * 4) {
-    set_error("%s: kept_lens must not be the memory of seq_lens", who);
+  // (a head's workgroup may read its sequence's length, or another sequence's its count, when another's has written the new length;
+  // a sequence's own count in its place does no harm, as the new length brings out itself)
+  const uintptr_t to = reinterpret_cast<uintptr_t>(kept_lens);
+  auto overlaps = [&](const int32_t* p) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+    return (from < to ? to - from : from - to) < static_cast<uintptr_t>(n_seqs) * 4;
+  };
+  if (overlaps(seq_lens) || (keep_lens != kept_lens && overlaps(keep_lens))) {
+    set_error("%s: kept_lens must not be the memory of seq_lens, nor a part of keep_lens'", who);
     return kErrArg;
   }
   const GqaEvictArgs args{(uint8_t*)kv_pages, gqa_page_bytes(kv_heads, head_dim), key_weights, block_table, seq_lens, keep_lens,

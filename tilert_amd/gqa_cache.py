@@ -165,7 +165,7 @@ def gqa_cache_evict(kv_pages: torch.Tensor, key_weights: torch.Tensor, block_tab
     of the others those of the largest ``key_weights`` (equal ones: the lowest position; NaN counts as the largest).  They
     go in ascending order, codes, scales and weights, into the pages of ``kept_table`` (int32 [sequences, pages], of the
     same pool); the sequences' own pages are left as they are, and may be given back afterwards.  ``kept_lens`` (int32
-    [sequences], not seq_lens itself; keep_lens may be it) receives the new lengths -- keep_lens, but no more than there are keys
+    [sequences], not in seq_lens' memory; it may be keep_lens itself, but not overlap it) receives the new lengths -- keep_lens, but no more than there are keys
     or kept_table has room for -- and ``kept_slots`` (int32 [sequences, kv_heads, 64 * pages]) the positions that were kept,
     -1 behind them.  kept_table names a page once, and none of the tables'; one outside the pool is not written."""
     name = "gqa_cache_evict"
