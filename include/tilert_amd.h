@@ -526,9 +526,14 @@ int tl_gqa_cache_write(const void* k_bf16, int64_t k_stride, const void* v_bf16,
  * elements apart); token t at position p sees the keys 0 .. p of its sequence:
  *   s[j] = q . k[j] * softmax_scale,  out = softmax(s) . v
  * out bf16 [n_tokens, heads, head_dim], lse fp32 [n_tokens, heads] (nullable) = ln sum e^s; 0 and
- * -inf where no key is seen.  Codes times scales are exact in bf16, statistics and sums fp32.  A row's
- * result follows from the keys that it sees and from no other row's.  n_tokens * heads < 2^27, n_seqs
- * <= 2^16, max_pages <= 2^20.  workspace: the bytes that tl_flash_paged_gqa_workspace_bytes names
+ * -inf where no key is seen.  Codes times scales are exact in bf16 (from a scale of 2^120 on, codes
+ * past bf16's largest are not finite to the rows that see them); scores (one past fp32 is infinite),
+ * statistics and sums fp32.  Probabilities go into the second product with 16 bits, or, where the
+ * batch has more than 32 rows (tokens * heads / kv_heads; 64 with head_dim 64) a sequence in the mean,
+ * with bf16's 8.  Within a call a row's result follows from its query and the keys that it sees and
+ * from no other row's; how its sums are split follows from the batch's sizes and lengths, so beside
+ * other sequences it may be rounded otherwise.  softmax_scale > 0, and finite times log2(e).
+ * n_tokens * heads < 2^27, n_seqs <= 2^16, max_pages <= 2^20.  workspace: the bytes that tl_flash_paged_gqa_workspace_bytes names
  * for these sizes (0: none), 16-byte aligned, its contents of no account before or after; calls
  * that overlap in time need one each. */
 size_t tl_flash_paged_gqa_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads,
@@ -541,10 +546,11 @@ int tl_flash_paged_gqa(const void* q_bf16, int64_t q_stride, const void* kv_page
 
 /* The attention weights that the keys gather from the batch's tokens: with q and lse as
  * tl_flash_paged_gqa took and gave them, key_weights fp32 [n_pages, kv_heads, 64] at the page and
- * row of each key j of a sequence with new tokens, j below its last token's position,
+ * row of each key j of a sequence with new tokens, j up to and with its last token's position,
  *   key_weights (+)= sum of e^(s[j] - lse) over the tokens that see j and the heads of the group,
- * added to what is there (accumulate = 1) or in its place (0); summed in fp32 in a fixed order.
- * Sequences must not share pages.  Limits as tl_flash_paged_gqa's. */
+ * added to what is there (accumulate = 1) or in its place (0); fp32, lse * log2(e) rounded to it
+ * too, summed in a fixed order.  Sequences must not share pages, and a sequence's table names a page
+ * once.  Limits as tl_flash_paged_gqa's. */
 int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const float* lse, const void* kv_pages, int64_t n_pages,
                          const int32_t* block_table, int64_t max_pages, const int32_t* cu_seqlens,
                          const int32_t* seq_lens, int64_t n_seqs, int64_t n_tokens, int64_t heads, int64_t kv_heads,

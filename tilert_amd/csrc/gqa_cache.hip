@@ -133,7 +133,7 @@ __device__ inline void norm_rope(float (&x)[8], int part, bool norm, const float
 
 // A workgroup takes one page of a sequence's new keys and one kv head (its scales need all of the block's rows), or, behind
 // those, 64 query rows; 8 or 16 lanes a row, 16 bytes each.  Values are transposed through LDS.  Bound by bytes and the loads'
-// latency, as a workgroup's work is one round of them: 4000 tokens, 32 heads over 8 of 128 dims, 92 MB, 25 us, 3.7 TB/s,
+// latency, as a workgroup's work is one round of them: 4040 tokens, 32 heads over 8 of 128 dims, 92 MB, 25 us, 3.7 TB/s,
 // vector instructions busy for 60 % of it (27 us with angles loaded row by row and for dims that are not turned).
 template <int D>
 __global__ __launch_bounds__(256) void gqa_write_kernel(const GqaWriteArgs A) {

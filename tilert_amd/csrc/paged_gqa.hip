@@ -94,7 +94,9 @@ struct GqaItem {
 // longest.  A piece costs kGqaPiece pages beside its own.  (With a fixed number of pieces wanted, 7 sequences of 2 to 700 new
 // tokens over 324 to 5000 keys took 57 us with 120, 53 with 330, 50 with 384 and 55 with 780; with the search 45.  32 sequences of
 // 1024 keys, 256 tiles of 32 rows: 33 uncut, as the search has it, and 52 with 512 pieces.)
-constexpr int kGqaPlanSeqs = 512;  // sequences that a launch plans for; with more, a workgroup takes a tile
+// Sequences that a launch plans for; with more, a workgroup takes a tile.  In us with one sequence of 32768 keys among 512 and 513 of
+// 1024, 64 heads over 8, head_dim 128: attention 357 / 424, key weights 176 / 599.
+constexpr int kGqaPlanSeqs = 512;
 constexpr int kGqaFew = 8;         // pages that are not cut
 constexpr int kGqaPlans = 16;
 constexpr float kGqaPiece = 9.f;
@@ -320,9 +322,12 @@ __device__ inline float2 load_scales(const float* s) { return float2{load_f32_ve
 // second), each with its own statistics, and are joined in LDS.  A wave has up to 32 rows, so that the codes, 128 conversions
 // of two a page and lane, are turned for all of them (16 rows a wave, two waves on the same pages: 4 tokens of 8 heads over
 // 131072 keys 76 us, 59 so).  Weights go into the second product as hi + lo in bf16, 16 bits of them.
-// Weights are relative to 2^24 times the row's largest: their sums of values then stay inside fp32 whatever the values.
+// Weights are relative to 2^24 times the row's largest: their sums of values then stay inside fp32 whatever the values, for up to
+// 2^24 keys as heavy as the heaviest.
 // Bound by bytes, two pages a wave on their way: 60 sequences of 2048 to 32768 keys, 1.42 GB, 238 us, 6.0 TB/s; 131072 keys, 268 MB,
-// 55 us and 6 to join, where a copy's rate takes 52.
+// 55 us and 6 to join, where a copy's rate takes 52.  One token over a table of up to 8 pages, which is not planned, is bound by
+// latency: 1 to 64 keys 5.6 us, loads one behind another (token ranges and lengths, table, page), the products, the waves' join;
+// 256, a page each for the four waves, 6.8; 500, two one behind another, 8.4.
 constexpr float kGqaHead = 24.f;
 template <int D, int RT>
 __global__ __launch_bounds__(256, D == 128 && RT > 1 ? 1 : 2) void gqa_attend_kernel(const GqaArgs A) {
@@ -552,7 +557,9 @@ __global__ __launch_bounds__(256, D == 128 && RT > 1 ? 1 : 2) void gqa_attend_ke
 // ---- many rows: the waves of a workgroup go through the pages together
 // A page's codes are turned into bf16 once, by the wave that loaded them, and lie in LDS as the products' operands, fragment
 // by fragment in lane order; each wave multiplies them with its own 32 rows.  Weights go into the second product in
-// bf16, 8 bits.  A row's reference m is set anew only where a score passes it by 2^8: hardly a page rescales anything.
+// bf16, 8 bits: the result's rms error is 0.0023 of it, 0.0017 with the 16 bits that few rows have, of which the result's own rounding
+// to bf16 is the most; a second product for the other 8 would be half of the matrix pipe's work again.
+// A row's reference m is set anew only where a score of its own passes it by 2^8: hardly a page rescales anything.
 //
 // The two waves of a SIMD are a third of a page apart: between two barriers waves 0 .. 3 make scores, weights and sums of page k,
 // waves 4 .. 7 weights and sums of page k - 1 and scores of page k, so that one's products run while the other makes
@@ -942,6 +949,9 @@ inline GqaLaunch gqa_launch(int64_t n_seqs, int64_t n_tokens, int64_t heads, int
   // us with 32-row, 64-row / kChunkRows tiles, 64 heads over 8, head_dim 128: 32 rows of 1 sequence over 131072 keys 66 / 95, of 8
   // over 4096 29 / 32, of 64 over 4096 142 / 184; 64 rows 91 / 98, 42 / 34, 204 / 191.  head_dim 64: 32 rows 35 / 73, 18 / 26,
   // 66 / 140; 64 rows 55 / 76, 26 / 27, 105 / 147; 96 rows of 8 over 4096 34 / 27.
+  // The rule goes by the batch's mean, so a batch of unlike sequences pays for it: 60 sequences of one token over 1000 to 8000 keys
+  // (119 us) and a chunk of 512 over 4096 (82) take 328 in one call, 64 heads over 8; 200 of one token over 200 to 2000 keys (113)
+  // and a prompt of 800 (30) 241, with one of 100 (12) 116, 32 heads over 8.
   d.bm = each <= 16 ? 16 : (each <= 32 ? 32 : (each <= 64 && head_dim == 64 ? 64 : kChunkRows));
   d.slots = gqa_slots(n_tokens, group, n_seqs, d.bm);
   d.at_once = d.bm == kChunkRows || (head_dim == 128 && d.bm > 16) ? 256 : 512;  // (by registers one workgroup a CU, or two)
@@ -987,8 +997,11 @@ struct GqaUnit {
 };
 
 // Few rows (a decode step): a wave takes every fourth page of a piece, one behind another, the next two's keys on their way;
-// their rows, RT tiles of 16 as a rule, stay in registers (more of them are loaded page by page).  Scores as in the
-// attention's first product, S^T = K Q^T: a lane sums its keys' weights over its column of rows.  Bound by bytes: 60
+// their rows, RT tiles of 16 as a rule, stay in registers (a sequence's more of them are loaded page by page: 200 sequences of one token
+// and a prompt of 800, 32 heads over 8, 70 and 30 us in a call each, 628 in one).  Scores as in the
+// attention's first product, S^T = K Q^T: a lane sums its keys' weights over its column of rows.  A weight is e^(s - lse) as
+// 2^(s' - lse'), lse' = lse log2 e rounded to fp32, which costs it up to 2^-24 lse': the sums' rms error is 2.0e-7, the
+// plain form's in fp32 1.2e-7.  Bound by bytes: 60
 // sequences of 2048 to 32768 keys, 730 MB, 157 us, 4.6 TB/s.  Pieces as the attention plans them (in groups of kSumPages
 // pages by the table's width they took 170 us).  Two tiles against the kernel for many rows below: 4 tokens of 8 heads over
 // 131072 keys 34 / 59 us, over 8192 keys of 40 sequences 90 / 147; four tiles, 8 tokens, 75 / 66.
@@ -1374,8 +1387,8 @@ extern "C" int tl_gqa_cache_weights(const void* q_bf16, int64_t q_stride, const 
   const int64_t each = cdiv(n_tokens * (heads / kv_heads), n_seqs);
   const bool few = each <= 32;
   // Pages a workgroup: as many as leave most CUs one, by the table's width, which of many sequences fewer fill.  In us with 1, 2, 4
-  // and 8: 32 tokens of 2 sequences of 1500 keys, 8 heads of 128 dims, 19 11 12 17; 2048 of 1 of 16384 928 709 575 528; 1000 of 1
-  // of 1000 63 93 152 264; 9 to 300 of 16 of 125 to 2000 98 68 72 91.
+  // and 8, all with 64 heads over 8 of 128 dims: 32 tokens each of 2 sequences of 1500 keys 19 11 12 17; 2048 of 1 of 16384 928 709
+  // 575 528; 1000 of 1 of 1000 63 93 152 264; 9 to 300 of 16 of 125 to 2000 98 68 72 91.  (The bound was set between these four.)
   int pw = 8;
   while (pw > 1 && cdiv(max_pages, pw) * kv_heads * n_seqs < std::min<int64_t>(128 + 32 * n_seqs, 768)) pw /= 2;
   // Pieces that few rows' pages are cut into: as many as run at once, or, where more than a few tiles may be of unlike

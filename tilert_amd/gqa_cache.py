@@ -140,7 +140,8 @@ def gqa_cache_weights(query: torch.Tensor, lse: torch.Tensor, kv_pages: torch.Te
     tokens, up to the last one's own, the sum over the tokens that see it and the query heads of its group of
     exp(score - lse), with ``query`` and ``lse`` as ``flash_paged_gqa`` took and gave them.  It is added to ``key_weights``
     (fp32 [n_pages, kv_heads, 64], at the key's page and row), or takes its place with ``accumulate=False``.  A batch of a
-    prompt's last tokens alone (their own cu_seqlens) gives the weights of that window.  Sequences must not share pages."""
+    prompt's last tokens alone (their own cu_seqlens) gives the weights of that window.  Sequences must not share pages, and a
+    sequence's table names a page once: a key's sum is one wave's."""
     name = "gqa_cache_weights"
     query_stride = _check_rows(name, "query", query)
     tokens, heads, head_dim = query.shape
